@@ -1,0 +1,314 @@
+// Attention over pages of int8 codes: the kernel on the CUDA cores, which takes every head size, float32 and bfloat16, the merge of key
+// slices, and the entry point that decides which kernel takes which requests.  Formulas in attention_q8.cuh.
+#include "attention_q8.cuh"
+
+#include <algorithm>
+#include <math.h>
+
+namespace {
+
+// ---- CUDA cores ------------------------------------------------------------------------------------
+// A CTA takes 32 rows and walks its keys in tiles of 64: codes are widened to float32 in shared memory, the keys' times their scale,
+// scores and outputs are register tiles of 4 rows by 4 keys (by HDP / 16 dimensions), the softmax runs online with float32 statistics.
+// The values' scales enter with the weights: the weight of a key that a row may not see is zero whatever its scale is, and a code is
+// always a number, so that what is not finite stays with the rows that see it.  Bound by the float32 units and shared memory; this is
+// the true 32-bit path, and the one of head sizes that the tensor-core kernels do not take.
+constexpr int BM = 32, BN = 64, THREADS = 128;
+
+template <int HDP> constexpr int lds_k() { return HDP + 4; }          // padded rows: sixteen lanes read sixteen keys without bank conflicts
+template <int HDP> constexpr size_t plain_smem() { return sizeof(float) * ((size_t)BM * lds_k<HDP>() + 2 * (size_t)BN * lds_k<HDP>() + BM * (BN + 4) + BN); }
+
+template <typename T, int HDP>
+__global__ void __launch_bounds__(THREADS) attention_q8_plain_kernel(const Q8Params p) {
+    pdl_launch_dependents();
+    constexpr int LD = lds_k<HDP>(), DV = HDP / 16, LP = BN + 4;
+    extern __shared__ __align__(16) float q8_smem[];
+    float *Q = q8_smem, *K = Q + BM * LD, *V = K + BN * LD, *P = V + BN * LD, *sv_s = P + BM * LP;
+    const int tid = threadIdx.x, kvh = blockIdx.y, slice = blockIdx.z;
+    const int rg = tid >> 4, kg = tid & 15;             // rows 4 rg .. + 3; keys kg + 16 j, dimensions 4 kg + 64 j
+    pdl_wait();
+    Q8Tile t;
+    if (!q8_find_tile(p, blockIdx.x, t)) return;
+    int lo, hi;
+    q8_slice(t, p.slices, slice, BN, lo, hi);
+    for (int i = tid; i < BM * HDP; i += THREADS) {
+        const int r = i / HDP, d = i % HDP;
+        float x = 0.f;
+        if (r < t.rows && d < p.hd) x = to_f32<T>(((const T *)p.q)[q8_out_row(p, t, kvh, r) * p.hd + d]);
+        Q[r * LD + d] = x;
+    }
+    float m[4], l[4], o[4][DV];
+    int pos[4], low[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DV; ++d) o[i][d] = 0.f;
+        const int r = 4 * rg + i;
+        pos[i] = r < t.rows ? t.pos_begin + (t.row0 + r) / t.G : -1;
+        low[i] = p.window > 0 ? max(0, pos[i] - p.window + 1) : 0;
+    }
+    const float scale_log2 = p.scale * 1.4426950408889634f;
+    for (int kb = lo / BN * BN; kb < hi; kb += BN) {
+        __syncthreads();
+        // four codes a thread and turn; keys outside the slice count as zero, whatever their page holds
+        for (int i = tid; i < BN * (HDP / 4); i += THREADS) {
+            const int r = i / (HDP / 4), d = i % (HDP / 4) * 4, key = kb + r;
+            float4 kf = make_float4(0.f, 0.f, 0.f, 0.f), vf = kf;
+            if (key >= lo && key < hi && d < p.hd) {
+                const long long row = q8_row_of(p, t.table, kvh, key);
+                const size_t at = (size_t)(row + key % Q8_BLOCK) * p.hd + d;
+                const char4 kc = *reinterpret_cast<const char4 *>(p.k + at), vc = *reinterpret_cast<const char4 *>(p.v + at);
+                const float sk = p.ks[row / Q8_BLOCK];
+                kf = make_float4(kc.x * sk, kc.y * sk, kc.z * sk, kc.w * sk);
+                vf = make_float4(vc.x, vc.y, vc.z, vc.w);
+                if (d == 0) sv_s[r] = p.vs[row / Q8_BLOCK];
+            }
+            *reinterpret_cast<float4 *>(K + r * LD + d) = kf;
+            *reinterpret_cast<float4 *>(V + r * LD + d) = vf;
+        }
+        __syncthreads();
+        float s[4][4] = {};
+#pragma unroll 4
+        for (int d = 0; d < HDP; d += 4) {
+            float4 a[4], b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4 *>(Q + (4 * rg + i) * LD + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4 *>(K + (kg + 16 * j) * LD + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[i][j] = fmaf(a[i].x, b[j].x, s[i][j]);
+                    s[i][j] = fmaf(a[i].y, b[j].y, s[i][j]);
+                    s[i][j] = fmaf(a[i].z, b[j].z, s[i][j]);
+                    s[i][j] = fmaf(a[i].w, b[j].w, s[i][j]);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float mx = -INFINITY;
+            bool seen[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = kb + kg + 16 * j;
+                seen[j] = key >= lo && key < hi && key <= pos[i] && key >= low[i];
+                s[i][j] = seen[j] ? s[i][j] * scale_log2 : -INFINITY;
+                mx = fmaxf(mx, s[i][j]);
+            }
+#pragma unroll
+            for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+            const float mn = fmaxf(m[i], mx), use = mn == -INFINITY ? 0.f : mn;
+            const float alpha = exp2f(m[i] - use);
+            m[i] = mn;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[i][j] = exp2f(s[i][j] - use);
+                sum += s[i][j];
+                P[(4 * rg + i) * LP + kg + 16 * j] = seen[j] ? s[i][j] * sv_s[kg + 16 * j] : 0.f;
+            }
+#pragma unroll
+            for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+            l[i] = l[i] * alpha + sum;
+#pragma unroll
+            for (int d = 0; d < DV; ++d) o[i][d] *= alpha;
+        }
+        __syncwarp();               // a row's probabilities are its own sixteen lanes'
+#pragma unroll 2
+        for (int j = 0; j < BN; j += 4) {
+            float pr[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 x = *reinterpret_cast<const float4 *>(P + (4 * rg + i) * LP + j);
+                pr[i][0] = x.x; pr[i][1] = x.y; pr[i][2] = x.z; pr[i][3] = x.w;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int d = 0; d < DV; d += 4) {
+                    const float4 x = *reinterpret_cast<const float4 *>(V + (j + k) * LD + 4 * kg + 16 * d);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        o[i][d] = fmaf(pr[i][k], x.x, o[i][d]);
+                        o[i][d + 1] = fmaf(pr[i][k], x.y, o[i][d + 1]);
+                        o[i][d + 2] = fmaf(pr[i][k], x.z, o[i][d + 2]);
+                        o[i][d + 3] = fmaf(pr[i][k], x.w, o[i][d + 3]);
+                    }
+                }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = 4 * rg + i;
+        if (r >= t.rows) continue;
+        const size_t row = q8_out_row(p, t, kvh, r);
+        if (p.slices > 1) {
+#pragma unroll
+            for (int d = 0; d < DV; ++d) {
+                const int at = 4 * kg + 16 * (d & ~3) + (d & 3);
+                if (at < p.hd) p.part_o[(row * p.slices + slice) * p.hd + at] = o[i][d];
+            }
+            if (kg == 0) {
+                p.part_ml[(row * p.slices + slice) * 2] = m[i];
+                p.part_ml[(row * p.slices + slice) * 2 + 1] = l[i];
+            }
+        } else {
+            const float inv = 1.0f / l[i];
+#pragma unroll
+            for (int d = 0; d < DV; ++d) {
+                const int at = 4 * kg + 16 * (d & ~3) + (d & 3);
+                if (at < p.hd) ((T *)p.out)[row * p.hd + at] = from_f32<T>(o[i][d] * inv);
+            }
+        }
+    }
+}
+
+// ---- merge -------------------------------------------------------------------------------------------
+// A warp takes a row: lane s holds slice s's maximum and sum, the outputs are added in ascending order of the slices.
+template <typename T>
+__global__ void __launch_bounds__(256) attention_q8_merge_kernel(const Q8Params p) {
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, kvh = blockIdx.y, r = blockIdx.z * 8 + (threadIdx.x >> 5);
+    pdl_wait();
+    Q8Tile t;
+    if (!q8_find_tile(p, blockIdx.x, t) || r >= t.rows) return;
+    const size_t row = q8_out_row(p, t, kvh, r);
+    const float2 ml = lane < p.slices ? *reinterpret_cast<const float2 *>(p.part_ml + (row * p.slices + lane) * 2) : make_float2(-INFINITY, 0.f);
+    const float M = warp_max(ml.x), f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+    const float inv = 1.0f / warp_sum(f == 0.f ? 0.f : ml.y * f);
+    for (int d = lane; d < p.hd; d += 32) {
+        float acc = 0.f;
+        for (int s = 0; s < p.slices; ++s) {
+            const float fs = __shfl_sync(__activemask(), f, s);
+            if (fs != 0.f) acc = fmaf(p.part_o[(row * p.slices + s) * p.hd + d], fs, acc);
+        }
+        ((T *)p.out)[row * p.hd + d] = from_f32<T>(acc * inv);
+    }
+}
+
+template <typename T, int HDP>
+int launch_plain(const Q8Params &p, int tiles, cudaStream_t stream) {
+    const size_t smem = plain_smem<HDP>();
+    if (cudaFuncSetAttribute(attention_q8_plain_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+        return kestrel_fail(-3, "attention_q8: cannot raise the shared-memory limit: %s", cudaGetErrorString(cudaGetLastError()));
+    kestrel_launch(attention_q8_plain_kernel<T, HDP>, dim3(tiles, p.nkv, p.slices), dim3(THREADS), smem, stream, p);
+    return kestrel_check_launch("attention_q8");
+}
+
+}  // namespace
+
+int q8_launch_plain(const Q8Params &p, int dtype, int tiles, cudaStream_t stream) {
+    if (dtype == KESTREL_F32)
+        return p.hd <= 64 ? launch_plain<float, 64>(p, tiles, stream) : p.hd <= 128 ? launch_plain<float, 128>(p, tiles, stream) : launch_plain<float, 256>(p, tiles, stream);
+    return p.hd <= 64 ? launch_plain<__nv_bfloat16, 64>(p, tiles, stream)
+                      : p.hd <= 128 ? launch_plain<__nv_bfloat16, 128>(p, tiles, stream) : launch_plain<__nv_bfloat16, 256>(p, tiles, stream);
+}
+
+int q8_launch_merge(const Q8Params &p, int dtype, int tiles, cudaStream_t stream) {
+    const dim3 grid(tiles, p.nkv, (p.rows_per_tile + 7) / 8);
+    if (dtype == KESTREL_F32) kestrel_launch(attention_q8_merge_kernel<float>, grid, dim3(256), 0, stream, p);
+    else kestrel_launch(attention_q8_merge_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, p);
+    return kestrel_check_launch("attention_q8 merge");
+}
+
+namespace {
+
+constexpr int MAX_SLICES = 32;
+
+// One launch of a step: the requests with rows_above < rows <= rows_upto, in tiles of rows_per_tile.
+struct Part {
+    int rows_above = 0, rows_upto = 0, rows_per_tile = 0, tiles = 0, slices = 1, longest = 0;
+};
+struct Plan {
+    Part part[2];
+    int parts = 0;
+};
+
+int slices_for(long long ctas, int slots, int keys, int least) {
+    if (ctas < 1 || keys < 1) return 1;
+    return (int)std::max<long long>(1, std::min<long long>(std::min<long long>(slots / ctas, keys / least), MAX_SLICES));
+}
+
+// counts of (token, head) rows follow from the host's copy of cu_seqlens; without it every request brings max_count tokens at most
+void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, int max_kv, int T, int nq, int nkv, int hd, int window, int dtype) {
+    const int G = nq / nkv;
+    (void)hd;
+    (void)dtype;
+    Part p;
+    p.rows_above = 0;
+    p.rows_upto = 0x7fffffff;
+    p.rows_per_tile = BM;
+    if (!cu) {
+        p.tiles = nseq * (int)(((long long)max_count * G + BM - 1) / BM);
+        p.longest = max_kv;
+    } else {
+        for (int i = 0; i < nseq; ++i) {
+            const long long rows = (long long)(cu[i + 1] - cu[i]) * G;
+            if (rows <= 0) continue;
+            p.tiles += (int)((rows + BM - 1) / BM);
+            p.longest = std::max(p.longest, kv[i]);
+        }
+    }
+    (void)T;
+    if (window > 0) p.longest = std::min(p.longest, window);
+    p.slices = slices_for((long long)p.tiles * nkv, kestrel_sms() * 2, p.longest, 256);
+    if (p.tiles) pl.part[pl.parts++] = p;
+}
+
+}  // namespace
+
+KESTREL_API long long kestrel_attention_q8_scratch(const int *cu_host, const int *kv_host, int nseq, int max_count, int max_kv, int T, int nq, int nkv, int hd,
+                                                   int window, int dtype) {
+    if (nseq <= 0 || T <= 0 || nq <= 0 || nkv <= 0 || nq % nkv) return 0;
+    Plan pl;
+    make_plan(pl, cu_host, kv_host, nseq, max_count, max_kv, T, nq, nkv, hd, window, dtype);
+    long long slices = 1;
+    for (int i = 0; i < pl.parts; ++i) slices = std::max<long long>(slices, pl.part[i].slices);
+    return slices > 1 ? (long long)T * nq * slices * (hd + 2) : 0;
+}
+
+KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, void *out, float *scratch,
+                                     long long scratch_floats, const int *cu_host, const int *kv_host, const int *cu_seqlens, const int *kv_lens,
+                                     const int *block_table, int nseq, int max_count, int max_kv, int table_width, int table_stride, int page_size,
+                                     int cache_pages, int T, int nq, int nkv, int hd, int window, float scale, int dtype, kestrel_stream_t stream) {
+    if (T == 0 || nseq == 0) return 0;
+    KESTREL_REQUIRE(T > 0 && nseq > 0 && max_count > 0 && max_kv >= max_count, "attention_q8: a step of %d tokens of %d requests, %d at most, %d keys at most", T, nseq, max_count, max_kv);
+    KESTREL_REQUIRE(dtype == KESTREL_F32 || dtype == KESTREL_BF16, "attention_q8: unknown dtype %d", dtype);
+    KESTREL_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "attention_q8: %d query heads over %d kv heads", nq, nkv);
+    KESTREL_REQUIRE(hd > 0 && hd % 16 == 0 && hd <= 256, "attention_q8: head size %d is no multiple of 16 up to 256", hd);
+    KESTREL_REQUIRE(page_size > 0 && page_size % Q8_BLOCK == 0, "attention_q8: pages of %d tokens are no whole blocks of %d", page_size, Q8_BLOCK);
+    KESTREL_REQUIRE(window >= 0 && scale > 0.f && isfinite(scale), "attention_q8: window %d, scale %g", window, scale);
+    KESTREL_REQUIRE(cache_pages > 0 && (long long)cache_pages * nkv * page_size < (1ll << 31), "attention_q8: a cache of %d pages is beyond the 32-bit row coordinate", cache_pages);
+    KESTREL_REQUIRE(table_width > 0 && table_stride >= table_width, "attention_q8: block table of %d entries a row, %d apart", table_width, table_stride);
+    KESTREL_REQUIRE(nkv <= 65535, "attention_q8: grid too large");
+    Plan pl;
+    make_plan(pl, cu_host, kv_host, nseq, max_count, max_kv, T, nq, nkv, hd, window, dtype);
+    int launches = 0;
+    for (int i = 0; i < pl.parts; ++i) {
+        const Part &part = pl.part[i];
+        Q8Params p = {};
+        p.q = q; p.out = out; p.k = (const int8_t *)k_cache; p.v = (const int8_t *)v_cache; p.ks = k_scale; p.vs = v_scale;
+        p.cu_seqlens = cu_seqlens; p.kv_lens = kv_lens; p.block_table = block_table;
+        p.nseq = nseq; p.table_width = table_width; p.table_stride = table_stride; p.page_size = page_size; p.cache_pages = cache_pages;
+        p.nq = nq; p.nkv = nkv; p.hd = hd; p.window = window; p.slices = part.slices; p.scale = scale;
+        p.rows_above = part.rows_above; p.rows_upto = part.rows_upto; p.rows_per_tile = part.rows_per_tile;
+        if (part.slices > 1) {
+            const long long need = (long long)T * nq * part.slices * (hd + 2);
+            KESTREL_REQUIRE(scratch && need <= scratch_floats, "attention_q8: %d slices need scratch of %lld floats, %lld given", part.slices, need, scratch_floats);
+            p.part_o = scratch;
+            p.part_ml = scratch + (long long)T * nq * part.slices * hd;
+        }
+        int rc = q8_launch_plain(p, dtype, part.tiles, stream);
+        if (rc) return rc;
+        launches++;
+        if (part.slices > 1) {
+            rc = q8_launch_merge(p, dtype, part.tiles, stream);
+            if (rc) return rc;
+            launches++;
+        }
+    }
+    return launches;
+}

@@ -1,0 +1,271 @@
+// Log probabilities of given tokens, the entropy, and the likeliest tokens of rows of logits.
+//
+// One pass over a row: every thread keeps the maximum m of its numbers, L = sum e^(x - m) and A = sum (x - m) e^(x - m), joined like any
+// online softmax's states - the sums move to a larger maximum m' as L' = f L, A' = f (A + (m - m') L) with f = e^(m - m') - so that
+//     log p(i) = (x_i - m) - log L,      entropy = log L - A / L,
+// both without a difference of large numbers.  A row's distances, exponentials and sums are float32.
+//
+// The likeliest tokens come from the threads' maxima, which the pass has made anyway: a value T that at least `top` threads' maxima reach
+// is at most the top-th largest number, so only threads whose maximum reaches T hold candidates.  T is found bit by bit over a count of
+// threads; the warps read those few threads' numbers again and keep the best of them, one a lane, in order.  Equal numbers go by index.
+//
+// A row is one block's, or a cluster's of up to 8 where the rows are few; a cluster's blocks meet once, in the first block's shared
+// memory.  Bound by the row's bytes; a number costs half a maximum, an add, a product, an
+// exponential, an add, a bound and a multiply-add.
+#include "common.cuh"
+
+#include <math.h>
+
+namespace {
+
+constexpr int THREADS = 512, WARPS = THREADS / 32, MOST = KESTREL_LOGPROBS_MAX_TOP, MAX_CLUSTER = 8;
+constexpr int FLIGHT = 4;               // vectors of four numbers that a thread has in flight
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct State {
+    float m, l, a;                      // m = -inf: nothing but -inf so far
+    __device__ __forceinline__ void rise(float to) {
+        if (to > m) {
+            const float f = m == -INFINITY ? 0.f : exp2f((m - to) * LOG2E);
+            a = f == 0.f ? 0.f : f * fmaf(m - to, l, a);
+            l *= f;
+            m = to;
+        }
+    }
+    __device__ __forceinline__ void join(State o) {
+        if (o.m > m) {
+            State t = o;
+            o = *this;
+            *this = t;
+        }
+        const float f = o.m == -INFINITY ? 0.f : exp2f((o.m - m) * LOG2E);
+        // sums that are no numbers stay that, whatever their maximum is
+        a += f == 0.f && o.a == o.a ? 0.f : f * fmaf(o.m - m, o.l, o.a);
+        l += f == 0.f && o.l == o.l ? 0.f : f * o.l;
+    }
+};
+
+// order of the numbers as that of unsigned integers, never 0
+__device__ __forceinline__ uint32_t key_of(float x) {
+    const uint32_t u = __float_as_uint(x + 0.f);                    // -0 counts as 0
+    const uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
+    return k ? k : 1u;
+}
+__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+// larger numbers first, equal ones by index
+__device__ __forceinline__ uint64_t entry_of(float x, uint32_t i) { return (uint64_t)key_of(x) << 32 | (uint32_t)~i; }
+
+__device__ __forceinline__ void add(State &s, float x, float m_use) {
+    const float d = x - m_use;                                      // first the difference: the lowest number times anything is -inf
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * LOG2E));
+    s.l += e;
+    s.a = fmaf(e, fmaxf(d, -1e30f), s.a);                           // e is 0 where d is -inf
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t in_first(const void *p) {       // this address in the cluster's first block
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(0));
+    return r;
+}
+
+// A warp's best `top` entries, one a lane, best first; e: a lane's new entry, 0 for none
+__device__ __forceinline__ void keep(uint64_t &best, uint64_t e, int top, int lane) {
+    const uint64_t last = __shfl_sync(0xffffffffu, best, top - 1);
+    for (uint32_t rest = __ballot_sync(0xffffffffu, e > last); rest; rest &= rest - 1) {
+        const uint64_t c = __shfl_sync(0xffffffffu, e, __ffs(rest) - 1);
+        const int at = __popc(__ballot_sync(0xffffffffu, best > c));
+        const uint64_t up = __shfl_up_sync(0xffffffffu, best, 1);
+        if (lane == at) best = c;
+        else if (lane > at) best = up;
+    }
+}
+
+__global__ void __launch_bounds__(THREADS, 2)
+token_logprobs_kernel(const float *__restrict__ logits, long long ld, int V, int cluster, const int *__restrict__ ids, int top, float *__restrict__ logprobs,
+                      float *__restrict__ entropy, int *__restrict__ top_ids, float *__restrict__ top_logprobs) {
+    pdl_launch_dependents();
+    __shared__ State joined[MAX_CLUSTER], parts[WARPS];
+    __shared__ uint64_t found[WARPS * MOST], block_best[MAX_CLUSTER * MOST];
+    __shared__ int n_found;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int row = blockIdx.x / cluster, rank = cluster > 1 ? (int)cluster_rank() : 0;
+    const float *x = logits + (size_t)row * ld;
+    // numbers in front of the first 16-byte boundary and behind the last vector go to single threads of the first and last block
+    const int head = min(V, (int)((16 - ((uintptr_t)x & 15)) & 15) / 4), nv = (V - head) / 4;
+    const float4 *xv = reinterpret_cast<const float4 *>(x + head);
+    const int v0 = (int)((long long)nv * rank / cluster), v1 = (int)((long long)nv * (rank + 1) / cluster);
+    int odd = -1;                       // index of this thread's number outside the vectors
+    if (rank == 0 && tid < head) odd = tid;
+    if (rank == cluster - 1 && tid >= 4 && tid - 4 < V - head - 4 * nv) odd = head + 4 * nv + tid - 4;
+    if (tid < WARPS * MOST) found[tid] = 0;
+    if (tid == 0) n_found = 0;
+    if (cluster > 1) cluster_arrive();  // the first block's shared memory may be written once every block has begun
+    pdl_wait();
+    float given = __uint_as_float(0x7fc00000u);
+    if (ids && rank == 0 && tid == 0) {
+        const int id = ids[row];
+        if (id >= 0 && id < V) given = x[id];
+    }
+
+    State s = {-INFINITY, 0.f, 0.f};
+    float big = -INFINITY;              // this thread's largest number
+    if (odd >= 0) {
+        const float o = x[odd];
+        big = fmaxf(big, o);
+        s.rise(big);
+        add(s, o, s.m == -INFINITY ? 0.f : s.m);
+    }
+    for (int v = v0 + tid; v < v1; v += FLIGHT * THREADS) {
+        float4 q[FLIGHT];
+#pragma unroll
+        for (int i = 0; i < FLIGHT; ++i)
+            q[i] = v + i * THREADS < v1 ? __ldcs(xv + v + i * THREADS) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < FLIGHT; ++i) mx = fmaxf(fmaxf(fmaxf(mx, q[i].x), fmaxf(q[i].y, q[i].z)), q[i].w);
+        big = fmaxf(big, mx);
+        s.rise(mx);
+        const float m_use = s.m == -INFINITY ? 0.f : s.m;
+#pragma unroll
+        for (int i = 0; i < FLIGHT; ++i) {
+            add(s, q[i].x, m_use);
+            add(s, q[i].y, m_use);
+            add(s, q[i].z, m_use);
+            add(s, q[i].w, m_use);
+        }
+    }
+    if (cluster > 1) cluster_wait();
+    // the block's state
+    State w = s;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        State t = {__shfl_xor_sync(0xffffffffu, w.m, o), __shfl_xor_sync(0xffffffffu, w.l, o), __shfl_xor_sync(0xffffffffu, w.a, o)};
+        w.join(t);
+    }
+    if (lane == 0) parts[warp] = w;
+
+    if (top > 0) {
+        // T: the largest value whose bits, from the highest down, leave at least `top` threads' maxima at or above it
+        const bool some = odd >= 0 || v0 + tid < v1;
+        const uint32_t mine = some ? key_of(big) : 0u;
+        uint32_t T = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t c = T | 1u << bit;
+            if (__syncthreads_count(mine >= c) >= top) T = c;
+        }
+        T = max(T, 1u);
+        uint64_t best = 0;
+        for (uint32_t rest = __ballot_sync(0xffffffffu, mine >= T); rest; rest &= rest - 1) {
+            const int l = __ffs(rest) - 1;
+            const int l_odd = __shfl_sync(0xffffffffu, odd, l);
+            if (l_odd >= 0) keep(best, lane == 0 ? entry_of(x[l_odd], l_odd) : 0, top, lane);
+            for (int v = v0 + 32 * warp + l; v < v1; v += 32 * THREADS) {
+                const int at = v + lane * THREADS;
+                float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (at < v1) q = xv[at];
+                const float e[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) keep(best, at < v1 && key_of(e[j]) >= T ? entry_of(e[j], head + 4 * at + j) : 0, top, lane);
+            }
+        }
+        // the warps' entries in one list, then each goes to the place that the number of better ones gives it
+        if (best && lane < top) found[atomicAdd(&n_found, 1)] = best;
+        __syncthreads();
+        const int n = n_found;
+        for (int i = tid; i < n; i += THREADS) {
+            const uint64_t e = found[i];
+            int at = 0;
+            for (int j = 0; j < n; ++j) at += found[j] > e;
+            if (at < top) {
+                if (cluster > 1) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(in_first(block_best + rank * MOST + at)), "l"(e) : "memory");
+                else block_best[at] = e;
+            }
+        }
+        for (int i = n + tid; i < top; i += THREADS) {              // a block with fewer numbers than that
+            if (cluster > 1) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(in_first(block_best + rank * MOST + i)), "l"(0ull) : "memory");
+            else block_best[i] = 0;
+        }
+    }
+    __syncthreads();
+    if (warp == 0) {
+        State b = lane < WARPS ? parts[lane] : State{-INFINITY, 0.f, 0.f};
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            State t = {__shfl_xor_sync(0xffffffffu, b.m, o), __shfl_xor_sync(0xffffffffu, b.l, o), __shfl_xor_sync(0xffffffffu, b.a, o)};
+            b.join(t);
+        }
+        if (lane == 0) {
+            if (cluster > 1) {
+                const uint32_t to = in_first(joined + rank);
+                asm volatile("st.shared::cluster.f32 [%0], %1;\n\tst.shared::cluster.f32 [%0 + 4], %2;\n\tst.shared::cluster.f32 [%0 + 8], %3;"
+                             ::"r"(to), "f"(b.m), "f"(b.l), "f"(b.a) : "memory");
+            } else {
+                joined[0] = b;
+            }
+        }
+    }
+    if (cluster > 1) {
+        cluster_arrive();
+        cluster_wait();
+    } else {
+        __syncthreads();
+    }
+    if (rank != 0) return;
+    State r = joined[0];
+    for (int c = 1; c < cluster; ++c) r.join(joined[c]);
+    const float log_l = logf(r.l), m_use = r.m == -INFINITY ? 0.f : r.m;
+    if (tid == 0) {
+        if (entropy) entropy[row] = log_l - r.a / r.l;
+        if (ids) logprobs[row] = (given - m_use) - log_l;
+    }
+    for (int i = tid; i < cluster * top; i += THREADS) {
+        const uint64_t e = block_best[i / top * MOST + i % top];
+        if (!e) continue;
+        int at = i % top;                                            // its own block's better ones
+        for (int c = 0; c < cluster; ++c) {
+            if (c == i / top) continue;
+            for (int j = 0; j < top && block_best[c * MOST + j] > e; ++j) ++at;
+        }
+        if (at < top) {
+            top_ids[(size_t)row * top + at] = (int)~(uint32_t)e;
+            top_logprobs[(size_t)row * top + at] = (value_of((uint32_t)(e >> 32)) - m_use) - log_l;
+        }
+    }
+}
+
+}  // namespace
+
+KESTREL_API int kestrel_token_logprobs(const float *logits, long long ld, int R, int V, const int *ids, int top, float *logprobs, float *entropy, int *top_ids,
+                                       float *top_logprobs, kestrel_stream_t stream) {
+    if (R == 0) return 0;
+    KESTREL_REQUIRE(R > 0 && V > 0 && ld >= V, "token_logprobs: %d rows of %d logits, %lld apart", R, V, ld);
+    KESTREL_REQUIRE(top >= 0 && top <= MOST && top <= V, "token_logprobs: the %d likeliest of %d; at most %d are picked", top, V, MOST);
+    KESTREL_REQUIRE((!ids || logprobs) && (top == 0 || (top_ids && top_logprobs)), "token_logprobs: no place for the results");
+    KESTREL_REQUIRE(((uintptr_t)logits & 3) == 0, "token_logprobs: logits must start on 4 bytes");
+    // blocks of a row: while twice as many would still be resident at once, two an SM
+    int cluster = 1;
+    while (cluster < MAX_CLUSTER && (long long)R * cluster * 2 <= 2ll * kestrel_sms() && V / (cluster * 2) >= 1024) cluster *= 2;
+    KESTREL_REQUIRE((long long)R * cluster < (1ll << 31), "token_logprobs: %d rows exceed the grid", R);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)R * cluster);
+    cfg.blockDim = dim3(THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = g_kestrel_pdl ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, token_logprobs_kernel, logits, ld, V, cluster, ids, top, logprobs, entropy, top_ids, top_logprobs);
+    return kestrel_check_launch("token_logprobs");
+}

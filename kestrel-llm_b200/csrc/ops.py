@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -82,6 +82,22 @@ def _stream():
     if _raw_stream is not None and _raw_device is not None:
         return _raw_stream(_raw_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_here = _Here()
+
+
+def _on(device: torch.device):
+    """A context in which ``device`` is the current one: kernels launch on the device of their tensors, on its current stream."""
+    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _need(t: torch.Tensor, name: str, dtype=None, dims: Optional[int] = None) -> None:
@@ -322,6 +338,156 @@ def attention_plain(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(),
         seq_of_token.data_ptr(), block_table.data_ptr(), block_table.stride(0), int(page_size),
         out.data_ptr(), _code(q, "attention.q"), T, nq, nkv, hd, int(window), float(scale), _stream()))
+
+
+# ---- pages of 8-bit codes -------------------------------------------------------------------------
+
+Q8_BLOCK = _cdecl.constants()["KESTREL_Q8_BLOCK"]       # tokens that share a scale
+
+
+def _need_q8(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, nkv: int, page_size: int, hd: int,
+             device: torch.device) -> None:
+    """Planes of the cache: int8 codes [pages, kv heads, page size, head size], float32 scales [pages, kv heads, page size / Q8_BLOCK]."""
+    if page_size % Q8_BLOCK:
+        raise KernelError(f"{what}: pages of {page_size} tokens are no whole blocks of {Q8_BLOCK}")
+    shape = (k_cache.shape[0], nkv, page_size, hd)
+    blocks = (k_cache.shape[0], nkv, page_size // Q8_BLOCK)
+    for t, name, dtype, want in ((k_cache, "k_cache", torch.int8, shape), (v_cache, "v_cache", torch.int8, shape),
+                                 (k_scale, "k_scale", torch.float32, blocks), (v_scale, "v_scale", torch.float32, blocks)):
+        if t.dtype != dtype or t.shape != want or not t.is_contiguous() or t.device != device:
+            _need(t, f"{what}.{name}", dtype, len(want))
+            if t.shape != want:
+                raise KernelError(f"{what}: {name} of shape {tuple(t.shape)}, expected {want}")
+            raise KernelError(f"{what}: {name} is on {t.device}, the queries on {device}")
+
+
+def _need_ints(what: str, device: torch.device, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != 1 or t.device != device:
+            _need(t, f"{what}.{name}", torch.int32, 1)
+            raise KernelError(f"{what}: {name} is on {t.device}, the queries on {device}")
+
+
+def _need_table(what: str, block_table: torch.Tensor, device: torch.device) -> None:
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.device != device or block_table.shape[1] < 1:
+        raise KernelError(f"{what}: the block table must be int32 [requests, pages] on {device} with neighbouring entries, "
+                          f"got {block_table.dtype} {tuple(block_table.shape)} on {block_table.device}")
+
+
+def attn_prepare_q8(qkv: Partials, q_norm_w: Optional[torch.Tensor], k_norm_w: Optional[torch.Tensor], norm_eps: float,
+                    inv_freq: Optional[torch.Tensor], rotary_dim: int, positions: torch.Tensor, cu_seqlens: torch.Tensor,
+                    block_table: torch.Tensor, page_size: int, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                    v_scale: torch.Tensor, q_out: torch.Tensor, nq: int, nkv: int, hd: int, write_kv: bool = True, rot_mode: int = 0,
+                    rot_scale: float = 1.0) -> None:
+    """`attn_prepare` into pages of 8-bit codes: bias, per-head RMSNorm, rotation (angles of any int32 position to float32 accuracy);
+    q to q_out (float32 or bfloat16), K and V as int8 codes in [-127, 127] and one float32 scale for every ``Q8_BLOCK`` tokens and head:
+    value = code * scale, scale = max(2^-64, largest magnitude / 127) over what the block has met, codes rounded to nearest even.
+    Where a step's tokens raise the scale of a block that earlier steps began, its codes are rounded again, so a block's codes depend on
+    how a sequence was cut into steps (by at most half a step of the scale for each rise).  A block that met a number that is not finite
+    has a scale that is not a number, until its page begins anew.  The tokens of request i are cu_seqlens[i] to cu_seqlens[i + 1] - 1, at
+    consecutive positions; rows of q_out behind the last request are left as they are, and so is a token whose page is absent."""
+    dev = q_out.device
+    _need(q_out, "attn_prepare_q8.q_out", dims=2)
+    T = q_out.shape[0]
+    if qkv.tokens != T or qkv.width != (nq + 2 * nkv) * hd or q_out.shape[1] != nq * hd:
+        raise KernelError("attn_prepare_q8: shapes differ")
+    _need_ints("attn_prepare_q8", dev, positions=positions, cu_seqlens=cu_seqlens)
+    _need_table("attn_prepare_q8", block_table, dev)
+    n = cu_seqlens.shape[0] - 1
+    if positions.shape[0] != T or n < 1 or block_table.shape[0] < n:
+        raise KernelError(f"attn_prepare_q8: {positions.shape[0]} positions and block tables of {block_table.shape[0]} requests for {T} tokens of {n} requests")
+    _need_q8("attn_prepare_q8", k_cache, v_cache, k_scale, v_scale, nkv, page_size, hd, dev)
+    for t, name, size in ((qkv.bias, "bias", qkv.width), (q_norm_w, "q_norm_w", hd), (k_norm_w, "k_norm_w", hd), (inv_freq, "inv_freq", rotary_dim // 2)):
+        if t is not None:
+            _need(t, f"attn_prepare_q8.{name}", torch.float32, 1)
+            if t.shape[0] < size or t.device != dev:
+                raise KernelError(f"attn_prepare_q8: {name} of {t.shape[0]} numbers on {t.device}, expected {size} on {dev}")
+    if qkv.data.device != dev:
+        raise KernelError(f"attn_prepare_q8: the product is on {qkv.data.device}, the queries on {dev}")
+    with _on(dev):
+        _check(library().kestrel_attn_prepare_q8(
+            qkv.data.data_ptr(), qkv.slices, qkv.slice_stride, _p(qkv.bias), _p(q_norm_w), _p(k_norm_w), norm_eps, _p(inv_freq),
+            rotary_dim, rot_mode, rot_scale, positions.data_ptr(), cu_seqlens.data_ptr(), n, block_table.data_ptr(), block_table.shape[1],
+            block_table.stride(0), page_size, k_cache.shape[0], k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), q_out.data_ptr(), _code(q_out, "attn_prepare_q8.q_out"), T, nq, nkv, hd, 1 if write_kv else 0, _stream()))
+
+
+def attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, out: torch.Tensor,
+                 batch, block_table: torch.Tensor, page_size: int, nq: int, nkv: int, hd: int, window: int, scale: float) -> None:
+    """Causal attention of this step's queries (float32 or bfloat16 [T, nq * hd]) over their requests' pages of 8-bit codes
+    (`attn_prepare_q8`), or over the last ``window`` keys.  ``batch`` is the step's description: ``num_tokens``, ``num_seqs``,
+    ``cu_seqlens`` and ``kv_lens`` (int32 on the device), their host copies ``cu_seqlens_host`` and ``kv_lens_host``, ``max_count``,
+    ``max_kv_len`` and ``captured`` (the launch is being recorded for replay with other lengths: every request then brings at most
+    ``max_count`` tokens).  Rows of ``out`` behind the last request are left as they are.  Kernels find their tiles on the device;
+    sums and softmax statistics are float32."""
+    dev = q.device
+    _need(q, "attention_q8.q", dims=2)
+    _need(out, "attention_q8.out", q.dtype, 2)
+    T, n = q.shape[0], batch.num_seqs
+    if q.shape[1] != nq * hd or out.shape != q.shape or out.device != dev:
+        raise KernelError(f"attention_q8: queries {tuple(q.shape)} and outputs {tuple(out.shape)} of {nq} heads of {hd}")
+    if T != batch.num_tokens:
+        raise KernelError(f"attention_q8: {T} query rows for a step of {batch.num_tokens} tokens")
+    _need_ints("attention_q8", dev, cu_seqlens=batch.cu_seqlens, kv_lens=batch.kv_lens)
+    _need_table("attention_q8", block_table, dev)
+    if batch.cu_seqlens.shape[0] < n + 1 or batch.kv_lens.shape[0] < n or block_table.shape[0] < n:
+        raise KernelError(f"attention_q8: a description of fewer than {n} requests")
+    _need_q8("attention_q8", k_cache, v_cache, k_scale, v_scale, nkv, page_size, hd, dev)
+    lib, code = library(), _code(q, "attention_q8.q")
+    max_count, max_kv = batch.max_count, batch.max_kv_len
+    cu = kv = None
+    if not batch.captured and max_count > 1:        # steps of single tokens need no look at the lengths
+        cu, kv = (ctypes.c_int * (n + 1))(*batch.cu_seqlens_host), (ctypes.c_int * n)(*batch.kv_lens_host)
+    with _on(dev):
+        floats = lib.kestrel_attention_q8_scratch(cu, kv, n, max_count, max_kv, T, nq, nkv, hd, window, code)
+        scratch = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
+        rc = lib.kestrel_attention_q8(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), out.data_ptr(), _p(scratch), floats,
+            cu, kv, batch.cu_seqlens.data_ptr(), batch.kv_lens.data_ptr(), block_table.data_ptr(), n, max_count, max_kv,
+            block_table.shape[1], block_table.stride(0), page_size, k_cache.shape[0], T, nq, nkv, hd, window, scale, code, _stream())
+    if rc < 0:
+        raise KernelError(lib.kestrel_last_error().decode("utf-8", "replace"))
+    global launches
+    launches += rc
+
+
+# ---- log probabilities ----------------------------------------------------------------------------
+
+class TokenLogprobs(NamedTuple):
+    """Of R rows: ``logprobs`` float32 [R] of the given tokens (None without them), ``entropy`` float32 [R] in nats, ``top_ids`` int32
+    and ``top_logprobs`` float32 [R, top]."""
+    logprobs: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+MAX_TOP_LOGPROBS = _cdecl.constants()["KESTREL_LOGPROBS_MAX_TOP"]
+
+
+def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, top: int = 0) -> TokenLogprobs:
+    """Natural log probabilities under softmax(logits[r]), logits float32 [R, V] with neighbouring columns (rows may be further apart):
+    of the given tokens ``ids`` (int32 [R]; an id outside the vocabulary gets NaN), and of the ``top`` likeliest tokens, at most
+    ``MAX_TOP_LOGPROBS`` of them, most likely first, equal ones by id; and every distribution's entropy.  A logit of minus infinity has
+    probability zero; a row of nothing else, or with a logit of plus infinity or NaN, has NaN for log probabilities and entropy."""
+    if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1 or not logits.is_cuda:
+        _need(logits, "token_logprobs.logits", torch.float32, 2)
+    R, V = logits.shape
+    dev = logits.device
+    if not 0 <= top <= min(V, MAX_TOP_LOGPROBS):
+        raise KernelError(f"token_logprobs: the {top} likeliest of {V} tokens; at most {MAX_TOP_LOGPROBS} are picked")
+    given = None
+    if ids is not None:
+        _need_ints("token_logprobs", dev, ids=ids)
+        if ids.shape[0] != R:
+            raise KernelError(f"token_logprobs: {ids.shape[0]} tokens for {R} rows")
+        given = torch.empty(R, dtype=torch.float32, device=dev)
+    got = TokenLogprobs(given, torch.empty(R, dtype=torch.float32, device=dev), torch.empty((R, top), dtype=torch.int32, device=dev),
+                        torch.empty((R, top), dtype=torch.float32, device=dev))
+    with _on(dev):
+        _check(library().kestrel_token_logprobs(logits.data_ptr(), logits.stride(0), R, V, _p(ids), top, _p(given), got.entropy.data_ptr(),
+                                                got.top_ids.data_ptr(), got.top_logprobs.data_ptr(), _stream()))
+    return got
 
 
 def argmax(logits: torch.Tensor, out: torch.Tensor) -> None:

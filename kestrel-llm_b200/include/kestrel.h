@@ -471,6 +471,27 @@ KESTREL_API int kestrel_attention(void *planner, long long step_serial, const in
 /* kernels launched by the planner's last kestrel_attention call */
 KESTREL_API int kestrel_attn_planner_last_launches(void *planner);
 
+/* ---- pages of 8-bit codes ----
+ * A plane of the cache is int8 codes [pages, nkv, page_size, hd] in [-127, 127] and float32 scales [pages, nkv, page_size / KESTREL_Q8_BLOCK];
+ * a value is code * scale, and KESTREL_Q8_BLOCK consecutive tokens share the scale of their head. */
+#define KESTREL_Q8_BLOCK 16
+/* Bias, per-head norm and rotation of a step's product (float32 [S, T, (nq + 2 nkv) hd]; rot_mode 0 rotate-half, 1 interleaved); queries to q_out
+ * (float32 or bfloat16), keys and values to their blocks.  A block's scale is max(2^-64, largest magnitude / 127) over what it has met since its
+ * first token; codes that earlier steps left in it are rounded again where it rises.  A block that met a value that is not finite has a scale that is
+ * not a number.  Requests' tokens are consecutive positions from positions[cu_seqlens[i]] on; tokens behind cu_seqlens[nseq] are left out. */
+KESTREL_API int kestrel_attn_prepare_q8(const float *partial, int S, long long slice_stride, const float *bias, const float *q_norm_w, const float *k_norm_w, float norm_eps, const float *inv_freq, int rot, int rot_mode, float rot_scale, const int *positions, const int *cu_seqlens, int nseq, const int *block_table, int table_width, int table_stride, int page_size, int cache_pages, void *k_cache, void *v_cache, float *k_scale, float *v_scale, void *q_out, int dtype, int T, int nq, int nkv, int hd, int write_kv, kestrel_stream_t stream);
+/* Causal attention of a step's queries over such pages; q and out float32 or bfloat16 [T, nq hd].  cu_host and kv_host are the host's copies of
+ * cu_seqlens and kv_lens, or NULL where only the bounds are known (a step recorded for replay).  scratch holds kestrel_attention_q8_scratch floats.
+ * Returns the number of kernels launched. */
+KESTREL_API long long kestrel_attention_q8_scratch(const int *cu_host, const int *kv_host, int nseq, int max_count, int max_kv, int T, int nq, int nkv, int hd, int window, int dtype);
+KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, void *out, float *scratch, long long scratch_floats, const int *cu_host, const int *kv_host, const int *cu_seqlens, const int *kv_lens, const int *block_table, int nseq, int max_count, int max_kv, int table_width, int table_stride, int page_size, int cache_pages, int T, int nq, int nkv, int hd, int window, float scale, int dtype, kestrel_stream_t stream);
+
+/* ---- log probabilities ---- */
+/* Of every row of logits float32 [R, ld], V of them: the log probability of ids[r] (ids may be NULL; an id outside [0, V) gives NaN), the entropy
+ * in nats (entropy may be NULL), and the `top` likeliest tokens, most likely first, ties to the lowest id. */
+#define KESTREL_LOGPROBS_MAX_TOP 32
+KESTREL_API int kestrel_token_logprobs(const float *logits, long long ld, int R, int V, const int *ids, int top, float *logprobs, float *entropy, int *top_ids, float *top_logprobs, kestrel_stream_t stream);
+
 /* ---- sampling ---- */
 KESTREL_API int kestrel_argmax(const float *logits, long long ld, int R, int V, int *out, float *cand_v, int *cand_i, kestrel_stream_t stream);
 KESTREL_API int kestrel_argmax_chunks(int V);
