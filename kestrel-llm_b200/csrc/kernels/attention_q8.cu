@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(256) attention_q8_merge_kernel(const Q8Params 
     const size_t row = q8_out_row(p, t, kvh, r);
     const float2 ml = lane < p.slices ? *reinterpret_cast<const float2 *>(p.part_ml + (row * p.slices + lane) * 2) : make_float2(-INFINITY, 0.f);
     const float M = warp_max(ml.x), f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-    const float inv = 1.0f / warp_sum(f == 0.f ? 0.f : ml.y * f);
+    const float inv = 1.0f / warp_sum(f == 0.f && ml.y == ml.y ? 0.f : ml.y * f);       // (a sum that is no number stays that)
     for (int d = lane; d < p.hd; d += 32) {
         float acc = 0.f;
         for (int s = 0; s < p.slices; ++s) {
@@ -219,7 +219,9 @@ namespace {
 constexpr int MAX_SLICES = 32;
 
 // One launch of a step: the requests with rows_above < rows <= rows_upto, in tiles of rows_per_tile.
+enum Kernel { CORES, DECODE };
 struct Part {
+    Kernel kernel = CORES;
     int rows_above = 0, rows_upto = 0, rows_per_tile = 0, tiles = 0, slices = 1, longest = 0;
 };
 struct Plan {
@@ -232,30 +234,38 @@ int slices_for(long long ctas, int slots, int keys, int least) {
     return (int)std::max<long long>(1, std::min<long long>(std::min<long long>(slots / ctas, keys / least), MAX_SLICES));
 }
 
-// counts of (token, head) rows follow from the host's copy of cu_seqlens; without it every request brings max_count tokens at most
-void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, int max_kv, int T, int nq, int nkv, int hd, int window, int dtype) {
+// Rows follow from the host's copy of cu_seqlens; without it every request brings max_count tokens at most.
+void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, int max_kv, int nq, int nkv, int hd, int window, int dtype) {
     const int G = nq / nkv;
-    (void)hd;
-    (void)dtype;
-    Part p;
-    p.rows_above = 0;
-    p.rows_upto = 0x7fffffff;
-    p.rows_per_tile = BM;
-    if (!cu) {
-        p.tiles = nseq * (int)(((long long)max_count * G + BM - 1) / BM);
-        p.longest = max_kv;
-    } else {
-        for (int i = 0; i < nseq; ++i) {
-            const long long rows = (long long)(cu[i + 1] - cu[i]) * G;
-            if (rows <= 0) continue;
-            p.tiles += (int)((rows + BM - 1) / BM);
-            p.longest = std::max(p.longest, kv[i]);
-        }
+    const bool cores = dtype != KESTREL_BF16 || (hd != 64 && hd != 128);
+    Part small, large;
+    small.kernel = cores ? CORES : DECODE;
+    small.rows_upto = cores ? 0x7fffffff : 16;
+    small.rows_per_tile = cores ? BM : 16;
+    large.kernel = CORES;
+    large.rows_above = small.rows_upto;
+    large.rows_upto = 0x7fffffff;
+    large.rows_per_tile = BM;
+    auto count = [&](long long rows, int keys, int times) {
+        if (rows <= 0) return;
+        Part &p = rows <= small.rows_upto ? small : large;
+        p.tiles += times * (int)((rows + p.rows_per_tile - 1) / p.rows_per_tile);
+        p.longest = std::max(p.longest, window > 0 ? std::min(keys, window + (int)((rows - 1) / G)) : keys);
+    };
+    if (cu) {
+        for (int i = 0; i < nseq; ++i) count((long long)(cu[i + 1] - cu[i]) * G, kv[i], 1);
+    } else if ((long long)max_count * G <= small.rows_upto) {
+        count((long long)max_count * G, max_kv, nseq);
+    } else {                            // any request may be of either kind: both launches are made for all of them
+        count(std::min<long long>(small.rows_upto, (long long)max_count * G), max_kv, nseq);
+        count((long long)max_count * G, max_kv, nseq);
     }
-    (void)T;
-    if (window > 0) p.longest = std::min(p.longest, window);
-    p.slices = slices_for((long long)p.tiles * nkv, kestrel_sms() * 2, p.longest, 256);
-    if (p.tiles) pl.part[pl.parts++] = p;
+    for (Part *p : {&small, &large}) {
+        if (!p->tiles) continue;
+        if (p->kernel == DECODE) p->slices = slices_for((long long)p->tiles * nkv, q8_decode_slots(hd), p->longest, 128);
+        else p->slices = slices_for((long long)p->tiles * nkv, kestrel_sms() * 2, p->longest, 256);
+        pl.part[pl.parts++] = *p;
+    }
 }
 
 }  // namespace
@@ -264,7 +274,7 @@ KESTREL_API long long kestrel_attention_q8_scratch(const int *cu_host, const int
                                                    int window, int dtype) {
     if (nseq <= 0 || T <= 0 || nq <= 0 || nkv <= 0 || nq % nkv) return 0;
     Plan pl;
-    make_plan(pl, cu_host, kv_host, nseq, max_count, max_kv, T, nq, nkv, hd, window, dtype);
+    make_plan(pl, cu_host, kv_host, nseq, max_count, max_kv, nq, nkv, hd, window, dtype);
     long long slices = 1;
     for (int i = 0; i < pl.parts; ++i) slices = std::max<long long>(slices, pl.part[i].slices);
     return slices > 1 ? (long long)T * nq * slices * (hd + 2) : 0;
@@ -285,7 +295,7 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
     KESTREL_REQUIRE(table_width > 0 && table_stride >= table_width, "attention_q8: block table of %d entries a row, %d apart", table_width, table_stride);
     KESTREL_REQUIRE(nkv <= 65535, "attention_q8: grid too large");
     Plan pl;
-    make_plan(pl, cu_host, kv_host, nseq, max_count, max_kv, T, nq, nkv, hd, window, dtype);
+    make_plan(pl, cu_host, kv_host, nseq, max_count, max_kv, nq, nkv, hd, window, dtype);
     int launches = 0;
     for (int i = 0; i < pl.parts; ++i) {
         const Part &part = pl.part[i];
@@ -301,7 +311,7 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
             p.part_o = scratch;
             p.part_ml = scratch + (long long)T * nq * part.slices * hd;
         }
-        int rc = q8_launch_plain(p, dtype, part.tiles, stream);
+        int rc = part.kernel == DECODE ? q8_launch_decode(p, part.tiles, stream) : q8_launch_plain(p, dtype, part.tiles, stream);
         if (rc) return rc;
         launches++;
         if (part.slices > 1) {
@@ -312,3 +322,5 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
     }
     return launches;
 }
+
+KESTREL_API int kestrel_attention_q8_error(void) { return q8_decode_error(); }

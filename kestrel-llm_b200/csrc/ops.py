@@ -976,6 +976,7 @@ def raise_on_kernel_error() -> None:
                                            ("attention_rows_tc", lib.kestrel_attention_rows_tc_error()),
                                            ("recurrence_blocks", lib.kestrel_recurrence_blocks_error()),
                                            ("attention_decode", lib.kestrel_attention_decode_error()),
+                                           ("attention_q8", lib.kestrel_attention_q8_error()),
                                            ("moe_tcgen05", lib.kestrel_moe_tc_error())) if code]
     if bad:
         raise KernelError("a bounded wait ran out in " + ", ".join(f"{n} (wait {c})" for n, c in bad) +

@@ -486,6 +486,9 @@ KESTREL_API int kestrel_attn_prepare_q8(const float *partial, int S, long long s
 KESTREL_API long long kestrel_attention_q8_scratch(const int *cu_host, const int *kv_host, int nseq, int max_count, int max_kv, int T, int nq, int nkv, int hd, int window, int dtype);
 KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, void *out, float *scratch, long long scratch_floats, const int *cu_host, const int *kv_host, const int *cu_seqlens, const int *kv_lens, const int *block_table, int nseq, int max_count, int max_kv, int table_width, int table_stride, int page_size, int cache_pages, int T, int nq, int nkv, int hd, int window, float scale, int dtype, kestrel_stream_t stream);
 
+/* error word of its kernels' bounded waits, 0 = none; synchronises the device and clears the word */
+KESTREL_API int kestrel_attention_q8_error(void);
+
 /* ---- log probabilities ---- */
 /* Of every row of logits float32 [R, ld], V of them: the log probability of ids[r] (ids may be NULL; an id outside [0, V) gives NaN), the entropy
  * in nats (entropy may be NULL), and the `top` likeliest tokens, most likely first, ties to the lowest id. */
