@@ -223,6 +223,9 @@ enum Kernel { CORES, DECODE };
 struct Part {
     Kernel kernel = CORES;
     int rows_above = 0, rows_upto = 0, rows_per_tile = 0, tiles = 0, slices = 1, longest = 0;
+    int ctas = 0;
+    long long scratch = 0;              // floats
+    long long key_tiles = 0;             // of 64, over all requests and kv heads
 };
 struct Plan {
     Part part[2];
@@ -235,7 +238,7 @@ int slices_for(long long ctas, int slots, int keys, int least) {
 }
 
 // Rows follow from the host's copy of cu_seqlens; without it every request brings max_count tokens at most.
-void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, int max_kv, int nq, int nkv, int hd, int window, int dtype) {
+void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, int max_kv, int T, int nq, int nkv, int hd, int window, int dtype) {
     const int G = nq / nkv;
     const bool cores = dtype != KESTREL_BF16 || (hd != 64 && hd != 128);
     Part small, large;
@@ -249,8 +252,10 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
     auto count = [&](long long rows, int keys, int times) {
         if (rows <= 0) return;
         Part &p = rows <= small.rows_upto ? small : large;
+        const int seen = window > 0 ? std::min(keys, window + (int)((rows - 1) / G)) : keys;
         p.tiles += times * (int)((rows + p.rows_per_tile - 1) / p.rows_per_tile);
-        p.longest = std::max(p.longest, window > 0 ? std::min(keys, window + (int)((rows - 1) / G)) : keys);
+        p.longest = std::max(p.longest, seen);
+        p.key_tiles += (long long)times * nkv * ((seen + 63) / 64);
     };
     if (cu) {
         for (int i = 0; i < nseq; ++i) count((long long)(cu[i + 1] - cu[i]) * G, kv[i], 1);
@@ -262,8 +267,13 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
     }
     for (Part *p : {&small, &large}) {
         if (!p->tiles) continue;
-        if (p->kernel == DECODE) p->slices = slices_for((long long)p->tiles * nkv, q8_decode_slots(hd), p->longest, 128);
-        else p->slices = slices_for((long long)p->tiles * nkv, kestrel_sms() * 2, p->longest, 256);
+        if (p->kernel == DECODE) {
+            p->ctas = q8_decode_ctas(p->key_tiles);
+            p->scratch = q8_decode_scratch(p->ctas, hd);
+        } else {
+            p->slices = slices_for((long long)p->tiles * nkv, kestrel_sms() * 2, p->longest, 256);
+            p->scratch = p->slices > 1 ? (long long)T * nq * p->slices * (hd + 2) : 0;
+        }
         pl.part[pl.parts++] = *p;
     }
 }
@@ -274,10 +284,10 @@ KESTREL_API long long kestrel_attention_q8_scratch(const int *cu_host, const int
                                                    int window, int dtype) {
     if (nseq <= 0 || T <= 0 || nq <= 0 || nkv <= 0 || nq % nkv) return 0;
     Plan pl;
-    make_plan(pl, cu_host, kv_host, nseq, max_count, max_kv, nq, nkv, hd, window, dtype);
-    long long slices = 1;
-    for (int i = 0; i < pl.parts; ++i) slices = std::max<long long>(slices, pl.part[i].slices);
-    return slices > 1 ? (long long)T * nq * slices * (hd + 2) : 0;
+    make_plan(pl, cu_host, kv_host, nseq, max_count, max_kv, T, nq, nkv, hd, window, dtype);
+    long long most = 0;
+    for (int i = 0; i < pl.parts; ++i) most = std::max(most, pl.part[i].scratch);
+    return most;
 }
 
 KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, void *out, float *scratch,
@@ -295,7 +305,7 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
     KESTREL_REQUIRE(table_width > 0 && table_stride >= table_width, "attention_q8: block table of %d entries a row, %d apart", table_width, table_stride);
     KESTREL_REQUIRE(nkv <= 65535, "attention_q8: grid too large");
     Plan pl;
-    make_plan(pl, cu_host, kv_host, nseq, max_count, max_kv, nq, nkv, hd, window, dtype);
+    make_plan(pl, cu_host, kv_host, nseq, max_count, max_kv, T, nq, nkv, hd, window, dtype);
     int launches = 0;
     for (int i = 0; i < pl.parts; ++i) {
         const Part &part = pl.part[i];
@@ -305,20 +315,20 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
         p.nseq = nseq; p.table_width = table_width; p.table_stride = table_stride; p.page_size = page_size; p.cache_pages = cache_pages;
         p.nq = nq; p.nkv = nkv; p.hd = hd; p.window = window; p.slices = part.slices; p.scale = scale;
         p.rows_above = part.rows_above; p.rows_upto = part.rows_upto; p.rows_per_tile = part.rows_per_tile;
-        if (part.slices > 1) {
-            const long long need = (long long)T * nq * part.slices * (hd + 2);
-            KESTREL_REQUIRE(scratch && need <= scratch_floats, "attention_q8: %d slices need scratch of %lld floats, %lld given", part.slices, need, scratch_floats);
-            p.part_o = scratch;
-            p.part_ml = scratch + (long long)T * nq * part.slices * hd;
+        KESTREL_REQUIRE(part.scratch == 0 || (scratch && part.scratch <= scratch_floats), "attention_q8: scratch of %lld floats is needed, %lld given", part.scratch, scratch_floats);
+        p.part_o = scratch;
+        int rc;
+        if (part.kernel == DECODE) {
+            p.part_ml = scratch + 2ll * part.ctas * 16 * hd;
+            rc = q8_launch_decode(p, part.ctas, stream);
+            launches += 2;
+        } else {
+            p.part_ml = scratch ? scratch + (long long)T * nq * part.slices * hd : nullptr;
+            rc = q8_launch_plain(p, dtype, part.tiles, stream);
+            if (rc == 0 && part.slices > 1) rc = q8_launch_merge(p, dtype, part.tiles, stream);
+            launches += part.slices > 1 ? 2 : 1;
         }
-        int rc = part.kernel == DECODE ? q8_launch_decode(p, part.tiles, stream) : q8_launch_plain(p, dtype, part.tiles, stream);
         if (rc) return rc;
-        launches++;
-        if (part.slices > 1) {
-            rc = q8_launch_merge(p, dtype, part.tiles, stream);
-            if (rc) return rc;
-            launches++;
-        }
     }
     return launches;
 }

@@ -98,8 +98,10 @@ __device__ __forceinline__ size_t q8_out_row(const Q8Params &p, const Q8Tile &t,
     return (size_t)(t.tok_begin + row / t.G) * p.nq + kvh * t.G + row % t.G;
 }
 
-int q8_launch_decode(const Q8Params &p, int tiles, cudaStream_t stream);     // tiles of up to 16 rows, head sizes 64 and 128, bfloat16
-int q8_decode_slots(int hd);                                                 // its CTAs that are resident at once
-int q8_decode_error();                                                       // its bounded waits' error word; synchronises
+// attention_q8_decode.cu: requests of up to 16 rows, head sizes 64 and 128, bfloat16; two kernels
+int q8_launch_decode(const Q8Params &p, int ctas, cudaStream_t stream);
+int q8_decode_ctas(long long tiles);                    // for so many (request, kv head, 64 keys)
+long long q8_decode_scratch(int ctas, int hd);          // floats: part_o, then part_ml
+int q8_decode_error();                                  // its bounded waits' error word; synchronises
 int q8_launch_plain(const Q8Params &p, int dtype, int tiles, cudaStream_t stream);
 int q8_launch_merge(const Q8Params &p, int dtype, int tiles, cudaStream_t stream);

@@ -1,18 +1,24 @@
 // Attention over pages of int8 codes with few rows: single tokens, and the ragged ends of short portions.  Head sizes 64 and 128, bfloat16
 // queries.  Formulas in attention_q8.cuh.
 //
-// A CTA takes up to 16 (token, query head) rows of one (request, kv head) and one slice of their keys.  A loader warp brings tiles of 64
-// keys by TMA into a ring of stages, codes of K and V side by side, and the scales of their four blocks beside them; four consumer warps
-// take one block of 16 keys each.  Codes go from shared memory straight into the fragments of mma.sync.m16n8k16 (float16, float32 sums):
-// a code c is the low byte of the float16 number 1024 + (c + 128), made by a byte permutation and freed of 1152 by one subtraction of
-// pairs.  The order of a product's inner index is free as long as both operands share it, which is used twice: a thread's 16 neighbouring
-// dimensions of a key are one 16-byte load and four k-steps of the scores, and the columns of the scores stand for keys in an order that
-// lets every load of a warp touch each bank once.  Bound by HBM: 2 hd bytes a key and kv head; about one instruction a code to widen it.
+// The work is cut evenly, whatever the requests' lengths: all key tiles of 64 of all (request, kv head) pairs stand in one line, and every
+// CTA takes as many of them as the next.  A CTA walks its stretch pair by pair, up to 16 (token, query head) rows at once.  A pair that lies
+// within one CTA's stretch is finished there; the others leave (maximum, sum, outputs) of their parts in scratch, two parts a CTA at most,
+// and the merge kernel below joins them in the order of the keys.
 //
-// Slices are merged through scratch by attention_q8_merge_kernel.
+// A loader warp brings tiles by TMA into a ring of stages, codes of K and V side by side, and the scales of their four blocks beside
+// them, running ahead over the pairs' borders; four consumer warps take one block of 16 keys each.  Codes go from shared memory straight
+// into the fragments of mma.sync.m16n8k16 (float16, float32 sums).  A code of V is the low byte of the float16 number 1024 + (c + 128), made
+// by a byte permutation and freed of 1152 by one subtraction of pairs.  A code of K is the float16 number (c + 128) 2^-24, a subnormal
+// one, which the permutation alone makes; the scores' sums begin with -128 2^-24 times the row's sum of queries instead of zero.  (The same
+// for V would leave 128 times the weights' sum in the outputs, of which they are a hundredth where many keys weigh alike.)
+// The order of a product's inner index is free as long as both operands share it, which is used twice: a thread's 16 neighbouring
+// dimensions of a key are one 16-byte load and four k-steps of the scores, and the columns of the scores stand for keys in an order that
+// lets every load of a warp touch each bank once.  Bound by HBM: 2 hd bytes a key and kv head; some 0.6 instructions a code to widen it.
 #include "attention_q8.cuh"
 #include "tcgen05.cuh"
 
+#include <cuda_fp16.h>
 #include <math.h>
 
 __device__ int g_q8d_error = 0;
@@ -23,10 +29,10 @@ constexpr int THREADS = 160, BN = 64;       // four consumer warps and the loade
 constexpr uint32_t MAGIC = 0x64646464u;     // high byte of the float16 numbers 1024 .. 1279
 
 template <int HD> struct Ring {
-    static constexpr int STAGES = HD == 128 ? 6 : 8;
-    static constexpr uint32_t PLANE = BN * HD, STAGE = 2 * PLANE;
-    static constexpr uint32_t SCALES = STAGES * STAGE, BARS = SCALES + STAGES * 32, BYTES = BARS + 16 * STAGES;
+    static constexpr int STAGES = HD == 128 ? 4 : 8;
     static constexpr int LDO = HD + 4;      // row of a warp's outputs, in floats, when the four warps meet
+    static constexpr uint32_t PLANE = BN * HD, STAGE = 2 * PLANE;
+    static constexpr uint32_t SCALES = STAGES * STAGE, BARS = SCALES + STAGES * 32, MEET = BARS + 16 * STAGES, BYTES = MEET + 4 * 16 * (LDO + 2) * 4;
 };
 
 __device__ __forceinline__ uint32_t hsub2(uint32_t a) {             // - 1152 from both halves
@@ -42,6 +48,16 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float log2_fast(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ void mma_f16(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
@@ -67,13 +83,118 @@ __device__ __forceinline__ uint2 lds64(uint32_t at) {
 template <int HD> __device__ __forceinline__ int key_of_column(int n) { return HD == 128 ? (n >> 1) + 4 * (n & 1) : n ^ ((n >> 1) & 1); }
 
 // address of 16-byte chunk c (of HD / 16) of key k in a tile
-template <int HD> __device__ __forceinline__ uint32_t chunk_at(uint32_t tile, int k, int c) {
+template <int HD> __device__ __forceinline__ uint32_t chunk_at(int k, int c) {
     const int line = HD == 128 ? k : k >> 1, at = HD == 128 ? c : 4 * (k & 1) + c;
-    return tile + line * 128 + ((at ^ (line & 7)) << 4);
+    return line * 128 + ((at ^ (line & 7)) << 4);
 }
 
+// The line of key tiles: request i's pairs lie behind those of the requests before it, kv head by kv head.
+struct Line {
+    const Q8Params &p;
+
+    __device__ __forceinline__ int tiles_of(int i) const {
+        if (i >= p.nseq) return 0;
+        const int n = p.cu_seqlens[i + 1] - p.cu_seqlens[i], kv = p.kv_lens[i];
+        const long long rows = (long long)n * (p.nq / p.nkv);
+        if (rows <= p.rows_above || rows > p.rows_upto) return 0;
+        const int first = p.window > 0 ? max(0, kv - n - p.window + 1) : 0;
+        return (kv + BN - 1) / BN - first / BN;
+    }
+    // all of it
+    __device__ __forceinline__ long long length() const {
+        int sum = 0;                                // of one kv head: below 2^31 tokens / 64
+        for (int i = threadIdx.x & 31; i < p.nseq; i += 32) sum += tiles_of(i);
+        return (long long)__reduce_add_sync(0xffffffffu, sum) * p.nkv;
+    }
+    // the request in which tile `at` lies, and its first tile's place
+    __device__ __forceinline__ int request_at(long long at, long long &begin) const {
+        const int lane = threadIdx.x & 31;
+        const int want = (int)(at / p.nkv);         // on one kv head's line a request holds its place
+        int before = 0;
+        for (int base = 0; base < p.nseq; base += 32) {
+            const int n = tiles_of(base + lane);
+            int end = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, end, o);
+                if (lane >= o) end += x;
+            }
+            const uint32_t behind = __ballot_sync(0xffffffffu, want < before + end);
+            if (behind) {
+                const int l = __ffs(behind) - 1;
+                begin = (long long)(before + __shfl_sync(0xffffffffu, end - n, l)) * p.nkv;
+                return base + l;
+            }
+            before += __shfl_sync(0xffffffffu, end, 31);
+        }
+        begin = 0;
+        return -1;
+    }
+};
+
+// CTA u's stretch begins here; the CTA whose stretch holds tile `at`
+__device__ __forceinline__ long long stretch(long long u, long long length, int ctas) { return u * length / ctas; }
+__device__ __forceinline__ int holder(long long at, long long length, int ctas) { return (int)(((at + 1) * ctas - 1) / length); }
+
+// One CTA's parts of pairs, one after the other
+struct Walk {
+    const Q8Params &p;
+    long long at, end, begin;           // next tile, end of the stretch, place of the pair's first tile
+    int seq, n, kvh;                    // the pair; n: its tiles
+    // the part
+    int G, rows, tok_begin, pos_begin, k_first, k_end, from, to;
+    const int *table;
+    bool whole;
+
+    __device__ __forceinline__ Walk(const Q8Params &p_, long long length) : p(p_), n(0) {
+        at = stretch(blockIdx.x, length, gridDim.x);
+        end = stretch(blockIdx.x + 1, length, gridDim.x);
+        G = p.nq / p.nkv;
+        if (at >= end) return;
+        const Line line{p};
+        seq = line.request_at(at, begin);
+        n = line.tiles_of(seq);
+        kvh = (int)((at - begin) / n);
+        begin += (long long)kvh * n;
+        describe();
+    }
+    __device__ __forceinline__ void describe() {
+        tok_begin = p.cu_seqlens[seq];
+        const int n_tok = p.cu_seqlens[seq + 1] - tok_begin;
+        k_end = p.kv_lens[seq];
+        pos_begin = k_end - n_tok;
+        rows = n_tok * G;
+        k_first = p.window > 0 ? max(0, pos_begin - p.window + 1) : 0;
+        table = p.block_table + (size_t)seq * p.table_stride;
+    }
+    // the next part: tiles [from, to) of the pair; false at the end of the stretch
+    __device__ __forceinline__ bool next() {
+        if (at >= end) return false;
+        if (at >= begin + n) {
+            begin += n;
+            if (++kvh == p.nkv) {
+                kvh = 0;
+                const Line line{p};
+                do n = line.tiles_of(++seq);
+                while (n == 0 && seq < p.nseq);
+                describe();
+            }
+        }
+        from = (int)(at - begin);
+        to = (int)min((long long)n, end - begin);
+        whole = from == 0 && to == n;
+        at = begin + to;
+        return true;
+    }
+    __device__ __forceinline__ size_t out_row(int r) const { return (size_t)(tok_begin + r / G) * p.nq + kvh * G + r % G; }
+};
+
+// Parts in scratch: 16 rows of HD outputs each, then 16 (maximum, sum) pairs each; a CTA's first part is its even one
+template <int HD> __device__ __forceinline__ float *part_out(const Q8Params &p, long long part, int row) { return p.part_o + (part * 16 + row) * HD; }
+__device__ __forceinline__ float2 *part_ml(const Q8Params &p, long long part, int row) { return reinterpret_cast<float2 *>(p.part_ml) + part * 16 + row; }
+
 template <int HD>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 2)
 attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Q8Params p) {
     pdl_launch_dependents();
     using R = Ring<HD>;
@@ -83,41 +204,44 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     uint8_t *ring = q8d_smem + (base - smem_u32(q8d_smem));
     auto full_bar = [&](int s) { return base + R::BARS + 8u * s; };
     auto empty_bar = [&](int s) { return base + R::BARS + 8u * (R::STAGES + s); };
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y, slice = blockIdx.z;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         // a stage is full when its codes are there (the loader's bytes) and eight lanes' scales
         for (int s = 0; s < R::STAGES; ++s) { mbar_init(full_bar(s), 1 + 8); mbar_init(empty_bar(s), 4); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    Q8Tile t;
     // the step's description was on the device before the kernel in front of this one began
-    if (!q8_find_tile(p, blockIdx.x, t)) { pdl_wait(); return; }
-    int lo, hi;
-    q8_slice(t, p.slices, slice, BN, lo, hi);
-    const int kb0 = lo / BN * BN, n_tiles = hi > lo ? (hi - kb0 + BN - 1) / BN : 0;
+    Walk w(p, Line{p}.length());
+    int stage = 0;
+    uint32_t phase = 0;
+    pdl_wait();
 
     if (warp == 4) {
         // ---- loader: lane l brings the l-th box of a tile, K and V; lanes 0-3 (4-7) bring its blocks' scales of K (V)
         const int box = p.page_size % 64 == 0 ? 64 : p.page_size % 32 == 0 ? 32 : 16, boxes = BN / box;
         const float *scales = lane < 4 ? p.ks : p.vs;
-        pdl_wait();
-        for (int i = 0; i < n_tiles; ++i) {
-            const int stage = i % R::STAGES, kb = kb0 + i * BN;
-            const long long box_row = lane < boxes ? q8_row_of(p, t.table, kvh, kb + lane * box) : 0;
-            const long long block_row = lane < 8 ? q8_row_of(p, t.table, kvh, kb + (lane & 3) * Q8_BLOCK) : 0;
-            if (!mbar_wait(empty_bar(stage), (uint32_t)(i / R::STAGES + 1) & 1u)) { atomicExch(&g_q8d_error, 1); break; }
-            if (lane == 0) mbar_expect_tx(full_bar(stage), R::STAGE);
-            __syncwarp();
-            if (lane < boxes) {
-                const uint32_t dst = base + stage * R::STAGE + lane * box * HD;
-                const int line = (int)(HD == 128 ? box_row : box_row >> 1);
-                tma_load_2d(dst, &map_k, full_bar(stage), 0, line);
-                tma_load_2d(dst + R::PLANE, &map_v, full_bar(stage), 0, line);
-            }
-            if (lane < 8) {
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(base + R::SCALES + stage * 32 + lane * 4), "l"(scales + block_row / Q8_BLOCK) : "memory");
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full_bar(stage)) : "memory");
+        bool ok = true;
+        while (ok && w.next()) {
+            const int kb0 = w.k_first / BN * BN;
+            for (int i = w.from; i < w.to; ++i) {
+                const int kb = kb0 + i * BN;
+                const long long box_row = lane < boxes ? q8_row_of(p, w.table, w.kvh, kb + lane * box) : 0;
+                const long long block_row = lane < 8 ? q8_row_of(p, w.table, w.kvh, kb + (lane & 3) * Q8_BLOCK) : 0;
+                if (!mbar_wait(empty_bar(stage), phase ^ 1u)) { atomicExch(&g_q8d_error, 1); ok = false; break; }
+                if (lane == 0) mbar_expect_tx(full_bar(stage), R::STAGE);
+                __syncwarp();
+                if (lane < boxes) {
+                    const uint32_t dst = base + stage * R::STAGE + lane * box * HD;
+                    const int line = (int)(HD == 128 ? box_row : box_row >> 1);
+                    tma_load_2d(dst, &map_k, full_bar(stage), 0, line);
+                    tma_load_2d(dst + R::PLANE, &map_v, full_bar(stage), 0, line);
+                }
+                if (lane < 8) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(base + R::SCALES + stage * 32 + lane * 4), "l"(scales + block_row / Q8_BLOCK) : "memory");
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full_bar(stage)) : "memory");
+                }
+                if (++stage == R::STAGES) stage = 0, phase ^= 1u;
             }
         }
         return;
@@ -125,229 +249,317 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 
     // ---- consumers
     const int g = lane >> 2, c = lane & 3;              // rows g and g + 8; a quarter of the inner index
-    pdl_wait();
-    // Queries as fragments, in float16: a row is multiplied by the power of two that brings its largest number to [64, 128), so that a
-    // bfloat16 number keeps its bits down to 2^-21 of that, and the rest is off by 2^-31 of it.
-    uint32_t qa[KS][4];
-    float row_scale[2];
-    int pos[2], low[2], min_pos = 0x7fffffff;           // (of the rows that are there)
+    // where this thread's codes lie in a stage: of the scores' first column tile (the second is 8 keys further), and of V
+    uint32_t k_off[HALVES], v_off[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = g + 8 * i;
-        const bool live = r < t.rows;
-        uint4 w[HALVES][2];
-        uint32_t big = 0;
+    for (int j = 0; j < HALVES; ++j) k_off[j] = warp * 16 * HD + chunk_at<HD>(key_of_column<HD>(g), 4 * j + c);
 #pragma unroll
-        for (int j = 0; j < HALVES; ++j) {
-            w[j][0] = w[j][1] = make_uint4(0, 0, 0, 0);
-            if (live) {
-                const uint4 *src = reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)p.q + q8_out_row(p, t, kvh, r) * HD + 64 * j + 16 * c);
-                w[j][0] = src[0];
-                w[j][1] = src[1];
-            }
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint32_t *u = reinterpret_cast<const uint32_t *>(&w[j][k]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) big = max(big, max(u[e] & 0x7fffu, (u[e] >> 16) & 0x7fffu));
-            }
-        }
-        big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        const int e = (int)(big >> 7);                  // biased exponent of the largest; 255: not finite, as it is
-        const int up = big == 0 || e == 255 ? 0 : 127 + 6 - max(e, 27);
-        const float f = __uint_as_float((uint32_t)(127 + up) << 23);
-        row_scale[i] = __uint_as_float((uint32_t)(127 - up) << 23) * p.scale * 1.4426950408889634f;
-#pragma unroll
-        for (int j = 0; j < HALVES; ++j)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {               // k-step 4 j + k: dimensions 64 j + 16 c + 4 k ..
-                const uint32_t a = reinterpret_cast<const uint32_t *>(&w[j][k >> 1])[2 * (k & 1)], b = reinterpret_cast<const uint32_t *>(&w[j][k >> 1])[2 * (k & 1) + 1];
-                qa[4 * j + k][i] = pack_f16(__uint_as_float(a << 16) * f, __uint_as_float(a & 0xffff0000u) * f);
-                qa[4 * j + k][2 + i] = pack_f16(__uint_as_float(b << 16) * f, __uint_as_float(b & 0xffff0000u) * f);
-            }
-        pos[i] = live ? t.pos_begin + (t.row0 + r) / t.G : -1;
-        low[i] = p.window > 0 ? max(0, pos[i] - p.window + 1) : 0;
-        if (live) min_pos = min(min_pos, pos[i]);
-    }
-    int max_low = max(low[0], low[1]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        min_pos = min(min_pos, __shfl_xor_sync(0xffffffffu, min_pos, o));
-        max_low = max(max_low, __shfl_xor_sync(0xffffffffu, max_low, o));
-    }
-    float o[NT_O][4];
-#pragma unroll
-    for (int i = 0; i < NT_O; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int j = 0; j < 2; ++j)
+        v_off[j] = R::PLANE + warp * 16 * HD + chunk_at<HD>(key_of_column<HD>(2 * c + j), HD == 128 ? (g >> 1) + 4 * (g & 1) : g >> 1) + (HD == 64 ? 8 * (g & 1) : 0);
+    // (8 keys are 8 lines at head size 128, which the swizzle repeats after, and 4 at 64, which turn its third bit)
+    auto second = [](uint32_t at) { return HD == 128 ? at + 1024 : (at + 512) ^ 64u; };
+    const int col0 = key_of_column<HD>(2 * c), col1 = key_of_column<HD>(2 * c + 1);     // keys of this thread's score columns
+    float *meet = reinterpret_cast<float *>(ring + R::MEET), *meet_ml = meet + 4 * 16 * R::LDO;
     bool ok = true;             // after a wait gave up the loop runs on without waiting, so that the warps still meet below
+    bool first_part = true;
 
-    for (int i = 0; i < n_tiles; ++i) {
-        const int stage = i % R::STAGES;
-        if (ok && !mbar_wait(full_bar(stage), (uint32_t)(i / R::STAGES) & 1u)) { atomicExch(&g_q8d_error, 2); ok = false; }
-        const int kbase = kb0 + i * BN + 16 * warp;     // this warp's block
-        if (ok && kbase < hi && kbase + 16 > lo) {
-            const uint32_t Kt = base + stage * R::STAGE, Vt = Kt + R::PLANE;
-            float s[2][4];
+    while (w.next()) {
+        // Queries as fragments, in float16: a row is multiplied by the power of two that brings its largest number to [64, 128), so that
+        // a bfloat16 number keeps its bits down to 2^-21 of that, and the rest is off by 2^-31 of it.
+        uint32_t qa[KS][4];
+        float row_scale[2], bias[2];
+        int pos[2], low[2], min_pos = 0x7fffffff;       // (of the rows that are there)
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-                s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-                const int key = 16 * warp + 8 * nt + key_of_column<HD>(g);
+        for (int i = 0; i < 2; ++i) {
+            const int r = g + 8 * i;
+            const bool live = r < w.rows;
+            uint4 q[HALVES][2];
+            uint32_t big = 0;
+#pragma unroll
+            for (int j = 0; j < HALVES; ++j) {
+                q[j][0] = q[j][1] = make_uint4(0, 0, 0, 0);
+                if (live) {
+                    const uint4 *src = reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)p.q + w.out_row(r) * HD + 64 * j + 16 * c);
+                    q[j][0] = src[0];
+                    q[j][1] = src[1];
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t *u = reinterpret_cast<const uint32_t *>(&q[j][k]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) big = max(big, max(u[e] & 0x7fffu, (u[e] >> 16) & 0x7fffu));
+                }
+            }
+            big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            const int e = (int)(big >> 7);              // biased exponent of the largest; 255: not finite, as it is
+            const int up = big == 0 || e == 255 ? 0 : 127 + 6 - max(e, 63);      // (below 2^-64 nothing weighs)
+            const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+            row_scale[i] = __uint_as_float((uint32_t)(127 - up) << 23) * p.scale * (1.4426950408889634f * 16777216.0f);
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < HALVES; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {           // k-step 4 j + k: dimensions 64 j + 16 c + 4 k ..
+                    const uint32_t a = reinterpret_cast<const uint32_t *>(&q[j][k >> 1])[2 * (k & 1)], b = reinterpret_cast<const uint32_t *>(&q[j][k >> 1])[2 * (k & 1) + 1];
+                    const uint32_t x = pack_f16(__uint_as_float(a << 16) * f, __uint_as_float(a & 0xffff0000u) * f);
+                    const uint32_t y = pack_f16(__uint_as_float(b << 16) * f, __uint_as_float(b & 0xffff0000u) * f);
+                    qa[4 * j + k][i] = x;
+                    qa[4 * j + k][2 + i] = y;
+                    const float2 fx = __half22float2(*reinterpret_cast<const __half2 *>(&x)), fy = __half22float2(*reinterpret_cast<const __half2 *>(&y));
+                    sum += (fx.x + fx.y) + (fy.x + fy.y);
+                }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            bias[i] = sum * (-128.0f / 16777216.0f);
+            pos[i] = live ? w.pos_begin + r / w.G : -1;
+            low[i] = p.window > 0 ? max(0, pos[i] - p.window + 1) : 0;
+            if (live) min_pos = min(min_pos, pos[i]);
+        }
+        int max_low = max(low[0], low[1]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            min_pos = min(min_pos, __shfl_xor_sync(0xffffffffu, min_pos, o));
+            max_low = max(max_low, __shfl_xor_sync(0xffffffffu, max_low, o));
+        }
+        float o[NT_O][4];
+#pragma unroll
+        for (int i = 0; i < NT_O; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        const int k_begin = w.k_first / BN * BN;
+
+        for (int i = w.from; i < w.to; ++i) {
+            if (ok && !mbar_wait(full_bar(stage), phase)) { atomicExch(&g_q8d_error, 2); ok = false; }
+            const int kbase = k_begin + i * BN + 16 * warp;     // this warp's block
+            if (ok && kbase < w.k_end && kbase + 16 > w.k_first) {
+                const uint32_t at = base + stage * R::STAGE;
+                float s[2][4];
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt) {
+                    s[nt][0] = s[nt][1] = bias[0];
+                    s[nt][2] = s[nt][3] = bias[1];
+                }
 #pragma unroll
                 for (int j = 0; j < HALVES; ++j) {
-                    const uint4 w = lds128(chunk_at<HD>(Kt, key, 4 * j + c));
-                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+                    const uint4 w0 = lds128(at + k_off[j]), w1 = lds128(at + second(k_off[j]));
+                    const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const uint32_t x = u[k] ^ 0x80808080u;
-                        mma_f16(s[nt], qa[4 * j + k], hsub2(__byte_perm(x, MAGIC, 0x4140)), hsub2(__byte_perm(x, MAGIC, 0x4342)));
+                        const uint32_t x0 = u0[k] ^ 0x80808080u, x1 = u1[k] ^ 0x80808080u;
+                        mma_f16(s[0], qa[4 * j + k], __byte_perm(x0, 0, 0x4140), __byte_perm(x0, 0, 0x4342));
+                        mma_f16(s[1], qa[4 * j + k], __byte_perm(x1, 0, 0x4140), __byte_perm(x1, 0, 0x4342));
                     }
                 }
-            }
-            const float *sc = reinterpret_cast<const float *>(ring + R::SCALES + stage * 32);
-            const float sk = sc[warp], sv = sc[4 + warp];
-            const float lv = __log2f(sv), rv = 1.0f / sv;
-            // scores with the value's scale in base-2 units, the mask where some row does not see the block whole, running reference
-            const bool whole = kbase >= lo && kbase + 16 <= hi && kbase + 15 <= min_pos && kbase >= max_low;
-            float mx[2] = {-INFINITY, -INFINITY};
+                const float *sc = reinterpret_cast<const float *>(ring + R::SCALES + stage * 32);
+                const float sk = sc[warp], sv = sc[4 + warp];
+                const float lv = log2_fast(sv), rv = rcp_fast(sv);
+                // scores with the value's scale, in base-2 units: x = s * ck + lv
+                const float ck[2] = {sk * row_scale[0], sk * row_scale[1]};
+                const bool whole = kbase >= w.k_first && kbase + 16 <= w.k_end && kbase + 15 <= min_pos && kbase >= max_low;
+                bool none[2] = {false, false};              // rows that see nothing of the block
+                if (!whole) {
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
+                    for (int r = 0; r < 2; ++r) {
+                        none[r] = kbase > pos[r] || kbase + 15 < low[r];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x = fmaf(s[nt][e], sk * row_scale[e >> 1], lv);
-                    if (!whole) {
-                        const int key = kbase + 8 * nt + key_of_column<HD>(2 * c + (e & 1));
-                        if (!(key <= pos[e >> 1] && key >= low[e >> 1] && key < hi && key >= lo)) x = -INFINITY;
+                        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int key = kbase + 8 * nt + (e ? col1 : col0);
+                                if (!(key <= pos[r] && key >= low[r])) s[nt][2 * r + e] = -INFINITY;
+                            }
                     }
-                    s[nt][e] = x;
-                    mx[e >> 1] = fmaxf(mx[e >> 1], x);
                 }
-            float use[2], alpha[2];
+                float mx[2];
+                bool grow = false;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                alpha[r] = 1.f;
+                for (int r = 0; r < 2; ++r) {
+                    mx[r] = fmaf(fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])), ck[r], lv);
+                    if (none[r]) mx[r] = -INFINITY;         // whatever the scales are
+                    grow |= mx[r] > m[r] + 8.f || (m[r] == -INFINITY && mx[r] > -INFINITY);
+                }
                 // the reference moves once the maximum has outgrown it by 8: weights stay below 2^8
-                if (mx[r] > m[r] + 8.f || (m[r] == -INFINITY && mx[r] > -INFINITY)) {
-                    alpha[r] = m[r] == -INFINITY ? 0.f : exp2_fast(m[r] - mx[r]);
-                    m[r] = mx[r];
+                if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+                        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+                        if (mx[r] > m[r]) {
+                            const float alpha = m[r] == -INFINITY ? 0.f : exp2_fast(m[r] - mx[r]);
+                            m[r] = mx[r];
+                            l[r] *= alpha;
+#pragma unroll
+                            for (int nt = 0; nt < NT_O; ++nt) o[nt][2 * r] *= alpha, o[nt][2 * r + 1] *= alpha;
+                        }
+                    }
                 }
-                use[r] = m[r] == -INFINITY ? 0.f : m[r];
-            }
-            if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-                l[0] *= alpha[0];
-                l[1] *= alpha[1];
 #pragma unroll
-                for (int nt = 0; nt < NT_O; ++nt) {
-                    o[nt][0] *= alpha[0]; o[nt][1] *= alpha[0];
-                    o[nt][2] *= alpha[1]; o[nt][3] *= alpha[1];
+                for (int r = 0; r < 2; ++r) {
+                    const float shift = lv - (m[r] == -INFINITY ? 0.f : m[r]);
+                    float sum = 0.f;
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float &x = s[nt][2 * r + e];
+                            x = exp2_fast(fmaf(x, ck[r], shift));
+                            if (!whole && none[r]) x = 0.f;
+                            sum += x;
+                        }
+                    if (!none[r]) l[r] = fmaf(sum, rv, l[r]);
+                }
+                // out += w V: columns 2 c, 2 c + 1 of both score tiles are the four keys of this thread's fragments
+                const uint32_t a[4] = {pack_f16(s[0][0], s[0][1]), pack_f16(s[0][2], s[0][3]), pack_f16(s[1][0], s[1][1]), pack_f16(s[1][2], s[1][3])};
+                uint32_t v[4][HD / 32];
+                if (HD == 128) {                            // this thread's 16 dimensions
+                    *reinterpret_cast<uint4 *>(v[0]) = lds128(at + v_off[0]);
+                    *reinterpret_cast<uint4 *>(v[1]) = lds128(at + v_off[1]);
+                    *reinterpret_cast<uint4 *>(v[2]) = lds128(at + second(v_off[0]));
+                    *reinterpret_cast<uint4 *>(v[3]) = lds128(at + second(v_off[1]));
+                } else {                                    // its 8
+                    *reinterpret_cast<uint2 *>(v[0]) = lds64(at + v_off[0]);
+                    *reinterpret_cast<uint2 *>(v[1]) = lds64(at + v_off[1]);
+                    *reinterpret_cast<uint2 *>(v[2]) = lds64(at + second(v_off[0]));
+                    *reinterpret_cast<uint2 *>(v[3]) = lds64(at + second(v_off[1]));
+                }
+#pragma unroll
+                for (int k = 0; k < HD / 32; ++k) {         // output column tiles 4 k .. 4 k + 3: dimensions 4 k .. 4 k + 3 of the thread's
+                    const uint32_t p0 = __byte_perm(v[0][k], v[1][k], 0x5140) ^ 0x80808080u, p1 = __byte_perm(v[0][k], v[1][k], 0x7362) ^ 0x80808080u;
+                    const uint32_t p2 = __byte_perm(v[2][k], v[3][k], 0x5140) ^ 0x80808080u, p3 = __byte_perm(v[2][k], v[3][k], 0x7362) ^ 0x80808080u;
+                    mma_f16(o[4 * k], a, hsub2(__byte_perm(p0, MAGIC, 0x4140)), hsub2(__byte_perm(p2, MAGIC, 0x4140)));
+                    mma_f16(o[4 * k + 1], a, hsub2(__byte_perm(p0, MAGIC, 0x4342)), hsub2(__byte_perm(p2, MAGIC, 0x4342)));
+                    mma_f16(o[4 * k + 2], a, hsub2(__byte_perm(p1, MAGIC, 0x4140)), hsub2(__byte_perm(p3, MAGIC, 0x4140)));
+                    mma_f16(o[4 * k + 3], a, hsub2(__byte_perm(p1, MAGIC, 0x4342)), hsub2(__byte_perm(p3, MAGIC, 0x4342)));
                 }
             }
-            float sum[2] = {0.f, 0.f};
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[nt][e] = exp2_fast(s[nt][e] - use[e >> 1]);
-                    sum[e >> 1] += s[nt][e];
-                }
-            // a block of which a row sees nothing adds nothing to its sum, whatever its scale is; a maximum passes over what is no number
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-                if (mx[r] > -INFINITY || sum[r] != sum[r]) l[r] = fmaf(sum[r], rv, l[r]);
-            // out += w V: columns 2 c, 2 c + 1 of both score tiles are the four keys of this thread's fragments
-            const uint32_t a[4] = {pack_f16(s[0][0], s[0][1]), pack_f16(s[0][2], s[0][3]), pack_f16(s[1][0], s[1][1]), pack_f16(s[1][2], s[1][3])};
-            const int ka = 16 * warp + key_of_column<HD>(2 * c), kb = 16 * warp + key_of_column<HD>(2 * c + 1);
-            uint32_t v[4][HD / 32];
-            if (HD == 128) {
-                const int ch = (g >> 1) + 4 * (g & 1);  // this thread's 16 dimensions: 16 ch ..
-                *reinterpret_cast<uint4 *>(v[0]) = lds128(chunk_at<HD>(Vt, ka, ch));
-                *reinterpret_cast<uint4 *>(v[1]) = lds128(chunk_at<HD>(Vt, kb, ch));
-                *reinterpret_cast<uint4 *>(v[2]) = lds128(chunk_at<HD>(Vt, ka + 8, ch));
-                *reinterpret_cast<uint4 *>(v[3]) = lds128(chunk_at<HD>(Vt, kb + 8, ch));
-            } else {                                    // its 8 dimensions: 8 g ..
-                *reinterpret_cast<uint2 *>(v[0]) = lds64(chunk_at<HD>(Vt, ka, g >> 1) + 8 * (g & 1));
-                *reinterpret_cast<uint2 *>(v[1]) = lds64(chunk_at<HD>(Vt, kb, g >> 1) + 8 * (g & 1));
-                *reinterpret_cast<uint2 *>(v[2]) = lds64(chunk_at<HD>(Vt, ka + 8, g >> 1) + 8 * (g & 1));
-                *reinterpret_cast<uint2 *>(v[3]) = lds64(chunk_at<HD>(Vt, kb + 8, g >> 1) + 8 * (g & 1));
-            }
-#pragma unroll
-            for (int k = 0; k < HD / 32; ++k) {         // output column tiles 4 k .. 4 k + 3: dimensions 4 k .. 4 k + 3 of the thread's
-                const uint32_t p0 = __byte_perm(v[0][k], v[1][k], 0x5140) ^ 0x80808080u, p1 = __byte_perm(v[0][k], v[1][k], 0x7362) ^ 0x80808080u;
-                const uint32_t p2 = __byte_perm(v[2][k], v[3][k], 0x5140) ^ 0x80808080u, p3 = __byte_perm(v[2][k], v[3][k], 0x7362) ^ 0x80808080u;
-                mma_f16(o[4 * k], a, hsub2(__byte_perm(p0, MAGIC, 0x4140)), hsub2(__byte_perm(p2, MAGIC, 0x4140)));
-                mma_f16(o[4 * k + 1], a, hsub2(__byte_perm(p0, MAGIC, 0x4342)), hsub2(__byte_perm(p2, MAGIC, 0x4342)));
-                mma_f16(o[4 * k + 2], a, hsub2(__byte_perm(p1, MAGIC, 0x4140)), hsub2(__byte_perm(p3, MAGIC, 0x4140)));
-                mma_f16(o[4 * k + 3], a, hsub2(__byte_perm(p1, MAGIC, 0x4342)), hsub2(__byte_perm(p3, MAGIC, 0x4342)));
-            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty_bar(stage));
+            if (++stage == R::STAGES) stage = 0, phase ^= 1u;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(empty_bar(stage));
-    }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    }
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        }
 
-    // the four warps' states, in warp order, in the ring's memory: every tile that was fetched has been consumed
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    float *mo = reinterpret_cast<float *>(ring);                // [4][16][LDO]
-    float *mml = mo + 4 * 16 * R::LDO;                          // [4][16][2]
-    // column n of output tile j is dimension j of thread n's: 2 c -> chunk c, 2 c + 1 -> chunk c + 4 (head size 64: 8 dimensions each)
-    const int d0 = HD == 128 ? 16 * c : 16 * c, d1 = HD == 128 ? 64 + 16 * c : 16 * c + 8;
+        // the four warps' states, in warp order
+        asm volatile("bar.sync 1, 128;" ::: "memory");      // the part before has been read
+        // column n of output tile j is dimension j of thread n's: 2 c and 2 c + 1
+        const int d0 = 16 * c, d1 = HD == 128 ? 64 + 16 * c : 16 * c + 8;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        float *row = mo + (warp * 16 + g + 8 * r) * R::LDO;
+        for (int r = 0; r < 2; ++r) {
+            if (8 * r >= w.rows) break;                     // no second half of rows
+            float *row = meet + (warp * 16 + g + 8 * r) * R::LDO;
 #pragma unroll
-        for (int j = 0; j < NT_O; j += 4) {
-            *reinterpret_cast<float4 *>(row + d0 + j) = make_float4(o[j][2 * r], o[j + 1][2 * r], o[j + 2][2 * r], o[j + 3][2 * r]);
-            *reinterpret_cast<float4 *>(row + d1 + j) = make_float4(o[j][2 * r + 1], o[j + 1][2 * r + 1], o[j + 2][2 * r + 1], o[j + 3][2 * r + 1]);
+            for (int j = 0; j < NT_O; j += 4) {
+                *reinterpret_cast<float4 *>(row + d0 + j) = make_float4(o[j][2 * r], o[j + 1][2 * r], o[j + 2][2 * r], o[j + 3][2 * r]);
+                *reinterpret_cast<float4 *>(row + d1 + j) = make_float4(o[j][2 * r + 1], o[j + 1][2 * r + 1], o[j + 2][2 * r + 1], o[j + 3][2 * r + 1]);
+            }
+            if (c == 0) {
+                meet_ml[(warp * 16 + g + 8 * r) * 2] = m[r];
+                meet_ml[(warp * 16 + g + 8 * r) * 2 + 1] = l[r];
+            }
         }
-        if (c == 0) {
-            mml[(warp * 16 + g + 8 * r) * 2] = m[r];
-            mml[(warp * 16 + g + 8 * r) * 2 + 1] = l[r];
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const long long part = 2ll * blockIdx.x + (first_part ? 0 : 1);
+        for (int idx = tid; idx < 16 * (HD / 8); idx += 128) {
+            const int r = idx / (HD / 8), d = (idx % (HD / 8)) * 8;
+            if (r >= w.rows) break;
+            float M = -INFINITY, L = 0.f, acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) M = fmaxf(M, meet_ml[(x * 16 + r) * 2]);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const float mw = meet_ml[(x * 16 + r) * 2], lw = meet_ml[(x * 16 + r) * 2 + 1];
+                const float f = mw == -INFINITY ? 0.f : exp2f(mw - M);
+                if (f == 0.f && lw == lw) continue;         // (a sum that is no number stays that)
+                L = fmaf(lw, f, L);
+                const float4 a = *reinterpret_cast<const float4 *>(meet + (x * 16 + r) * R::LDO + d), b = *reinterpret_cast<const float4 *>(meet + (x * 16 + r) * R::LDO + d + 4);
+                acc[0] = fmaf(a.x, f, acc[0]); acc[1] = fmaf(a.y, f, acc[1]); acc[2] = fmaf(a.z, f, acc[2]); acc[3] = fmaf(a.w, f, acc[3]);
+                acc[4] = fmaf(b.x, f, acc[4]); acc[5] = fmaf(b.y, f, acc[5]); acc[6] = fmaf(b.z, f, acc[6]); acc[7] = fmaf(b.w, f, acc[7]);
+            }
+            if (!ok) continue;                              // a wait gave up: nothing is written
+            if (w.whole) {
+                const float inv = 1.0f / L;
+                __nv_bfloat162 b[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) b[j] = __floats2bfloat162_rn(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+                *reinterpret_cast<uint4 *>((__nv_bfloat16 *)p.out + w.out_row(r) * HD + d) = *reinterpret_cast<uint4 *>(b);
+            } else {
+                float *po = part_out<HD>(p, part, r) + d;
+                *reinterpret_cast<float4 *>(po) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                *reinterpret_cast<float4 *>(po + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                if (d == 0) *part_ml(p, part, r) = make_float2(M, L);
+            }
         }
+        first_part = false;
     }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    for (int idx = tid; idx < 16 * (HD / 8); idx += 128) {
-        const int r = idx / (HD / 8), d = (idx % (HD / 8)) * 8;
-        if (r >= t.rows) continue;
-        float M = -INFINITY, L = 0.f, acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+}
+
+// Joins the parts of the pairs that lie in several CTAs' stretches: a warp a row, HD / 32 neighbouring dimensions a lane, eight parts'
+// outputs in flight.
+template <int HD>
+__global__ void __launch_bounds__(256) attention_q8_join_kernel(const Q8Params p, int ctas) {
+    pdl_launch_dependents();
+    constexpr int DL = HD / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.x, kvh = blockIdx.y, G = p.nq / p.nkv;
+    const Line line{p};
+    int before = 0, all = 0;
+    for (int i = lane; i < p.nseq; i += 32) {
+        const int n = line.tiles_of(i);
+        all += n;
+        if (i < seq) before += n;
+    }
+    const long long length = (long long)__reduce_add_sync(0xffffffffu, all) * p.nkv;
+    const int n = line.tiles_of(seq);
+    const long long begin = (long long)__reduce_add_sync(0xffffffffu, before) * p.nkv + (long long)kvh * n;
+    pdl_wait();
+    if (n == 0) return;
+    const int u0 = holder(begin, length, ctas), u1 = holder(begin + n - 1, length, ctas);
+    if (u0 == u1) return;
+    const int tok_begin = p.cu_seqlens[seq], rows = (p.cu_seqlens[seq + 1] - tok_begin) * G;
+    const long long first = 2ll * u0 + (begin > stretch(u0, length, ctas) ? 1 : 0);      // in its own CTA the pair's part is the last one
+    auto part_of = [&](int k) { return k == 0 ? first : 2ll * (u0 + k); };
+    const int parts = u1 - u0 + 1;
+    for (int r = warp; r < rows; r += 8) {
+        float M = -INFINITY;
+        for (int k = lane; k < parts; k += 32) M = fmaxf(M, part_ml(p, part_of(k), r)->x);
+        M = warp_max(M);
+        float L = 0.f, acc[DL] = {};
+        for (int k0 = 0; k0 < parts; k0 += 32) {
+            const float2 ml = k0 + lane < parts ? *part_ml(p, part_of(k0 + lane), r) : make_float2(-INFINITY, 0.f);
+            const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+            L += warp_sum(f == 0.f && ml.y == ml.y ? 0.f : ml.y * f);            // (a sum that is no number stays that)
+            for (int k = 0; k < min(32, parts - k0); k += 8) {
+                float x[8][DL];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, mml[(w * 16 + r) * 2]);
+                for (int j = 0; j < 8; ++j)
+                    if (k0 + k + j < parts) {
+                        const float *src = part_out<HD>(p, part_of(k0 + k + j), r) + lane * DL;
+                        if (DL == 4) *reinterpret_cast<float4 *>(x[j]) = *reinterpret_cast<const float4 *>(src);
+                        else *reinterpret_cast<float2 *>(x[j]) = *reinterpret_cast<const float2 *>(src);
+                    }
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float mw = mml[(w * 16 + r) * 2], lw = mml[(w * 16 + r) * 2 + 1];
-            const float f = mw == -INFINITY ? 0.f : exp2f(mw - M);
-            if (f == 0.f && lw == lw) continue;         // (a sum that is no number stays that)
-            L = fmaf(lw, f, L);
-            const float4 a = *reinterpret_cast<const float4 *>(mo + (w * 16 + r) * R::LDO + d), b = *reinterpret_cast<const float4 *>(mo + (w * 16 + r) * R::LDO + d + 4);
-            acc[0] = fmaf(a.x, f, acc[0]); acc[1] = fmaf(a.y, f, acc[1]); acc[2] = fmaf(a.z, f, acc[2]); acc[3] = fmaf(a.w, f, acc[3]);
-            acc[4] = fmaf(b.x, f, acc[4]); acc[5] = fmaf(b.y, f, acc[5]); acc[6] = fmaf(b.z, f, acc[6]); acc[7] = fmaf(b.w, f, acc[7]);
+                for (int j = 0; j < 8; ++j) {
+                    if (k0 + k + j >= parts) break;
+                    const float fs = __shfl_sync(0xffffffffu, f, k + j);
+                    if (fs == 0.f) continue;
+#pragma unroll
+                    for (int d = 0; d < DL; ++d) acc[d] = fmaf(x[j][d], fs, acc[d]);
+                }
+            }
         }
-        if (!ok) continue;                              // a wait gave up: nothing is written
-        const size_t row = q8_out_row(p, t, kvh, r);
-        if (p.slices > 1) {
-            float *po = p.part_o + (row * p.slices + slice) * HD + d;
-            *reinterpret_cast<float4 *>(po) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-            *reinterpret_cast<float4 *>(po + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
-            if (d == 0) *reinterpret_cast<float2 *>(p.part_ml + (row * p.slices + slice) * 2) = make_float2(M, L);
-        } else {
-            const float inv = 1.0f / L;
-            __nv_bfloat162 w[4];
+        const float inv = 1.0f / L;
+        __nv_bfloat16 *out = (__nv_bfloat16 *)p.out + ((size_t)(tok_begin + r / G) * p.nq + kvh * G + r % G) * HD + lane * DL;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = __floats2bfloat162_rn(acc[2 * j] * inv, acc[2 * j + 1] * inv);
-            *reinterpret_cast<uint4 *>((__nv_bfloat16 *)p.out + row * HD + d) = *reinterpret_cast<uint4 *>(w);
-        }
+        for (int d = 0; d < DL; d += 2) *reinterpret_cast<__nv_bfloat162 *>(out + d) = __floats2bfloat162_rn(acc[d] * inv, acc[d + 1] * inv);
     }
 }
 
 template <int HD> constexpr size_t decode_smem() { return Ring<HD>::BYTES + 1024; }
 
 template <int HD>
-int launch_decode(const Q8Params &p, int tiles, cudaStream_t stream) {
+int launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
     CUtensorMap mk, mv;
     const long long lines = (long long)p.cache_pages * p.nkv * p.page_size * HD / 128;
     const int box = (p.page_size % 64 == 0 ? 64 : p.page_size % 32 == 0 ? 32 : 16) * HD / 128;
@@ -357,21 +569,26 @@ int launch_decode(const Q8Params &p, int tiles, cudaStream_t stream) {
     if (rc) return rc;
     if (cudaFuncSetAttribute(attention_q8_decode_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)decode_smem<HD>()) != cudaSuccess)
         return kestrel_fail(-3, "attention_q8: cannot raise the shared-memory limit: %s", cudaGetErrorString(cudaGetLastError()));
-    kestrel_launch(attention_q8_decode_kernel<HD>, dim3(tiles, p.nkv, p.slices), dim3(THREADS), decode_smem<HD>(), stream, mk, mv, p);
-    return kestrel_check_launch("attention_q8 decode");
+    kestrel_launch(attention_q8_decode_kernel<HD>, dim3(ctas), dim3(THREADS), decode_smem<HD>(), stream, mk, mv, p);
+    rc = kestrel_check_launch("attention_q8 decode");
+    if (rc) return rc;
+    kestrel_launch(attention_q8_join_kernel<HD>, dim3(p.nseq, p.nkv), dim3(256), 0, stream, p, ctas);
+    return kestrel_check_launch("attention_q8 join");
 }
 
 }  // namespace
 
-int q8_launch_decode(const Q8Params &p, int tiles, cudaStream_t stream) {
-    return p.hd == 64 ? launch_decode<64>(p, tiles, stream) : launch_decode<128>(p, tiles, stream);
+int q8_launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
+    return p.hd == 64 ? launch_decode<64>(p, ctas, stream) : launch_decode<128>(p, ctas, stream);
 }
 
-// CTAs that the SMs hold at once, by shared memory
-int q8_decode_slots(int hd) {
-    const size_t smem = hd == 64 ? decode_smem<64>() : decode_smem<128>();
-    return kestrel_sms() * (int)((227 * 1024) / (smem + 1024));
+// Every SM holds two CTAs.  A stretch of fewer than two tiles costs more to begin and to join than it takes.
+int q8_decode_ctas(long long tiles) {
+    const long long most = 2ll * kestrel_sms();
+    return (int)(tiles / 2 < 1 ? 1 : tiles / 2 < most ? tiles / 2 : most);
 }
+
+long long q8_decode_scratch(int ctas, int hd) { return 2ll * ctas * 16 * (hd + 2); }
 
 int q8_decode_error() {
     int v = 0, zero = 0;
