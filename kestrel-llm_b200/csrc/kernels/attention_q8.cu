@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(THREADS) attention_q8_plain_kernel(const Q8Par
             const int r = i / (HDP / 4), d = i % (HDP / 4) * 4, key = kb + r;
             float4 kf = make_float4(0.f, 0.f, 0.f, 0.f), vf = kf;
             if (key >= lo && key < hi && d < p.hd) {
-                const long long row = q8_row_of(p, t.table, kvh, key);
+                const int row = q8_row_of(p, t.table, kvh, key);
                 const size_t at = (size_t)(row + key % Q8_BLOCK) * p.hd + d;
                 const char4 kc = *reinterpret_cast<const char4 *>(p.k + at), vc = *reinterpret_cast<const char4 *>(p.v + at);
                 const float sk = p.ks[row / Q8_BLOCK];
@@ -223,7 +223,7 @@ enum Kernel { CORES, DECODE };
 struct Part {
     Kernel kernel = CORES;
     int rows_above = 0, rows_upto = 0, rows_per_tile = 0, tiles = 0, slices = 1, longest = 0;
-    int ctas = 0;
+    int ctas = 0, most_rows = 0;
     long long scratch = 0;              // floats
     long long key_tiles = 0;             // of 64, over all requests and kv heads
 };
@@ -255,6 +255,7 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
         const int seen = window > 0 ? std::min(keys, window + (int)((rows - 1) / G)) : keys;
         p.tiles += times * (int)((rows + p.rows_per_tile - 1) / p.rows_per_tile);
         p.longest = std::max(p.longest, seen);
+        p.most_rows = std::max(p.most_rows, (int)std::min<long long>(rows, p.rows_upto));
         p.key_tiles += (long long)times * nkv * ((seen + 63) / 64);
     };
     if (cu) {
@@ -268,7 +269,7 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
     for (Part *p : {&small, &large}) {
         if (!p->tiles) continue;
         if (p->kernel == DECODE) {
-            p->ctas = q8_decode_ctas(p->key_tiles);
+            p->ctas = q8_decode_ctas(p->key_tiles, hd, p->most_rows);
             p->scratch = q8_decode_scratch(p->ctas, hd);
         } else {
             p->slices = slices_for((long long)p->tiles * nkv, kestrel_sms() * 2, p->longest, 256);
@@ -314,13 +315,14 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
         p.cu_seqlens = cu_seqlens; p.kv_lens = kv_lens; p.block_table = block_table;
         p.nseq = nseq; p.table_width = table_width; p.table_stride = table_stride; p.page_size = page_size; p.cache_pages = cache_pages;
         p.nq = nq; p.nkv = nkv; p.hd = hd; p.window = window; p.slices = part.slices; p.scale = scale;
+        p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1;
         p.rows_above = part.rows_above; p.rows_upto = part.rows_upto; p.rows_per_tile = part.rows_per_tile;
         KESTREL_REQUIRE(part.scratch == 0 || (scratch && part.scratch <= scratch_floats), "attention_q8: scratch of %lld floats is needed, %lld given", part.scratch, scratch_floats);
         p.part_o = scratch;
         int rc;
         if (part.kernel == DECODE) {
             p.part_ml = scratch + 2ll * part.ctas * 16 * hd;
-            rc = q8_launch_decode(p, part.ctas, stream);
+            rc = q8_launch_decode(p, part.ctas, part.most_rows, stream);
             launches += 2;
         } else {
             p.part_ml = scratch ? scratch + (long long)T * nq * part.slices * hd : nullptr;

@@ -27,6 +27,7 @@ struct Q8Params {
     int nseq, table_width, table_stride, page_size, cache_pages, nq, nkv, hd, window, slices;
     int rows_above, rows_upto;      // this launch takes the requests with rows_above < (token, head) rows per kv head <= rows_upto
     int rows_per_tile;
+    int page_shift;                 // log2 of the page size, or -1
     float scale;
 };
 
@@ -86,11 +87,11 @@ __device__ __forceinline__ void q8_slice(const Q8Tile &t, int slices, int slice,
 
 // Row (in units of one token's codes of one head) of the first token of the block that holds position `pos`; a released or absent page,
 // whose keys no row may see, stands for page 0.
-__device__ __forceinline__ long long q8_row_of(const Q8Params &p, const int *table, int kvh, int pos) {
-    const int idx = pos / p.page_size;
+__device__ __forceinline__ int q8_row_of(const Q8Params &p, const int *table, int kvh, int pos) {
+    const int idx = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
     int page = idx < p.table_width ? table[idx] : 0;
     if (page < 0 || page >= p.cache_pages) page = 0;
-    return ((long long)page * p.nkv + kvh) * p.page_size + (pos - idx * p.page_size) / Q8_BLOCK * Q8_BLOCK;
+    return (page * p.nkv + kvh) * p.page_size + (pos - idx * p.page_size) / Q8_BLOCK * Q8_BLOCK;       // below 2^31: checked on the host
 }
 
 __device__ __forceinline__ size_t q8_out_row(const Q8Params &p, const Q8Tile &t, int kvh, int r) {
@@ -99,8 +100,8 @@ __device__ __forceinline__ size_t q8_out_row(const Q8Params &p, const Q8Tile &t,
 }
 
 // attention_q8_decode.cu: requests of up to 16 rows, head sizes 64 and 128, bfloat16; two kernels
-int q8_launch_decode(const Q8Params &p, int ctas, cudaStream_t stream);
-int q8_decode_ctas(long long tiles);                    // for so many (request, kv head, 64 keys)
+int q8_launch_decode(const Q8Params &p, int ctas, int most_rows, cudaStream_t stream);
+int q8_decode_ctas(long long tiles, int hd, int most_rows);      // for so many (request, kv head, 64 keys), requests of at most so many rows
 long long q8_decode_scratch(int ctas, int hd);          // floats: part_o, then part_ml
 int q8_decode_error();                                  // its bounded waits' error word; synchronises
 int q8_launch_plain(const Q8Params &p, int dtype, int tiles, cudaStream_t stream);

@@ -8,7 +8,9 @@
 //
 // A loader warp brings tiles by TMA into a ring of stages, codes of K and V side by side, and the scales of their four blocks beside
 // them, running ahead over the pairs' borders; four consumer warps take one block of 16 keys each.  Codes go from shared memory straight
-// into the fragments of mma.sync.m16n8k16 (float16, float32 sums).  A code of V is the low byte of the float16 number 1024 + (c + 128), made
+// into the fragments of mma.sync.m16n8k16 (float16, float32 sums), as the operand of sixteen rows: 16 keys by 8 query rows of scores,
+// 16 dimensions by 8 query rows of outputs, so that four heads a group leave half of a product unused and not three quarters, and a
+// thread's softmax holds four scores.  The weights change places between the two products by transposing 8 by 8 tiles.  A code of V is the low byte of the float16 number 1024 + (c + 128), made
 // by a byte permutation and freed of 1152 by one subtraction of pairs.  A code of K is the float16 number (c + 128) 2^-24, a subnormal
 // one, which the permutation alone makes; the scores' sums begin with -128 2^-24 times the row's sum of queries instead of zero.  (The same
 // for V would leave 128 times the weights' sum in the outputs, of which they are a hundredth where many keys weigh alike.)
@@ -28,11 +30,12 @@ namespace {
 constexpr int THREADS = 160, BN = 64;       // four consumer warps and the loader; keys of a tile
 constexpr uint32_t MAGIC = 0x64646464u;     // high byte of the float16 numbers 1024 .. 1279
 
-template <int HD> struct Ring {
-    static constexpr int STAGES = HD == 128 ? 4 : 8;
+// NT: column tiles of eight rows.  One: three CTAs an SM; two: two.
+template <int HD, int NT> struct Ring {
+    static constexpr int STAGES = (NT == 1 ? 3 : 4) * (128 / HD), CTAS = NT == 1 ? 3 : 2;
     static constexpr int LDO = HD + 4;      // row of a warp's outputs, in floats, when the four warps meet
     static constexpr uint32_t PLANE = BN * HD, STAGE = 2 * PLANE;
-    static constexpr uint32_t SCALES = STAGES * STAGE, BARS = SCALES + STAGES * 32, MEET = BARS + 16 * STAGES, BYTES = MEET + 4 * 16 * (LDO + 2) * 4;
+    static constexpr uint32_t SCALES = STAGES * STAGE, BARS = SCALES + STAGES * 32, MEET = BARS + 16 * STAGES, BYTES = MEET + 4 * 8 * NT * (LDO + 2) * 4;
 };
 
 __device__ __forceinline__ uint32_t hsub2(uint32_t a) {             // - 1152 from both halves
@@ -65,6 +68,11 @@ __device__ __forceinline__ void mma_f16(float *d, const uint32_t *a, uint32_t b0
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ uint32_t transpose(uint32_t a) {        // of an 8 by 8 tile of 16-bit numbers
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
 __device__ __forceinline__ uint4 lds128(uint32_t at) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
@@ -76,11 +84,11 @@ __device__ __forceinline__ uint2 lds64(uint32_t at) {
     return v;
 }
 
-// Key, among the eight of a column tile, that column n of the scores stands for.  A tile's lines of 128 bytes are swizzled as TMA writes
-// them: 16-byte chunk c of line i lies at c ^ (i % 8).  Head size 128: a key is a line; eight lanes of a 16-byte load hold columns
+// Key, among the eight of a half tile, that row n of the scores stands for.  A tile's lines of 128 bytes are swizzled as TMA writes
+// them: 16-byte chunk c of line i lies at c ^ (i % 8).  Head size 128: a key is a line; eight lanes of a 16-byte load hold rows
 // 2 i and 2 i + 1, whose keys are four lines apart, so that their chunks fall into different halves of the banks; the values' loads of
-// sixteen lanes hold the even (or odd) columns, which are neighbouring keys.  Head size 64: a line is two keys.
-template <int HD> __device__ __forceinline__ int key_of_column(int n) { return HD == 128 ? (n >> 1) + 4 * (n & 1) : n ^ ((n >> 1) & 1); }
+// sixteen lanes hold the even (or odd) rows, which are neighbouring keys.  Head size 64: a line is two keys.
+template <int HD> __device__ __forceinline__ int key_of_row(int n) { return HD == 128 ? (n >> 1) + 4 * (n & 1) : n ^ ((n >> 1) & 1); }
 
 // address of 16-byte chunk c (of HD / 16) of key k in a tile
 template <int HD> __device__ __forceinline__ uint32_t chunk_at(int k, int c) {
@@ -193,12 +201,67 @@ struct Walk {
 template <int HD> __device__ __forceinline__ float *part_out(const Q8Params &p, long long part, int row) { return p.part_o + (part * 16 + row) * HD; }
 __device__ __forceinline__ float2 *part_ml(const Q8Params &p, long long part, int row) { return reinterpret_cast<float2 *>(p.part_ml) + part * 16 + row; }
 
-template <int HD>
-__global__ void __launch_bounds__(THREADS, 2)
+// A block's scores s - (key g, rows 2 c and 2 c + 1), (key g + 8, the same) - become weights; the rows' references, sums and outputs follow.
+// sk: the keys' scale, lv and rv: log2 and reciprocal of the values'.  MASKED: some row does not see the block whole.
+template <int NT, bool MASKED, int NO>
+__device__ __forceinline__ void weigh(float (&s)[NT][4], float (&o)[NT][NO][4], float (&m)[NT][2], float (&l)[NT][2], const float (&row_scale)[NT][2], float sk,
+                                      float lv, float rv, int kbase, int my_key, const int (&pos)[NT][2], const int (&low)[NT][2]) {
+    float mx[NT][2], ck[NT][2];
+    bool none[NT][2], grow = false;             // none: rows that see nothing of the block, whatever its scales are
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            none[nt][i] = MASKED && (kbase > pos[nt][i] || kbase + 15 < low[nt][i]);
+            if (MASKED) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int key = kbase + my_key + 8 * h;
+                    if (!(key <= pos[nt][i] && key >= low[nt][i])) s[nt][2 * h + i] = -INFINITY;
+                }
+            }
+            ck[nt][i] = sk * row_scale[nt][i];
+            // in base-2 units, with the value's scale: x = s * ck + lv
+            mx[nt][i] = fmaf(fmaxf(s[nt][i], s[nt][2 + i]), ck[nt][i], lv);
+            if (MASKED && none[nt][i]) mx[nt][i] = -INFINITY;
+            grow |= mx[nt][i] > m[nt][i] + 8.f || (m[nt][i] == -INFINITY && mx[nt][i] > -INFINITY);
+        }
+    // the reference moves once the maximum has outgrown it by 8: weights stay below 2^8
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) mx[nt][i] = fmaxf(mx[nt][i], __shfl_xor_sync(0xffffffffu, mx[nt][i], x));
+                if (mx[nt][i] > m[nt][i]) {
+                    const float alpha = m[nt][i] == -INFINITY ? 0.f : exp2_fast(m[nt][i] - mx[nt][i]);
+                    m[nt][i] = mx[nt][i];
+                    l[nt][i] *= alpha;
+#pragma unroll
+                    for (int j = 0; j < NO; ++j) o[nt][j][i] *= alpha, o[nt][j][2 + i] *= alpha;
+                }
+            }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float shift = lv - (m[nt][i] == -INFINITY ? 0.f : m[nt][i]);
+            float &a = s[nt][i], &b = s[nt][2 + i];
+            a = exp2_fast(fmaf(a, ck[nt][i], shift));
+            b = exp2_fast(fmaf(b, ck[nt][i], shift));
+            if (MASKED && none[nt][i]) a = b = 0.f;
+            else l[nt][i] = fmaf(a + b, rv, l[nt][i]);
+        }
+}
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(THREADS, Ring<HD, NT>::CTAS)
 attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Q8Params p) {
     pdl_launch_dependents();
-    using R = Ring<HD>;
-    constexpr int KS = HD / 16, HALVES = HD / 64, NT_O = HD / 8;
+    using R = Ring<HD, NT>;
+    constexpr int KS = HD / 16, HALVES = HD / 64, ROWS = 8 * NT;
     extern __shared__ uint8_t q8d_smem[];
     const uint32_t base = (smem_u32(q8d_smem) + 1023u) & ~1023u;
     uint8_t *ring = q8d_smem + (base - smem_u32(q8d_smem));
@@ -226,14 +289,14 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
             const int kb0 = w.k_first / BN * BN;
             for (int i = w.from; i < w.to; ++i) {
                 const int kb = kb0 + i * BN;
-                const long long box_row = lane < boxes ? q8_row_of(p, w.table, w.kvh, kb + lane * box) : 0;
-                const long long block_row = lane < 8 ? q8_row_of(p, w.table, w.kvh, kb + (lane & 3) * Q8_BLOCK) : 0;
+                const int box_row = lane < boxes ? q8_row_of(p, w.table, w.kvh, kb + lane * box) : 0;
+                const int block_row = lane < 8 ? q8_row_of(p, w.table, w.kvh, kb + (lane & 3) * Q8_BLOCK) : 0;
                 if (!mbar_wait(empty_bar(stage), phase ^ 1u)) { atomicExch(&g_q8d_error, 1); ok = false; break; }
                 if (lane == 0) mbar_expect_tx(full_bar(stage), R::STAGE);
                 __syncwarp();
                 if (lane < boxes) {
                     const uint32_t dst = base + stage * R::STAGE + lane * box * HD;
-                    const int line = (int)(HD == 128 ? box_row : box_row >> 1);
+                    const int line = HD == 128 ? box_row : box_row >> 1;
                     tma_load_2d(dst, &map_k, full_bar(stage), 0, line);
                     tma_load_2d(dst + R::PLANE, &map_v, full_bar(stage), 0, line);
                 }
@@ -248,37 +311,37 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     }
 
     // ---- consumers
-    const int g = lane >> 2, c = lane & 3;              // rows g and g + 8; a quarter of the inner index
-    // where this thread's codes lie in a stage: of the scores' first column tile (the second is 8 keys further), and of V
+    // a lane (g, c) holds rows g of the first operands, row g of the queries, and of a product keys g and g + 8 for rows 2 c and 2 c + 1
+    const int g = lane >> 2, c = lane & 3;
+    // where this thread's codes lie in a stage: of K for the block's first eight keys, and of V
     uint32_t k_off[HALVES], v_off[2];
 #pragma unroll
-    for (int j = 0; j < HALVES; ++j) k_off[j] = warp * 16 * HD + chunk_at<HD>(key_of_column<HD>(g), 4 * j + c);
+    for (int j = 0; j < HALVES; ++j) k_off[j] = warp * 16 * HD + chunk_at<HD>(key_of_row<HD>(g), 4 * j + c);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
-        v_off[j] = R::PLANE + warp * 16 * HD + chunk_at<HD>(key_of_column<HD>(2 * c + j), HD == 128 ? (g >> 1) + 4 * (g & 1) : g >> 1) + (HD == 64 ? 8 * (g & 1) : 0);
-    // (8 keys are 8 lines at head size 128, which the swizzle repeats after, and 4 at 64, which turn its third bit)
+        v_off[j] = R::PLANE + warp * 16 * HD + chunk_at<HD>(key_of_row<HD>(2 * c + j), HD == 128 ? (g >> 1) + 4 * (g & 1) : g >> 1) + (HD == 64 ? 8 * (g & 1) : 0);
+    // the other eight keys: 8 lines further at head size 128, which the swizzle repeats after, 4 at 64, which turn its third bit
     auto second = [](uint32_t at) { return HD == 128 ? at + 1024 : (at + 512) ^ 64u; };
-    const int col0 = key_of_column<HD>(2 * c), col1 = key_of_column<HD>(2 * c + 1);     // keys of this thread's score columns
-    float *meet = reinterpret_cast<float *>(ring + R::MEET), *meet_ml = meet + 4 * 16 * R::LDO;
+    const int my_key = key_of_row<HD>(g);
+    float *meet = reinterpret_cast<float *>(ring + R::MEET), *meet_ml = meet + 4 * ROWS * R::LDO;
     bool ok = true;             // after a wait gave up the loop runs on without waiting, so that the warps still meet below
     bool first_part = true;
 
     while (w.next()) {
         // Queries as fragments, in float16: a row is multiplied by the power of two that brings its largest number to [64, 128), so that
         // a bfloat16 number keeps its bits down to 2^-21 of that, and the rest is off by 2^-31 of it.
-        uint32_t qa[KS][4];
-        float row_scale[2], bias[2];
-        int pos[2], low[2], min_pos = 0x7fffffff;       // (of the rows that are there)
+        uint32_t qb[NT][KS][2];
+        float row_scale[NT][2], bias[NT][2];            // of rows 2 c and 2 c + 1
+        int pos[NT][2], low[NT][2], min_pos = 0x7fffffff, max_low = 0;      // (the last two of the rows that are there)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = g + 8 * i;
-            const bool live = r < w.rows;
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = 8 * nt + g;
             uint4 q[HALVES][2];
             uint32_t big = 0;
 #pragma unroll
             for (int j = 0; j < HALVES; ++j) {
                 q[j][0] = q[j][1] = make_uint4(0, 0, 0, 0);
-                if (live) {
+                if (r < w.rows) {
                     const uint4 *src = reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)p.q + w.out_row(r) * HD + 64 * j + 16 * c);
                     q[j][0] = src[0];
                     q[j][1] = src[1];
@@ -295,7 +358,6 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
             const int e = (int)(big >> 7);              // biased exponent of the largest; 255: not finite, as it is
             const int up = big == 0 || e == 255 ? 0 : 127 + 6 - max(e, 63);      // (below 2^-64 nothing weighs)
             const float f = __uint_as_float((uint32_t)(127 + up) << 23);
-            row_scale[i] = __uint_as_float((uint32_t)(127 - up) << 23) * p.scale * (1.4426950408889634f * 16777216.0f);
             float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < HALVES; ++j)
@@ -304,28 +366,42 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                     const uint32_t a = reinterpret_cast<const uint32_t *>(&q[j][k >> 1])[2 * (k & 1)], b = reinterpret_cast<const uint32_t *>(&q[j][k >> 1])[2 * (k & 1) + 1];
                     const uint32_t x = pack_f16(__uint_as_float(a << 16) * f, __uint_as_float(a & 0xffff0000u) * f);
                     const uint32_t y = pack_f16(__uint_as_float(b << 16) * f, __uint_as_float(b & 0xffff0000u) * f);
-                    qa[4 * j + k][i] = x;
-                    qa[4 * j + k][2 + i] = y;
+                    qb[nt][4 * j + k][0] = x;
+                    qb[nt][4 * j + k][1] = y;
                     const float2 fx = __half22float2(*reinterpret_cast<const __half2 *>(&x)), fy = __half22float2(*reinterpret_cast<const __half2 *>(&y));
                     sum += (fx.x + fx.y) + (fy.x + fy.y);
                 }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            bias[i] = sum * (-128.0f / 16777216.0f);
-            pos[i] = live ? w.pos_begin + r / w.G : -1;
-            low[i] = p.window > 0 ? max(0, pos[i] - p.window + 1) : 0;
-            if (live) min_pos = min(min_pos, pos[i]);
-        }
-        int max_low = max(low[0], low[1]);
+            const float scale_g = __uint_as_float((uint32_t)(127 - up) << 23) * p.scale * (1.4426950408889634f * 16777216.0f);
+            const float bias_g = sum * (-128.0f / 16777216.0f);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            min_pos = min(min_pos, __shfl_xor_sync(0xffffffffu, min_pos, o));
-            max_low = max(max_low, __shfl_xor_sync(0xffffffffu, max_low, o));
+            for (int i = 0; i < 2; ++i) {
+                row_scale[nt][i] = __shfl_sync(0xffffffffu, scale_g, 8 * c + 4 * i);
+                bias[nt][i] = __shfl_sync(0xffffffffu, bias_g, 8 * c + 4 * i);
+                const int row = 8 * nt + 2 * c + i;
+                const bool live = row < w.rows;
+                pos[nt][i] = live ? w.pos_begin + row / w.G : -1;
+                low[nt][i] = p.window > 0 ? max(0, pos[nt][i] - p.window + 1) : 0;
+                if (live) min_pos = min(min_pos, pos[nt][i]);
+                max_low = max(max_low, low[nt][i]);
+            }
         }
-        float o[NT_O][4];
+        min_pos = min(min_pos, __shfl_xor_sync(0xffffffffu, min_pos, 1));
+        min_pos = min(min_pos, __shfl_xor_sync(0xffffffffu, min_pos, 2));
+        max_low = max(max_low, __shfl_xor_sync(0xffffffffu, max_low, 1));
+        max_low = max(max_low, __shfl_xor_sync(0xffffffffu, max_low, 2));
+        float o[NT][HD / 16][4];
 #pragma unroll
-        for (int i = 0; i < NT_O; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+        float m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+        }
         const int k_begin = w.k_first / BN * BN;
 
         for (int i = w.from; i < w.to; ++i) {
@@ -333,11 +409,11 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
             const int kbase = k_begin + i * BN + 16 * warp;     // this warp's block
             if (ok && kbase < w.k_end && kbase + 16 > w.k_first) {
                 const uint32_t at = base + stage * R::STAGE;
-                float s[2][4];
+                float s[NT][4];
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    s[nt][0] = s[nt][1] = bias[0];
-                    s[nt][2] = s[nt][3] = bias[1];
+                for (int nt = 0; nt < NT; ++nt) {
+                    s[nt][0] = s[nt][2] = bias[nt][0];
+                    s[nt][1] = s[nt][3] = bias[nt][1];
                 }
 #pragma unroll
                 for (int j = 0; j < HALVES; ++j) {
@@ -346,70 +422,26 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const uint32_t x0 = u0[k] ^ 0x80808080u, x1 = u1[k] ^ 0x80808080u;
-                        mma_f16(s[0], qa[4 * j + k], __byte_perm(x0, 0, 0x4140), __byte_perm(x0, 0, 0x4342));
-                        mma_f16(s[1], qa[4 * j + k], __byte_perm(x1, 0, 0x4140), __byte_perm(x1, 0, 0x4342));
+                        const uint32_t a[4] = {__byte_perm(x0, 0, 0x4140), __byte_perm(x1, 0, 0x4140), __byte_perm(x0, 0, 0x4342), __byte_perm(x1, 0, 0x4342)};
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a, qb[nt][4 * j + k][0], qb[nt][4 * j + k][1]);
                     }
                 }
                 const float *sc = reinterpret_cast<const float *>(ring + R::SCALES + stage * 32);
                 const float sk = sc[warp], sv = sc[4 + warp];
                 const float lv = log2_fast(sv), rv = rcp_fast(sv);
-                // scores with the value's scale, in base-2 units: x = s * ck + lv
-                const float ck[2] = {sk * row_scale[0], sk * row_scale[1]};
-                const bool whole = kbase >= w.k_first && kbase + 16 <= w.k_end && kbase + 15 <= min_pos && kbase >= max_low;
-                bool none[2] = {false, false};              // rows that see nothing of the block
-                if (!whole) {
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        none[r] = kbase > pos[r] || kbase + 15 < low[r];
-#pragma unroll
-                        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int key = kbase + 8 * nt + (e ? col1 : col0);
-                                if (!(key <= pos[r] && key >= low[r])) s[nt][2 * r + e] = -INFINITY;
-                            }
-                    }
+                if (kbase >= w.k_first && kbase + 16 <= w.k_end && kbase + 15 <= min_pos && kbase >= max_low) {
+                    weigh<NT, false>(s, o, m, l, row_scale, sk, lv, rv, kbase, my_key, pos, low);
+                } else {
+                    weigh<NT, true>(s, o, m, l, row_scale, sk, lv, rv, kbase, my_key, pos, low);
                 }
-                float mx[2];
-                bool grow = false;
+                // out += w V: the transposed weights' pairs are keys 2 c, 2 c + 1 of both halves
+                uint32_t b[NT][2];
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    mx[r] = fmaf(fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])), ck[r], lv);
-                    if (none[r]) mx[r] = -INFINITY;         // whatever the scales are
-                    grow |= mx[r] > m[r] + 8.f || (m[r] == -INFINITY && mx[r] > -INFINITY);
+                for (int nt = 0; nt < NT; ++nt) {
+                    b[nt][0] = transpose(pack_f16(s[nt][0], s[nt][1]));
+                    b[nt][1] = transpose(pack_f16(s[nt][2], s[nt][3]));
                 }
-                // the reference moves once the maximum has outgrown it by 8: weights stay below 2^8
-                if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                        if (mx[r] > m[r]) {
-                            const float alpha = m[r] == -INFINITY ? 0.f : exp2_fast(m[r] - mx[r]);
-                            m[r] = mx[r];
-                            l[r] *= alpha;
-#pragma unroll
-                            for (int nt = 0; nt < NT_O; ++nt) o[nt][2 * r] *= alpha, o[nt][2 * r + 1] *= alpha;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float shift = lv - (m[r] == -INFINITY ? 0.f : m[r]);
-                    float sum = 0.f;
-#pragma unroll
-                    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float &x = s[nt][2 * r + e];
-                            x = exp2_fast(fmaf(x, ck[r], shift));
-                            if (!whole && none[r]) x = 0.f;
-                            sum += x;
-                        }
-                    if (!none[r]) l[r] = fmaf(sum, rv, l[r]);
-                }
-                // out += w V: columns 2 c, 2 c + 1 of both score tiles are the four keys of this thread's fragments
-                const uint32_t a[4] = {pack_f16(s[0][0], s[0][1]), pack_f16(s[0][2], s[0][3]), pack_f16(s[1][0], s[1][1]), pack_f16(s[1][2], s[1][3])};
                 uint32_t v[4][HD / 32];
                 if (HD == 128) {                            // this thread's 16 dimensions
                     *reinterpret_cast<uint4 *>(v[0]) = lds128(at + v_off[0]);
@@ -423,58 +455,61 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                     *reinterpret_cast<uint2 *>(v[3]) = lds64(at + second(v_off[1]));
                 }
 #pragma unroll
-                for (int k = 0; k < HD / 32; ++k) {         // output column tiles 4 k .. 4 k + 3: dimensions 4 k .. 4 k + 3 of the thread's
+                for (int k = 0; k < HD / 32; ++k) {         // dimensions 4 k .. 4 k + 3 of the thread's, two to a product
                     const uint32_t p0 = __byte_perm(v[0][k], v[1][k], 0x5140) ^ 0x80808080u, p1 = __byte_perm(v[0][k], v[1][k], 0x7362) ^ 0x80808080u;
                     const uint32_t p2 = __byte_perm(v[2][k], v[3][k], 0x5140) ^ 0x80808080u, p3 = __byte_perm(v[2][k], v[3][k], 0x7362) ^ 0x80808080u;
-                    mma_f16(o[4 * k], a, hsub2(__byte_perm(p0, MAGIC, 0x4140)), hsub2(__byte_perm(p2, MAGIC, 0x4140)));
-                    mma_f16(o[4 * k + 1], a, hsub2(__byte_perm(p0, MAGIC, 0x4342)), hsub2(__byte_perm(p2, MAGIC, 0x4342)));
-                    mma_f16(o[4 * k + 2], a, hsub2(__byte_perm(p1, MAGIC, 0x4140)), hsub2(__byte_perm(p3, MAGIC, 0x4140)));
-                    mma_f16(o[4 * k + 3], a, hsub2(__byte_perm(p1, MAGIC, 0x4342)), hsub2(__byte_perm(p3, MAGIC, 0x4342)));
+                    const uint32_t a0[4] = {hsub2(__byte_perm(p0, MAGIC, 0x4140)), hsub2(__byte_perm(p0, MAGIC, 0x4342)),
+                                            hsub2(__byte_perm(p2, MAGIC, 0x4140)), hsub2(__byte_perm(p2, MAGIC, 0x4342))};
+                    const uint32_t a1[4] = {hsub2(__byte_perm(p1, MAGIC, 0x4140)), hsub2(__byte_perm(p1, MAGIC, 0x4342)),
+                                            hsub2(__byte_perm(p3, MAGIC, 0x4140)), hsub2(__byte_perm(p3, MAGIC, 0x4342))};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_f16(o[nt][2 * k], a0, b[nt][0], b[nt][1]);
+                        mma_f16(o[nt][2 * k + 1], a1, b[nt][0], b[nt][1]);
+                    }
                 }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty_bar(stage));
             if (++stage == R::STAGES) stage = 0, phase ^= 1u;
         }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        }
 
         // the four warps' states, in warp order
         asm volatile("bar.sync 1, 128;" ::: "memory");      // the part before has been read
-        // column n of output tile j is dimension j of thread n's: 2 c and 2 c + 1
-        const int d0 = 16 * c, d1 = HD == 128 ? 64 + 16 * c : 16 * c + 8;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            if (8 * r >= w.rows) break;                     // no second half of rows
-            float *row = meet + (warp * 16 + g + 8 * r) * R::LDO;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < NT_O; j += 4) {
-                *reinterpret_cast<float4 *>(row + d0 + j) = make_float4(o[j][2 * r], o[j + 1][2 * r], o[j + 2][2 * r], o[j + 3][2 * r]);
-                *reinterpret_cast<float4 *>(row + d1 + j) = make_float4(o[j][2 * r + 1], o[j + 1][2 * r + 1], o[j + 2][2 * r + 1], o[j + 3][2 * r + 1]);
+            for (int i = 0; i < 2; ++i) {
+                float sum = l[nt][i];
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                const int r = 8 * nt + 2 * c + i;
+                // rows 2 c + i of this thread's dimensions: chunk (g >> 1) + 4 (g & 1) of 16, or 8 g ..
+                float *row = meet + (warp * ROWS + r) * R::LDO + (HD == 128 ? 16 * ((g >> 1) + 4 * (g & 1)) : 8 * g);
+#pragma unroll
+                for (int k = 0; k < HD / 32; ++k)
+                    *reinterpret_cast<float4 *>(row + 4 * k) = make_float4(o[nt][2 * k][i], o[nt][2 * k][2 + i], o[nt][2 * k + 1][i], o[nt][2 * k + 1][2 + i]);
+                if (g == 0) {
+                    meet_ml[(warp * ROWS + r) * 2] = m[nt][i];
+                    meet_ml[(warp * ROWS + r) * 2 + 1] = sum;
+                }
             }
-            if (c == 0) {
-                meet_ml[(warp * 16 + g + 8 * r) * 2] = m[r];
-                meet_ml[(warp * 16 + g + 8 * r) * 2 + 1] = l[r];
-            }
-        }
         asm volatile("bar.sync 1, 128;" ::: "memory");
         const long long part = 2ll * blockIdx.x + (first_part ? 0 : 1);
-        for (int idx = tid; idx < 16 * (HD / 8); idx += 128) {
+        for (int idx = tid; idx < ROWS * (HD / 8); idx += 128) {
             const int r = idx / (HD / 8), d = (idx % (HD / 8)) * 8;
             if (r >= w.rows) break;
             float M = -INFINITY, L = 0.f, acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-            for (int x = 0; x < 4; ++x) M = fmaxf(M, meet_ml[(x * 16 + r) * 2]);
+            for (int x = 0; x < 4; ++x) M = fmaxf(M, meet_ml[(x * ROWS + r) * 2]);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const float mw = meet_ml[(x * 16 + r) * 2], lw = meet_ml[(x * 16 + r) * 2 + 1];
+                const float mw = meet_ml[(x * ROWS + r) * 2], lw = meet_ml[(x * ROWS + r) * 2 + 1];
                 const float f = mw == -INFINITY ? 0.f : exp2f(mw - M);
                 if (f == 0.f && lw == lw) continue;         // (a sum that is no number stays that)
                 L = fmaf(lw, f, L);
-                const float4 a = *reinterpret_cast<const float4 *>(meet + (x * 16 + r) * R::LDO + d), b = *reinterpret_cast<const float4 *>(meet + (x * 16 + r) * R::LDO + d + 4);
+                const float *src = meet + (x * ROWS + r) * R::LDO + d;
+                const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
                 acc[0] = fmaf(a.x, f, acc[0]); acc[1] = fmaf(a.y, f, acc[1]); acc[2] = fmaf(a.z, f, acc[2]); acc[3] = fmaf(a.w, f, acc[3]);
                 acc[4] = fmaf(b.x, f, acc[4]); acc[5] = fmaf(b.y, f, acc[5]); acc[6] = fmaf(b.z, f, acc[6]); acc[7] = fmaf(b.w, f, acc[7]);
             }
@@ -556,9 +591,9 @@ __global__ void __launch_bounds__(256) attention_q8_join_kernel(const Q8Params p
     }
 }
 
-template <int HD> constexpr size_t decode_smem() { return Ring<HD>::BYTES + 1024; }
+template <int HD, int NT> constexpr size_t decode_smem() { return Ring<HD, NT>::BYTES + 1024; }
 
-template <int HD>
+template <int HD, int NT>
 int launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
     CUtensorMap mk, mv;
     const long long lines = (long long)p.cache_pages * p.nkv * p.page_size * HD / 128;
@@ -567,9 +602,9 @@ int launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
     int rc = kestrel_tensor_map_bf16(&mk, p.k, lines, 64, 64, box);
     if (rc == 0) rc = kestrel_tensor_map_bf16(&mv, p.v, lines, 64, 64, box);
     if (rc) return rc;
-    if (cudaFuncSetAttribute(attention_q8_decode_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)decode_smem<HD>()) != cudaSuccess)
+    if (cudaFuncSetAttribute(attention_q8_decode_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)decode_smem<HD, NT>()) != cudaSuccess)
         return kestrel_fail(-3, "attention_q8: cannot raise the shared-memory limit: %s", cudaGetErrorString(cudaGetLastError()));
-    kestrel_launch(attention_q8_decode_kernel<HD>, dim3(ctas), dim3(THREADS), decode_smem<HD>(), stream, mk, mv, p);
+    kestrel_launch(attention_q8_decode_kernel<HD, NT>, dim3(ctas), dim3(THREADS), decode_smem<HD, NT>(), stream, mk, mv, p);
     rc = kestrel_check_launch("attention_q8 decode");
     if (rc) return rc;
     kestrel_launch(attention_q8_join_kernel<HD>, dim3(p.nseq, p.nkv), dim3(256), 0, stream, p, ctas);
@@ -578,13 +613,14 @@ int launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
 
 }  // namespace
 
-int q8_launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
-    return p.hd == 64 ? launch_decode<64>(p, ctas, stream) : launch_decode<128>(p, ctas, stream);
+int q8_launch_decode(const Q8Params &p, int ctas, int most_rows, cudaStream_t stream) {
+    if (most_rows <= 8) return p.hd == 64 ? launch_decode<64, 1>(p, ctas, stream) : launch_decode<128, 1>(p, ctas, stream);
+    return p.hd == 64 ? launch_decode<64, 2>(p, ctas, stream) : launch_decode<128, 2>(p, ctas, stream);
 }
 
-// Every SM holds two CTAs.  A stretch of fewer than two tiles costs more to begin and to join than it takes.
-int q8_decode_ctas(long long tiles) {
-    const long long most = 2ll * kestrel_sms();
+// As many as are resident at once.  A stretch of fewer than two tiles costs more to begin and to join than it takes.
+int q8_decode_ctas(long long tiles, int hd, int most_rows) {
+    const long long most = (most_rows <= 8 ? (hd == 64 ? Ring<64, 1>::CTAS : Ring<128, 1>::CTAS) : (hd == 64 ? Ring<64, 2>::CTAS : Ring<128, 2>::CTAS)) * (long long)kestrel_sms();
     return (int)(tiles / 2 < 1 ? 1 : tiles / 2 < most ? tiles / 2 : most);
 }
 
