@@ -219,7 +219,7 @@ namespace {
 constexpr int MAX_SLICES = 32;
 
 // One launch of a step: the requests with rows_above < rows <= rows_upto, in tiles of rows_per_tile.
-enum Kernel { CORES, DECODE };
+enum Kernel { CORES, DECODE, TC };
 struct Part {
     Kernel kernel = CORES;
     int rows_above = 0, rows_upto = 0, rows_per_tile = 0, tiles = 0, slices = 1, longest = 0;
@@ -245,10 +245,19 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
     small.kernel = cores ? CORES : DECODE;
     small.rows_upto = cores ? 0x7fffffff : 16;
     small.rows_per_tile = cores ? BM : 16;
-    large.kernel = CORES;
+    large.kernel = TC;
     large.rows_above = small.rows_upto;
     large.rows_upto = 0x7fffffff;
-    large.rows_per_tile = BM;
+    large.rows_per_tile = 256;
+    if (!cores && cu) {
+        // while tiles of 128 rows fit the SMs at once, a CTA takes one and its key tiles go to the two streams in turn
+        long long tiles = 0;
+        for (int i = 0; i < nseq; ++i) {
+            const long long rows = (long long)(cu[i + 1] - cu[i]) * G;
+            if (rows > small.rows_upto) tiles += (rows + 127) / 128;
+        }
+        if (tiles * nkv <= kestrel_sms()) large.rows_per_tile = 128;
+    }
     auto count = [&](long long rows, int keys, int times) {
         if (rows <= 0) return;
         Part &p = rows <= small.rows_upto ? small : large;
@@ -272,7 +281,9 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
             p->ctas = q8_decode_ctas(p->key_tiles, hd, p->most_rows);
             p->scratch = q8_decode_scratch(p->ctas, hd);
         } else {
-            p->slices = slices_for((long long)p->tiles * nkv, kestrel_sms() * 2, p->longest, 256);
+            // the tensor cores: one CTA an SM, slices of 512 keys at least
+            p->slices = p->kernel == TC ? slices_for((long long)p->tiles * nkv, kestrel_sms(), p->longest, 512)
+                                        : slices_for((long long)p->tiles * nkv, kestrel_sms() * 2, p->longest, 256);
             p->scratch = p->slices > 1 ? (long long)T * nq * p->slices * (hd + 2) : 0;
         }
         pl.part[pl.parts++] = *p;
@@ -304,7 +315,8 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
     KESTREL_REQUIRE(window >= 0 && scale > 0.f && isfinite(scale), "attention_q8: window %d, scale %g", window, scale);
     KESTREL_REQUIRE(cache_pages > 0 && (long long)cache_pages * nkv * page_size < (1ll << 31), "attention_q8: a cache of %d pages is beyond the 32-bit row coordinate", cache_pages);
     KESTREL_REQUIRE(table_width > 0 && table_stride >= table_width, "attention_q8: block table of %d entries a row, %d apart", table_width, table_stride);
-    KESTREL_REQUIRE(nkv <= 65535, "attention_q8: grid too large");
+    KESTREL_REQUIRE(nkv <= 65535 && nseq <= 0x7fffffff / nkv, "attention_q8: grid too large");
+    KESTREL_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)scratch) & 15) == 0, "attention_q8: tensors must start on 16 bytes");
     Plan pl;
     make_plan(pl, cu_host, kv_host, nseq, max_count, max_kv, T, nq, nkv, hd, window, dtype);
     int launches = 0;
@@ -326,7 +338,7 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
             launches += 2;
         } else {
             p.part_ml = scratch ? scratch + (long long)T * nq * part.slices * hd : nullptr;
-            rc = q8_launch_plain(p, dtype, part.tiles, stream);
+            rc = part.kernel == TC ? q8_launch_tc(p, part.tiles, stream) : q8_launch_plain(p, dtype, part.tiles, stream);
             if (rc == 0 && part.slices > 1) rc = q8_launch_merge(p, dtype, part.tiles, stream);
             launches += part.slices > 1 ? 2 : 1;
         }
@@ -335,4 +347,8 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
     return launches;
 }
 
-KESTREL_API int kestrel_attention_q8_error(void) { return q8_decode_error(); }
+// 1, 2: the decode kernel's loader and consumers; 100 and more: the portion kernel's wait
+KESTREL_API int kestrel_attention_q8_error(void) {
+    const int decode = q8_decode_error(), tc = q8_tc_error();
+    return tc ? 100 + tc : decode;
+}

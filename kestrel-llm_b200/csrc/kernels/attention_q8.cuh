@@ -104,5 +104,9 @@ int q8_launch_decode(const Q8Params &p, int ctas, int most_rows, cudaStream_t st
 int q8_decode_ctas(long long tiles, int hd, int most_rows);      // for so many (request, kv head, 64 keys), requests of at most so many rows
 long long q8_decode_scratch(int ctas, int hd);          // floats: part_o, then part_ml
 int q8_decode_error();                                  // its bounded waits' error word; synchronises
+// attention_q8_tc.cu: tiles of up to 256 rows, head sizes 64 and 128, bfloat16
+int q8_launch_tc(const Q8Params &p, int tiles, cudaStream_t stream);
+int q8_tc_error();
+// attention_q8.cu
 int q8_launch_plain(const Q8Params &p, int dtype, int tiles, cudaStream_t stream);
 int q8_launch_merge(const Q8Params &p, int dtype, int tiles, cudaStream_t stream);

@@ -1,0 +1,572 @@
+// Attention over pages of int8 codes for prompt portions, on the 5th-generation tensor cores.  Head sizes 64 and 128, bfloat16 queries.
+// Formulas in attention_q8.cuh.
+//
+// A CTA owns up to 256 rows - (token, query head of one kv group) pairs, token-major - as two row tiles A and B of 128, and walks the keys
+// its rows may see in tiles of 128.  Sixteen warps in four groups, coupled by mbarriers:
+//   warps 0-3, 4-7   softmax of A and of B: a thread owns a row, its 128 scores in registers; P goes back over S in TMEM as float16;
+//   warp 8           one thread issues S_X = Q_X K^T and O_X += P_X V, tcgen05.mma M = 128, N = 128 (N = head size), in the order
+//                    S_A S_B | PV_A S_A' PV_B S_B' | ..., so that one row tile is multiplied while the other is softmaxed;
+//   warps 9-11       read the codes of K from the cache, 16 bytes a lane, widen them to float16 in registers and write them to shared
+//                    memory in the swizzled layout of an operand, two stages ahead of the products at most; one lane in eight of warp 9
+//                    brings a block's scales along;
+//   warps 12-15      the same for V.
+// A code is widened as the low byte of the float16 number 1024 + (c + 128), less 1152: a permutation for two codes and a subtraction of
+// pairs.  Reading codes and not 16-bit numbers halves what a CTA fetches; the widening, 32,768 codes a key tile, takes some 1,800 of the
+// four schedulers' issue slots, beside 4,100 of the softmax and 2,048 cycles of products at head size 128.
+// The softmax groups hold 184 registers a thread, the others 72: what the 512 threads were launched with, dealt out again.
+//
+// Scores enter the softmax as x = s * ck + lv with ck = (the key's scale) * (the row's), lv = log2 of the value's scale, both the same for
+// 16 keys: the maximum is taken per block before the scales, and the exponent is one multiply-add as without them.  The sum of a block's
+// weights is divided by its value's scale once.  The output accumulates in TMEM against a reference that moves only when a row's maximum
+// has outgrown it by 8.  Codes are numbers whatever a stale page holds, so nothing has to be cleared; a block that a row sees nothing of
+// counts as without scales.
+//
+// HALVES: a CTA with one row tile (up to 128 rows), whose even key tiles go to stream A and odd ones to B, over the same queries; the rows'
+// two states are merged at the end.  Every wait is bounded.
+#include "attention_q8.cuh"
+#include "tcgen05.cuh"
+
+#include <math.h>
+
+__device__ int g_q8t_error = 0;
+
+namespace {
+
+constexpr int THREADS = 512, BM = 128, BN = 128, BLOCKS = BN / Q8_BLOCK;
+constexpr int SOFTMAX_REGS = 184, OTHER_REGS = 72;      // 2 x 128 threads each: 65,536 in all, the launch's 512 x 128
+constexpr uint32_t MAGIC = 0x64646464u;
+constexpr float STEP = 8.0f;                            // log2 units by which a row's maximum may outgrow its reference
+
+enum { Q_FULL = 0, K_FULL = 1, K_EMPTY = 3, V_FULL = 5, V_EMPTY = 7, S_FULL = 9, P_FULL = 11, PV_DONE = 13, SCALES_FULL = 15, BARS = 19 };
+
+template <int HD> struct Lay {
+    static constexpr uint32_t PANEL = 128 * 128, PANELS = HD / 64, TILE = PANELS * PANEL;       // 128 rows of HD float16 numbers
+    static constexpr uint32_t Q = 0, K = 2 * TILE, V = 4 * TILE, SCALES = 6 * TILE;             // Q_A Q_B | two stages of K | of V
+    static constexpr uint32_t ROWS = SCALES + 4 * BLOCKS * 16, BARRIERS = ROWS + 256 * 4, TMEM = BARRIERS + 8 * BARS, BYTES = TMEM + 16;
+    static constexpr uint32_t TMEM_COLS = 512, O = 256;                                         // S_A S_B at 0 and 128, O_A O_B behind
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float log2_fast(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+__device__ __forceinline__ uint32_t hsub2(uint32_t a) {             // - 1152 from both halves
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(0x64806480u));
+    return d;
+}
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 32 consecutive TMEM columns of this thread's lane; ld_wait() before they are used
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st8(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D (TMEM) = or += A (TMEM, M x 16 packed two to a column) x B (shared memory)
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 ldg128(const int8_t *p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+// eight codes as eight float16 numbers
+__device__ __forceinline__ uint4 widen(uint32_t a, uint32_t b) {
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    return make_uint4(hsub2(__byte_perm(a, MAGIC, 0x4140)), hsub2(__byte_perm(a, MAGIC, 0x4342)),
+                      hsub2(__byte_perm(b, MAGIC, 0x4140)), hsub2(__byte_perm(b, MAGIC, 0x4342)));
+}
+
+// One plane's widening, by WARPS warps of which this is the w-th: key tiles of 128 into a ring of two stages at `ring`.  A warp's load is
+// one unit: 512 bytes, 4 keys at head size 128 and 8 at 64; a quarter-warp's stores of 16 bytes go to two keys and every other chunk, which
+// the swizzle spreads over all banks.
+template <int HD, int WARPS, bool SCALED>
+__device__ __forceinline__ void convert(const Q8Params &p, const Q8Tile &t, int kvh, const int8_t *plane, int w, int lane, int k_lo, int n_tiles,
+                                        uint32_t base, uint32_t ring, int full0, int empty0, int error) {
+    using L = Lay<HD>;
+    constexpr int KEYS = 512 / HD, UNITS = BN / KEYS, MINE = (UNITS + WARPS - 1) / WARPS;
+    auto bar = [&](int i) { return base + L::BARRIERS + 8u * (uint32_t)i; };
+    const int key = HD == 128 ? (lane >> 2) & 3 : lane >> 2, chunk = HD == 128 ? (lane & 3) + 4 * (lane >> 4) : lane & 3;
+    // lane l < 8 knows the cache row of a tile's l-th block
+    auto rows_of = [&](int i) { return i < n_tiles ? q8_row_of(p, t.table, kvh, k_lo + i * BN + (lane & 7) * Q8_BLOCK) : 0; };
+    uint4 q[MINE];
+    float sk = 0.f, sv = 1.f;
+    auto fetch = [&](int rows) {
+#pragma unroll
+        for (int u = 0; u < MINE; ++u) {
+            const int k = (w + u * WARPS) * KEYS;           // the unit's first key of the tile
+            const int row = __shfl_sync(0xffffffffu, rows, (k / Q8_BLOCK) & 7) + k % Q8_BLOCK + key;
+            if (w + u * WARPS < UNITS) q[u] = ldg128(plane + (size_t)row * HD + 16 * chunk);
+        }
+        if (SCALED && lane < BLOCKS) sk = p.ks[rows / Q8_BLOCK], sv = p.vs[rows / Q8_BLOCK];
+    };
+    int ahead = rows_of(0);
+    if (n_tiles > 0) fetch(ahead);
+    ahead = rows_of(1);
+    for (int i = 0; i < n_tiles; ++i) {
+        const int b = i & 1;
+        if (!mbar_wait(bar(empty0 + b), (uint32_t)((i >> 1) + 1) & 1u)) { atomicExch(&g_q8t_error, error); break; }
+        const uint32_t stage = base + ring + b * L::TILE;
+#pragma unroll
+        for (int u = 0; u < MINE; ++u) {
+            if (w + u * WARPS >= UNITS) break;
+            const int k = (w + u * WARPS) * KEYS + key;
+            const uint32_t panel = stage + (uint32_t)(chunk >> 2) * L::PANEL;
+            sts128(panel + swizzle128(k, 2 * (chunk & 3)), widen(q[u].x, q[u].y));
+            sts128(panel + swizzle128(k, 2 * (chunk & 3) + 1), widen(q[u].z, q[u].w));
+        }
+        if (SCALED) {
+            // Slot i % 4 is free: tile i's stage was, so S(i - 2) is done, before which every thread was through with tile i - 4.
+            if (lane < BLOCKS)
+                sts128(base + L::SCALES + ((i & 3) * BLOCKS + lane) * 16, make_uint4(__float_as_uint(sk), __float_as_uint(log2_fast(sv)), __float_as_uint(1.0f / sv), 0));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(SCALES_FULL + (i & 3)));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // these writes -> tensor-core reads
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(full0 + b));
+        if (i + 1 < n_tiles) {
+            fetch(ahead);
+            ahead = rows_of(i + 2);
+        }
+    }
+}
+
+template <int HD, bool HALVES>
+__global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Params p) {
+    pdl_launch_dependents();
+    using L = Lay<HD>;
+    // float16 x float16 -> float32, M = 128; S: both operands K-major, N = 128; PV: B is MN-major, N = head size
+    constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+    constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+    extern __shared__ uint8_t q8t_smem[];
+    const uint32_t base = (smem_u32(q8t_smem) + 1023u) & ~1023u;
+    uint8_t *aligned = q8t_smem + (base - smem_u32(q8t_smem));
+    auto bar = [&](int i) { return base + L::BARRIERS + 8u * (uint32_t)i; };
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    // late tiles, which see the most keys, come first - across all kv heads
+    const int kvh = blockIdx.x % p.nkv, slice = blockIdx.z;
+    Q8Tile t;
+    if (!q8_find_tile(p, (int)(gridDim.x / p.nkv) - 1 - (int)(blockIdx.x / p.nkv), t)) { pdl_wait(); return; }
+
+    if (tid == 0) {
+        mbar_init(bar(Q_FULL), 8);
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(bar(K_FULL + b), 3);  mbar_init(bar(K_EMPTY + b), 1);
+            mbar_init(bar(V_FULL + b), 4);  mbar_init(bar(V_EMPTY + b), 1);
+            mbar_init(bar(S_FULL + b), 1);  mbar_init(bar(P_FULL + b), 4);
+            mbar_init(bar(PV_DONE + b), 1);
+        }
+        for (int b = 0; b < 4; ++b) mbar_init(bar(SCALES_FULL + b), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::TMEM), "r"(L::TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *(volatile uint32_t *)(aligned + L::TMEM);
+    pdl_wait();
+
+    int k_first, k_hi;                                  // keys that this CTA's rows may see in its slice
+    q8_slice(t, p.slices, slice, BN, k_first, k_hi);
+    const int k_lo = k_first / BN * BN;
+    const int n_tiles = k_hi > k_first ? (k_hi - k_lo + BN - 1) / BN : 0;
+    // row tile A ends earlier: it skips the key tiles beyond its last row
+    const int rows_a = min(t.rows, BM);
+    const bool has_b = HALVES || t.rows > BM;
+    const int k_hi_a = HALVES ? k_hi : min(t.pos_begin + (t.row0 + rows_a - 1) / t.G + 1, k_hi);
+    const int n_tiles_a = HALVES ? (n_tiles + 1) / 2 : k_hi_a > k_lo ? min(n_tiles, (k_hi_a - k_lo + BN - 1) / BN) : 0;
+
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+        convert<HD, 4, false>(p, t, kvh, p.v, warp - 12, lane, k_lo, n_tiles, base, L::V, V_FULL, V_EMPTY, 4);
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+        if (warp == 9) {
+            convert<HD, 3, true>(p, t, kvh, p.k, 0, lane, k_lo, n_tiles, base, L::K, K_FULL, K_EMPTY, 3);
+        } else if (warp > 9) {
+            convert<HD, 3, false>(p, t, kvh, p.k, warp - 9, lane, k_lo, n_tiles, base, L::K, K_FULL, K_EMPTY, 3);
+        } else if (lane == 0 && n_tiles > 0) {
+            // ---- issuer
+            bool ok = mbar_wait(bar(Q_FULL), 0);
+            if (!ok) atomicExch(&g_q8t_error, 5);
+            auto issue_s = [&](int x, int i) {
+                const uint32_t q = base + L::Q + (HALVES ? 0 : x * L::TILE), k = base + L::K + (i & 1) * L::TILE;
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks) {
+                    const uint32_t off = (ks >> 2) * L::PANEL + (ks & 3) * 32;
+                    tc_mma(tmem + x * 128, smem_desc(q + off), smem_desc(k + off), IDESC_S, ks > 0 ? 1u : 0u);
+                }
+                tc_commit(bar(S_FULL + x));
+            };
+            auto issue_pv = [&](int x, int i) {
+                if (!mbar_wait(bar(P_FULL + x), (uint32_t)(HALVES ? i >> 1 : i) & 1u)) { atomicExch(&g_q8t_error, 2); return false; }
+                tc_fence_after();
+#pragma unroll
+                for (int ks = 0; ks < BN / 16; ++ks)
+                    // A = P: keys 16 ks.. are columns 8 ks..; B = V: 16 keys down = 2 groups of 8 rows
+                    mma_ts(tmem + L::O + x * 128, tmem + x * 128 + ks * 8, smem_desc_mn_major(base + L::V + (i & 1) * L::TILE + ks * 2048, L::PANEL), IDESC_PV,
+                           (i > (HALVES ? 1 : 0) || ks > 0) ? 1u : 0u);
+                tc_commit(bar(PV_DONE + x));
+                return true;
+            };
+            auto wait_k = [&](int i) {
+                if (mbar_wait(bar(K_FULL + (i & 1)), (uint32_t)(i >> 1) & 1u)) { tc_fence_after(); return true; }
+                atomicExch(&g_q8t_error, 1);
+                return false;
+            };
+            auto wait_v = [&](int i) {
+                if (mbar_wait(bar(V_FULL + (i & 1)), (uint32_t)(i >> 1) & 1u)) { tc_fence_after(); return true; }
+                atomicExch(&g_q8t_error, 6);
+                return false;
+            };
+            if (HALVES) {
+                // per stream: S(i) | PV(i), S(i + 2); tile i is stream i % 2's step i / 2, and so is its stage
+                for (int i = 0; i < min(2, n_tiles) && ok; ++i) {
+                    if (!(ok = wait_k(i))) break;
+                    issue_s(i, i);
+                    tc_commit(bar(K_EMPTY + i));
+                }
+                for (int i = 0; i < n_tiles && ok; ++i) {
+                    const int x = i & 1;
+                    if (!(ok = wait_v(i)) || !(ok = issue_pv(x, i))) break;
+                    tc_commit(bar(V_EMPTY + x));
+                    if (i + 2 < n_tiles) {
+                        if (!(ok = wait_k(i + 2))) break;
+                        issue_s(x, i + 2);
+                        tc_commit(bar(K_EMPTY + x));
+                    }
+                }
+            } else {
+                if (ok && (ok = wait_k(0))) {
+                    if (n_tiles_a > 0) issue_s(0, 0);
+                    if (has_b) issue_s(1, 0);
+                    tc_commit(bar(K_EMPTY + 0));
+                }
+                for (int i = 0; i < n_tiles && ok; ++i) {
+                    const bool next = i + 1 < n_tiles;
+                    if (!(ok = wait_v(i))) break;
+                    if (next && !(ok = wait_k(i + 1))) break;
+                    // PV_A(i), S_A(i+1), PV_B(i), S_B(i+1): the products of one row tile fill the time the other's softmax takes
+                    if (i < n_tiles_a && !(ok = issue_pv(0, i))) break;
+                    if (next && i + 1 < n_tiles_a) issue_s(0, i + 1);
+                    if (has_b && !(ok = issue_pv(1, i))) break;
+                    if (next && has_b) issue_s(1, i + 1);
+                    if (next) tc_commit(bar(K_EMPTY + ((i + 1) & 1)));
+                    tc_commit(bar(V_EMPTY + (i & 1)));
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
+        // ---- softmax: thread r of a row tile owns row r (TMEM lane r)
+        const int x = warp >> 2, r = tid & 127;
+        float *row_up = reinterpret_cast<float *>(aligned + L::ROWS);
+        {
+            // Queries, in float16: a row is multiplied by the power of two that brings its largest number to [64, 128), so that a bfloat16
+            // number keeps its bits down to 2^-21 of that, and the rest is off by 2^-31 of it.  LPR lanes hold a row, 8 numbers each.
+            constexpr int LPR = HD / 8, RPT = LPR / 2;          // 256 threads take 512 / LPR .. rows of a tile each
+            const int ld_c = tid % LPR, ld_r0 = tid / LPR * RPT;
+#pragma unroll
+            for (int xt = 0; xt < (HALVES ? 1 : 2); ++xt) {
+                uint4 v[RPT];
+#pragma unroll
+                for (int j = 0; j < RPT; ++j) {
+                    const int rr = xt * BM + ld_r0 + j;
+                    v[j] = make_uint4(0, 0, 0, 0);
+                    if (rr < t.rows) v[j] = *reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)p.q + q8_out_row(p, t, kvh, rr) * HD + 8 * ld_c);
+                }
+#pragma unroll
+                for (int j = 0; j < RPT; ++j) {
+                    const uint32_t u[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+                    uint32_t big = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) big = max(big, max(u[e] & 0x7fffu, (u[e] >> 16) & 0x7fffu));
+#pragma unroll
+                    for (int o = LPR / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+                    const int e = (int)(big >> 7);              // biased exponent of the largest; 255: not finite, as it is
+                    const int up = big == 0 || e == 255 ? 0 : 127 + 6 - max(e, 63);      // (below 2^-64 nothing weighs)
+                    const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+                    uint32_t h[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) h[k] = pack_f16(__uint_as_float(u[k] << 16) * f, __uint_as_float(u[k] & 0xffff0000u) * f);
+                    sts128(base + L::Q + xt * L::TILE + (ld_c >> 3) * L::PANEL + swizzle128(ld_r0 + j, ld_c & 7), make_uint4(h[0], h[1], h[2], h[3]));
+                    if (ld_c == 0) row_up[xt * BM + ld_r0 + j] = __uint_as_float((uint32_t)(127 - up) << 23);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(Q_FULL));
+            asm volatile("bar.sync 1, 256;" ::: "memory");      // the rows' powers
+        }
+        const int tile_row = HALVES ? t.row0 : t.row0 + x * BM;
+        const int rows_x = x == 0 || HALVES ? rows_a : t.rows - BM;                // rows of this row tile (<= 0: none)
+        const int n_tiles_x = x == 0 ? n_tiles_a : HALVES ? n_tiles / 2 : (has_b ? n_tiles : 0);
+        const int k_hi_x = x == 0 ? k_hi_a : k_hi;
+        const bool row_ok = r < rows_x;
+        const int my_pos = row_ok ? t.pos_begin + (tile_row + r) / t.G : -1;
+        // the keys that this row sees in this slice: [see_lo, see_hi)
+        const int see_lo = max(k_first, p.window > 0 ? my_pos - p.window + 1 : 0), see_hi = min(my_pos + 1, k_hi_x);
+        const float row_scale = row_up[HALVES ? r : x * BM + r] * p.scale * 1.4426950408889634f;
+        // warps none of whose 32 rows exist skip the arithmetic
+        const bool warp_has_rows = 32 * (warp & 3) < rows_x;
+        const uint32_t lane_base = ((uint32_t)(32 * (warp & 3))) << 16;
+        const uint32_t s_addr = tmem + lane_base + x * 128, o_addr = tmem + lane_base + L::O + x * 128;
+        float m_ref = -INFINITY, l_run = 0.f;       // the reference the output is accumulated against, and the row's sum
+        bool ok = true;             // after a wait gave up the loop runs on without waiting, so that the warps still meet
+
+        for (int step = 0; step < n_tiles_x; ++step) {
+            const int i = HALVES ? 2 * step + x : step;
+            const int kbase = k_lo + i * BN;
+            // S_X(i) is done - and with it, in the issuer's order, O_X += P_X V of the step before
+            if (ok && !mbar_wait(bar(S_FULL + x), (uint32_t)step & 1u)) { atomicExch(&g_q8t_error, 7); ok = false; }
+            if (ok && !mbar_wait(bar(SCALES_FULL + (i & 3)), (uint32_t)(i >> 2) & 1u)) { atomicExch(&g_q8t_error, 10); ok = false; }
+            tc_fence_after();
+            if (warp_has_rows) {
+                const uint4 *scales = reinterpret_cast<const uint4 *>(aligned + L::SCALES) + (i & 3) * BLOCKS;      // (s_k, log2 s_v, 1 / s_v)
+                uint32_t sr[BN];
+#pragma unroll
+                for (int c = 0; c < BN; c += 32) ld32(s_addr + c, sr + c);
+                ld_wait();
+                const bool whole = __all_sync(0xffffffffu, kbase >= see_lo && kbase + BN <= see_hi);
+                if (!whole) {
+                    // keys this row may not see count as minus infinity
+#pragma unroll
+                    for (int j = 0; j < BN; ++j)
+                        if (kbase + j < see_lo || kbase + j >= see_hi) sr[j] = 0xff800000u;
+                }
+                // a block of which the row sees nothing has no scales, whatever they are
+                auto block = [&](int b, float &ck, float &lv, float &rv) {
+                    const uint4 s = scales[b];
+                    ck = __uint_as_float(s.x) * row_scale;
+                    lv = __uint_as_float(s.y);
+                    rv = __uint_as_float(s.z);
+                    if (!whole && (kbase + 16 * b + 15 < see_lo || kbase + 16 * b >= see_hi)) ck = 1.f, lv = rv = 0.f;
+                };
+                float mx = -INFINITY;
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) {
+                    float ck, lv, rv, m2[2] = {-INFINITY, -INFINITY};
+                    block(b, ck, lv, rv);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        m2[0] = max3(m2[0], __uint_as_float(sr[16 * b + j]), __uint_as_float(sr[16 * b + j + 1]));
+                        m2[1] = max3(m2[1], __uint_as_float(sr[16 * b + j + 2]), __uint_as_float(sr[16 * b + j + 3]));
+                    }
+                    mx = fmaxf(mx, fmaf(fmaxf(m2[0], m2[1]), ck, lv));
+                }
+                float alpha = 1.f;
+                if (mx > m_ref + STEP || (m_ref == -INFINITY && mx > -INFINITY)) {
+                    if (m_ref != -INFINITY) alpha = exp2_fast(m_ref - mx);
+                    m_ref = mx;
+                }
+                l_run *= alpha;
+                const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+                // P over this row's own scores; a block is stored while the next is computed
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) {
+                    float ck, lv, rv;
+                    block(b, ck, lv, rv);
+                    const uint64_t scale2 = pack2(ck, ck), shift2 = pack2(lv - m_use, lv - m_use);
+                    uint64_t l2[2] = {0ull, 0ull};
+                    uint32_t w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        float x0, x1;
+                        unpack2(fma2(pack2(__uint_as_float(sr[16 * b + 2 * j]), __uint_as_float(sr[16 * b + 2 * j + 1])), scale2, shift2), x0, x1);
+                        const float e0 = exp2_fast(x0), e1 = exp2_fast(x1);
+                        l2[j & 1] = add2(l2[j & 1], pack2(e0, e1));
+                        w[j] = pack_f16(e0, e1);
+                    }
+                    st8(s_addr + 8 * b, w);
+                    float a0, a1;
+                    unpack2(add2(l2[0], l2[1]), a0, a1);
+                    l_run = fmaf(a0 + a1, rv, l_run);
+                }
+                if (__any_sync(0xffffffffu, alpha != 1.f)) {
+                    // the whole warp walks its rows' outputs; rows whose reference stays are multiplied by one.  O_X is idle: its last
+                    // product is done.
+#pragma unroll
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t o[32];
+                        ld32(o_addr + c, o);
+                        ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 8) st8(o_addr + c + j, o + j);
+                    }
+                }
+                st_wait();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(P_FULL + x));
+        }
+
+        // the last product of this row tile
+        if (n_tiles_x > 0 && ok && !mbar_wait(bar(PV_DONE + x), (uint32_t)(n_tiles_x - 1) & 1u)) { atomicExch(&g_q8t_error, 9); ok = false; }
+        tc_fence_after();
+        const bool write = row_ok && ok;
+        const size_t qrow = write ? (size_t)(t.tok_begin + (tile_row + r) / t.G) * p.nq + kvh * t.G + (tile_row + r) % t.G : 0;
+        // columns [c0, c0 + 32) of the row's output
+        auto put = [&](int c0, const uint32_t *o, float inv) {
+            if (p.slices > 1) {
+                float *po = p.part_o + (qrow * p.slices + slice) * HD + c0;
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4 *>(po + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            } else {
+                __nv_bfloat16 *po = (__nv_bfloat16 *)p.out + qrow * HD + c0;
+#pragma unroll
+                for (int j = 0; j < 32; j += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const __nv_bfloat162 b2 = __floats2bfloat162_rn(__uint_as_float(o[j + 2 * k]) * inv, __uint_as_float(o[j + 2 * k + 1]) * inv);
+                        w[k] = *reinterpret_cast<const uint32_t *>(&b2);
+                    }
+                    *reinterpret_cast<uint4 *>(po + j) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+        };
+        if (HALVES) {
+            // both streams' last products, then the two states of a row as one: the threads of A take the first half of the columns
+            const int n_other = x == 0 ? n_tiles / 2 : n_tiles_a;
+            if (n_other > 0 && ok && !mbar_wait(bar(PV_DONE + (x ^ 1)), (uint32_t)(n_other - 1) & 1u)) { atomicExch(&g_q8t_error, 9); ok = false; }
+            tc_fence_after();
+            float m_a = -INFINITY, l_a = 0.f, m_b = -INFINITY, l_b = 0.f;
+            if (n_tiles > 0) {
+                float2 *meet = reinterpret_cast<float2 *>(aligned + L::Q);          // Q's memory: every product that read it is done
+                meet[x * 128 + r] = make_float2(m_ref, l_run);
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                m_a = meet[r].x, l_a = meet[r].y, m_b = meet[128 + r].x, l_b = meet[128 + r].y;
+            }
+            const float m = fmaxf(m_a, m_b), f_a = m_a == -INFINITY ? 0.f : exp2_fast(m_a - m), f_b = m_b == -INFINITY ? 0.f : exp2_fast(m_b - m);
+            // (a sum that is no number stays that)
+            const float l = (f_a == 0.f && l_a == l_a ? 0.f : l_a * f_a) + (f_b == 0.f && l_b == l_b ? 0.f : l_b * f_b);
+            if (warp_has_rows) {
+#pragma unroll
+                for (int c = 0; c < HD / 2; c += 32) {
+                    const int c0 = x * (HD / 2) + c;
+                    uint32_t oa[32], ob[32];
+                    ld32(tmem + lane_base + L::O + c0, oa);             // warp-wide, whatever rows exist
+                    ld32(tmem + lane_base + L::O + 128 + c0, ob);
+                    ld_wait();
+                    if (!write) continue;
+                    // a stream without a tile has left its columns as they were: not a number, perhaps
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        oa[j] = __float_as_uint((n_tiles > 0 ? __uint_as_float(oa[j]) * f_a : 0.f) + (n_tiles > 1 ? __uint_as_float(ob[j]) * f_b : 0.f));
+                    put(c0, oa, 1.0f / l);
+                }
+                if (write && p.slices > 1 && x == 0) *reinterpret_cast<float2 *>(p.part_ml + (qrow * p.slices + slice) * 2) = make_float2(m, l);
+            }
+        } else if (warp_has_rows) {
+#pragma unroll
+            for (int c = 0; c < HD; c += 32) {
+                uint32_t o[32];
+                if (n_tiles_x > 0) {
+                    ld32(o_addr + c, o);                // warp-wide, whatever rows exist
+                    ld_wait();
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] = 0u;
+                }
+                if (write) put(c, o, 1.0f / l_run);
+            }
+            if (write && p.slices > 1) *reinterpret_cast<float2 *>(p.part_ml + (qrow * p.slices + slice) * 2) = make_float2(m_ref, l_run);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM_COLS) : "memory");
+    }
+}
+
+template <int HD, bool HALVES>
+int launch_tc(const Q8Params &p, int tiles, cudaStream_t stream) {
+    constexpr int smem = Lay<HD>::BYTES + 1024;
+    // the registers dealt out inside are those of the launch: with fewer the softmax groups would wait for the difference
+    static const int regs = [] {
+        cudaFuncAttributes a;
+        return cudaFuncGetAttributes(&a, attention_q8_tc_kernel<HD, HALVES>) == cudaSuccess ? a.numRegs : 0;
+    }();
+    KESTREL_REQUIRE(regs * THREADS >= 256 * (SOFTMAX_REGS + OTHER_REGS), "attention_q8: the kernel was built with %d registers a thread, %d are dealt out", regs,
+                    (SOFTMAX_REGS + OTHER_REGS) / 2);
+    if (cudaFuncSetAttribute(attention_q8_tc_kernel<HD, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return kestrel_fail(-3, "attention_q8: cannot raise the shared-memory limit: %s", cudaGetErrorString(cudaGetLastError()));
+    kestrel_launch(attention_q8_tc_kernel<HD, HALVES>, dim3((unsigned)tiles * p.nkv, 1, p.slices), dim3(THREADS), smem, stream, p);
+    return kestrel_check_launch("attention_q8 tc");
+}
+
+}  // namespace
+
+int q8_launch_tc(const Q8Params &p, int tiles, cudaStream_t stream) {
+    if (p.rows_per_tile <= BM) return p.hd == 64 ? launch_tc<64, true>(p, tiles, stream) : launch_tc<128, true>(p, tiles, stream);
+    return p.hd == 64 ? launch_tc<64, false>(p, tiles, stream) : launch_tc<128, false>(p, tiles, stream);
+}
+
+int q8_tc_error() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_q8t_error, sizeof(int)) != cudaSuccess) return -1;
+    if (v) cudaMemcpyToSymbol(g_q8t_error, &zero, sizeof(int));
+    return v;
+}
