@@ -428,7 +428,8 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                     }
                 }
                 const float *sc = reinterpret_cast<const float *>(ring + R::SCALES + stage * 32);
-                const float sk = sc[warp], sv = sc[4 + warp];
+                // zero counts as 2^-100; what is no number stays that
+                const float sk = sc[warp] < 7.9e-31f ? 7.9e-31f : sc[warp], sv = sc[4 + warp] < 7.9e-31f ? 7.9e-31f : sc[4 + warp];
                 const float lv = log2_fast(sv), rv = rcp_fast(sv);
                 if (kbase >= w.k_first && kbase + 16 <= w.k_end && kbase + 15 <= min_pos && kbase >= max_low) {
                     weigh<NT, false>(s, o, m, l, row_scale, sk, lv, rv, kbase, my_key, pos, low);

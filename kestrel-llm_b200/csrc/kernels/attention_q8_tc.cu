@@ -6,10 +6,10 @@
 //   warps 0-3, 4-7   softmax of A and of B: a thread owns a row, its 128 scores in registers; P goes back over S in TMEM as float16;
 //   warp 8           one thread issues S_X = Q_X K^T and O_X += P_X V, tcgen05.mma M = 128, N = 128 (N = head size), in the order
 //                    S_A S_B | PV_A S_A' PV_B S_B' | ..., so that one row tile is multiplied while the other is softmaxed;
-//   warps 9-11       read the codes of K from the cache, 16 bytes a lane, widen them to float16 in registers and write them to shared
-//                    memory in the swizzled layout of an operand, two stages ahead of the products at most; one lane in eight of warp 9
-//                    brings a block's scales along;
-//   warps 12-15      the same for V.
+//   warps 10-12      read the codes of K from the cache, 16 bytes a lane, widen them to float16 in registers and write them to shared
+//                    memory in the swizzled layout of an operand, two stages ahead of the products at most; eight lanes of warp 10 bring
+//                    the blocks' scales along;
+//   warps 13-15      the same for V.
 // A code is widened as the low byte of the float16 number 1024 + (c + 128), less 1152: a permutation for two codes and a subtraction of
 // pairs.  Reading codes and not 16-bit numbers halves what a CTA fetches; the widening, 32,768 codes a key tile, takes some 1,800 of the
 // four schedulers' issue slots, beside 4,100 of the softmax and 2,048 cycles of products at head size 128.
@@ -18,8 +18,7 @@
 // Scores enter the softmax as x = s * ck + lv with ck = (the key's scale) * (the row's), lv = log2 of the value's scale, both the same for
 // 16 keys: the maximum is taken per block before the scales, and the exponent is one multiply-add as without them.  The sum of a block's
 // weights is divided by its value's scale once.  The output accumulates in TMEM against a reference that moves only when a row's maximum
-// has outgrown it by 8.  Codes are numbers whatever a stale page holds, so nothing has to be cleared; a block that a row sees nothing of
-// counts as without scales.
+// has outgrown it by 8.  Codes are numbers whatever a stale page holds, so nothing has to be cleared.
 //
 // HALVES: a CTA with one row tile (up to 128 rows), whose even key tiles go to stream A and odd ones to B, over the same queries; the rows'
 // two states are merged at the end.  Every wait is bounded.
@@ -128,14 +127,14 @@ __device__ __forceinline__ uint4 widen(uint32_t a, uint32_t b) {
                       hsub2(__byte_perm(b, MAGIC, 0x4140)), hsub2(__byte_perm(b, MAGIC, 0x4342)));
 }
 
-// One plane's widening, by WARPS warps of which this is the w-th: key tiles of 128 into a ring of two stages at `ring`.  A warp's load is
+// One plane's widening, by three warps of which this is the w-th: key tiles of 128 into a ring of two stages at `ring`.  A warp's load is
 // one unit: 512 bytes, 4 keys at head size 128 and 8 at 64; a quarter-warp's stores of 16 bytes go to two keys and every other chunk, which
-// the swizzle spreads over all banks.
-template <int HD, int WARPS, bool SCALED>
-__device__ __forceinline__ void convert(const Q8Params &p, const Q8Tile &t, int kvh, const int8_t *plane, int w, int lane, int k_lo, int n_tiles,
+// the swizzle spreads over all banks.  Both planes' warps run the same instructions: with a copy for each the kernel waited for its code.
+template <int HD>
+__device__ __forceinline__ void convert(const Q8Params &p, const Q8Tile &t, int kvh, const int8_t *plane, int w, bool scaled, int lane, int k_lo, int n_tiles,
                                         uint32_t base, uint32_t ring, int full0, int empty0, int error) {
     using L = Lay<HD>;
-    constexpr int KEYS = 512 / HD, UNITS = BN / KEYS, MINE = (UNITS + WARPS - 1) / WARPS;
+    constexpr int KEYS = 512 / HD, UNITS = BN / KEYS, MINE = (UNITS + 2) / 3;
     auto bar = [&](int i) { return base + L::BARRIERS + 8u * (uint32_t)i; };
     const int key = HD == 128 ? (lane >> 2) & 3 : lane >> 2, chunk = HD == 128 ? (lane & 3) + 4 * (lane >> 4) : lane & 3;
     // lane l < 8 knows the cache row of a tile's l-th block
@@ -145,31 +144,35 @@ __device__ __forceinline__ void convert(const Q8Params &p, const Q8Tile &t, int 
     auto fetch = [&](int rows) {
 #pragma unroll
         for (int u = 0; u < MINE; ++u) {
-            const int k = (w + u * WARPS) * KEYS;           // the unit's first key of the tile
+            const int k = (w + u * 3) * KEYS;               // the unit's first key of the tile
             const int row = __shfl_sync(0xffffffffu, rows, (k / Q8_BLOCK) & 7) + k % Q8_BLOCK + key;
-            if (w + u * WARPS < UNITS) q[u] = ldg128(plane + (size_t)row * HD + 16 * chunk);
+            if (w + u * 3 < UNITS) q[u] = ldg128(plane + (size_t)row * HD + 16 * chunk);
         }
-        if (SCALED && lane < BLOCKS) sk = p.ks[rows / Q8_BLOCK], sv = p.vs[rows / Q8_BLOCK];
+        if (scaled && lane < BLOCKS) sk = p.ks[rows / Q8_BLOCK], sv = p.vs[rows / Q8_BLOCK];
     };
     int ahead = rows_of(0);
-    if (n_tiles > 0) fetch(ahead);
+    fetch(ahead);
     ahead = rows_of(1);
     for (int i = 0; i < n_tiles; ++i) {
         const int b = i & 1;
         if (!mbar_wait(bar(empty0 + b), (uint32_t)((i >> 1) + 1) & 1u)) { atomicExch(&g_q8t_error, error); break; }
-        const uint32_t stage = base + ring + b * L::TILE;
+        const uint32_t stage = base + ring + b * L::TILE + (uint32_t)(chunk >> 2) * L::PANEL;
 #pragma unroll
         for (int u = 0; u < MINE; ++u) {
-            if (w + u * WARPS >= UNITS) break;
-            const int k = (w + u * WARPS) * KEYS + key;
-            const uint32_t panel = stage + (uint32_t)(chunk >> 2) * L::PANEL;
-            sts128(panel + swizzle128(k, 2 * (chunk & 3)), widen(q[u].x, q[u].y));
-            sts128(panel + swizzle128(k, 2 * (chunk & 3) + 1), widen(q[u].z, q[u].w));
+            if (w + u * 3 >= UNITS) break;
+            const int k = (w + u * 3) * KEYS + key;
+            sts128(stage + swizzle128(k, 2 * (chunk & 3)), widen(q[u].x, q[u].y));
+            sts128(stage + swizzle128(k, 2 * (chunk & 3) + 1), widen(q[u].z, q[u].w));
         }
-        if (SCALED) {
+        if (scaled) {
             // Slot i % 4 is free: tile i's stage was, so S(i - 2) is done, before which every thread was through with tile i - 4.
+            // A scale that is no positive number becomes one that makes the sum of a row that sees the block no number, and no other's:
+            // the weights of such a row come out as 2^0 against a reference that nothing else reaches, and 1 / s_v is NaN.
+            const bool bad = !(sk >= 0.f && sk <= 3.4e38f && sv >= 0.f && sv <= 3.4e38f);
+            const float k = bad ? 1e-30f : fmaxf(sk, 7.9e-31f), v = fmaxf(sv, 7.9e-31f);      // zero counts as 2^-100
             if (lane < BLOCKS)
-                sts128(base + L::SCALES + ((i & 3) * BLOCKS + lane) * 16, make_uint4(__float_as_uint(sk), __float_as_uint(log2_fast(sv)), __float_as_uint(1.0f / sv), 0));
+                sts128(base + L::SCALES + ((i & 3) * BLOCKS + lane) * 16, make_uint4(__float_as_uint(k), __float_as_uint(bad ? 3e4f : log2_fast(v)),
+                                                                                     bad ? 0x7fc00000u : __float_as_uint(1.0f / v), 0));
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(SCALES_FULL + (i & 3)));
         }
@@ -205,7 +208,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
         mbar_init(bar(Q_FULL), 8);
         for (int b = 0; b < 2; ++b) {
             mbar_init(bar(K_FULL + b), 3);  mbar_init(bar(K_EMPTY + b), 1);
-            mbar_init(bar(V_FULL + b), 4);  mbar_init(bar(V_EMPTY + b), 1);
+            mbar_init(bar(V_FULL + b), 3);  mbar_init(bar(V_EMPTY + b), 1);
             mbar_init(bar(S_FULL + b), 1);  mbar_init(bar(P_FULL + b), 4);
             mbar_init(bar(PV_DONE + b), 1);
         }
@@ -232,16 +235,14 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
     const int k_hi_a = HALVES ? k_hi : min(t.pos_begin + (t.row0 + rows_a - 1) / t.G + 1, k_hi);
     const int n_tiles_a = HALVES ? (n_tiles + 1) / 2 : k_hi_a > k_lo ? min(n_tiles, (k_hi_a - k_lo + BN - 1) / BN) : 0;
 
-    if (warp >= 12) {
+    if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-        convert<HD, 4, false>(p, t, kvh, p.v, warp - 12, lane, k_lo, n_tiles, base, L::V, V_FULL, V_EMPTY, 4);
-    } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-        if (warp == 9) {
-            convert<HD, 3, true>(p, t, kvh, p.k, 0, lane, k_lo, n_tiles, base, L::K, K_FULL, K_EMPTY, 3);
-        } else if (warp > 9) {
-            convert<HD, 3, false>(p, t, kvh, p.k, warp - 9, lane, k_lo, n_tiles, base, L::K, K_FULL, K_EMPTY, 3);
-        } else if (lane == 0 && n_tiles > 0) {
+        if (warp >= 10) {
+            const bool is_v = warp >= 13;
+            if (n_tiles > 0)
+                convert<HD>(p, t, kvh, is_v ? p.v : p.k, is_v ? warp - 13 : warp - 10, warp == 10, lane, k_lo, n_tiles, base, is_v ? L::V : L::K,
+                            is_v ? V_FULL : K_FULL, is_v ? V_EMPTY : K_EMPTY, is_v ? 4 : 3);
+        } else if (warp == 8 && lane == 0 && n_tiles > 0) {
             // ---- issuer
             bool ok = mbar_wait(bar(Q_FULL), 0);
             if (!ok) atomicExch(&g_q8t_error, 5);
@@ -391,25 +392,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
                     for (int j = 0; j < BN; ++j)
                         if (kbase + j < see_lo || kbase + j >= see_hi) sr[j] = 0xff800000u;
                 }
-                // a block of which the row sees nothing has no scales, whatever they are
-                auto block = [&](int b, float &ck, float &lv, float &rv) {
-                    const uint4 s = scales[b];
-                    ck = __uint_as_float(s.x) * row_scale;
-                    lv = __uint_as_float(s.y);
-                    rv = __uint_as_float(s.z);
-                    if (!whole && (kbase + 16 * b + 15 < see_lo || kbase + 16 * b >= see_hi)) ck = 1.f, lv = rv = 0.f;
-                };
                 float mx = -INFINITY;
 #pragma unroll
                 for (int b = 0; b < BLOCKS; ++b) {
-                    float ck, lv, rv, m2[2] = {-INFINITY, -INFINITY};
-                    block(b, ck, lv, rv);
+                    const uint4 sc = scales[b];
+                    float m2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                     for (int j = 0; j < 16; j += 4) {
                         m2[0] = max3(m2[0], __uint_as_float(sr[16 * b + j]), __uint_as_float(sr[16 * b + j + 1]));
                         m2[1] = max3(m2[1], __uint_as_float(sr[16 * b + j + 2]), __uint_as_float(sr[16 * b + j + 3]));
                     }
-                    mx = fmaxf(mx, fmaf(fmaxf(m2[0], m2[1]), ck, lv));
+                    mx = fmaxf(mx, fmaf(fmaxf(m2[0], m2[1]), __uint_as_float(sc.x) * row_scale, __uint_as_float(sc.y)));
                 }
                 float alpha = 1.f;
                 if (mx > m_ref + STEP || (m_ref == -INFINITY && mx > -INFINITY)) {
@@ -421,9 +414,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
                 // P over this row's own scores; a block is stored while the next is computed
 #pragma unroll
                 for (int b = 0; b < BLOCKS; ++b) {
-                    float ck, lv, rv;
-                    block(b, ck, lv, rv);
-                    const uint64_t scale2 = pack2(ck, ck), shift2 = pack2(lv - m_use, lv - m_use);
+                    const uint4 sc = scales[b];
+                    const float ck = __uint_as_float(sc.x) * row_scale, shift = __uint_as_float(sc.y) - m_use;
+                    const uint64_t scale2 = pack2(ck, ck), shift2 = pack2(shift, shift);
                     uint64_t l2[2] = {0ull, 0ull};
                     uint32_t w[8];
 #pragma unroll
@@ -437,7 +430,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
                     st8(s_addr + 8 * b, w);
                     float a0, a1;
                     unpack2(add2(l2[0], l2[1]), a0, a1);
-                    l_run = fmaf(a0 + a1, rv, l_run);
+                    if (a0 + a1 != 0.f) l_run = fmaf(a0 + a1, __uint_as_float(sc.z), l_run);      // (nothing seen: whatever the scale is)
                 }
                 if (__any_sync(0xffffffffu, alpha != 1.f)) {
                     // the whole warp walks its rows' outputs; rows whose reference stays are multiplied by one.  O_X is idle: its last
