@@ -2,18 +2,20 @@
 // Formulas in attention_q8.cuh.
 //
 // A CTA owns up to 256 rows - (token, query head of one kv group) pairs, token-major - as two row tiles A and B of 128, and walks the keys
-// its rows may see in tiles of 128.  Sixteen warps in four groups, coupled by mbarriers:
+// its rows may see in tiles of 128.  Twenty warps in five groups, coupled by mbarriers:
 //   warps 0-3, 4-7   softmax of A and of B: a thread owns a row, its 128 scores in registers; P goes back over S in TMEM as float16;
 //   warp 8           one thread issues S_X = Q_X K^T and O_X += P_X V, tcgen05.mma M = 128, N = 128 (N = head size), in the order
 //                    S_A S_B | PV_A S_A' PV_B S_B' | ..., so that one row tile is multiplied while the other is softmaxed;
-//   warps 10-12      read the codes of K from the cache, 16 bytes a lane, widen them to float16 in registers and write them to shared
-//                    memory in the swizzled layout of an operand, two stages ahead of the products at most; eight lanes of warp 10 bring
+//   warps 12-15      read the codes of K from the cache, 16 bytes a lane, widen them to float16 in registers and write them to shared
+//                    memory in the swizzled layout of an operand, two stages ahead of the products at most; eight lanes of warp 12 bring
 //                    the blocks' scales along;
-//   warps 13-15      the same for V.
+//   warps 16-19      the same for V.
 // A code is widened as the low byte of the float16 number 1024 + (c + 128), less 1152: a permutation for two codes and a subtraction of
 // pairs.  Reading codes and not 16-bit numbers halves what a CTA fetches; the widening, 32,768 codes a key tile, takes some 1,800 of the
 // four schedulers' issue slots, beside 4,100 of the softmax and 2,048 cycles of products at head size 128.
-// The softmax groups hold 184 registers a thread, the others 72: what the 512 threads were launched with, dealt out again.
+// The softmax groups hold 176 registers a thread, the others 40: what the 640 threads were launched with, dealt out again.  The roles share
+// the SM's instruction caches, and the softmax is long, so the others are loops of a hundred instructions: with its eight products and their
+// descriptors unrolled the issuing thread took 3,000 cycles for products of 64 each to have its code fetched.
 //
 // Scores enter the softmax as x = s * ck + lv with ck = (the key's scale) * (the row's), lv = log2 of the value's scale, both the same for
 // 16 keys: the maximum is taken per block before the scales, and the exponent is one multiply-add as without them.  The sum of a block's
@@ -31,8 +33,8 @@ __device__ int g_q8t_error = 0;
 
 namespace {
 
-constexpr int THREADS = 512, BM = 128, BN = 128, BLOCKS = BN / Q8_BLOCK;
-constexpr int SOFTMAX_REGS = 184, OTHER_REGS = 72;      // 2 x 128 threads each: 65,536 in all, the launch's 512 x 128
+constexpr int THREADS = 640, BM = 128, BN = 128, BLOCKS = BN / Q8_BLOCK;
+constexpr int SOFTMAX_REGS = 176, OTHER_REGS = 40;      // of 256 and of 384 threads: 60,416 in all; the launch has 640 x 96
 constexpr uint32_t MAGIC = 0x64646464u;
 constexpr float STEP = 8.0f;                            // log2 units by which a row's maximum may outgrow its reference
 
@@ -98,9 +100,13 @@ __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t *r) {
         : "r"(taddr));
 }
 __device__ __forceinline__ void ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void st8(uint32_t taddr, const uint32_t *r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+// 16 packed words into 16 consecutive TMEM columns of this thread's lane
+__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
 }
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // D (TMEM) = or += A (TMEM, M x 16 packed two to a column) x B (shared memory)
@@ -127,42 +133,49 @@ __device__ __forceinline__ uint4 widen(uint32_t a, uint32_t b) {
                       hsub2(__byte_perm(b, MAGIC, 0x4140)), hsub2(__byte_perm(b, MAGIC, 0x4342)));
 }
 
-// One plane's widening, by three warps of which this is the w-th: key tiles of 128 into a ring of two stages at `ring`.  A warp's load is
-// one unit: 512 bytes, 4 keys at head size 128 and 8 at 64; a quarter-warp's stores of 16 bytes go to two keys and every other chunk, which
-// the swizzle spreads over all banks.  Both planes' warps run the same instructions: with a copy for each the kernel waited for its code.
+// One plane's widening, by four warps of which this is the w-th: key tiles of 128 into a ring of two stages at `ring`.  A warp's load is one
+// unit: 512 bytes, 4 keys at head size 128 and 8 at 64.  A warp always has four units in flight: once one is widened the load of the fourth
+// after it starts, over the tiles' borders.  A quarter-warp's stores of 16 bytes go to two keys and every other chunk, which the swizzle
+// spreads over all banks.  Both planes' warps run the same instructions: with a copy for each, and all of a tile unrolled, the kernel
+// waited for its code, and for what did not fit its registers.
 template <int HD>
-__device__ __forceinline__ void convert(const Q8Params &p, const Q8Tile &t, int kvh, const int8_t *plane, int w, bool scaled, int lane, int k_lo, int n_tiles,
+__device__ __forceinline__ void convert(const Q8Params &p, const int *table, int kvh, const int8_t *plane, int w, bool scaled, int lane, int k_lo, int n_tiles,
                                         uint32_t base, uint32_t ring, int full0, int empty0, int error) {
     using L = Lay<HD>;
-    constexpr int KEYS = 512 / HD, UNITS = BN / KEYS, MINE = (UNITS + 2) / 3;
+    constexpr int KEYS = 512 / HD, MINE = BN / KEYS / 4, DEEP = 4;         // units of a tile that are this warp's: 8, or 4
     auto bar = [&](int i) { return base + L::BARRIERS + 8u * (uint32_t)i; };
-    const int key = HD == 128 ? (lane >> 2) & 3 : lane >> 2, chunk = HD == 128 ? (lane & 3) + 4 * (lane >> 4) : lane & 3;
-    // lane l < 8 knows the cache row of a tile's l-th block
-    auto rows_of = [&](int i) { return i < n_tiles ? q8_row_of(p, t.table, kvh, k_lo + i * BN + (lane & 7) * Q8_BLOCK) : 0; };
-    uint4 q[MINE];
-    float sk = 0.f, sv = 1.f;
-    auto fetch = [&](int rows) {
-#pragma unroll
-        for (int u = 0; u < MINE; ++u) {
-            const int k = (w + u * 3) * KEYS;               // the unit's first key of the tile
-            const int row = __shfl_sync(0xffffffffu, rows, (k / Q8_BLOCK) & 7) + k % Q8_BLOCK + key;
-            if (w + u * 3 < UNITS) q[u] = ldg128(plane + (size_t)row * HD + 16 * chunk);
-        }
-        if (scaled && lane < BLOCKS) sk = p.ks[rows / Q8_BLOCK], sv = p.vs[rows / Q8_BLOCK];
+    const int key = w * KEYS + (HD == 128 ? (lane >> 2) & 3 : lane >> 2);                   // among the keys of the four warps' units: 16, or 32
+    const int chunk = HD == 128 ? (lane & 3) + 4 * (lane >> 4) : lane & 3;
+    const uint32_t at0 = base + ring + (uint32_t)(chunk >> 2) * L::PANEL + swizzle128(key, 2 * (chunk & 3));
+    const uint32_t at1 = base + ring + (uint32_t)(chunk >> 2) * L::PANEL + swizzle128(key, 2 * (chunk & 3) + 1);
+    plane += (size_t)(key % Q8_BLOCK) * HD + 16 * chunk;
+    // lane l (modulo 8) knows the cache row of a tile's l-th block
+    auto rows_of = [&](int i) { return i < n_tiles ? q8_row_of(p, table, kvh, k_lo + i * BN + (lane & 7) * Q8_BLOCK) : 0; };
+    auto load = [&](int rows, int u) {
+        const int row = __shfl_sync(0xffffffffu, rows, HD == 128 ? u : 2 * u + (w >> 1));
+        return ldg128(plane + (size_t)row * HD);
     };
-    int ahead = rows_of(0);
-    fetch(ahead);
-    ahead = rows_of(1);
+    int rows = rows_of(0), rows_next = rows_of(1);
+    uint4 q[DEEP];
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u) q[u] = load(rows, u);
+#pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {
         const int b = i & 1;
+        float sk = 0.f, sv = 0.f;
+        if (scaled && lane < BLOCKS) sk = p.ks[rows / Q8_BLOCK], sv = p.vs[rows / Q8_BLOCK];
+        const int rows_after = rows_of(i + 2);
         if (!mbar_wait(bar(empty0 + b), (uint32_t)((i >> 1) + 1) & 1u)) { atomicExch(&g_q8t_error, error); break; }
-        const uint32_t stage = base + ring + b * L::TILE + (uint32_t)(chunk >> 2) * L::PANEL;
+#pragma unroll 1
+        for (int h = 0; h < MINE; h += DEEP) {
 #pragma unroll
-        for (int u = 0; u < MINE; ++u) {
-            if (w + u * 3 >= UNITS) break;
-            const int k = (w + u * 3) * KEYS + key;
-            sts128(stage + swizzle128(k, 2 * (chunk & 3)), widen(q[u].x, q[u].y));
-            sts128(stage + swizzle128(k, 2 * (chunk & 3) + 1), widen(q[u].z, q[u].w));
+            for (int u = 0; u < DEEP; ++u) {
+                const uint32_t off = b * L::TILE + (uint32_t)(h + u) * (4 * KEYS * 128);
+                sts128(at0 + off, widen(q[u].x, q[u].y));
+                sts128(at1 + off, widen(q[u].z, q[u].w));
+                // behind the last tile the rows are 0: a load that nothing waits for
+                q[u] = h + DEEP < MINE ? load(rows, h + DEEP + u) : load(rows_next, u);
+            }
         }
         if (scaled) {
             // Slot i % 4 is free: tile i's stage was, so S(i - 2) is done, before which every thread was through with tile i - 4.
@@ -179,10 +192,8 @@ __device__ __forceinline__ void convert(const Q8Params &p, const Q8Tile &t, int 
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // these writes -> tensor-core reads
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(full0 + b));
-        if (i + 1 < n_tiles) {
-            fetch(ahead);
-            ahead = rows_of(i + 2);
-        }
+        rows = rows_next;
+        rows_next = rows_after;
     }
 }
 
@@ -207,8 +218,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
     if (tid == 0) {
         mbar_init(bar(Q_FULL), 8);
         for (int b = 0; b < 2; ++b) {
-            mbar_init(bar(K_FULL + b), 3);  mbar_init(bar(K_EMPTY + b), 1);
-            mbar_init(bar(V_FULL + b), 3);  mbar_init(bar(V_EMPTY + b), 1);
+            mbar_init(bar(K_FULL + b), 4);  mbar_init(bar(K_EMPTY + b), 1);
+            mbar_init(bar(V_FULL + b), 4);  mbar_init(bar(V_EMPTY + b), 1);
             mbar_init(bar(S_FULL + b), 1);  mbar_init(bar(P_FULL + b), 4);
             mbar_init(bar(PV_DONE + b), 1);
         }
@@ -237,32 +248,41 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-        if (warp >= 10) {
-            const bool is_v = warp >= 13;
+        if (warp >= 12) {
+            const bool is_v = warp >= 16;
             if (n_tiles > 0)
-                convert<HD>(p, t, kvh, is_v ? p.v : p.k, is_v ? warp - 13 : warp - 10, warp == 10, lane, k_lo, n_tiles, base, is_v ? L::V : L::K,
-                            is_v ? V_FULL : K_FULL, is_v ? V_EMPTY : K_EMPTY, is_v ? 4 : 3);
+                convert<HD>(p, t.table, kvh, is_v ? p.v : p.k, warp & 3, warp == 12, lane, k_lo, n_tiles, base, is_v ? L::V : L::K, is_v ? V_FULL : K_FULL,
+                            is_v ? V_EMPTY : K_EMPTY, is_v ? 4 : 3);
         } else if (warp == 8 && lane == 0 && n_tiles > 0) {
             // ---- issuer
             bool ok = mbar_wait(bar(Q_FULL), 0);
             if (!ok) atomicExch(&g_q8t_error, 5);
+            const uint64_t q_desc = smem_desc(base + L::Q), k_desc = smem_desc(base + L::K), v_desc = smem_desc_mn_major(base + L::V, L::PANEL);
             auto issue_s = [&](int x, int i) {
-                const uint32_t q = base + L::Q + (HALVES ? 0 : x * L::TILE), k = base + L::K + (i & 1) * L::TILE;
+                uint64_t dq = q_desc + (HALVES ? 0 : x * (L::TILE >> 4)), dk = k_desc + (i & 1) * (L::TILE >> 4);
+#pragma unroll 1
+                for (int pn = 0; pn < (int)L::PANELS; ++pn) {
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) {
-                    const uint32_t off = (ks >> 2) * L::PANEL + (ks & 3) * 32;
-                    tc_mma(tmem + x * 128, smem_desc(q + off), smem_desc(k + off), IDESC_S, ks > 0 ? 1u : 0u);
+                    for (int ks = 0; ks < 4; ++ks) tc_mma(tmem + x * 128, dq + 2 * ks, dk + 2 * ks, IDESC_S, (pn > 0 || ks > 0) ? 1u : 0u);      // 32 bytes on
+                    dq += L::PANEL >> 4;
+                    dk += L::PANEL >> 4;
                 }
                 tc_commit(bar(S_FULL + x));
             };
             auto issue_pv = [&](int x, int i) {
                 if (!mbar_wait(bar(P_FULL + x), (uint32_t)(HALVES ? i >> 1 : i) & 1u)) { atomicExch(&g_q8t_error, 2); return false; }
                 tc_fence_after();
+                // A = P: keys 16 ks.. are columns 8 ks..; B = V: 16 keys down = 2 groups of 8 rows = 2,048 bytes
+                uint64_t dv = v_desc + (i & 1) * (L::TILE >> 4);
+                uint32_t pa = tmem + x * 128;
+                const bool more = i > (HALVES ? 1 : 0);
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int ks = 0; ks < BN / 16; ++ks)
-                    // A = P: keys 16 ks.. are columns 8 ks..; B = V: 16 keys down = 2 groups of 8 rows
-                    mma_ts(tmem + L::O + x * 128, tmem + x * 128 + ks * 8, smem_desc_mn_major(base + L::V + (i & 1) * L::TILE + ks * 2048, L::PANEL), IDESC_PV,
-                           (i > (HALVES ? 1 : 0) || ks > 0) ? 1u : 0u);
+                    for (int ks = 0; ks < 4; ++ks) mma_ts(tmem + L::O + x * 128, pa + 8 * ks, dv + 128 * ks, IDESC_PV, (more || h > 0 || ks > 0) ? 1u : 0u);
+                    dv += 512;
+                    pa += 32;
+                }
                 tc_commit(bar(PV_DONE + x));
                 return true;
             };
@@ -324,14 +344,16 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
             // number keeps its bits down to 2^-21 of that, and the rest is off by 2^-31 of it.  LPR lanes hold a row, 8 numbers each.
             constexpr int LPR = HD / 8, RPT = LPR / 2;          // 256 threads take 512 / LPR .. rows of a tile each
             const int ld_c = tid % LPR, ld_r0 = tid / LPR * RPT;
-#pragma unroll
+#pragma unroll 1
             for (int xt = 0; xt < (HALVES ? 1 : 2); ++xt) {
                 uint4 v[RPT];
+                int tok = (t.row0 + xt * BM + ld_r0) / t.G, head = (t.row0 + xt * BM + ld_r0) - tok * t.G;
 #pragma unroll
                 for (int j = 0; j < RPT; ++j) {
-                    const int rr = xt * BM + ld_r0 + j;
                     v[j] = make_uint4(0, 0, 0, 0);
-                    if (rr < t.rows) v[j] = *reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)p.q + q8_out_row(p, t, kvh, rr) * HD + 8 * ld_c);
+                    if (xt * BM + ld_r0 + j < t.rows)
+                        v[j] = *reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)p.q + ((size_t)(t.tok_begin + tok) * p.nq + kvh * t.G + head) * HD + 8 * ld_c);
+                    if (++head == t.G) head = 0, ++tok;
                 }
 #pragma unroll
                 for (int j = 0; j < RPT; ++j) {
@@ -381,16 +403,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
             tc_fence_after();
             if (warp_has_rows) {
                 const uint4 *scales = reinterpret_cast<const uint4 *>(aligned + L::SCALES) + (i & 3) * BLOCKS;      // (s_k, log2 s_v, 1 / s_v)
-                uint32_t sr[BN];
-#pragma unroll
-                for (int c = 0; c < BN; c += 32) ld32(s_addr + c, sr + c);
-                ld_wait();
                 const bool whole = __all_sync(0xffffffffu, kbase >= see_lo && kbase + BN <= see_hi);
+                uint32_t a[BN];
+#pragma unroll
+                for (int c = 0; c < BN; c += 32) ld32(s_addr + c, a + c);
+                ld_wait();
                 if (!whole) {
                     // keys this row may not see count as minus infinity
+                    const int lo = see_lo - kbase, hi = see_hi - kbase;
 #pragma unroll
                     for (int j = 0; j < BN; ++j)
-                        if (kbase + j < see_lo || kbase + j >= see_hi) sr[j] = 0xff800000u;
+                        if (j < lo || j >= hi) a[j] = 0xff800000u;
                 }
                 float mx = -INFINITY;
 #pragma unroll
@@ -399,8 +422,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
                     float m2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                     for (int j = 0; j < 16; j += 4) {
-                        m2[0] = max3(m2[0], __uint_as_float(sr[16 * b + j]), __uint_as_float(sr[16 * b + j + 1]));
-                        m2[1] = max3(m2[1], __uint_as_float(sr[16 * b + j + 2]), __uint_as_float(sr[16 * b + j + 3]));
+                        m2[0] = max3(m2[0], __uint_as_float(a[16 * b + j]), __uint_as_float(a[16 * b + j + 1]));
+                        m2[1] = max3(m2[1], __uint_as_float(a[16 * b + j + 2]), __uint_as_float(a[16 * b + j + 3]));
                     }
                     mx = fmaxf(mx, fmaf(fmaxf(m2[0], m2[1]), __uint_as_float(sc.x) * row_scale, __uint_as_float(sc.y)));
                 }
@@ -411,39 +434,41 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
                 }
                 l_run *= alpha;
                 const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-                // P over this row's own scores; a block is stored while the next is computed
+                // P over this row's own scores; two blocks are stored while the next are computed
 #pragma unroll
-                for (int b = 0; b < BLOCKS; ++b) {
-                    const uint4 sc = scales[b];
-                    const float ck = __uint_as_float(sc.x) * row_scale, shift = __uint_as_float(sc.y) - m_use;
-                    const uint64_t scale2 = pack2(ck, ck), shift2 = pack2(shift, shift);
-                    uint64_t l2[2] = {0ull, 0ull};
-                    uint32_t w[8];
+                for (int b = 0; b < BLOCKS; b += 2) {
+                    uint32_t w[16];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        float x0, x1;
-                        unpack2(fma2(pack2(__uint_as_float(sr[16 * b + 2 * j]), __uint_as_float(sr[16 * b + 2 * j + 1])), scale2, shift2), x0, x1);
-                        const float e0 = exp2_fast(x0), e1 = exp2_fast(x1);
-                        l2[j & 1] = add2(l2[j & 1], pack2(e0, e1));
-                        w[j] = pack_f16(e0, e1);
+                    for (int d = 0; d < 2; ++d) {
+                        const uint4 sc = scales[b + d];
+                        const float ck = __uint_as_float(sc.x) * row_scale, shift = __uint_as_float(sc.y) - m_use;
+                        const uint64_t scale2 = pack2(ck, ck), shift2 = pack2(shift, shift);
+                        uint64_t l2[2] = {0ull, 0ull};
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            float x0, x1;
+                            unpack2(fma2(pack2(__uint_as_float(a[16 * (b + d) + 2 * j]), __uint_as_float(a[16 * (b + d) + 2 * j + 1])), scale2, shift2), x0, x1);
+                            const float e0 = exp2_fast(x0), e1 = exp2_fast(x1);
+                            l2[j & 1] = add2(l2[j & 1], pack2(e0, e1));
+                            w[8 * d + j] = pack_f16(e0, e1);
+                        }
+                        float a0, a1;
+                        unpack2(add2(l2[0], l2[1]), a0, a1);
+                        if (a0 + a1 != 0.f) l_run = fmaf(a0 + a1, __uint_as_float(sc.z), l_run);      // (nothing seen: whatever the scale is)
                     }
-                    st8(s_addr + 8 * b, w);
-                    float a0, a1;
-                    unpack2(add2(l2[0], l2[1]), a0, a1);
-                    if (a0 + a1 != 0.f) l_run = fmaf(a0 + a1, __uint_as_float(sc.z), l_run);      // (nothing seen: whatever the scale is)
+                    st16(s_addr + 8 * b, w);
                 }
                 if (__any_sync(0xffffffffu, alpha != 1.f)) {
                     // the whole warp walks its rows' outputs; rows whose reference stays are multiplied by one.  O_X is idle: its last
                     // product is done.
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < HD; c += 32) {
-                        uint32_t o[32];
-                        ld32(o_addr + c, o);
+                        ld32(o_addr + c, a);
                         ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-#pragma unroll
-                        for (int j = 0; j < 32; j += 8) st8(o_addr + c + j, o + j);
+                        for (int j = 0; j < 32; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * alpha);
+                        st16(o_addr + c, a);
+                        st16(o_addr + c + 16, a + 16);
                     }
                 }
                 st_wait();
@@ -494,7 +519,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
             // (a sum that is no number stays that)
             const float l = (f_a == 0.f && l_a == l_a ? 0.f : l_a * f_a) + (f_b == 0.f && l_b == l_b ? 0.f : l_b * f_b);
             if (warp_has_rows) {
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < HD / 2; c += 32) {
                     const int c0 = x * (HD / 2) + c;
                     uint32_t oa[32], ob[32];
@@ -511,7 +536,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
                 if (write && p.slices > 1 && x == 0) *reinterpret_cast<float2 *>(p.part_ml + (qrow * p.slices + slice) * 2) = make_float2(m, l);
             }
         } else if (warp_has_rows) {
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 uint32_t o[32];
                 if (n_tiles_x > 0) {
@@ -542,8 +567,8 @@ int launch_tc(const Q8Params &p, int tiles, cudaStream_t stream) {
         cudaFuncAttributes a;
         return cudaFuncGetAttributes(&a, attention_q8_tc_kernel<HD, HALVES>) == cudaSuccess ? a.numRegs : 0;
     }();
-    KESTREL_REQUIRE(regs * THREADS >= 256 * (SOFTMAX_REGS + OTHER_REGS), "attention_q8: the kernel was built with %d registers a thread, %d are dealt out", regs,
-                    (SOFTMAX_REGS + OTHER_REGS) / 2);
+    KESTREL_REQUIRE(regs * THREADS >= 256 * SOFTMAX_REGS + 384 * OTHER_REGS, "attention_q8: the kernel was built with %d registers a thread, %d are dealt out", regs,
+                    (256 * SOFTMAX_REGS + 384 * OTHER_REGS) / THREADS);
     if (cudaFuncSetAttribute(attention_q8_tc_kernel<HD, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return kestrel_fail(-3, "attention_q8: cannot raise the shared-memory limit: %s", cudaGetErrorString(cudaGetLastError()));
     kestrel_launch(attention_q8_tc_kernel<HD, HALVES>, dim3((unsigned)tiles * p.nkv, 1, p.slices), dim3(THREADS), smem, stream, p);
