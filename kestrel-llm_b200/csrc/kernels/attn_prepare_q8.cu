@@ -123,9 +123,12 @@ struct Row {
     }
 };
 
-__device__ __forceinline__ int code_of(float x, float scale) { return max(-127, min(127, __float2int_rn(x / scale))); }
-__device__ __forceinline__ char4 codes_of(float4 x, float scale) {
-    return make_char4((signed char)code_of(x.x, scale), (signed char)code_of(x.y, scale), (signed char)code_of(x.z, scale), (signed char)code_of(x.w, scale));
+// Four codes as one word.  x / scale as a product with the reciprocal: off by 2^-23 of at most 127 steps.  Added to 1.5 * 2^23 a number is
+// rounded to a whole one, ties to even, whose two's complement is the low byte; no number is above the one that the scale came from.
+__device__ __forceinline__ uint32_t codes_word(float a, float b, float c, float d, float inv) {
+    constexpr float M = 12582912.0f;
+    const uint32_t x = __float_as_uint(fmaf(a, inv, M)), y = __float_as_uint(fmaf(b, inv, M)), z = __float_as_uint(fmaf(c, inv, M)), w = __float_as_uint(fmaf(d, inv, M));
+    return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
 }
 
 // A block's scale from the largest magnitude among the new tokens (its bits) and, where earlier steps began the block, its scale so far
@@ -133,6 +136,242 @@ __device__ __forceinline__ float block_scale(unsigned largest, bool begun, float
     if (largest >= 0x7f800000u || (begun && !(before <= 3.4e38f))) return __uint_as_float(0x7fc00000u);
     const float s = fmaxf(__uint_as_float(largest) / 127.0f, 5.421010862427522e-20f);          // 2^-64
     return begun ? fmaxf(s, before) : s;
+}
+
+// The unit-th block of 16 positions among those that the step's requests touch
+struct Block {
+    int seq, t0, pos0, count;           // its request, first token, first position, tokens; seq -1: there are fewer
+};
+__device__ __forceinline__ Block find_block(const PrepParams &p, int unit) {
+    const int lane = threadIdx.x & 31;
+    Block r = {-1, 0, 0, 0};
+    int left = unit;
+    for (int base = 0; base < p.nseq && r.seq < 0; base += 32) {
+        const int i = base + lane;
+        int n = 0, first = 0, pos = 0, tokens = 0;
+        if (i < p.nseq) {
+            first = p.cu[i];
+            tokens = p.cu[i + 1] - first;
+            if (tokens > 0) {
+                pos = p.positions[first];
+                n = (pos + tokens - 1) / Q8_BLOCK - pos / Q8_BLOCK + 1;
+            }
+        }
+        int end = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end += x;
+        }
+        const unsigned behind = __ballot_sync(0xffffffffu, left < end);
+        if (behind) {
+            const int at = __ffs(behind) - 1;
+            const int nth = left - __shfl_sync(0xffffffffu, end - n, at);            // among the request's blocks
+            const int from = __shfl_sync(0xffffffffu, pos, at), cu = __shfl_sync(0xffffffffu, first, at), all = __shfl_sync(0xffffffffu, tokens, at);
+            r.seq = base + at;
+            r.pos0 = nth == 0 ? from : (from / Q8_BLOCK + nth) * Q8_BLOCK;
+            r.t0 = cu + r.pos0 - from;
+            r.count = min(from + all, (r.pos0 / Q8_BLOCK + 1) * Q8_BLOCK) - r.pos0;
+        } else {
+            left -= __shfl_sync(0xffffffffu, end, 31);
+        }
+    }
+    return r;
+}
+
+// Codes that earlier steps left in a block, against a scale that has risen
+__device__ __forceinline__ void round_again(int8_t *codes, int n, float ratio) {
+    if (!(ratio < 1.0f)) return;                    // the same scale, or none
+    char4 *c4 = reinterpret_cast<char4 *>(codes);
+    for (int i = threadIdx.x; i < n / 4; i += THREADS) {
+        const char4 c = c4[i];
+        c4[i] = make_char4((signed char)__float2int_rn(c.x * ratio), (signed char)__float2int_rn(c.y * ratio), (signed char)__float2int_rn(c.z * ratio),
+                           (signed char)__float2int_rn(c.w * ratio));
+    }
+}
+
+// Head sizes 64 and 128 without rotation, with rotate-half pairs over the whole head (TURN 1) or neighbouring pairs (TURN 2).  Eight lanes
+// hold a row, each the dimensions [n s, n s + n) and [HD / 2 + n s, ...) with n = HD / 16, so that both members of a pair are in one lane
+// and a warp works on four rows: a third of the instructions of the general form, which is bound by them.
+enum { TURN_NONE, TURN_HALF, TURN_NEXT };
+
+// (cosine, sine) as the codes and bfloat16 queries need them: within 2^-21
+__device__ __forceinline__ float2 turn_fast(int pos, float freq, float scale) {
+    const double angle = (double)pos * (double)freq, turns = rint(angle * 0.15915494309189535);
+    const float r = (float)fma(turns, -6.283185307179586, angle);
+    return make_float2(scale * __cosf(r), scale * __sinf(r));
+}
+
+template <typename T, int HD, int TURN>
+struct Eighth {
+    static constexpr int N = HD / 16, N4 = N / 4;
+    float x[2][N];                      // the two runs of dimensions
+
+    __device__ __forceinline__ static int dim(int sub, int h) { return h * (HD / 2) + N * sub; }
+
+    __device__ __forceinline__ void load(const PrepParams &p, int t, int h, int sub, bool live) {
+        const float *at = p.partial + ((size_t)t * (p.nq + 2 * p.nkv) + h) * HD + N * sub;
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i) x[i / N][i % N] = 0.f;
+        if (!live) return;
+        for (int s = 0; s < p.S; ++s, at += p.slice_stride) {
+            float4 v[2][N4];
+#pragma unroll
+            for (int i = 0; i < 2 * N4; ++i) v[i / N4][i % N4] = __ldcs(reinterpret_cast<const float4 *>(at + (i / N4) * (HD / 2)) + i % N4);
+#pragma unroll
+            for (int i = 0; i < 2 * N; ++i) x[i / N][i % N] += reinterpret_cast<const float *>(&v[i / N][(i % N) / 4])[i % 4];
+        }
+        if (p.bias) {
+#pragma unroll
+            for (int i = 0; i < 2 * N; ++i) x[i / N][i % N] += p.bias[(size_t)h * HD + dim(sub, i / N) + i % N];
+        }
+    }
+    __device__ __forceinline__ void norm(const PrepParams &p, const float *w, int sub) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i) ss = fmaf(x[i / N][i % N], x[i / N][i % N], ss);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float rinv = 1.0f / sqrtf(ss * (1.0f / HD) + p.eps);
+#pragma unroll
+        for (int i = 0; i < 2 * N4; ++i) {
+            const float4 g = *(reinterpret_cast<const float4 *>(w + dim(sub, i / N4)) + i % N4);
+            float *e = &x[i / N4][4 * (i % N4)];
+            e[0] *= rinv * g.x; e[1] *= rinv * g.y; e[2] *= rinv * g.z; e[3] *= rinv * g.w;
+        }
+    }
+    // cs: (cosine, sine) of every pair of the token
+    __device__ __forceinline__ void rotate(const PrepParams &p, const float2 *cs, int sub) {
+        if (TURN == TURN_HALF) {
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                const float4 c = *reinterpret_cast<const float4 *>(cs + N * sub + i);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float co = j ? c.z : c.x, si = j ? c.w : c.y, a = x[0][i + j], b = x[1][i + j];
+                    x[0][i + j] = fmaf(a, co, -b * si);
+                    x[1][i + j] = fmaf(b, co, a * si);
+                }
+            }
+        } else if (TURN == TURN_NEXT) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < N; i += 2) {
+                    const int d = dim(sub, h) + i;
+                    if (d >= p.rot) continue;
+                    const float2 c = cs[d >> 1];
+                    const float a = x[h][i], b = x[h][i + 1];
+                    x[h][i] = fmaf(a, c.x, -b * c.y);
+                    x[h][i + 1] = fmaf(b, c.x, a * c.y);
+                }
+        }
+    }
+    __device__ __forceinline__ unsigned largest() const {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i) m = max(m, __float_as_uint(x[i / N][i % N]) & 0x7fffffffu);
+        return m;
+    }
+    __device__ __forceinline__ void put(T *o, int sub) const {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (sizeof(T) == 4) {
+#pragma unroll
+                for (int i = 0; i < N; i += 4) *reinterpret_cast<float4 *>(o + dim(sub, h) + i) = make_float4(x[h][i], x[h][i + 1], x[h][i + 2], x[h][i + 3]);
+            } else {
+                __nv_bfloat162 w[N / 2];
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i) w[i] = __floats2bfloat162_rn(x[h][2 * i], x[h][2 * i + 1]);
+                if (N == 8) *reinterpret_cast<uint4 *>(o + dim(sub, h)) = *reinterpret_cast<uint4 *>(w);
+                else *reinterpret_cast<uint2 *>(o + dim(sub, h)) = *reinterpret_cast<uint2 *>(w);
+            }
+        }
+    }
+    __device__ __forceinline__ void put_codes(int8_t *o, int sub, float inv) const {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t w[N4];
+#pragma unroll
+            for (int i = 0; i < N4; ++i) w[i] = codes_word(x[h][4 * i], x[h][4 * i + 1], x[h][4 * i + 2], x[h][4 * i + 3], inv);
+            if (N == 8) *reinterpret_cast<uint2 *>(o + dim(sub, h)) = make_uint2(w[0], w[1 % N4]);
+            else *reinterpret_cast<uint32_t *>(o + dim(sub, h)) = w[0];
+        }
+    }
+};
+
+template <typename T, int HD, int TURN>
+__global__ void __launch_bounds__(THREADS) attn_prepare_q8_fast_kernel(const PrepParams p) {
+    pdl_launch_dependents();
+    __shared__ __align__(16) float2 cs[Q8_BLOCK][HD / 2];
+    __shared__ unsigned big[WARPS];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane & 7, mine = tid >> 3;
+    const int half = TURN == TURN_NONE ? 0 : TURN == TURN_HALF ? HD / 2 : p.rot >> 1;
+    const int kv_ctas = p.units * p.nkv;
+
+    if ((int)blockIdx.x >= kv_ctas) {
+        // ---- one token's queries, 32 heads at a time
+        const int t = blockIdx.x - kv_ctas;
+        if (t >= p.cu[p.nseq]) { pdl_wait(); return; }      // the step's description was there before the kernel in front of this one began
+        if (TURN != TURN_NONE) {
+            const int pos = p.positions[t];
+            for (int j = tid; j < half; j += THREADS) cs[0][j] = sizeof(T) == 4 ? turn(pos, p.inv_freq[j], p.rot_scale) : turn_fast(pos, p.inv_freq[j], p.rot_scale);
+        }
+        pdl_wait();
+        Eighth<T, HD, TURN> r;
+        r.load(p, t, mine, sub, mine < p.nq);
+        __syncthreads();
+        for (int h0 = 0;;) {
+            const int h = h0 + mine;
+            if (p.q_w) r.norm(p, p.q_w, sub);
+            r.rotate(p, cs[0], sub);
+            if (h < p.nq) r.put((T *)p.q_out + ((size_t)t * p.nq + h) * HD, sub);
+            h0 += THREADS / 8;
+            if (h0 >= p.nq) break;
+            r.load(p, t, h0 + mine, sub, h0 + mine < p.nq);
+        }
+        return;
+    }
+
+    // ---- one block of one (request, kv head): rows 0-15 are its tokens' keys, 16-31 their values
+    const int kvh = blockIdx.x % p.nkv;
+    const Block bl = find_block(p, blockIdx.x / p.nkv);
+    if (bl.seq < 0) { pdl_wait(); return; }
+    const int there = bl.pos0 % Q8_BLOCK;           // codes that earlier steps left in the block
+    const int idx = bl.pos0 / p.page_size;
+    const int page = idx < p.table_width ? p.table[(size_t)bl.seq * p.table_stride + idx] : -1;
+    if (TURN != TURN_NONE) {
+        for (int i = tid; i < bl.count * half; i += THREADS) {
+            const int n = TURN == TURN_HALF ? i / (HD / 2) : i / half, j = i - n * half;
+            cs[n][j] = sizeof(T) == 4 ? turn(bl.pos0 + n, p.inv_freq[j], p.rot_scale) : turn_fast(bl.pos0 + n, p.inv_freq[j], p.rot_scale);
+        }
+    }
+    pdl_wait();
+    if (page < 0 || page >= p.cache_pages) return;  // no page to write to
+    const size_t row0 = ((size_t)page * p.nkv + kvh) * p.page_size + (bl.pos0 - idx * p.page_size) - there;
+    const bool is_k = warp < WARPS / 2;
+    const int n = mine & (Q8_BLOCK - 1);
+    float *scales = is_k ? p.ks : p.vs;
+    int8_t *codes = (is_k ? p.k : p.v) + row0 * HD;
+    const float k_before = there ? p.ks[row0 / Q8_BLOCK] : 0.f, v_before = there ? p.vs[row0 / Q8_BLOCK] : 0.f;
+    Eighth<T, HD, TURN> r;
+    r.load(p, bl.t0 + n, p.nq + (is_k ? 0 : p.nkv) + kvh, sub, n < bl.count);
+    __syncthreads();                                // the cosines and sines
+    if (is_k) {
+        if (p.k_w) r.norm(p, p.k_w, sub);
+        r.rotate(p, cs[n < bl.count ? n : 0], sub);
+    }
+    const unsigned m = __reduce_max_sync(0xffffffffu, n < bl.count ? r.largest() : 0u);
+    if (lane == 0) big[warp] = m;
+    __syncthreads();
+    const unsigned k_big = max(max(big[0], big[1]), max(big[2], big[3])), v_big = max(max(big[4], big[5]), max(big[6], big[7]));
+    const float k_s = block_scale(k_big, there > 0, k_before), v_s = block_scale(v_big, there > 0, v_before);
+    if (n < bl.count) r.put_codes(codes + (size_t)(there + n) * HD, sub, 1.0f / (is_k ? k_s : v_s));
+    if (there) {
+        round_again(p.k + row0 * HD, there * HD, k_before / k_s);
+        round_again(p.v + row0 * HD, there * HD, v_before / v_s);
+    }
+    if (tid == 0 || tid == THREADS / 2) scales[row0 / Q8_BLOCK] = is_k ? k_s : v_s;
 }
 
 template <typename T, int LPR, int NV>
@@ -181,38 +420,9 @@ __global__ void __launch_bounds__(THREADS) attn_prepare_q8_kernel(const PrepPara
     }
 
     // ---- one block of one (request, kv head)
-    const int unit = blockIdx.x / p.nkv, kvh = blockIdx.x % p.nkv;
-    int left = unit, seq = -1, t0 = 0, pos0 = 0, count = 0;
-    for (int base = 0; base < p.nseq && seq < 0; base += 32) {
-        const int i = base + lane;
-        int n = 0, first = 0, pos = 0, tokens = 0;
-        if (i < p.nseq) {
-            first = p.cu[i];
-            tokens = p.cu[i + 1] - first;
-            if (tokens > 0) {
-                pos = p.positions[first];
-                n = (pos + tokens - 1) / Q8_BLOCK - pos / Q8_BLOCK + 1;
-            }
-        }
-        int end = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, end, o);
-            if (lane >= o) end += x;
-        }
-        const unsigned behind = __ballot_sync(0xffffffffu, left < end);
-        if (behind) {
-            const int at = __ffs(behind) - 1;
-            const int nth = left - __shfl_sync(0xffffffffu, end - n, at);            // among the request's blocks
-            const int from = __shfl_sync(0xffffffffu, pos, at), cu = __shfl_sync(0xffffffffu, first, at), all = __shfl_sync(0xffffffffu, tokens, at);
-            seq = base + at;
-            pos0 = nth == 0 ? from : (from / Q8_BLOCK + nth) * Q8_BLOCK;
-            t0 = cu + pos0 - from;
-            count = min(from + all, (pos0 / Q8_BLOCK + 1) * Q8_BLOCK) - pos0;
-        } else {
-            left -= __shfl_sync(0xffffffffu, end, 31);
-        }
-    }
+    const int kvh = blockIdx.x % p.nkv;
+    const Block bl = find_block(p, blockIdx.x / p.nkv);
+    const int seq = bl.seq, t0 = bl.t0, pos0 = bl.pos0, count = bl.count;
     if (seq < 0) { pdl_wait(); return; }
     const int there = pos0 % Q8_BLOCK;              // codes that earlier steps left in the block
     const int idx = pos0 / p.page_size;
@@ -257,29 +467,30 @@ __global__ void __launch_bounds__(THREADS) attn_prepare_q8_kernel(const PrepPara
             const int d = k[i].dim(sub, c);
             if (d >= p.hd) continue;
             const size_t at = (row0 + there + n) * p.hd + d;
-            *reinterpret_cast<char4 *>(p.k + at) = codes_of(k[i].x[c], k_s);
-            *reinterpret_cast<char4 *>(p.v + at) = codes_of(v[i].x[c], v_s);
+            *reinterpret_cast<uint32_t *>(p.k + at) = codes_word(k[i].x[c].x, k[i].x[c].y, k[i].x[c].z, k[i].x[c].w, 1.0f / k_s);
+            *reinterpret_cast<uint32_t *>(p.v + at) = codes_word(v[i].x[c].x, v[i].x[c].y, v[i].x[c].z, v[i].x[c].w, 1.0f / v_s);
         }
     }
-    // codes that were there, against a scale that has risen
-    const float again[2] = {k_before / k_s, v_before / v_s};
-#pragma unroll
-    for (int plane = 0; plane < 2; ++plane) {
-        if (!(again[plane] < 1.0f)) continue;       // the same scale, or none
-        char4 *c4 = reinterpret_cast<char4 *>((plane ? p.v : p.k) + row0 * p.hd);
-        for (int i = tid; i < there * p.hd / 4; i += THREADS) {
-            const char4 c = c4[i];
-            c4[i] = make_char4((signed char)__float2int_rn(c.x * again[plane]), (signed char)__float2int_rn(c.y * again[plane]),
-                               (signed char)__float2int_rn(c.z * again[plane]), (signed char)__float2int_rn(c.w * again[plane]));
-        }
-    }
+    round_again(p.k + row0 * p.hd, there * p.hd, k_before / k_s);
+    round_again(p.v + row0 * p.hd, there * p.hd, v_before / v_s);
     if (tid == 0) p.ks[row0 / Q8_BLOCK] = k_s, p.vs[row0 / Q8_BLOCK] = v_s;
+}
+
+template <typename T, int HD>
+int launch_fast(const PrepParams &p, unsigned ctas, cudaStream_t stream) {
+    const dim3 grid(ctas), block(THREADS);
+    if (p.rot == 0) kestrel_launch(attn_prepare_q8_fast_kernel<T, HD, TURN_NONE>, grid, block, 0, stream, p);
+    else if (p.rot_mode == 0) kestrel_launch(attn_prepare_q8_fast_kernel<T, HD, TURN_HALF>, grid, block, 0, stream, p);
+    else kestrel_launch(attn_prepare_q8_fast_kernel<T, HD, TURN_NEXT>, grid, block, 0, stream, p);
+    return kestrel_check_launch("attn_prepare_q8");
 }
 
 template <typename T>
 int launch(const PrepParams &p, unsigned ctas, cudaStream_t stream) {
-    if (p.hd == 64) kestrel_launch(attn_prepare_q8_kernel<T, 16, 1>, dim3(ctas), dim3(THREADS), 0, stream, p);
-    else if (p.hd <= 128) kestrel_launch(attn_prepare_q8_kernel<T, 32, 1>, dim3(ctas), dim3(THREADS), 0, stream, p);
+    const bool whole = p.rot == 0 || p.rot_mode == 1 || p.rot == p.hd;
+    if (whole && p.hd == 64) return launch_fast<T, 64>(p, ctas, stream);
+    if (whole && p.hd == 128) return launch_fast<T, 128>(p, ctas, stream);
+    if (p.hd <= 128) kestrel_launch(attn_prepare_q8_kernel<T, 32, 1>, dim3(ctas), dim3(THREADS), 0, stream, p);
     else kestrel_launch(attn_prepare_q8_kernel<T, 32, 2>, dim3(ctas), dim3(THREADS), 0, stream, p);
     return kestrel_check_launch("attn_prepare_q8");
 }
