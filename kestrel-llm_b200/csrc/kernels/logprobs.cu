@@ -6,12 +6,13 @@
 // both without a difference of large numbers.  A row's distances, exponentials and sums are float32.
 //
 // The likeliest tokens come from the threads' maxima, which the pass has made anyway: a value T that at least `top` threads' maxima reach
-// is at most the top-th largest number, so only threads whose maximum reaches T hold candidates.  T is found bit by bit over a count of
-// threads; the warps read those few threads' numbers again and keep the best of them, one a lane, in order.  Equal numbers go by index.
+// is at most the top-th largest number, so only threads whose maximum reaches T hold candidates.  T is a number's upper 16 bits, found four
+// at a time over counts of threads.  A thread remembers the largest of its runs of 16 numbers, and the largest number outside that run:
+// most candidates' threads read one run again, all at once, and the warps of the others all of their numbers.  Rows with very many equal
+// numbers leave more candidates than there is room for; their warps keep the best, one a lane, in order.  Equal numbers go by index.
 //
-// A row is one block's, or a cluster's of up to 8 where the rows are few; a cluster's blocks meet once, in the first block's shared
-// memory.  Bound by the row's bytes; a number costs half a maximum, an add, a product, an
-// exponential, an add, a bound and a multiply-add.
+// A row is one block's, or a cluster's of up to 8; a cluster's blocks meet once, in the first block's shared memory.  Bound by the row's
+// bytes; a number costs half a maximum, an add, a product, an exponential, an add, a bound and a multiply-add.
 #include "common.cuh"
 
 #include <math.h>
@@ -19,7 +20,8 @@
 namespace {
 
 constexpr int THREADS = 512, WARPS = THREADS / 32, MOST = KESTREL_LOGPROBS_MAX_TOP, MAX_CLUSTER = 8;
-constexpr int FLIGHT = 4;               // vectors of four numbers that a thread has in flight
+constexpr int FLIGHT = 4;               // vectors of four numbers that a thread has in flight: a run
+constexpr int ROOM = 512;               // candidates of a block
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct State {
@@ -32,16 +34,22 @@ struct State {
             m = to;
         }
     }
-    __device__ __forceinline__ void join(State o) {
-        if (o.m > m) {
-            State t = o;
-            o = *this;
-            *this = t;
+    // the state against a maximum that is at least its own; sums that are no numbers stay that
+    __device__ __forceinline__ void move(float to) {
+        const float f = m == -INFINITY ? 0.f : exp2f((m - to) * LOG2E);
+        a = f == 0.f && a == a ? 0.f : f * fmaf(m - to, l, a);
+        l = f == 0.f && l == l ? 0.f : f * l;
+        m = to;
+    }
+    // over the first n lanes of a warp, n a power of two: every lane has all of it
+    __device__ __forceinline__ void over(int n) {
+        float to = m;
+        for (int o = n / 2; o > 0; o >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, o));
+        move(to);
+        for (int o = n / 2; o > 0; o >>= 1) {
+            l += __shfl_xor_sync(0xffffffffu, l, o);
+            a += __shfl_xor_sync(0xffffffffu, a, o);
         }
-        const float f = o.m == -INFINITY ? 0.f : exp2f((o.m - m) * LOG2E);
-        // sums that are no numbers stay that, whatever their maximum is
-        a += f == 0.f && o.a == o.a ? 0.f : f * fmaf(o.m - m, o.l, o.a);
-        l += f == 0.f && o.l == o.l ? 0.f : f * o.l;
     }
 };
 
@@ -93,8 +101,9 @@ token_logprobs_kernel(const float *__restrict__ logits, long long ld, int V, int
                       float *__restrict__ entropy, int *__restrict__ top_ids, float *__restrict__ top_logprobs) {
     pdl_launch_dependents();
     __shared__ State joined[MAX_CLUSTER], parts[WARPS];
-    __shared__ uint64_t found[WARPS * MOST], block_best[MAX_CLUSTER * MOST];
-    __shared__ int n_found;
+    __shared__ uint64_t found[ROOM], block_best[MAX_CLUSTER * MOST];
+    __shared__ int n_found, counts[4][16];
+    static_assert(ROOM >= WARPS * MOST && ROOM == THREADS, "a thread an entry, and room for what all warps keep");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row = blockIdx.x / cluster, rank = cluster > 1 ? (int)cluster_rank() : 0;
     const float *x = logits + (size_t)row * ld;
@@ -105,7 +114,7 @@ token_logprobs_kernel(const float *__restrict__ logits, long long ld, int V, int
     int odd = -1;                       // index of this thread's number outside the vectors
     if (rank == 0 && tid < head) odd = tid;
     if (rank == cluster - 1 && tid >= 4 && tid - 4 < V - head - 4 * nv) odd = head + 4 * nv + tid - 4;
-    if (tid < WARPS * MOST) found[tid] = 0;
+    if (tid < 64) counts[tid >> 4][tid & 15] = 0;
     if (tid == 0) n_found = 0;
     if (cluster > 1) cluster_arrive();  // the first block's shared memory may be written once every block has begun
     pdl_wait();
@@ -116,7 +125,8 @@ token_logprobs_kernel(const float *__restrict__ logits, long long ld, int V, int
     }
 
     State s = {-INFINITY, 0.f, 0.f};
-    float big = -INFINITY;              // this thread's largest number
+    float big = -INFINITY, other = -INFINITY;       // this thread's largest number, and the largest outside its run
+    int run = -1;                       // the run's first vector; -1: the number outside the vectors
     if (odd >= 0) {
         const float o = x[odd];
         big = fmaxf(big, o);
@@ -131,7 +141,8 @@ token_logprobs_kernel(const float *__restrict__ logits, long long ld, int V, int
         float mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < FLIGHT; ++i) mx = fmaxf(fmaxf(fmaxf(mx, q[i].x), fmaxf(q[i].y, q[i].z)), q[i].w);
-        big = fmaxf(big, mx);
+        if (mx > big) other = big, big = mx, run = v;
+        else other = fmaxf(other, mx);
         s.rise(mx);
         const float m_use = s.m == -INFINITY ? 0.f : s.m;
 #pragma unroll
@@ -145,44 +156,93 @@ token_logprobs_kernel(const float *__restrict__ logits, long long ld, int V, int
     if (cluster > 1) cluster_wait();
     // the block's state
     State w = s;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        State t = {__shfl_xor_sync(0xffffffffu, w.m, o), __shfl_xor_sync(0xffffffffu, w.l, o), __shfl_xor_sync(0xffffffffu, w.a, o)};
-        w.join(t);
-    }
+    w.over(32);
     if (lane == 0) parts[warp] = w;
 
     if (top > 0) {
-        // T: the largest value whose bits, from the highest down, leave at least `top` threads' maxima at or above it
+        // T: the largest value of 16 bits that leaves at least `top` threads' maxima at or above it
         const bool some = odd >= 0 || v0 + tid < v1;
         const uint32_t mine = some ? key_of(big) : 0u;
         uint32_t T = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t c = T | 1u << bit;
-            if (__syncthreads_count(mine >= c) >= top) T = c;
+        __syncthreads();                    // the counts are zero
+#pragma unroll
+        for (int round = 0; round < 4; ++round) {
+            const int shift = 28 - 4 * round;
+            // how many lanes reach T + c * 2^shift, for c = 1 .. 15: lane c keeps that count
+            int n = 0;
+#pragma unroll
+            for (int c = 1; c < 16; ++c) {
+                const int k = __popc(__ballot_sync(0xffffffffu, mine >= T + ((uint32_t)c << shift)));
+                if (lane == c) n = k;
+            }
+            if (n) atomicAdd(&counts[round][lane], n);
+            __syncthreads();
+            const int reach = lane > 0 && lane < 16 ? counts[round][lane] : 0;
+            T += (uint32_t)__popc(__ballot_sync(0xffffffffu, reach >= top)) << shift;       // the counts fall with c
         }
         T = max(T, 1u);
-        uint64_t best = 0;
-        for (uint32_t rest = __ballot_sync(0xffffffffu, mine >= T); rest; rest &= rest - 1) {
-            const int l = __ffs(rest) - 1;
-            const int l_odd = __shfl_sync(0xffffffffu, odd, l);
-            if (l_odd >= 0) keep(best, lane == 0 ? entry_of(x[l_odd], l_odd) : 0, top, lane);
-            for (int v = v0 + 32 * warp + l; v < v1; v += 32 * THREADS) {
-                const int at = v + lane * THREADS;
-                float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (at < v1) q = xv[at];
-                const float e[4] = {q.x, q.y, q.z, q.w};
+        auto offer = [&](float e, int i) {
+            if (key_of(e) >= T) {
+                const int at = atomicAdd(&n_found, 1);
+                if (at < ROOM) found[at] = entry_of(e, i);
+            }
+        };
+        if (mine >= T && odd >= 0) offer(x[odd], odd);
+        const bool several = mine >= T && (key_of(other) >= T || run < 0);       // (numbers that are none have no run)
+        if (mine >= T && !several) {
+            float4 q[FLIGHT];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) keep(best, at < v1 && key_of(e[j]) >= T ? entry_of(e[j], head + 4 * at + j) : 0, top, lane);
+            for (int i = 0; i < FLIGHT; ++i)
+                if (run + i * THREADS < v1) q[i] = xv[run + i * THREADS];
+#pragma unroll
+            for (int i = 0; i < FLIGHT; ++i) {
+                const int at = run + i * THREADS;
+                if (at >= v1) break;
+                offer(q[i].x, head + 4 * at);
+                offer(q[i].y, head + 4 * at + 1);
+                offer(q[i].z, head + 4 * at + 2);
+                offer(q[i].w, head + 4 * at + 3);
             }
         }
-        // the warps' entries in one list, then each goes to the place that the number of better ones gives it
-        if (best && lane < top) found[atomicAdd(&n_found, 1)] = best;
+        // threads with candidates in several runs: their warp reads all of their numbers
+        for (uint32_t rest = __ballot_sync(0xffffffffu, several); rest; rest &= rest - 1) {
+            const int l = __ffs(rest) - 1;
+            for (int at = v0 + 32 * warp + l + lane * THREADS; at < v1; at += 32 * THREADS) {
+                const float4 q = xv[at];
+                offer(q.x, head + 4 * at);
+                offer(q.y, head + 4 * at + 1);
+                offer(q.z, head + 4 * at + 2);
+                offer(q.w, head + 4 * at + 3);
+            }
+        }
         __syncthreads();
+        if (n_found > ROOM) {               // too many: every warp keeps the best of its threads'
+            __syncthreads();
+            if (tid == 0) n_found = 0;
+            uint64_t best = 0;
+            for (uint32_t rest = __ballot_sync(0xffffffffu, mine >= T); rest; rest &= rest - 1) {
+                const int l = __ffs(rest) - 1;
+                const int l_odd = __shfl_sync(0xffffffffu, odd, l);
+                if (l_odd >= 0) keep(best, lane == 0 ? entry_of(x[l_odd], l_odd) : 0, top, lane);
+                for (int v = v0 + 32 * warp + l; v < v1; v += 32 * THREADS) {
+                    const int at = v + lane * THREADS;
+                    float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (at < v1) q = xv[at];
+                    const float e[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) keep(best, at < v1 && key_of(e[j]) >= T ? entry_of(e[j], head + 4 * at + j) : 0, top, lane);
+                }
+            }
+            __syncthreads();
+            if (best && lane < top) found[atomicAdd(&n_found, 1)] = best;
+            __syncthreads();
+        }
+        // each goes to the place that the number of better ones gives it
         const int n = n_found;
-        for (int i = tid; i < n; i += THREADS) {
-            const uint64_t e = found[i];
+        if (tid < n) {
+            const uint64_t e = found[tid];
             int at = 0;
+#pragma unroll 8
             for (int j = 0; j < n; ++j) at += found[j] > e;
             if (at < top) {
                 if (cluster > 1) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(in_first(block_best + rank * MOST + at)), "l"(e) : "memory");
@@ -196,12 +256,8 @@ token_logprobs_kernel(const float *__restrict__ logits, long long ld, int V, int
     }
     __syncthreads();
     if (warp == 0) {
-        State b = lane < WARPS ? parts[lane] : State{-INFINITY, 0.f, 0.f};
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            State t = {__shfl_xor_sync(0xffffffffu, b.m, o), __shfl_xor_sync(0xffffffffu, b.l, o), __shfl_xor_sync(0xffffffffu, b.a, o)};
-            b.join(t);
-        }
+        State b = parts[lane % WARPS];
+        b.over(WARPS);
         if (lane == 0) {
             if (cluster > 1) {
                 const uint32_t to = in_first(joined + rank);
@@ -219,8 +275,8 @@ token_logprobs_kernel(const float *__restrict__ logits, long long ld, int V, int
         __syncthreads();
     }
     if (rank != 0) return;
-    State r = joined[0];
-    for (int c = 1; c < cluster; ++c) r.join(joined[c]);
+    State r = joined[lane & (cluster - 1)];
+    r.over(cluster);
     const float log_l = logf(r.l), m_use = r.m == -INFINITY ? 0.f : r.m;
     if (tid == 0) {
         if (entropy) entropy[row] = log_l - r.a / r.l;
@@ -230,9 +286,11 @@ token_logprobs_kernel(const float *__restrict__ logits, long long ld, int V, int
         const uint64_t e = block_best[i / top * MOST + i % top];
         if (!e) continue;
         int at = i % top;                                            // its own block's better ones
-        for (int c = 0; c < cluster; ++c) {
-            if (c == i / top) continue;
-            for (int j = 0; j < top && block_best[c * MOST + j] > e; ++j) ++at;
+        if (cluster > 1) {
+            at = 0;
+            for (int c = 0; c < cluster; ++c)
+#pragma unroll 8
+                for (int j = 0; j < top; ++j) at += block_best[c * MOST + j] > e;
         }
         if (at < top) {
             top_ids[(size_t)row * top + at] = (int)~(uint32_t)e;
@@ -250,7 +308,9 @@ KESTREL_API int kestrel_token_logprobs(const float *logits, long long ld, int R,
     KESTREL_REQUIRE(top >= 0 && top <= MOST && top <= V, "token_logprobs: the %d likeliest of %d; at most %d are picked", top, V, MOST);
     KESTREL_REQUIRE((!ids || logprobs) && (top == 0 || (top_ids && top_logprobs)), "token_logprobs: no place for the results");
     KESTREL_REQUIRE(((uintptr_t)logits & 3) == 0, "token_logprobs: logits must start on 4 bytes");
-    // blocks of a row: while twice as many would still be resident at once, two an SM
+    // Blocks of a row: while twice as many would still be resident at once, two an SM.  (128 rows of 151,936, 20 likeliest: 29 us with clusters
+    // of 2, 44 and 38 with 1 and 4; 64 rows 18.5 with 4, 23 and 28 with 2 and 8; 1,024 rows 121 with one block, 143 with clusters of 2,
+    // although these leave the last round fuller.)
     int cluster = 1;
     while (cluster < MAX_CLUSTER && (long long)R * cluster * 2 <= 2ll * kestrel_sms() && V / (cluster * 2) >= 1024) cluster *= 2;
     KESTREL_REQUIRE((long long)R * cluster < (1ll << 31), "token_logprobs: %d rows exceed the grid", R);
