@@ -6,8 +6,8 @@
 // both without a difference of large numbers.  A row's distances, exponentials and sums are float32.
 //
 // The likeliest tokens come from the threads' maxima, which the pass has made anyway: a value T that at least `top` threads' maxima reach
-// is at most the top-th largest number, so only threads whose maximum reaches T hold candidates.  T is a number's upper 16 bits, found four
-// at a time over counts of threads.  A thread remembers the largest of its runs of 16 numbers, and the largest number outside that run:
+// is at most the top-th largest number, so only threads whose maximum reaches T hold candidates.  T is the top-th largest among the two
+// largest maxima of every warp: no more than its threads', and found in two steps.  A thread remembers the largest of its runs of 16 numbers, and the largest number outside that run:
 // most candidates' threads read one run again, all at once, and the warps of the others all of their numbers.  Rows with very many equal
 // numbers leave more candidates than there is room for; their warps keep the best, one a lane, in order.  Equal numbers go by index.
 //
@@ -102,8 +102,9 @@ token_logprobs_kernel(const float *__restrict__ logits, long long ld, int V, int
     pdl_launch_dependents();
     __shared__ State joined[MAX_CLUSTER], parts[WARPS];
     __shared__ uint64_t found[ROOM], block_best[MAX_CLUSTER * MOST];
-    __shared__ int n_found, counts[4][16];
-    static_assert(ROOM >= WARPS * MOST && ROOM == THREADS, "a thread an entry, and room for what all warps keep");
+    __shared__ int n_found, place[MAX_CLUSTER * MOST];
+    __shared__ uint32_t maxima[2 * WARPS];
+    static_assert(ROOM >= WARPS * MOST && ROOM == THREADS && 2 * WARPS == 32 && MOST == 32, "a thread an entry, room for what all warps keep, a lane a maximum");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row = blockIdx.x / cluster, rank = cluster > 1 ? (int)cluster_rank() : 0;
     const float *x = logits + (size_t)row * ld;
@@ -114,7 +115,6 @@ token_logprobs_kernel(const float *__restrict__ logits, long long ld, int V, int
     int odd = -1;                       // index of this thread's number outside the vectors
     if (rank == 0 && tid < head) odd = tid;
     if (rank == cluster - 1 && tid >= 4 && tid - 4 < V - head - 4 * nv) odd = head + 4 * nv + tid - 4;
-    if (tid < 64) counts[tid >> 4][tid & 15] = 0;
     if (tid == 0) n_found = 0;
     if (cluster > 1) cluster_arrive();  // the first block's shared memory may be written once every block has begun
     pdl_wait();
@@ -160,27 +160,22 @@ token_logprobs_kernel(const float *__restrict__ logits, long long ld, int V, int
     if (lane == 0) parts[warp] = w;
 
     if (top > 0) {
-        // T: the largest value of 16 bits that leaves at least `top` threads' maxima at or above it
+        // T: the top-th largest of the warps' two largest maxima each, which are as many threads'
         const bool some = odd >= 0 || v0 + tid < v1;
         const uint32_t mine = some ? key_of(big) : 0u;
-        uint32_t T = 0;
-        __syncthreads();                    // the counts are zero
-#pragma unroll
-        for (int round = 0; round < 4; ++round) {
-            const int shift = 28 - 4 * round;
-            // how many lanes reach T + c * 2^shift, for c = 1 .. 15: lane c keeps that count
-            int n = 0;
-#pragma unroll
-            for (int c = 1; c < 16; ++c) {
-                const int k = __popc(__ballot_sync(0xffffffffu, mine >= T + ((uint32_t)c << shift)));
-                if (lane == c) n = k;
-            }
-            if (n) atomicAdd(&counts[round][lane], n);
-            __syncthreads();
-            const int reach = lane > 0 && lane < 16 ? counts[round][lane] : 0;
-            T += (uint32_t)__popc(__ballot_sync(0xffffffffu, reach >= top)) << shift;       // the counts fall with c
+        const uint32_t m1 = __reduce_max_sync(0xffffffffu, mine);
+        const int at1 = __ffs(__ballot_sync(0xffffffffu, mine == m1)) - 1;
+        const uint32_t m2 = __reduce_max_sync(0xffffffffu, lane == at1 ? 0u : mine);
+        if (lane < 2) maxima[2 * warp + lane] = lane ? m2 : m1;
+        __syncthreads();
+        const uint32_t v = maxima[lane];
+        int better = 0;
+#pragma unroll 4
+        for (int i = 0; i < 32; ++i) {
+            const uint32_t u = __shfl_sync(0xffffffffu, v, i);
+            better += u > v || (u == v && i < lane);
         }
-        T = max(T, 1u);
+        const uint32_t T = max(__shfl_sync(0xffffffffu, v, __ffs(__ballot_sync(0xffffffffu, better == top - 1)) - 1), 1u);
         auto offer = [&](float e, int i) {
             if (key_of(e) >= T) {
                 const int at = atomicAdd(&n_found, 1);
@@ -282,17 +277,29 @@ token_logprobs_kernel(const float *__restrict__ logits, long long ld, int V, int
         if (entropy) entropy[row] = log_l - r.a / r.l;
         if (ids) logprobs[row] = (given - m_use) - log_l;
     }
-    for (int i = tid; i < cluster * top; i += THREADS) {
-        const uint64_t e = block_best[i / top * MOST + i % top];
-        if (!e) continue;
-        int at = i % top;                                            // its own block's better ones
-        if (cluster > 1) {
-            at = 0;
-            for (int c = 0; c < cluster; ++c)
-#pragma unroll 8
-                for (int j = 0; j < top; ++j) at += block_best[c * MOST + j] > e;
+    // An entry's place: its own in its block's list, and of every other list, which are in order, as many as a search by halves finds; a
+    // thread a pair of entry and list.  (Rolled: what runs once a row costs what its code takes to arrive.)
+    if (cluster > 1) {
+        if (tid < MAX_CLUSTER * MOST) place[tid] = 0;
+        __syncthreads();
+#pragma unroll 1
+        for (int j = tid; j < cluster * MOST * cluster; j += THREADS) {
+            const int i = j / cluster, c = j & (cluster - 1);
+            if (i % MOST >= top || i / MOST == c) continue;
+            const uint64_t e = block_best[i], *list = block_best + c * MOST;
+            int n = 0;
+#pragma unroll 1
+            for (int step = MOST; step > 0; step /= 2)
+                if (n + step <= top && list[n + step - 1] > e) n += step;
+            if (n) atomicAdd(&place[i], n);
         }
-        if (at < top) {
+        __syncthreads();
+    }
+#pragma unroll 1
+    for (int i = tid; i < cluster * MOST; i += THREADS) {
+        const uint64_t e = block_best[i];
+        const int at = i % MOST + (cluster > 1 ? place[i] : 0);
+        if (i % MOST < top && e && at < top) {
             top_ids[(size_t)row * top + at] = (int)~(uint32_t)e;
             top_logprobs[(size_t)row * top + at] = (value_of((uint32_t)(e >> 32)) - m_use) - log_l;
         }
