@@ -279,7 +279,8 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
         if (!p->tiles) continue;
         if (p->kernel == DECODE) {
             p->ctas = q8_decode_ctas(p->key_tiles, hd, p->most_rows);
-            p->scratch = q8_decode_scratch(p->ctas, hd);
+            p->slices = q8_decode_cluster((long long)nseq * nkv, (p->longest + 63) / 64, p->key_tiles, hd, p->most_rows);
+            p->scratch = p->slices ? 0 : q8_decode_scratch(p->ctas, hd);
         } else {
             // the tensor cores: one CTA an SM, slices of 512 keys at least
             p->slices = p->kernel == TC ? slices_for((long long)p->tiles * nkv, kestrel_sms(), p->longest, 512)
@@ -333,9 +334,9 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
         p.part_o = scratch;
         int rc;
         if (part.kernel == DECODE) {
-            p.part_ml = scratch + 2ll * part.ctas * 16 * hd;
+            p.part_ml = scratch ? scratch + 2ll * part.ctas * 16 * hd : nullptr;
             rc = q8_launch_decode(p, part.ctas, part.most_rows, stream);
-            launches += 2;
+            launches += part.slices ? 1 : 2;
         } else {
             p.part_ml = scratch ? scratch + (long long)T * nq * part.slices * hd : nullptr;
             rc = part.kernel == TC ? q8_launch_tc(p, part.tiles, stream) : q8_launch_plain(p, dtype, part.tiles, stream);

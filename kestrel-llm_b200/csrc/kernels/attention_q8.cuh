@@ -102,6 +102,7 @@ __device__ __forceinline__ size_t q8_out_row(const Q8Params &p, const Q8Tile &t,
 // attention_q8_decode.cu: requests of up to 16 rows, head sizes 64 and 128, bfloat16; two kernels
 int q8_launch_decode(const Q8Params &p, int ctas, int most_rows, cudaStream_t stream);
 int q8_decode_ctas(long long tiles, int hd, int most_rows);      // for so many (request, kv head, 64 keys), requests of at most so many rows
+int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int hd, int most_rows);      // CTAs a pair (Q8Params.slices), or 0: ctas in stretches
 long long q8_decode_scratch(int ctas, int hd);          // floats: part_o, then part_ml
 int q8_decode_error();                                  // its bounded waits' error word; synchronises
 // attention_q8_tc.cu: tiles of up to 256 rows, head sizes 64 and 128, bfloat16

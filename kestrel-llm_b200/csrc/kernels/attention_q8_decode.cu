@@ -4,7 +4,8 @@
 // The work is cut evenly, whatever the requests' lengths: all key tiles of 64 of all (request, kv head) pairs stand in one line, and every
 // CTA takes as many of them as the next.  A CTA walks its stretch pair by pair, up to 16 (token, query head) rows at once.  A pair that lies
 // within one CTA's stretch is finished there; the others leave (maximum, sum, outputs) of their parts in scratch, two parts a CTA at most,
-// and the merge kernel below joins them in the order of the keys.
+// and the merge kernel below joins them in the order of the keys.  Where the pairs are few and short (CLUSTER) the CTAs of a cluster share one
+// pair instead, evenly, and join their parts in each other's shared memory: a kernel less.
 //
 // A loader warp brings tiles by TMA into a ring of stages, codes of K and V side by side, and the scales of their four blocks beside
 // them, running ahead over the pairs' borders; four consumer warps take one block of 16 keys each.  Codes go from shared memory straight
@@ -20,6 +21,8 @@
 #include "attention_q8.cuh"
 #include "tcgen05.cuh"
 
+#include "device_table.h"
+
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -27,7 +30,7 @@ __device__ int g_q8d_error = 0;
 
 namespace {
 
-constexpr int THREADS = 160, BN = 64;       // four consumer warps and the loader; keys of a tile
+constexpr int THREADS = 160, BN = 64, MAX_CLUSTER = 8;      // four consumer warps and the loader; keys of a tile
 constexpr uint32_t MAGIC = 0x64646464u;     // high byte of the float16 numbers 1024 .. 1279
 
 // NT: column tiles of eight rows.  One: three CTAs an SM; two: two.
@@ -67,6 +70,22 @@ __device__ __forceinline__ void mma_f16(float *d, const uint32_t *a, uint32_t b0
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// shared memory of the rank-th CTA of this cluster at this one's address `at`
+__device__ __forceinline__ uint32_t in_cluster(uint32_t at, int rank) {
+    uint32_t remote;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(rank));
+    return remote;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t at) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
 }
 __device__ __forceinline__ uint32_t transpose(uint32_t a) {        // of an 8 by 8 tile of 16-bit numbers
     uint32_t d;
@@ -154,6 +173,16 @@ struct Walk {
     const int *table;
     bool whole;
 
+    // the rank-th of `ranks` equal parts of a pair
+    __device__ __forceinline__ Walk(const Q8Params &p_, int pair, int rank, int ranks) : p(p_), at(0), end(0), begin(0), seq(pair / p_.nkv), kvh(pair % p_.nkv) {
+        G = p.nq / p.nkv;
+        n = Line{p}.tiles_of(seq);
+        if (n == 0) return;
+        describe();
+        from = (int)((long long)n * rank / ranks);
+        to = (int)((long long)n * (rank + 1) / ranks);
+        whole = ranks == 1;
+    }
     __device__ __forceinline__ Walk(const Q8Params &p_, long long length) : p(p_), n(0) {
         at = stretch(blockIdx.x, length, gridDim.x);
         end = stretch(blockIdx.x + 1, length, gridDim.x);
@@ -256,12 +285,13 @@ __device__ __forceinline__ void weigh(float (&s)[NT][4], float (&o)[NT][NO][4], 
         }
 }
 
-template <int HD, int NT>
+template <int HD, int NT, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, Ring<HD, NT>::CTAS)
 attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Q8Params p) {
     pdl_launch_dependents();
     using R = Ring<HD, NT>;
     constexpr int KS = HD / 16, HALVES = HD / 64, ROWS = 8 * NT;
+    constexpr uint32_t FIN_ML = ROWS * HD * 4;
     extern __shared__ uint8_t q8d_smem[];
     const uint32_t base = (smem_u32(q8d_smem) + 1023u) & ~1023u;
     uint8_t *ring = q8d_smem + (base - smem_u32(q8d_smem));
@@ -275,17 +305,34 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     }
     __syncthreads();
     // the step's description was on the device before the kernel in front of this one began
-    Walk w(p, Line{p}.length());
+    Walk w = CLUSTER ? Walk(p, (int)blockIdx.x / p.slices, (int)blockIdx.x % p.slices, p.slices) : Walk(p, Line{p}.length());
     int stage = 0;
     uint32_t phase = 0;
     pdl_wait();
+    if (CLUSTER && w.n == 0) return;                    // another launch's request: all of the cluster
+    bool more = true;
+    auto next = [&] {
+        if (!CLUSTER) return w.next();
+        const bool now = more;
+        more = false;
+        return now;
+    };
+
+    // eight neighbouring numbers of an output row
+    auto store = [&](size_t at, const float *acc, float L) {
+        const float inv = 1.0f / L;
+        __nv_bfloat162 b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = __floats2bfloat162_rn(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+        *reinterpret_cast<uint4 *>((__nv_bfloat16 *)p.out + at) = *reinterpret_cast<uint4 *>(b);
+    };
 
     if (warp == 4) {
         // ---- loader: lane l brings the l-th box of a tile, K and V; lanes 0-3 (4-7) bring its blocks' scales of K (V)
         const int box = p.page_size % 64 == 0 ? 64 : p.page_size % 32 == 0 ? 32 : 16, boxes = BN / box;
         const float *scales = lane < 4 ? p.ks : p.vs;
         bool ok = true;
-        while (ok && w.next()) {
+        while (ok && next()) {
             const int kb0 = w.k_first / BN * BN;
             for (int i = w.from; i < w.to; ++i) {
                 const int kb = kb0 + i * BN;
@@ -307,8 +354,7 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                 if (++stage == R::STAGES) stage = 0, phase ^= 1u;
             }
         }
-        return;
-    }
+    } else {
 
     // ---- consumers
     // a lane (g, c) holds rows g of the first operands, row g of the queries, and of a product keys g and g + 8 for rows 2 c and 2 c + 1
@@ -327,7 +373,7 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     bool ok = true;             // after a wait gave up the loop runs on without waiting, so that the warps still meet below
     bool first_part = true;
 
-    while (w.next()) {
+    while (next()) {
         // Queries as fragments, in float16: a row is multiplied by the power of two that brings its largest number to [64, 128), so that
         // a bfloat16 number keeps its bits down to 2^-21 of that, and the rest is off by 2^-31 of it.
         uint32_t qb[NT][KS][2];
@@ -514,13 +560,17 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                 acc[0] = fmaf(a.x, f, acc[0]); acc[1] = fmaf(a.y, f, acc[1]); acc[2] = fmaf(a.z, f, acc[2]); acc[3] = fmaf(a.w, f, acc[3]);
                 acc[4] = fmaf(b.x, f, acc[4]); acc[5] = fmaf(b.y, f, acc[5]); acc[6] = fmaf(b.z, f, acc[6]); acc[7] = fmaf(b.w, f, acc[7]);
             }
+            if (CLUSTER && !w.whole) {
+                // this part's sums stay in the ring's memory, whose tiles have all been consumed, for the cluster
+                float *fin = reinterpret_cast<float *>(ring) + r * HD + d;
+                *reinterpret_cast<float4 *>(fin) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                *reinterpret_cast<float4 *>(fin + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                if (d == 0) *reinterpret_cast<float2 *>(ring + FIN_ML + 8 * r) = make_float2(ok ? M : __uint_as_float(0x7fc00000u), L);
+                continue;
+            }
             if (!ok) continue;                              // a wait gave up: nothing is written
             if (w.whole) {
-                const float inv = 1.0f / L;
-                __nv_bfloat162 b[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) b[j] = __floats2bfloat162_rn(acc[2 * j] * inv, acc[2 * j + 1] * inv);
-                *reinterpret_cast<uint4 *>((__nv_bfloat16 *)p.out + w.out_row(r) * HD + d) = *reinterpret_cast<uint4 *>(b);
+                store(w.out_row(r) * HD + d, acc, L);
             } else {
                 float *po = part_out<HD>(p, part, r) + d;
                 *reinterpret_cast<float4 *>(po) = make_float4(acc[0], acc[1], acc[2], acc[3]);
@@ -529,6 +579,49 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
             }
         }
         first_part = false;
+    }
+    }   // consumers
+
+    if (CLUSTER && !w.whole) {
+        // the parts of one pair, in ascending order of the keys; the rows are shared out among the CTAs.  Every thread takes part in the
+        // barriers; no CTA leaves while its shared memory may still be read.
+        const int rank = blockIdx.x % p.slices;
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (warp < 4) {
+            for (int idx = tid; idx < ROWS * (HD / 8); idx += 128) {
+                const int r = idx / (HD / 8), d = (idx % (HD / 8)) * 8;
+                if (r >= w.rows) break;
+                if (r % p.slices != rank) continue;
+                // all parts' numbers in flight at once
+                float2 ml[MAX_CLUSTER];
+                float4 x[MAX_CLUSTER][2];
+#pragma unroll
+                for (int s = 0; s < MAX_CLUSTER; ++s) {
+                    ml[s] = make_float2(-INFINITY, 0.f);
+                    if (s >= p.slices) continue;
+                    ml[s] = ld_cluster2(in_cluster(base + FIN_ML + 8 * r, s));
+                    x[s][0] = ld_cluster4(in_cluster(base + (r * HD + d) * 4, s));
+                    x[s][1] = ld_cluster4(in_cluster(base + (r * HD + d + 4) * 4, s));
+                }
+                float M = -INFINITY, L = 0.f, acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                bool fine = true;
+#pragma unroll
+                for (int s = 0; s < MAX_CLUSTER; ++s) {
+                    fine = fine && ml[s].x == ml[s].x;      // a wait gave up: nothing is written
+                    M = fmaxf(M, ml[s].x);
+                }
+#pragma unroll
+                for (int s = 0; s < MAX_CLUSTER; ++s) {
+                    const float f = ml[s].x == -INFINITY ? 0.f : exp2_fast(ml[s].x - M);
+                    if (s >= p.slices || (f == 0.f && ml[s].y == ml[s].y)) continue;       // (a sum that is no number stays that)
+                    L = fmaf(ml[s].y, f, L);
+                    acc[0] = fmaf(x[s][0].x, f, acc[0]); acc[1] = fmaf(x[s][0].y, f, acc[1]); acc[2] = fmaf(x[s][0].z, f, acc[2]); acc[3] = fmaf(x[s][0].w, f, acc[3]);
+                    acc[4] = fmaf(x[s][1].x, f, acc[4]); acc[5] = fmaf(x[s][1].y, f, acc[5]); acc[6] = fmaf(x[s][1].z, f, acc[6]); acc[7] = fmaf(x[s][1].w, f, acc[7]);
+                }
+                if (fine) store(w.out_row(r) * HD + d, acc, L);
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
 }
 
@@ -594,6 +687,21 @@ __global__ void __launch_bounds__(256) attention_q8_join_kernel(const Q8Params p
 
 template <int HD, int NT> constexpr size_t decode_smem() { return Ring<HD, NT>::BYTES + 1024; }
 
+// all but the grid and the stream of a launch in clusters
+template <int HD, int NT>
+int cluster_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int size) {
+    if (cudaFuncSetAttribute(attention_q8_decode_kernel<HD, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)decode_smem<HD, NT>()) != cudaSuccess)
+        return kestrel_fail(-3, "attention_q8: cannot raise the shared-memory limit: %s", cudaGetErrorString(cudaGetLastError()));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = decode_smem<HD, NT>();
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return 0;
+}
+
 template <int HD, int NT>
 int launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
     CUtensorMap mk, mv;
@@ -603,13 +711,43 @@ int launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
     int rc = kestrel_tensor_map_bf16(&mk, p.k, lines, 64, 64, box);
     if (rc == 0) rc = kestrel_tensor_map_bf16(&mv, p.v, lines, 64, 64, box);
     if (rc) return rc;
-    if (cudaFuncSetAttribute(attention_q8_decode_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)decode_smem<HD, NT>()) != cudaSuccess)
+    if (p.slices > 0) {
+        // a CTA, or a cluster of them, a pair
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[2];
+        rc = cluster_config<HD, NT>(cfg, attr, p.slices);
+        if (rc) return rc;
+        cfg.gridDim = dim3((unsigned)p.nseq * p.nkv * p.slices);
+        cfg.stream = stream;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = g_kestrel_pdl ? 2 : 1;
+        cudaLaunchKernelEx(&cfg, attention_q8_decode_kernel<HD, NT, true>, mk, mv, p);
+        return kestrel_check_launch("attention_q8 decode");
+    }
+    if (cudaFuncSetAttribute(attention_q8_decode_kernel<HD, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)decode_smem<HD, NT>()) != cudaSuccess)
         return kestrel_fail(-3, "attention_q8: cannot raise the shared-memory limit: %s", cudaGetErrorString(cudaGetLastError()));
-    kestrel_launch(attention_q8_decode_kernel<HD, NT>, dim3(ctas), dim3(THREADS), decode_smem<HD, NT>(), stream, mk, mv, p);
+    kestrel_launch(attention_q8_decode_kernel<HD, NT, false>, dim3(ctas), dim3(THREADS), decode_smem<HD, NT>(), stream, mk, mv, p);
     rc = kestrel_check_launch("attention_q8 decode");
     if (rc) return rc;
     kestrel_launch(attention_q8_join_kernel<HD>, dim3(p.nseq, p.nkv), dim3(256), 0, stream, p, ctas);
     return kestrel_check_launch("attention_q8 join");
+}
+
+// Clusters of `size` CTAs that the current device holds at once.  A cluster lies within one GPC, so they are fewer than the CTAs' places
+// divided by their size.  Asked of the runtime once a device, head size, rows and size.
+template <int HD, int NT>
+int resident_clusters(int size) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    if (cluster_config<HD, NT>(cfg, attr, size)) return 0;
+    cfg.gridDim = dim3(size);
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, attention_q8_decode_kernel<HD, NT, true>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    return n;
 }
 
 }  // namespace
@@ -623,6 +761,28 @@ int q8_launch_decode(const Q8Params &p, int ctas, int most_rows, cudaStream_t st
 int q8_decode_ctas(long long tiles, int hd, int most_rows) {
     const long long most = (most_rows <= 8 ? (hd == 64 ? Ring<64, 1>::CTAS : Ring<128, 1>::CTAS) : (hd == 64 ? Ring<64, 2>::CTAS : Ring<128, 2>::CTAS)) * (long long)kestrel_sms();
     return (int)(tiles / 2 < 1 ? 1 : tiles / 2 < most ? tiles / 2 : most);
+}
+
+// CTAs a pair, or 0 for stretches.  As many as let every cluster be resident, up to 8, and two tiles each; taken where the longest pair's
+// share is no more than six tiles above a stretch, which is about what the join kernel takes.
+int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int hd, int most_rows) {
+    static DeviceTable<4 * (MAX_CLUSTER + 1)> known;
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) {
+        cudaGetLastError();
+        dev = -1;
+    }
+    const long long stretch = (tiles + q8_decode_ctas(tiles, hd, most_rows) - 1) / q8_decode_ctas(tiles, hd, most_rows);
+    for (int size = longest_tiles / 2 < MAX_CLUSTER ? (longest_tiles < 2 ? 1 : longest_tiles / 2) : MAX_CLUSTER; size >= 1; --size) {
+        if ((longest_tiles + size - 1) / size > stretch + 6) return 0;
+        const int at = ((hd == 64 ? 2 : 0) + (most_rows <= 8 ? 1 : 0)) * (MAX_CLUSTER + 1) + size;
+        const int n = known.get(dev, at, [&] {
+            return hd == 64 ? (most_rows <= 8 ? resident_clusters<64, 1>(size) : resident_clusters<64, 2>(size))
+                            : (most_rows <= 8 ? resident_clusters<128, 1>(size) : resident_clusters<128, 2>(size));
+        });
+        if (pairs <= n) return size;
+    }
+    return 0;
 }
 
 long long q8_decode_scratch(int ctas, int hd) { return 2ll * ctas * 16 * (hd + 2); }
