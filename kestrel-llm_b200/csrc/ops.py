@@ -8,6 +8,7 @@ first call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import NamedTuple, Optional
 
@@ -97,7 +98,7 @@ _here = _Here()
 
 def _on(device: torch.device):
     """A context in which ``device`` is the current one: kernels launch on the device of their tensors, on its current stream."""
-    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _here if device.index == (_raw_device or torch.cuda.current_device)() else torch.cuda.device(device)
 
 
 def _need(t: torch.Tensor, name: str, dtype=None, dims: Optional[int] = None) -> None:
@@ -348,28 +349,34 @@ Q8_BLOCK = _cdecl.constants()["KESTREL_Q8_BLOCK"]       # tokens that share a sc
 def _need_q8(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, nkv: int, page_size: int, hd: int,
              device: torch.device) -> None:
     """Planes of the cache: int8 codes [pages, kv heads, page size, head size], float32 scales [pages, kv heads, page size / Q8_BLOCK]."""
+    shape = (k_cache.shape[0], nkv, page_size, hd)
+    blocks = (shape[0], nkv, page_size // Q8_BLOCK)
+    d = device.index
+    if (page_size % Q8_BLOCK == 0 and k_cache.dtype is v_cache.dtype is torch.int8 and k_scale.dtype is v_scale.dtype is torch.float32
+            and k_cache.shape == shape and v_cache.shape == shape and k_scale.shape == blocks and v_scale.shape == blocks
+            and k_cache.get_device() == v_cache.get_device() == k_scale.get_device() == v_scale.get_device() == d
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+        return
     if page_size % Q8_BLOCK:
         raise KernelError(f"{what}: pages of {page_size} tokens are no whole blocks of {Q8_BLOCK}")
-    shape = (k_cache.shape[0], nkv, page_size, hd)
-    blocks = (k_cache.shape[0], nkv, page_size // Q8_BLOCK)
     for t, name, dtype, want in ((k_cache, "k_cache", torch.int8, shape), (v_cache, "v_cache", torch.int8, shape),
                                  (k_scale, "k_scale", torch.float32, blocks), (v_scale, "v_scale", torch.float32, blocks)):
-        if t.dtype != dtype or t.shape != want or not t.is_contiguous() or t.device != device:
-            _need(t, f"{what}.{name}", dtype, len(want))
-            if t.shape != want:
-                raise KernelError(f"{what}: {name} of shape {tuple(t.shape)}, expected {want}")
+        _need(t, f"{what}.{name}", dtype, len(want))
+        if t.shape != want:
+            raise KernelError(f"{what}: {name} of shape {tuple(t.shape)}, expected {want}")
+        if t.device != device:
             raise KernelError(f"{what}: {name} is on {t.device}, the queries on {device}")
 
 
 def _need_ints(what: str, device: torch.device, **tensors: torch.Tensor) -> None:
     for name, t in tensors.items():
-        if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != 1 or t.device != device:
+        if t.dtype is not torch.int32 or t.dim() != 1 or t.get_device() != device.index or not t.is_contiguous():
             _need(t, f"{what}.{name}", torch.int32, 1)
             raise KernelError(f"{what}: {name} is on {t.device}, the queries on {device}")
 
 
 def _need_table(what: str, block_table: torch.Tensor, device: torch.device) -> None:
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.device != device or block_table.shape[1] < 1:
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.get_device() != device.index or block_table.shape[1] < 1:
         raise KernelError(f"{what}: the block table must be int32 [requests, pages] on {device} with neighbouring entries, "
                           f"got {block_table.dtype} {tuple(block_table.shape)} on {block_table.device}")
 
@@ -412,6 +419,12 @@ def attn_prepare_q8(qkv: Partials, q_norm_w: Optional[torch.Tensor], k_norm_w: O
             v_scale.data_ptr(), q_out.data_ptr(), _code(q_out, "attn_prepare_q8.q_out"), T, nq, nkv, hd, 1 if write_kv else 0, _stream()))
 
 
+@functools.lru_cache(maxsize=1024)
+def _q8_scratch(device: int, n: int, max_count: int, max_kv: int, T: int, nq: int, nkv: int, hd: int, window: int, code: int) -> int:
+    """Floats of scratch that a step of single tokens, or a recorded one, needs on the current device: a matter of its sizes."""
+    return library().kestrel_attention_q8_scratch(None, None, n, max_count, max_kv, T, nq, nkv, hd, window, code)
+
+
 def attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, out: torch.Tensor,
                  batch, block_table: torch.Tensor, page_size: int, nq: int, nkv: int, hd: int, window: int, scale: float) -> None:
     """Causal attention of this step's queries (float32 or bfloat16 [T, nq * hd]) over their requests' pages of 8-bit codes
@@ -439,7 +452,10 @@ def attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     if not batch.captured and max_count > 1:        # steps of single tokens need no look at the lengths
         cu, kv = (ctypes.c_int * (n + 1))(*batch.cu_seqlens_host), (ctypes.c_int * n)(*batch.kv_lens_host)
     with _on(dev):
-        floats = lib.kestrel_attention_q8_scratch(cu, kv, n, max_count, max_kv, T, nq, nkv, hd, window, code)
+        if cu is None:
+            floats = _q8_scratch(dev.index, n, max_count, max_kv, T, nq, nkv, hd, window, code)
+        else:
+            floats = lib.kestrel_attention_q8_scratch(cu, kv, n, max_count, max_kv, T, nq, nkv, hd, window, code)
         scratch = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
         rc = lib.kestrel_attention_q8(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), out.data_ptr(), _p(scratch), floats,
@@ -481,9 +497,10 @@ def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, top
         _need_ints("token_logprobs", dev, ids=ids)
         if ids.shape[0] != R:
             raise KernelError(f"token_logprobs: {ids.shape[0]} tokens for {R} rows")
-        given = torch.empty(R, dtype=torch.float32, device=dev)
-    got = TokenLogprobs(given, torch.empty(R, dtype=torch.float32, device=dev), torch.empty((R, top), dtype=torch.int32, device=dev),
-                        torch.empty((R, top), dtype=torch.float32, device=dev))
+        given, entropy = logits.new_empty((2, R)).unbind()
+    else:
+        entropy = logits.new_empty(R)
+    got = TokenLogprobs(given, entropy, torch.empty((R, top), dtype=torch.int32, device=dev), logits.new_empty((R, top)))
     with _on(dev):
         _check(library().kestrel_token_logprobs(logits.data_ptr(), logits.stride(0), R, V, _p(ids), top, _p(given), got.entropy.data_ptr(),
                                                 got.top_ids.data_ptr(), got.top_logprobs.data_ptr(), _stream()))
