@@ -405,7 +405,7 @@ def attn_prepare_q8(qkv: Partials, q_norm_w: Optional[torch.Tensor], k_norm_w: O
         raise KernelError(f"attn_prepare_q8: {positions.shape[0]} positions and block tables of {block_table.shape[0]} requests for {T} tokens of {n} requests")
     _need_q8("attn_prepare_q8", k_cache, v_cache, k_scale, v_scale, nkv, page_size, hd, dev)
     for t, name, size in ((qkv.bias, "bias", qkv.width), (q_norm_w, "q_norm_w", hd), (k_norm_w, "k_norm_w", hd), (inv_freq, "inv_freq", rotary_dim // 2)):
-        if t is not None:
+        if t is not None and not (t.dtype is torch.float32 and t.dim() == 1 and t.shape[0] >= size and t.get_device() == dev.index and t.is_contiguous()):
             _need(t, f"attn_prepare_q8.{name}", torch.float32, 1)
             if t.shape[0] < size or t.device != dev:
                 raise KernelError(f"attn_prepare_q8: {name} of {t.shape[0]} numbers on {t.device}, expected {size} on {dev}")
@@ -492,17 +492,15 @@ def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, top
     dev = logits.device
     if not 0 <= top <= min(V, MAX_TOP_LOGPROBS):
         raise KernelError(f"token_logprobs: the {top} likeliest of {V} tokens; at most {MAX_TOP_LOGPROBS} are picked")
-    given = None
     if ids is not None:
         _need_ints("token_logprobs", dev, ids=ids)
         if ids.shape[0] != R:
             raise KernelError(f"token_logprobs: {ids.shape[0]} tokens for {R} rows")
-        given, entropy = logits.new_empty((2, R)).unbind()
-    else:
-        entropy = logits.new_empty(R)
-    got = TokenLogprobs(given, entropy, torch.empty((R, top), dtype=torch.int32, device=dev), logits.new_empty((R, top)))
+    buf = logits.new_empty(2 * R * (1 + top))       # one piece of memory: an allocation costs the host as much as a launch
+    got = TokenLogprobs(None if ids is None else buf.as_strided((R,), (1,), 0), buf.as_strided((R,), (1,), R),
+                        buf.view(torch.int32).as_strided((R, top), (top or 1, 1), 2 * R), buf.as_strided((R, top), (top or 1, 1), (2 + top) * R))
     with _on(dev):
-        _check(library().kestrel_token_logprobs(logits.data_ptr(), logits.stride(0), R, V, _p(ids), top, _p(given), got.entropy.data_ptr(),
+        _check(library().kestrel_token_logprobs(logits.data_ptr(), logits.stride(0), R, V, _p(ids), top, _p(got.logprobs), got.entropy.data_ptr(),
                                                 got.top_ids.data_ptr(), got.top_logprobs.data_ptr(), _stream()))
     return got
 
