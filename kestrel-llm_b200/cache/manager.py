@@ -3,7 +3,8 @@ device memory it describes.
 
 Layers are sorted into groups by what they must keep: all keys, or a window of them.  Each
 group has its own pool of pages and its own block table per request; layers of a group share
-the table, each with K and V planes of its own laid out [page][kv_head][slot][head_dim].
+the table, each with K and V planes of its own laid out [page][kv_head][slot][head_dim], in the model's
+type or as int8 codes beside one float32 scale for every 16 tokens and head [page][kv_head][slot / 16].
 Beside the pages, every live request owns one slot; layers that keep fixed-size state get a
 tensor [slots, *shape] indexed by it.
 """
@@ -19,6 +20,9 @@ import torch
 from ..csrc import build as _build
 from ..csrc import cdecl as _cdecl
 from ..parts.base import CacheSpec, FixedStateSpec, PagedKVSpec, paged_part, state_part
+
+
+Q8_BLOCK = _cdecl.constants()["KESTREL_Q8_BLOCK"]       # tokens that share a scale of 8-bit codes
 
 
 class CacheError(RuntimeError):
@@ -54,11 +58,12 @@ class GroupInfo:
 class LayerCache:
     """What one layer call sees of the cache."""
 
-    __slots__ = ("index", "group", "page_size", "k", "v", "state", "writable", "spec")
+    __slots__ = ("index", "group", "page_size", "k", "v", "state", "writable", "spec", "k_scale", "v_scale")
 
-    def __init__(self, index, group, page_size, k, v, state, writable, spec):
+    def __init__(self, index, group, page_size, k, v, state, writable, spec, k_scale=None, v_scale=None):
         self.index, self.group, self.page_size = index, group, page_size
         self.k, self.v, self.state, self.writable, self.spec = k, v, state, writable, spec
+        self.k_scale, self.v_scale = k_scale, v_scale       # of pages of 8-bit codes, else None
 
 
 class PageTable:
@@ -215,10 +220,17 @@ class CacheManager(PageTable):
     """Bookkeeping plus the device memory of every cache layer.
 
     ``specs[i]`` is what cache layer i keeps (a `PagedKVSpec`, a `FixedStateSpec` or None).
-    ``num_pages`` pages go to every group."""
+    ``num_pages`` pages go to every group.  ``codes``: pages hold 8-bit codes and scales; every paged
+    layer must say that it takes them."""
 
     def __init__(self, specs: Sequence[CacheSpec], dtype: torch.dtype, device, page_size: int,
-                 num_pages: int, max_requests: int, max_model_len: int):
+                 num_pages: int, max_requests: int, max_model_len: int, codes: bool = False):
+        if codes:
+            if page_size % Q8_BLOCK:
+                raise CacheError(f"pages of 8-bit codes hold whole blocks of {Q8_BLOCK} tokens, not {page_size}")
+            for i, sp in enumerate(map(paged_part, specs)):
+                if sp is not None and not sp.codes:
+                    raise CacheError(f"cache layer {i} has no form with 8-bit codes: its mixer reads keys and values in the model's type only")
         kinds: List[Tuple[int, int]] = []          # (window, kept first tokens) of each group
         members: List[List[int]] = []
         self.layer_group: List[int] = []
@@ -246,6 +258,9 @@ class CacheManager(PageTable):
         self.dtype, self.device = dtype, torch.device(device)
         self.k: List[Optional[torch.Tensor]] = []
         self.v: List[Optional[torch.Tensor]] = []
+        self.codes = bool(codes)
+        self.k_scale: List[Optional[torch.Tensor]] = []
+        self.v_scale: List[Optional[torch.Tensor]] = []
         self.state: List[Optional[torch.Tensor]] = []
         for spec in specs:            # a layer may keep pages, a state slot, both (`CombinedSpec`) or nothing
             sp, st = paged_part(spec), state_part(spec)
@@ -253,6 +268,14 @@ class CacheManager(PageTable):
                 # one page more than the manager hands out: the "null page", where padding tokens
                 # of a captured step write their keys and values
                 shape = (num_pages + 1, sp.kv_heads, page_size, sp.head_dim)
+                scales = shape[:2] + (page_size // Q8_BLOCK,) if codes else None
+                self.k_scale.append(torch.zeros(scales, dtype=torch.float32, device=device) if codes else None)
+                self.v_scale.append(torch.zeros(scales, dtype=torch.float32, device=device) if codes else None)
+                if codes:
+                    self.k.append(torch.zeros(shape, dtype=torch.int8, device=device))
+                    self.v.append(torch.zeros(shape, dtype=torch.int8, device=device))
+                    self.state.append(self._state_plane(st, max_requests))
+                    continue
                 self.k.append(torch.zeros(shape, dtype=dtype, device=device))
                 if sp.values_are_keys:
                     if sp.value_dim != sp.head_dim:
@@ -263,12 +286,16 @@ class CacheManager(PageTable):
             else:
                 self.k.append(None)
                 self.v.append(None)
-            if st is not None:
-                # one slot more than there are requests: the spare slot, which padding rows of a
-                # captured step use so that they never touch a live request's state
-                self.state.append(torch.zeros((max_requests + 1,) + tuple(st.shape), dtype=st.dtype, device=device))
-            else:
-                self.state.append(None)
+                self.k_scale.append(None)
+                self.v_scale.append(None)
+            self.state.append(self._state_plane(st, max_requests))
+
+    def _state_plane(self, st: Optional[FixedStateSpec], max_requests: int) -> Optional[torch.Tensor]:
+        if st is None:
+            return None
+        # one slot more than there are requests: the spare slot, which padding rows of a
+        # captured step use so that they never touch a live request's state
+        return torch.zeros((max_requests + 1,) + tuple(st.shape), dtype=st.dtype, device=self.device)
 
     def admit(self, rid: int) -> int:
         slot = super().admit(rid)
@@ -290,11 +317,14 @@ class CacheManager(PageTable):
 
     def layer(self, index: int, writable: bool = True) -> LayerCache:
         return LayerCache(index, self.layer_group[index], self.page_size, self.k[index], self.v[index],
-                          self.state[index], writable, self.specs[index])
+                          self.state[index], writable, self.specs[index], self.k_scale[index], self.v_scale[index])
 
-    def bytes_per_token(self) -> int:
-        n = 0
-        for sp in map(paged_part, self.specs):
-            if sp is not None:
-                n += sp.kv_heads * (sp.head_dim + (0 if sp.values_are_keys else sp.value_dim)) * torch.empty((), dtype=self.dtype).element_size()
-        return n
+    def bytes_per_token(self) -> float:
+        return sum(paged_bytes_per_token(sp, self.dtype, self.codes) for sp in map(paged_part, self.specs) if sp is not None)
+
+
+def paged_bytes_per_token(sp: PagedKVSpec, dtype: torch.dtype, codes: bool = False) -> float:
+    """Bytes of keys and values that one token takes in a layer's pages, its share of the scales of 8-bit codes included."""
+    if codes:
+        return sp.kv_heads * (sp.head_dim + sp.value_dim + 8 / Q8_BLOCK)
+    return sp.kv_heads * (sp.head_dim + (0 if sp.values_are_keys else sp.value_dim)) * torch.empty((), dtype=dtype).element_size()

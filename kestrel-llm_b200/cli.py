@@ -75,6 +75,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--prompt-file", default=None, help="one prompt a line, comma-separated token ids")
     ap.add_argument("--random-prompts", default=None, metavar="N:LEN:SEED")
     ap.add_argument("--page-size", type=int, default=16)
+    ap.add_argument("--cache-dtype", default="", choices=["", "int8"], help="how the cache keeps keys and values: as the model computes, or as 8-bit codes")
     ap.add_argument("--max-tokens", type=int, default=0, help="tokens the cache holds (0: batch-max * max-model-len)")
     ap.add_argument("--max-model-len", type=int, default=0)
     ap.add_argument("--max-step-tokens", type=int, default=2048)
@@ -133,7 +134,7 @@ def main(argv=None) -> int:
               max_queued=max(args.max_queued, 1), prefill_batch=args.prefill_batch,
               max_step_tokens=args.max_step_tokens, max_tokens=args.max_tokens,
               max_model_len=args.max_model_len, seed=args.seed, profile=args.profile, debug_guards=args.debug_guards,
-              cuda_graphs=bool(args.cuda_graphs))
+              cuda_graphs=bool(args.cuda_graphs), cache_dtype=args.cache_dtype)
     c = llm.model.config
     # sizes every architecture's configuration has; head counts where this one names them
     heads = "".join(f" {tag}={getattr(c, key)}" for tag, key in (("heads", "num_attention_heads"), ("kv", "num_key_value_heads"))

@@ -12,6 +12,7 @@ from dataclasses import dataclass
 @dataclass
 class EngineOptions:
     dtype: str = "bfloat16"          # "bfloat16" (serving kernels) or "float32" (true 32-bit path)
+    cache_dtype: str = ""            # how keys and values are kept: "" as the model computes, "int8" codes with a scale for every 16 tokens and head
     page_size: int = 16              # tokens per cache page
     num_pages: int = 0               # pages per cache group; 0 = derive from max_tokens
     max_tokens: int = 0              # tokens all live requests may hold; 0 = what fits the device's free memory, at most batch_max * max_model_len
@@ -27,6 +28,13 @@ class EngineOptions:
     profile: bool = False            # time the phases of every step with CUDA events and print them in the reference's formats
     debug_guards: bool = False       # check every step's description on the device and guard words behind every activation
     device: str = "cuda:0"
+
+    @property
+    def cache_codes(self) -> bool:
+        """Whether the cache holds 8-bit codes."""
+        if self.cache_dtype not in ("", "int8"):
+            raise ValueError(f"cache_dtype '{self.cache_dtype}' is neither '' (the model's) nor 'int8'")
+        return self.cache_dtype == "int8"
 
     def normalised_dtype(self) -> str:
         d = {"bf16": "bfloat16", "bfloat16": "bfloat16", "fp32": "float32", "float32": "float32",

@@ -45,6 +45,7 @@ struct Op {
     const float *bias = nullptr;
     const float *w2 = nullptr, *w3 = nullptr;      // norm weights of attn_prepare; inv_freq
     const void *k_cache = nullptr, *v_cache = nullptr;
+    float *k_scale = nullptr, *v_scale = nullptr;  // pages of 8-bit codes (null: pages of the program's type)
     void *planner = nullptr;
     int N = 0, K = 0, width = 0, dtype = 0, flag = 0;
     int nq = 0, nkv = 0, hd = 0, window = 0, group = 0, page_size = 0, cache_pages = 0, rot = 0, rot_mode = 0;
@@ -195,7 +196,7 @@ struct Walk {
                             break;
                         }
                     }
-                    if (!dry && bf16 && op.b < 0 && oi + 1 < pg.ops.size() && pg.ops[oi + 1].kind == OP_ATTN_PREPARE && pg.ops[oi + 1].a == op.out) {
+                    if (!dry && bf16 && op.b < 0 && oi + 1 < pg.ops.size() && pg.ops[oi + 1].kind == OP_ATTN_PREPARE && pg.ops[oi + 1].a == op.out && !pg.ops[oi + 1].k_scale) {
                         // a q, k, v product of many tokens does its consumer's work in its epilogue, where
                         // that kernel takes the sizes; the product's float32 plane is then never made (a
                         // dry walk counts both the plane and the queries: an upper bound)
@@ -275,11 +276,18 @@ struct Walk {
                             return kestrel_fail(-2, "step program: op %zu: the register is not a q, k, v product of %d + 2 x %d heads", oi, op.nq, op.nkv);
                         if (op.group < 0 || op.group >= layout[KB_NUM_GROUPS])
                             return kestrel_fail(-2, "step program: op %zu: cache group %d of %d", oi, op.group, layout[KB_NUM_GROUPS]);
-                        rc = kestrel_attn_prepare((const float *)qkv.ptr, qkv.slices, (long long)T * qkv.cols, qkv.bias, op.w2, op.w3, op.eps,
-                                                  (const float *)op.w, op.rot, op.rot_mode, op.rot_scale, dev + layout[KB_O_POSITIONS],
-                                                  dev + layout[KB_O_SEQ_OF_TOKEN], dev + layout[KB_O_TABLES] + (size_t)op.group * n * W, W,
-                                                  op.page_size, (void *)op.k_cache, (void *)op.v_cache, o.ptr, pg.dtype, T, op.nq, op.nkv,
-                                                  op.hd, op.flag, stream);
+                        if (op.k_scale)
+                            rc = kestrel_attn_prepare_q8((const float *)qkv.ptr, qkv.slices, (long long)T * qkv.cols, qkv.bias, op.w2, op.w3, op.eps,
+                                                         (const float *)op.w, op.rot, op.rot_mode, op.rot_scale, dev + layout[KB_O_POSITIONS],
+                                                         dev + layout[KB_O_CU_SEQLENS], n, dev + layout[KB_O_TABLES] + (size_t)op.group * n * W, W, W,
+                                                         op.page_size, op.cache_pages, (void *)op.k_cache, (void *)op.v_cache, op.k_scale, op.v_scale, o.ptr,
+                                                         pg.dtype, T, op.nq, op.nkv, op.hd, op.flag, stream);
+                        else
+                            rc = kestrel_attn_prepare((const float *)qkv.ptr, qkv.slices, (long long)T * qkv.cols, qkv.bias, op.w2, op.w3, op.eps,
+                                                      (const float *)op.w, op.rot, op.rot_mode, op.rot_scale, dev + layout[KB_O_POSITIONS],
+                                                      dev + layout[KB_O_SEQ_OF_TOKEN], dev + layout[KB_O_TABLES] + (size_t)op.group * n * W, W,
+                                                      op.page_size, (void *)op.k_cache, (void *)op.v_cache, o.ptr, pg.dtype, T, op.nq, op.nkv,
+                                                      op.hd, op.flag, stream);
                         launches++;
                     }
                     break;
@@ -289,6 +297,22 @@ struct Walk {
                     Reg &o = regs[op.out];
                     o.rows = T; o.cols = op.nq * op.hd; o.dtype = pg.dtype;
                     o.ptr = take((size_t)T * o.cols * elem_size(pg.dtype), false);
+                    if (op.k_scale) {
+                        if (op.group < 0 || op.group >= layout[KB_NUM_GROUPS])
+                            return kestrel_fail(-2, "step program: op %zu: cache group %d of %d", oi, op.group, layout[KB_NUM_GROUPS]);
+                        const int *cu_h = host + layout[KB_O_CU_SEQLENS], *kv_h = host + layout[KB_O_KV_LENS];
+                        const long long floats = kestrel_attention_q8_scratch(cu_h, kv_h, n, layout[KB_MAX_COUNT], layout[KB_MAX_KV_LEN], T, op.nq, op.nkv,
+                                                                              op.hd, op.window, pg.dtype);
+                        float *scratch = floats ? (float *)take((size_t)floats * 4, false) : nullptr;
+                        if (!dry) {
+                            rc = kestrel_attention_q8(q.ptr, op.k_cache, op.v_cache, op.k_scale, op.v_scale, o.ptr, scratch, floats, cu_h, kv_h,
+                                                      dev + layout[KB_O_CU_SEQLENS], dev + layout[KB_O_KV_LENS],
+                                                      dev + layout[KB_O_TABLES] + (size_t)op.group * n * W, n, layout[KB_MAX_COUNT], layout[KB_MAX_KV_LEN], W, W,
+                                                      op.page_size, op.cache_pages, T, op.nq, op.nkv, op.hd, op.window, op.scale, pg.dtype, stream);
+                            if (rc > 0) launches += rc, rc = 0;
+                        }
+                        break;
+                    }
                     if (!dry) {
                         rc = kestrel_attention(op.planner, r.serial, host, dev, layout, op.group, 0, q.ptr, op.k_cache, op.v_cache, o.ptr, pg.dtype,
                                                op.cache_pages, op.page_size, op.nq, op.nkv, op.hd, op.window, op.scale, stream);
@@ -439,6 +463,29 @@ KESTREL_API int kprog_attention(void *prog, int q, void *planner, int group, int
     op.window = window; op.scale = scale; op.out = pg.new_reg();
     pg.ops.push_back(op);
     return op.out;
+}
+
+// The same two over pages of 8-bit codes (kestrel_attn_prepare_q8, kestrel_attention_q8)
+KESTREL_API int kprog_attn_prepare_q8(void *prog, int qkv, const float *q_norm_w, const float *k_norm_w, float norm_eps, const float *inv_freq, int rot,
+                                      int rot_mode, float rot_scale, int group, int page_size, int cache_pages, void *k_cache, void *v_cache,
+                                      float *k_scale, float *v_scale, int nq, int nkv, int hd, int write_kv, int tag) {
+    KESTREL_REQUIRE(k_scale && v_scale && cache_pages > 0, "step program: attn_prepare_q8 without scales");
+    const int out = kprog_attn_prepare(prog, qkv, q_norm_w, k_norm_w, norm_eps, inv_freq, rot, rot_mode, rot_scale, group, page_size, k_cache, v_cache, nq, nkv,
+                                       hd, write_kv, tag);
+    if (out < 0) return out;
+    Op &op = ((Program *)prog)->ops.back();
+    op.k_scale = k_scale; op.v_scale = v_scale; op.cache_pages = cache_pages;
+    return out;
+}
+
+KESTREL_API int kprog_attention_q8(void *prog, int q, int group, int page_size, int cache_pages, const void *k_cache, const void *v_cache,
+                                   const float *k_scale, const float *v_scale, int nq, int nkv, int hd, int window, float scale, int tag) {
+    KESTREL_REQUIRE(k_scale && v_scale, "step program: attention_q8 without scales");
+    const int out = kprog_attention(prog, q, nullptr, group, page_size, cache_pages, k_cache, v_cache, nq, nkv, hd, window, scale, tag);
+    if (out < 0) return out;
+    Op &op = ((Program *)prog)->ops.back();
+    op.k_scale = (float *)k_scale; op.v_scale = (float *)v_scale;
+    return out;
 }
 
 KESTREL_API int kprog_logits(void *prog, int x, const void *w, long long ldw, int V, int K, int tag) {

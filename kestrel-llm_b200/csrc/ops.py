@@ -2831,6 +2831,23 @@ class StepProgram:
             self._ptr(k_cache, "k_cache", self.dtype), self._ptr(v_cache, "v_cache", self.dtype), nq, nkv, hd, int(window),
             float(scale), PHASES[phase]))
 
+    def attn_prepare_q8(self, qkv: int, q_norm_w, k_norm_w, norm_eps: float, inv_freq, rotary_dim: int, rot_mode: int, rot_scale: float, group: int,
+                        page_size: int, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, nq: int, nkv: int,
+                        hd: int, write_kv: bool, phase: str = "rope") -> int:
+        _need_q8("program.attn_prepare_q8", k_cache, v_cache, k_scale, v_scale, nkv, page_size, hd, k_cache.device)
+        return self._reg(self._lib.kprog_attn_prepare_q8(
+            self._h, qkv, self._ptr(q_norm_w, "q_norm", torch.float32), self._ptr(k_norm_w, "k_norm", torch.float32),
+            float(norm_eps), self._ptr(inv_freq, "inv_freq", torch.float32), int(rotary_dim), int(rot_mode), float(rot_scale),
+            int(group), int(page_size), int(k_cache.shape[0]), self._ptr(k_cache, "k_cache"), self._ptr(v_cache, "v_cache"),
+            self._ptr(k_scale, "k_scale"), self._ptr(v_scale, "v_scale"), nq, nkv, hd, 1 if write_kv else 0, PHASES[phase]))
+
+    def attention_q8(self, q: int, group: int, page_size: int, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                     v_scale: torch.Tensor, nq: int, nkv: int, hd: int, window: int, scale: float, phase: str = "attn") -> int:
+        _need_q8("program.attention_q8", k_cache, v_cache, k_scale, v_scale, nkv, page_size, hd, k_cache.device)
+        return self._reg(self._lib.kprog_attention_q8(
+            self._h, q, int(group), int(page_size), int(k_cache.shape[0]), self._ptr(k_cache, "k_cache"), self._ptr(v_cache, "v_cache"),
+            self._ptr(k_scale, "k_scale"), self._ptr(v_scale, "v_scale"), nq, nkv, hd, int(window), float(scale), PHASES[phase]))
+
     def logits(self, x: int, weight: torch.Tensor, phase: str = "lm_head") -> None:
         _need(weight, "program.logits.weight", self.dtype, 2)
         self._reg(self._lib.kprog_logits(self._h, x, self._ptr(weight, "weight"), weight.stride(0), weight.shape[0],

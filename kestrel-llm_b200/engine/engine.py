@@ -16,7 +16,7 @@ from typing import Dict, List, Optional, Sequence
 import numpy as np
 import torch
 
-from ..cache.manager import CacheManager, OutOfPages
+from ..cache.manager import CacheManager, OutOfPages, paged_bytes_per_token
 from ..config.engine_options import EngineOptions
 from ..csrc import ops
 from .batch import Entry, StepBatch
@@ -42,7 +42,7 @@ class Engine:
         else:
             num_pages = self._pages_that_fit(model, options, page)
         self.cache = CacheManager(model.cache_specs(), model.dtype, dev, page, num_pages,
-                                  options.batch_max, self.max_model_len)
+                                  options.batch_max, self.max_model_len, codes=options.cache_codes)
         self.vocab_size = model.vocab_size
         self.graphs = None
         if options.cuda_graphs and getattr(model, "graph_safe", False):
@@ -73,9 +73,7 @@ class Engine:
         import sys
         from ..parts.base import paged_part
         want = options.batch_max * self.max_model_len
-        esize = torch.empty((), dtype=model.dtype).element_size()
-        per_token = sum(sp.kv_heads * (sp.head_dim + (0 if sp.values_are_keys else sp.value_dim)) * esize for sp in map(paged_part, model.cache_specs())
-                        if sp is not None)
+        per_token = sum(paged_bytes_per_token(sp, model.dtype, options.cache_codes) for sp in map(paged_part, model.cache_specs()) if sp is not None)
         if per_token == 0:
             return max(1, (want + page - 1) // page)
         free, _total = torch.cuda.mem_get_info(model.device)
@@ -84,7 +82,7 @@ class Engine:
         fit = int(max(0, free * options.memory_fraction - reserve) // per_token)
         tokens = min(want, fit)
         if tokens < self.max_model_len:
-            raise RuntimeError(f"the device has room for a cache of {fit} tokens ({per_token} bytes a token), less than one "
+            raise RuntimeError(f"the device has room for a cache of {fit} tokens ({per_token:g} bytes a token), less than one "
                                f"request of max_model_len {self.max_model_len}; lower max_model_len")
         if tokens < want:
             print(f"[kestrel] cache: {tokens} tokens ({tokens * per_token / 2**30:.1f} GiB) fit the device's free memory; "

@@ -19,7 +19,7 @@ from __future__ import annotations
 
 import time
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional, Sequence, Union
+from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -47,12 +47,24 @@ class RequestMetrics:
 
 
 @dataclass
+class TokenScore:
+    """A token under the softmax of the logits that it was picked from, or that a prompt's tokens before it led to (repetition penalties
+    included, temperature and filters not): its natural log probability, the distribution's entropy in nats, and the likeliest tokens with
+    their log probabilities, most likely first, equal ones by id."""
+    token_id: int
+    logprob: float
+    entropy: float
+    top: List[Tuple[int, float]] = field(default_factory=list)
+
+
+@dataclass
 class RequestOutput:
     request_id: int
     prompt_token_ids: List[int]
     token_ids: List[int] = field(default_factory=list)
     finish_reason: Optional[str] = None       # "stop" | "length", as the reference reports them
     preemptions: int = 0
+    logprobs: Optional[List[TokenScore]] = None       # one entry a token, if the request asked for them
     metrics: RequestMetrics = field(default_factory=RequestMetrics)
 
 
@@ -77,6 +89,32 @@ class _InFlight:
     decode_only: bool           # every entry of the step was a single decode token
     counted: bool = False       # the scheduler already counts these tokens
     discard: set = field(default_factory=set)      # requests that ended before this step's token was read
+    scores: Optional["_HostScores"] = None          # of the sampled tokens, if a request asked for them
+
+
+class _HostScores:
+    """Pinned memory for the results of one `ops.token_logprobs` call, and what is on its way there."""
+
+    def __init__(self, rows: int, top: int):
+        self.rows, self.top = rows, top
+        self.floats = torch.empty(2 * rows * (1 + top), dtype=torch.float32).pin_memory()
+        self.n = self.k = 0
+
+    def fetch(self, got: ops.TokenLogprobs) -> int:
+        """Starts the copies; returns their bytes."""
+        self.n, self.k = got.top_ids.shape
+        for part, t in zip(self._parts(), got):
+            part.copy_(t, non_blocking=True)
+        return 8 * self.n * (1 + self.k)
+
+    def _parts(self):
+        n, k, f = self.n, self.k, self.floats
+        return (f[:n], f[n:2 * n], f[2 * n:(2 + k) * n].view(torch.int32).view(n, k), f[(2 + k) * n:2 * (1 + k) * n].view(n, k))
+
+    def scores(self, tokens: Sequence[int], tops: Sequence[int]) -> List[TokenScore]:
+        """Once the copies have run: row r's token and its ``tops[r]`` likeliest alternatives."""
+        lp, h, ids, tlp = (t.tolist() for t in self._parts())
+        return [TokenScore(int(t), lp[r], h[r], list(zip(ids[r][:k], tlp[r][:k]))) for r, (t, k) in enumerate(zip(tokens, tops))]
 
 
 @dataclass
@@ -126,6 +164,7 @@ class LLM:
         self._ahead: Optional[_InFlight] = None
         self._pinned = [torch.empty(opts.batch_max + 8, dtype=torch.int32).pin_memory() for _ in range(3)]
         self._pinned_turn = 0
+        self._scores: List[Optional[_HostScores]] = [None] * len(self._pinned)
         self.run_ahead = not opts.profile   # False: every step's ids are read before the next step is built
         self.record_steps = False       # True: every step leaves a `StepRecord` in `step_records`
         self.step_records: List[StepRecord] = []
@@ -147,6 +186,8 @@ class LLM:
         seed = params.seed if params.seed is not None else (self.options.seed * 1000003 + rid)
         lv = _Live(RequestOutput(rid, prompt), params, seed, frozenset(stop), t_start=time.perf_counter())
         lv.out.metrics.prompt_tokens = len(prompt)
+        if params.logprobs is not None:
+            lv.out.logprobs = []
         self._live[rid] = lv
         return rid
 
@@ -246,25 +287,37 @@ class LLM:
                                       [lv.sampled for lv in lives], [lv.out.token_ids for lv in lives])
         for lv in lives:
             lv.sampled += 1
-        host = self._pinned[self._pinned_turn]
-        self._pinned_turn = (self._pinned_turn + 1) % len(self._pinned)
+        turn = self._pinned_turn
+        host = self._pinned[turn]
+        self._pinned_turn = (turn + 1) % len(self._pinned)
         host[:len(lives)].copy_(ids_dev, non_blocking=True)
+        scores = None
+        if any(lv.params.logprobs is not None for lv in lives):
+            top = min(max(lv.params.logprobs or 0 for lv in lives), self.engine.vocab_size)
+            got = ops.token_logprobs(logits, ids_dev, top)
+            scores = self._scores[turn]
+            if scores is None or scores.rows < len(lives) or scores.top < top:
+                scores = self._scores[turn] = _HostScores(len(host), top)
+            self.stats.d2h_bytes += scores.fetch(got)
         done = torch.cuda.Event()
         done.record()
         self.stats.d2h_bytes += 4 * len(lives)
-        return _InFlight(lives, ids_dev, host, done, decode_only)
+        return _InFlight(lives, ids_dev, host, done, decode_only, scores=scores)
 
     def _finalize(self, flight: _InFlight, newer: Optional[_InFlight]) -> List[RequestOutput]:
         """Waits for a step's ids, appends them and ends the requests that are over; a request
         that ends is struck from ``newer``, the step launched after this one."""
         flight.done.synchronize()
         ids = flight.ids_host[:len(flight.lives)].tolist()          # the step's only read-back: one id per request
+        scores = flight.scores.scores(ids, [lv.params.logprobs or 0 for lv in flight.lives]) if flight.scores is not None else None
         finished: List[RequestOutput] = []
-        for lv, tok in zip(flight.lives, ids):
+        for row, (lv, tok) in enumerate(zip(flight.lives, ids)):
             rid = lv.out.request_id
             if rid in flight.discard or self._live.get(rid) is not lv:
                 continue
             lv.out.token_ids.append(int(tok))
+            if lv.out.logprobs is not None:
+                lv.out.logprobs.append(scores[row])
             self.stats.generated_tokens += 1
             now = time.perf_counter()
             m = lv.out.metrics
@@ -343,6 +396,74 @@ class LLM:
         done = self.run_until_done()
         self.stats.seconds += time.perf_counter() - t0
         return [done[r] for r in rids]
+
+    def score(self, prompts: Sequence[Sequence[int]], top: int = 0) -> List[List[TokenScore]]:
+        """The log probability of every token of every prompt after its first, given the tokens before it, with the ``top`` likeliest tokens
+        at its place: how well the model foresees a text, and what a cache of another type changes.  Runs steps of its own, while no request
+        is live; nothing of the prompts stays in the cache."""
+        if self.has_unfinished():
+            raise RuntimeError("score() runs steps of its own: requests are live")
+        if not 0 <= top <= min(ops.MAX_TOP_LOGPROBS, self.engine.vocab_size):
+            raise ValueError(f"the {top} likeliest tokens are not within 0..{min(ops.MAX_TOP_LOGPROBS, self.engine.vocab_size)}")
+        texts = [[int(t) for t in p] for p in prompts]
+        for p in texts:
+            for t in p:
+                if not 0 <= t < self.engine.vocab_size:
+                    raise ValueError(f"token id {t} outside the vocabulary of {self.engine.vocab_size}")
+            if len(p) > self.engine.max_model_len:
+                raise ValueError(f"a prompt of {len(p)} tokens exceeds max_model_len {self.engine.max_model_len}")
+        out: List[List[TokenScore]] = [[] for _ in texts]
+        engine, cache = self.engine, self.engine.cache
+        budget = min(self.options.max_step_tokens, self.options.prefill_batch)
+        waiting = [i for i, p in enumerate(texts) if len(p) > 1]
+        running: List[Tuple[int, int]] = []              # (text, request id)
+        try:
+            while waiting or running:
+                # as many texts at once as the step has tokens, and the cache slots and pages for all of their tokens
+                left = budget - sum(min(budget, len(texts[i]) - 1 - cache.length(r)) for i, r in running)
+                while waiting and left > 0 and cache.free_slots() > 0:
+                    i = waiting[0]
+                    pages = -(-(sum(len(texts[j]) for j, _ in running) + len(texts[i])) // cache.page_size) + len(running)
+                    held = [sum(cache.num_blocks(r, g) for _, r in running) for g in range(cache.num_groups)]
+                    if running and any(pages > cache.free_pages(g) + held[g] for g in range(cache.num_groups)):
+                        break
+                    rid = self._next_id
+                    self._next_id += 1
+                    engine.admit(rid)
+                    running.append((i, rid))
+                    waiting.pop(0)
+                    left -= min(budget, len(texts[i]) - 1)
+                entries, given, room = [], [], budget
+                for i, r in running:
+                    at = cache.length(r)
+                    n = min(room, len(texts[i]) - 1 - at)          # the last token has nothing behind it to score
+                    if n > 0:
+                        entries.append(Entry(r, texts[i][at:at + n], range(n)))
+                        given += texts[i][at + 1:at + 1 + n]
+                        room -= n
+                logits = engine.step(entries, checked=True)
+                ids = torch.tensor(given, dtype=torch.int32).to(logits.device)
+                got = ops.token_logprobs(logits, ids, top)
+                host = _HostScores(len(given), top)
+                host.fetch(got)
+                torch.cuda.current_stream(logits.device).synchronize()
+                rows = iter(host.scores(given, [top] * len(given)))
+                owner = {r: i for i, r in running}
+                for e in entries:
+                    out[owner[e.rid]] += [next(rows) for _ in e.tokens]
+                still = []
+                for i, r in running:
+                    if cache.length(r) >= len(texts[i]) - 1:
+                        engine.release(r)
+                    else:
+                        still.append((i, r))
+                running = still
+            ops.raise_on_kernel_error()
+        finally:
+            for _, r in running:
+                if cache.is_live(r):
+                    engine.release(r)
+        return out
 
     def run_until_done(self, on_step=None) -> Dict[int, RequestOutput]:
         """Steps until no request is left; returns the finished requests by id.  ``on_step`` is

@@ -538,6 +538,9 @@ KESTREL_API int kprog_gate_up_swiglu(void *prog, int x, const void *w, long long
 KESTREL_API int kprog_attn_prepare(void *prog, int qkv, const float *q_norm_w, const float *k_norm_w, float norm_eps, const float *inv_freq, int rot, int rot_mode, float rot_scale, int group, int page_size, void *k_cache, void *v_cache, int nq, int nkv, int hd, int write_kv, int tag);
 /* causal attention of the step's queries over their requests' pages */
 KESTREL_API int kprog_attention(void *prog, int q, void *planner, int group, int page_size, int cache_pages, const void *k_cache, const void *v_cache, int nq, int nkv, int hd, int window, float scale, int tag);
+/* the two over pages of 8-bit codes (kestrel_attn_prepare_q8, kestrel_attention_q8) */
+KESTREL_API int kprog_attn_prepare_q8(void *prog, int qkv, const float *q_norm_w, const float *k_norm_w, float norm_eps, const float *inv_freq, int rot, int rot_mode, float rot_scale, int group, int page_size, int cache_pages, void *k_cache, void *v_cache, float *k_scale, float *v_scale, int nq, int nkv, int hd, int write_kv, int tag);
+KESTREL_API int kprog_attention_q8(void *prog, int q, int group, int page_size, int cache_pages, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, int nq, int nkv, int hd, int window, float scale, int tag);
 /* float32 logits [R, V] = x w^T for the wanted rows: the program's result */
 KESTREL_API int kprog_logits(void *prog, int x, const void *w, long long ldw, int V, int K, int tag);
 KESTREL_API int kprog_num_ops(void *prog);

@@ -4,7 +4,9 @@ q, k, v = W{q,k,v} x (+bias) in one fused product; optional per-head RMSNorm of 
 (st.c:9541-9561); rotation (st.c:8950-8991); K and V written to the request's pages; each
 query attends to the keys of its request up to itself, or to the last ``window`` of them;
 kv head of query head h is (h * kv_heads) / heads (st.c:10782); scale 1/sqrt(head_dim)
-(st.c:16549); output projection (st.c:16622-16626).  With ``reads_cache_only`` the layer
+(st.c:16549); output projection (st.c:16622-16626).  The pages may hold 8-bit codes with a scale for
+every 16 tokens and head (the reference keeps int8 rows with a scale per token and head by default,
+st.c:8432-8461, 16497-16526).  With ``reads_cache_only`` the layer
 writes nothing and attends over a cache that an earlier layer of the same step filled.
 """
 from __future__ import annotations
@@ -52,7 +54,7 @@ class GroupedQueryAttention(Mixer):
         self.graph_safe = heads // kv_heads <= 16
 
     def cache_spec(self) -> PagedKVSpec:
-        return PagedKVSpec(self.kv_heads, self.head_dim, self.window)
+        return PagedKVSpec(self.kv_heads, self.head_dim, self.window, codes=self.head_dim % 16 == 0)
 
     def weight_slots(self) -> List[WeightSlot]:
         p = self.prefix
@@ -74,6 +76,15 @@ class GroupedQueryAttention(Mixer):
         q = torch.empty((T, self.heads * self.head_dim), dtype=self.dtype, device=x.device)
         rot = self.position.rotary() if self.position is not None else None
         table = batch.block_table(cache.group)
+        if cache.k_scale is not None:
+            ops.attn_prepare_q8(self.qkv.forward(x), self.q_norm, self.k_norm, self.qk_norm_eps or 0.0, rot.inv_freq if rot else None,
+                                rot.dim if rot else 0, batch.positions, batch.cu_seqlens, table, cache.page_size, cache.k, cache.v, cache.k_scale,
+                                cache.v_scale, q, self.heads, self.kv_heads, self.head_dim, cache.writable, rot.mode if rot else 0,
+                                rot.scale if rot else 1.0)
+            a = torch.empty_like(q)
+            ops.attention_q8(q, cache.k, cache.v, cache.k_scale, cache.v_scale, a, batch, table, cache.page_size, self.heads, self.kv_heads,
+                             self.head_dim, self.window, self.scale)
+            return self.out.forward(a, residual=residual)
         prepare = dict(q_norm_w=self.q_norm, k_norm_w=self.k_norm, norm_eps=self.qk_norm_eps or 0.0,
                        inv_freq=rot.inv_freq if rot else None, rotary_dim=rot.dim if rot else 0, positions=batch.positions,
                        seq_of_token=batch.seq_of_token, block_table=table, page_size=cache.page_size, k_cache=cache.k,
@@ -90,6 +101,13 @@ class GroupedQueryAttention(Mixer):
     def emit(self, prog, x: int, residual: Optional[int], cache) -> int:
         qkv = self.qkv.emit(prog, x, phase="qkv")
         rot = self.position.rotary() if self.position is not None else None
+        if cache.k_scale is not None:
+            q = prog.attn_prepare_q8(qkv, self.q_norm, self.k_norm, self.qk_norm_eps or 0.0, rot.inv_freq if rot else None,
+                                     rot.dim if rot else 0, rot.mode if rot else 0, rot.scale if rot else 1.0, cache.group, cache.page_size,
+                                     cache.k, cache.v, cache.k_scale, cache.v_scale, self.heads, self.kv_heads, self.head_dim, cache.writable)
+            a = prog.attention_q8(q, cache.group, cache.page_size, cache.k, cache.v, cache.k_scale, cache.v_scale, self.heads, self.kv_heads,
+                                  self.head_dim, self.window, self.scale)
+            return self.out.emit(prog, a, residual=residual, phase="o")
         q = prog.attn_prepare(qkv, self.q_norm, self.k_norm, self.qk_norm_eps or 0.0, rot.inv_freq if rot else None,
                               rot.dim if rot else 0, rot.mode if rot else 0, rot.scale if rot else 1.0, cache.group,
                               cache.page_size, cache.k, cache.v, self.heads, self.kv_heads, self.head_dim, cache.writable)

@@ -40,13 +40,14 @@ class PagedKVSpec:
     layer may keep a request's first ``keep_first`` tokens visible (their pages are then never
     given back); values may have a size of their own.  With ``values_are_keys`` the layer caches ONE
     vector a token and head, read both as its key and as its value (a latent that both are expanded
-    from): the V plane is the K plane."""
+    from): the V plane is the K plane.  ``codes``: the mixer reads and writes pages of 8-bit codes too, where the engine asks for them."""
     kv_heads: int
     head_dim: int
     window: int = 0          # 0 = all keys
     keep_first: int = 0      # with a window: the first tokens of a request stay
     v_head_dim: int = 0      # 0 = head_dim
     values_are_keys: bool = False
+    codes: bool = False
 
     @property
     def value_dim(self) -> int:

@@ -20,8 +20,11 @@ class SamplingParams:
     seed: Optional[int] = None    # None: derived from the engine's seed and the request's number
     stop_token_ids: Tuple[int, ...] = ()
     ignore_eos: bool = False
+    logprobs: Optional[int] = None    # report every token's log probability and this many of the likeliest alternatives (0..32); None: no report
 
     def __post_init__(self):
+        if self.logprobs is not None and not 0 <= int(self.logprobs) <= 32:
+            raise ValueError(f"logprobs {self.logprobs} outside 0..32")
         if not 1 <= int(self.repetition_window) <= 64:
             raise ValueError(f"repetition_window {self.repetition_window} outside 1..64")
         if self.repetition_penalty >= 1e3:
