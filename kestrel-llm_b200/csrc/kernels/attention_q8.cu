@@ -167,7 +167,8 @@ __global__ void __launch_bounds__(THREADS) attention_q8_plain_kernel(const Q8Par
 }
 
 // ---- merge -------------------------------------------------------------------------------------------
-// A warp takes a row: lane s holds slice s's maximum and sum, the outputs are added in ascending order of the slices.
+// A warp takes a row: lane s holds slice s's maximum and sum, the outputs are added in ascending order of the slices; a lane takes four
+// neighbouring dimensions, four slices' in flight.
 template <typename T>
 __global__ void __launch_bounds__(256) attention_q8_merge_kernel(const Q8Params p) {
     pdl_launch_dependents();
@@ -179,13 +180,25 @@ __global__ void __launch_bounds__(256) attention_q8_merge_kernel(const Q8Params 
     const float2 ml = lane < p.slices ? *reinterpret_cast<const float2 *>(p.part_ml + (row * p.slices + lane) * 2) : make_float2(-INFINITY, 0.f);
     const float M = warp_max(ml.x), f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
     const float inv = 1.0f / warp_sum(f == 0.f && ml.y == ml.y ? 0.f : ml.y * f);       // (a sum that is no number stays that)
-    for (int d = lane; d < p.hd; d += 32) {
-        float acc = 0.f;
-        for (int s = 0; s < p.slices; ++s) {
-            const float fs = __shfl_sync(__activemask(), f, s);
-            if (fs != 0.f) acc = fmaf(p.part_o[(row * p.slices + s) * p.hd + d], fs, acc);
+    for (int d0 = 0; d0 < p.hd; d0 += 128) {
+        const int d = d0 + 4 * lane;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s0 = 0; s0 < p.slices; s0 += 4) {
+            float4 x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (s0 + j < p.slices && d < p.hd) x[j] = *reinterpret_cast<const float4 *>(p.part_o + (row * p.slices + s0 + j) * p.hd + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float fs = __shfl_sync(0xffffffffu, f, (s0 + j) & 31);
+                if (s0 + j >= p.slices || d >= p.hd || fs == 0.f) continue;
+                acc.x = fmaf(x[j].x, fs, acc.x); acc.y = fmaf(x[j].y, fs, acc.y); acc.z = fmaf(x[j].z, fs, acc.z); acc.w = fmaf(x[j].w, fs, acc.w);
+            }
         }
-        ((T *)p.out)[row * p.hd + d] = from_f32<T>(acc * inv);
+        if (d < p.hd) {
+            T *o = (T *)p.out + row * p.hd + d;
+            o[0] = from_f32<T>(acc.x * inv); o[1] = from_f32<T>(acc.y * inv); o[2] = from_f32<T>(acc.z * inv); o[3] = from_f32<T>(acc.w * inv);
+        }
     }
 }
 
@@ -223,7 +236,7 @@ enum Kernel { CORES, DECODE, TC };
 struct Part {
     Kernel kernel = CORES;
     int rows_above = 0, rows_upto = 0, rows_per_tile = 0, tiles = 0, slices = 1, longest = 0;
-    int ctas = 0, most_rows = 0;
+    int ctas = 0, most_rows = 0, row_tiles = 0;
     long long scratch = 0;              // floats
     long long key_tiles = 0;             // of 64, over all requests and kv heads
 };
@@ -240,11 +253,36 @@ int slices_for(long long ctas, int slots, int keys, int least) {
 // Rows follow from the host's copy of cu_seqlens; without it every request brings max_count tokens at most.
 void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, int max_kv, int T, int nq, int nkv, int hd, int window, int dtype) {
     const int G = nq / nkv;
+    auto seen_of = [&](int keys, long long rows) { return window > 0 ? std::min(keys, window + (int)((rows - 1) / G)) : keys; };
+    constexpr int FEW = 512;                // rows of a portion that may go to the decode kernel
     const bool cores = dtype != KESTREL_BF16 || (hd != 64 && hd != 128);
     Part small, large;
     small.kernel = cores ? CORES : DECODE;
     small.rows_upto = cores ? 0x7fffffff : 16;
-    small.rows_per_tile = cores ? BM : 16;
+    if (!cores && cu) {
+        // Short portions go to the decode kernel, which reads a request's keys again for every 16 rows, if that leaves no portion to the other
+        // kernel: where every pair has its CTAs at once and their work is little (32 / 8 heads of 128, one request, behind 500 keys: 16 tokens
+        // 10.9 us against 14.9, 64 tokens 13.8 against 16.7, 128 tokens 16.9 against 17.8; 64 tokens behind 2,000 keys 27 against 19; four
+        // requests of about 64 tokens, more pairs than CTAs, 30 against 10), and beside single tokens, which are a launch of the kernel anyway,
+        // for three times that (four requests of 2 to 8 tokens behind 2,000 keys 15 against 32, behind 8,000 34 against 51).
+        long long tiles = 0;
+        int most = 0, longest = 0;
+        bool single = false, all = true;
+        for (int i = 0; i < nseq; ++i) {
+            const long long rows = (long long)(cu[i + 1] - cu[i]) * G;
+            if (rows <= 0) continue;
+            single |= rows <= 16;
+            all &= rows <= FEW;
+            if (!all) break;
+            most = std::max(most, (int)rows);
+            longest = std::max(longest, seen_of(kv[i], rows));
+            tiles += (rows + 15) / 16 * nkv * ((seen_of(kv[i], rows) + 63) / 64);
+        }
+        const long long pairs = (long long)nseq * ((most + 15) / 16) * nkv;
+        if (all && most > 16 && tiles <= (single ? 24 : 8) * 2ll * kestrel_sms() &&
+            (q8_decode_cluster(pairs, (longest + 63) / 64, tiles, hd, most) > 0 || (single && pairs <= q8_decode_ctas(tiles, hd, most))))
+            small.rows_upto = FEW;
+    }
     large.kernel = TC;
     large.rows_above = small.rows_upto;
     large.rows_upto = 0x7fffffff;
@@ -258,14 +296,15 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
         }
         if (tiles * nkv <= kestrel_sms()) large.rows_per_tile = 128;
     }
+    small.rows_per_tile = cores ? BM : 16;
     auto count = [&](long long rows, int keys, int times) {
         if (rows <= 0) return;
         Part &p = rows <= small.rows_upto ? small : large;
-        const int seen = window > 0 ? std::min(keys, window + (int)((rows - 1) / G)) : keys;
+        const int seen = seen_of(keys, rows);
         p.tiles += times * (int)((rows + p.rows_per_tile - 1) / p.rows_per_tile);
         p.longest = std::max(p.longest, seen);
         p.most_rows = std::max(p.most_rows, (int)std::min<long long>(rows, p.rows_upto));
-        p.key_tiles += (long long)times * nkv * ((seen + 63) / 64);
+        p.key_tiles += (long long)times * nkv * ((seen + 63) / 64) * ((rows + p.rows_per_tile - 1) / p.rows_per_tile);
     };
     if (cu) {
         for (int i = 0; i < nseq; ++i) count((long long)(cu[i + 1] - cu[i]) * G, kv[i], 1);
@@ -278,12 +317,14 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
     for (Part *p : {&small, &large}) {
         if (!p->tiles) continue;
         if (p->kernel == DECODE) {
+            if (p->most_rows <= 8) p->rows_per_tile = 8;
             p->ctas = q8_decode_ctas(p->key_tiles, hd, p->most_rows);
-            p->slices = q8_decode_cluster((long long)nseq * nkv, (p->longest + 63) / 64, p->key_tiles, hd, p->most_rows);
+            p->row_tiles = (p->most_rows + p->rows_per_tile - 1) / p->rows_per_tile;
+            p->slices = q8_decode_cluster((long long)nseq * p->row_tiles * nkv, (p->longest + 63) / 64, p->key_tiles, hd, p->most_rows);
             p->scratch = p->slices ? 0 : q8_decode_scratch(p->ctas, hd);
         } else {
-            // the tensor cores: one CTA an SM, slices of 512 keys at least
-            p->slices = p->kernel == TC ? slices_for((long long)p->tiles * nkv, kestrel_sms(), p->longest, 512)
+            // the tensor cores: one CTA an SM, slices of two key tiles at least
+            p->slices = p->kernel == TC ? slices_for((long long)p->tiles * nkv, kestrel_sms(), p->longest, 256)
                                         : slices_for((long long)p->tiles * nkv, kestrel_sms() * 2, p->longest, 256);
             p->scratch = p->slices > 1 ? (long long)T * nq * p->slices * (hd + 2) : 0;
         }
@@ -329,13 +370,13 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
         p.nseq = nseq; p.table_width = table_width; p.table_stride = table_stride; p.page_size = page_size; p.cache_pages = cache_pages;
         p.nq = nq; p.nkv = nkv; p.hd = hd; p.window = window; p.slices = part.slices; p.scale = scale;
         p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1;
-        p.rows_above = part.rows_above; p.rows_upto = part.rows_upto; p.rows_per_tile = part.rows_per_tile;
+        p.rows_above = part.rows_above; p.rows_upto = part.rows_upto; p.rows_per_tile = part.rows_per_tile; p.row_tiles = part.row_tiles;
         KESTREL_REQUIRE(part.scratch == 0 || (scratch && part.scratch <= scratch_floats), "attention_q8: scratch of %lld floats is needed, %lld given", part.scratch, scratch_floats);
         p.part_o = scratch;
         int rc;
         if (part.kernel == DECODE) {
             p.part_ml = scratch ? scratch + 2ll * part.ctas * 16 * hd : nullptr;
-            rc = q8_launch_decode(p, part.ctas, part.most_rows, stream);
+            rc = q8_launch_decode(p, part.ctas, stream);
             launches += part.slices ? 1 : 2;
         } else {
             p.part_ml = scratch ? scratch + (long long)T * nq * part.slices * hd : nullptr;

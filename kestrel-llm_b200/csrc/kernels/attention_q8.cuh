@@ -26,7 +26,7 @@ struct Q8Params {
     const int *block_table;         // [nseq, table_stride], table_width entries of a row are read
     int nseq, table_width, table_stride, page_size, cache_pages, nq, nkv, hd, window, slices;
     int rows_above, rows_upto;      // this launch takes the requests with rows_above < (token, head) rows per kv head <= rows_upto
-    int rows_per_tile;
+    int rows_per_tile, row_tiles;   // row_tiles: most of a request
     int page_shift;                 // log2 of the page size, or -1
     float scale;
 };
@@ -99,8 +99,8 @@ __device__ __forceinline__ size_t q8_out_row(const Q8Params &p, const Q8Tile &t,
     return (size_t)(t.tok_begin + row / t.G) * p.nq + kvh * t.G + row % t.G;
 }
 
-// attention_q8_decode.cu: requests of up to 16 rows, head sizes 64 and 128, bfloat16; two kernels
-int q8_launch_decode(const Q8Params &p, int ctas, int most_rows, cudaStream_t stream);
+// attention_q8_decode.cu: requests of few rows, in tiles of 8 or 16 (Q8Params.rows_per_tile), head sizes 64 and 128, bfloat16; one or two kernels
+int q8_launch_decode(const Q8Params &p, int ctas, cudaStream_t stream);
 int q8_decode_ctas(long long tiles, int hd, int most_rows);      // for so many (request, kv head, 64 keys), requests of at most so many rows
 int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int hd, int most_rows);      // CTAs a pair (Q8Params.slices), or 0: ctas in stretches
 long long q8_decode_scratch(int ctas, int hd);          // floats: part_o, then part_ml

@@ -1,8 +1,8 @@
-// Attention over pages of int8 codes with few rows: single tokens, and the ragged ends of short portions.  Head sizes 64 and 128, bfloat16
+// Attention over pages of int8 codes with few rows: single tokens and short portions.  Head sizes 64 and 128, bfloat16
 // queries.  Formulas in attention_q8.cuh.
 //
-// The work is cut evenly, whatever the requests' lengths: all key tiles of 64 of all (request, kv head) pairs stand in one line, and every
-// CTA takes as many of them as the next.  A CTA walks its stretch pair by pair, up to 16 (token, query head) rows at once.  A pair that lies
+// The work is cut evenly, whatever the requests' lengths: all key tiles of 64 of all pairs - of a kv head and up to 16 (token, query head)
+// rows of a request - stand in one line, and every CTA takes as many of them as the next.  A CTA walks its stretch pair by pair.  A pair that lies
 // within one CTA's stretch is finished there; the others leave (maximum, sum, outputs) of their parts in scratch, two parts a CTA at most,
 // and the merge kernel below joins them in the order of the keys.  Where the pairs are few and short (CLUSTER) the CTAs of a cluster share one
 // pair instead, evenly, and join their parts in each other's shared memory: a kernel less.
@@ -115,22 +115,32 @@ template <int HD> __device__ __forceinline__ uint32_t chunk_at(int k, int c) {
     return line * 128 + ((at ^ (line & 7)) << 4);
 }
 
-// The line of key tiles: request i's pairs lie behind those of the requests before it, kv head by kv head.
+// The line of key tiles: request i's pairs lie behind those of the requests before it, row tile by row tile and in these kv head by kv head.
+// All pairs of a request have the tiles that its first or its last row sees.
 struct Line {
     const Q8Params &p;
 
-    __device__ __forceinline__ int tiles_of(int i) const {
+    // key tiles of a pair of request i; sets its row tiles
+    __device__ __forceinline__ int tiles_of(int i, int &row_tiles) const {
+        row_tiles = 0;
         if (i >= p.nseq) return 0;
         const int n = p.cu_seqlens[i + 1] - p.cu_seqlens[i], kv = p.kv_lens[i];
         const long long rows = (long long)n * (p.nq / p.nkv);
         if (rows <= p.rows_above || rows > p.rows_upto) return 0;
         const int first = p.window > 0 ? max(0, kv - n - p.window + 1) : 0;
+        row_tiles = ((int)rows + p.rows_per_tile - 1) / p.rows_per_tile;
         return (kv + BN - 1) / BN - first / BN;
+    }
+    // of one kv head: below 2^31, which the host sees to
+    __device__ __forceinline__ int place_of(int i) const {
+        int rt;
+        const int n = tiles_of(i, rt);
+        return n * rt;
     }
     // all of it
     __device__ __forceinline__ long long length() const {
-        int sum = 0;                                // of one kv head: below 2^31 tokens / 64
-        for (int i = threadIdx.x & 31; i < p.nseq; i += 32) sum += tiles_of(i);
+        int sum = 0;
+        for (int i = threadIdx.x & 31; i < p.nseq; i += 32) sum += place_of(i);
         return (long long)__reduce_add_sync(0xffffffffu, sum) * p.nkv;
     }
     // the request in which tile `at` lies, and its first tile's place
@@ -139,7 +149,7 @@ struct Line {
         const int want = (int)(at / p.nkv);         // on one kv head's line a request holds its place
         int before = 0;
         for (int base = 0; base < p.nseq; base += 32) {
-            const int n = tiles_of(base + lane);
+            const int n = place_of(base + lane);
             int end = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -167,18 +177,23 @@ __device__ __forceinline__ int holder(long long at, long long length, int ctas) 
 struct Walk {
     const Q8Params &p;
     long long at, end, begin;           // next tile, end of the stretch, place of the pair's first tile
-    int seq, n, kvh;                    // the pair; n: its tiles
+    int seq, n, kvh, row0;              // the pair; n: its tiles, row0: its first row among the request's
     // the part
-    int G, rows, tok_begin, pos_begin, k_first, k_end, from, to;
+    int G, row_tiles, all_rows, rows, tok_begin, pos_begin, k_first, k_end, from, to;
     const int *table;
     bool whole;
 
     // the rank-th of `ranks` equal parts of a pair
-    __device__ __forceinline__ Walk(const Q8Params &p_, int pair, int rank, int ranks) : p(p_), at(0), end(0), begin(0), seq(pair / p_.nkv), kvh(pair % p_.nkv) {
+    __device__ __forceinline__ Walk(const Q8Params &p_, int pair, int rank, int ranks) : p(p_), at(0), end(0), begin(0), kvh(pair % p_.nkv) {
         G = p.nq / p.nkv;
-        n = Line{p}.tiles_of(seq);
+        seq = pair / p.nkv / p.row_tiles;
+        const int rt = pair / p.nkv - seq * p.row_tiles;
+        n = Line{p}.tiles_of(seq, row_tiles);
+        if (rt >= row_tiles) n = 0;
         if (n == 0) return;
+        row0 = rt * p.rows_per_tile;
         describe();
+        rows = min(p.rows_per_tile, all_rows - row0);
         from = (int)((long long)n * rank / ranks);
         to = (int)((long long)n * (rank + 1) / ranks);
         whole = ranks == 1;
@@ -190,9 +205,11 @@ struct Walk {
         if (at >= end) return;
         const Line line{p};
         seq = line.request_at(at, begin);
-        n = line.tiles_of(seq);
-        kvh = (int)((at - begin) / n);
-        begin += (long long)kvh * n;
+        n = line.tiles_of(seq, row_tiles);
+        const int pair = (int)((at - begin) / n);
+        begin += (long long)pair * n;
+        kvh = pair % p.nkv;
+        row0 = pair / p.nkv * p.rows_per_tile;
         describe();
     }
     __device__ __forceinline__ void describe() {
@@ -200,7 +217,7 @@ struct Walk {
         const int n_tok = p.cu_seqlens[seq + 1] - tok_begin;
         k_end = p.kv_lens[seq];
         pos_begin = k_end - n_tok;
-        rows = n_tok * G;
+        all_rows = n_tok * G;
         k_first = p.window > 0 ? max(0, pos_begin - p.window + 1) : 0;
         table = p.block_table + (size_t)seq * p.table_stride;
     }
@@ -211,19 +228,24 @@ struct Walk {
             begin += n;
             if (++kvh == p.nkv) {
                 kvh = 0;
-                const Line line{p};
-                do n = line.tiles_of(++seq);
-                while (n == 0 && seq < p.nseq);
-                describe();
+                row0 += p.rows_per_tile;
+                if (row0 >= all_rows) {
+                    row0 = 0;
+                    const Line line{p};
+                    do n = line.tiles_of(++seq, row_tiles);
+                    while (n == 0 && seq < p.nseq);
+                    describe();
+                }
             }
         }
+        rows = min(p.rows_per_tile, all_rows - row0);
         from = (int)(at - begin);
         to = (int)min((long long)n, end - begin);
         whole = from == 0 && to == n;
         at = begin + to;
         return true;
     }
-    __device__ __forceinline__ size_t out_row(int r) const { return (size_t)(tok_begin + r / G) * p.nq + kvh * G + r % G; }
+    __device__ __forceinline__ size_t out_row(int r) const { return (size_t)(tok_begin + (row0 + r) / G) * p.nq + kvh * G + (row0 + r) % G; }
 };
 
 // Parts in scratch: 16 rows of HD outputs each, then 16 (maximum, sum) pairs each; a CTA's first part is its even one
@@ -309,7 +331,7 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     int stage = 0;
     uint32_t phase = 0;
     pdl_wait();
-    if (CLUSTER && w.n == 0) return;                    // another launch's request: all of the cluster
+    if (CLUSTER && w.n == 0) return;                    // another launch's request, or fewer rows than another's: all of the cluster
     bool more = true;
     auto next = [&] {
         if (!CLUSTER) return w.next();
@@ -427,7 +449,7 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                 bias[nt][i] = __shfl_sync(0xffffffffu, bias_g, 8 * c + 4 * i);
                 const int row = 8 * nt + 2 * c + i;
                 const bool live = row < w.rows;
-                pos[nt][i] = live ? w.pos_begin + row / w.G : -1;
+                pos[nt][i] = live ? w.pos_begin + (w.row0 + row) / w.G : -1;
                 low[nt][i] = p.window > 0 ? max(0, pos[nt][i] - p.window + 1) : 0;
                 if (live) min_pos = min(min_pos, pos[nt][i]);
                 max_low = max(max_low, low[nt][i]);
@@ -633,20 +655,20 @@ __global__ void __launch_bounds__(256) attention_q8_join_kernel(const Q8Params p
     constexpr int DL = HD / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.x, kvh = blockIdx.y, G = p.nq / p.nkv;
     const Line line{p};
-    int before = 0, all = 0;
+    int before = 0, all = 0, row_tiles;
     for (int i = lane; i < p.nseq; i += 32) {
-        const int n = line.tiles_of(i);
+        const int n = line.place_of(i);
         all += n;
         if (i < seq) before += n;
     }
     const long long length = (long long)__reduce_add_sync(0xffffffffu, all) * p.nkv;
-    const int n = line.tiles_of(seq);
-    const long long begin = (long long)__reduce_add_sync(0xffffffffu, before) * p.nkv + (long long)kvh * n;
+    const int n = line.tiles_of(seq, row_tiles);
+    const long long begin = (long long)__reduce_add_sync(0xffffffffu, before) * p.nkv + ((long long)blockIdx.z * p.nkv + kvh) * n;
     pdl_wait();
-    if (n == 0) return;
+    if (n == 0 || (int)blockIdx.z >= row_tiles) return;
     const int u0 = holder(begin, length, ctas), u1 = holder(begin + n - 1, length, ctas);
     if (u0 == u1) return;
-    const int tok_begin = p.cu_seqlens[seq], rows = (p.cu_seqlens[seq + 1] - tok_begin) * G;
+    const int tok_begin = p.cu_seqlens[seq], row0 = blockIdx.z * p.rows_per_tile, rows = min(p.rows_per_tile, (p.cu_seqlens[seq + 1] - tok_begin) * G - row0);
     const long long first = 2ll * u0 + (begin > stretch(u0, length, ctas) ? 1 : 0);      // in its own CTA the pair's part is the last one
     auto part_of = [&](int k) { return k == 0 ? first : 2ll * (u0 + k); };
     const int parts = u1 - u0 + 1;
@@ -679,7 +701,7 @@ __global__ void __launch_bounds__(256) attention_q8_join_kernel(const Q8Params p
             }
         }
         const float inv = 1.0f / L;
-        __nv_bfloat16 *out = (__nv_bfloat16 *)p.out + ((size_t)(tok_begin + r / G) * p.nq + kvh * G + r % G) * HD + lane * DL;
+        __nv_bfloat16 *out = (__nv_bfloat16 *)p.out + ((size_t)(tok_begin + (row0 + r) / G) * p.nq + kvh * G + (row0 + r) % G) * HD + lane * DL;
 #pragma unroll
         for (int d = 0; d < DL; d += 2) *reinterpret_cast<__nv_bfloat162 *>(out + d) = __floats2bfloat162_rn(acc[d] * inv, acc[d + 1] * inv);
     }
@@ -717,7 +739,7 @@ int launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
         cudaLaunchAttribute attr[2];
         rc = cluster_config<HD, NT>(cfg, attr, p.slices);
         if (rc) return rc;
-        cfg.gridDim = dim3((unsigned)p.nseq * p.nkv * p.slices);
+        cfg.gridDim = dim3((unsigned)p.nseq * p.row_tiles * p.nkv * p.slices);
         cfg.stream = stream;
         attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[1].val.programmaticStreamSerializationAllowed = 1;
@@ -730,7 +752,7 @@ int launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
     kestrel_launch(attention_q8_decode_kernel<HD, NT, false>, dim3(ctas), dim3(THREADS), decode_smem<HD, NT>(), stream, mk, mv, p);
     rc = kestrel_check_launch("attention_q8 decode");
     if (rc) return rc;
-    kestrel_launch(attention_q8_join_kernel<HD>, dim3(p.nseq, p.nkv), dim3(256), 0, stream, p, ctas);
+    kestrel_launch(attention_q8_join_kernel<HD>, dim3(p.nseq, p.nkv, p.row_tiles), dim3(256), 0, stream, p, ctas);
     return kestrel_check_launch("attention_q8 join");
 }
 
@@ -752,8 +774,8 @@ int resident_clusters(int size) {
 
 }  // namespace
 
-int q8_launch_decode(const Q8Params &p, int ctas, int most_rows, cudaStream_t stream) {
-    if (most_rows <= 8) return p.hd == 64 ? launch_decode<64, 1>(p, ctas, stream) : launch_decode<128, 1>(p, ctas, stream);
+int q8_launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
+    if (p.rows_per_tile == 8) return p.hd == 64 ? launch_decode<64, 1>(p, ctas, stream) : launch_decode<128, 1>(p, ctas, stream);
     return p.hd == 64 ? launch_decode<64, 2>(p, ctas, stream) : launch_decode<128, 2>(p, ctas, stream);
 }
 
