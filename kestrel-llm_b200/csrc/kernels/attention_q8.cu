@@ -50,25 +50,42 @@ __global__ void __launch_bounds__(THREADS) attention_q8_plain_kernel(const Q8Par
         low[i] = p.window > 0 ? max(0, pos[i] - p.window + 1) : 0;
     }
     const float scale_log2 = p.scale * 1.4426950408889634f;
+    // sixteen codes a thread and load; those of the next tile are on their way while this one is worked on
+    constexpr int LOADS = BN * (HDP / 16) / THREADS;
+    uint4 kq[LOADS], vq[LOADS];
+    float ks[LOADS], vs[LOADS];
+    auto fetch = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int r = (tid + i * THREADS) / (HDP / 16), d = (tid + i * THREADS) % (HDP / 16) * 16, key = kb + r;
+            kq[i] = vq[i] = make_uint4(0, 0, 0, 0);         // keys outside the slice count as zero, whatever their page holds
+            ks[i] = vs[i] = 0.f;
+            if (key < lo || key >= hi || d >= p.hd) continue;
+            const int row = q8_row_of(p, t.table, kvh, key);
+            const size_t at = (size_t)(row + key % Q8_BLOCK) * p.hd + d;
+            kq[i] = *reinterpret_cast<const uint4 *>(p.k + at);
+            vq[i] = *reinterpret_cast<const uint4 *>(p.v + at);
+            ks[i] = p.ks[row / Q8_BLOCK];
+            vs[i] = p.vs[row / Q8_BLOCK];
+        }
+    };
+    if (lo < hi) fetch(lo / BN * BN);
     for (int kb = lo / BN * BN; kb < hi; kb += BN) {
         __syncthreads();
-        // four codes a thread and turn; keys outside the slice count as zero, whatever their page holds
-        for (int i = tid; i < BN * (HDP / 4); i += THREADS) {
-            const int r = i / (HDP / 4), d = i % (HDP / 4) * 4, key = kb + r;
-            float4 kf = make_float4(0.f, 0.f, 0.f, 0.f), vf = kf;
-            if (key >= lo && key < hi && d < p.hd) {
-                const int row = q8_row_of(p, t.table, kvh, key);
-                const size_t at = (size_t)(row + key % Q8_BLOCK) * p.hd + d;
-                const char4 kc = *reinterpret_cast<const char4 *>(p.k + at), vc = *reinterpret_cast<const char4 *>(p.v + at);
-                const float sk = p.ks[row / Q8_BLOCK];
-                kf = make_float4(kc.x * sk, kc.y * sk, kc.z * sk, kc.w * sk);
-                vf = make_float4(vc.x, vc.y, vc.z, vc.w);
-                if (d == 0) sv_s[r] = p.vs[row / Q8_BLOCK];
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int r = (tid + i * THREADS) / (HDP / 16), d = (tid + i * THREADS) % (HDP / 16) * 16;
+            const uint32_t kw[4] = {kq[i].x, kq[i].y, kq[i].z, kq[i].w}, vw[4] = {vq[i].x, vq[i].y, vq[i].z, vq[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const char4 k = *reinterpret_cast<const char4 *>(&kw[j]), v = *reinterpret_cast<const char4 *>(&vw[j]);
+                *reinterpret_cast<float4 *>(K + r * LD + d + 4 * j) = make_float4(k.x * ks[i], k.y * ks[i], k.z * ks[i], k.w * ks[i]);
+                *reinterpret_cast<float4 *>(V + r * LD + d + 4 * j) = make_float4(v.x, v.y, v.z, v.w);
             }
-            *reinterpret_cast<float4 *>(K + r * LD + d) = kf;
-            *reinterpret_cast<float4 *>(V + r * LD + d) = vf;
+            if (d == 0) sv_s[r] = vs[i];
         }
         __syncthreads();
+        if (kb + BN < hi) fetch(kb + BN);
         float s[4][4] = {};
 #pragma unroll 4
         for (int d = 0; d < HDP; d += 4) {
