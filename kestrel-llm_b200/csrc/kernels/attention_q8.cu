@@ -364,7 +364,8 @@ KESTREL_API long long kestrel_attention_q8_scratch(const int *cu_host, const int
 KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, void *out, float *scratch,
                                      long long scratch_floats, const int *cu_host, const int *kv_host, const int *cu_seqlens, const int *kv_lens,
                                      const int *block_table, int nseq, int max_count, int max_kv, int table_width, int table_stride, int page_size,
-                                     int cache_pages, int T, int nq, int nkv, int hd, int window, float scale, int dtype, kestrel_stream_t stream) {
+                                     int cache_pages, int T, int nq, int nkv, int hd, int window, float scale, int dtype, int described,
+                                     kestrel_stream_t stream) {
     if (T == 0 || nseq == 0) return 0;
     KESTREL_REQUIRE(T > 0 && nseq > 0 && max_count > 0 && max_kv >= max_count, "attention_q8: a step of %d tokens of %d requests, %d at most, %d keys at most", T, nseq, max_count, max_kv);
     KESTREL_REQUIRE(dtype == KESTREL_F32 || dtype == KESTREL_BF16, "attention_q8: unknown dtype %d", dtype);
@@ -385,7 +386,7 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
         p.q = q; p.out = out; p.k = (const int8_t *)k_cache; p.v = (const int8_t *)v_cache; p.ks = k_scale; p.vs = v_scale;
         p.cu_seqlens = cu_seqlens; p.kv_lens = kv_lens; p.block_table = block_table;
         p.nseq = nseq; p.table_width = table_width; p.table_stride = table_stride; p.page_size = page_size; p.cache_pages = cache_pages;
-        p.nq = nq; p.nkv = nkv; p.hd = hd; p.window = window; p.slices = part.slices; p.scale = scale;
+        p.nq = nq; p.nkv = nkv; p.hd = hd; p.window = window; p.slices = part.slices; p.scale = scale; p.described = described;
         p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1;
         p.rows_above = part.rows_above; p.rows_upto = part.rows_upto; p.rows_per_tile = part.rows_per_tile; p.row_tiles = part.row_tiles;
         KESTREL_REQUIRE(part.scratch == 0 || (scratch && part.scratch <= scratch_floats), "attention_q8: scratch of %lld floats is needed, %lld given", part.scratch, scratch_floats);

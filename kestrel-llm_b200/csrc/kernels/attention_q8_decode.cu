@@ -326,7 +326,7 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    // the step's description was on the device before the kernel in front of this one began
+    if (!p.described) pdl_wait();
     Walk w = CLUSTER ? Walk(p, (int)blockIdx.x / p.slices, (int)blockIdx.x % p.slices, p.slices) : Walk(p, Line{p}.length());
     int stage = 0;
     uint32_t phase = 0;
@@ -654,6 +654,7 @@ __global__ void __launch_bounds__(256) attention_q8_join_kernel(const Q8Params p
     pdl_launch_dependents();
     constexpr int DL = HD / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.x, kvh = blockIdx.y, G = p.nq / p.nkv;
+    if (!p.described) pdl_wait();
     const Line line{p};
     int before = 0, all = 0, row_tiles;
     for (int i = lane; i < p.nseq; i += 32) {

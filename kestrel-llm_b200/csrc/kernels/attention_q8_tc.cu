@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
     auto bar = [&](int i) { return base + L::BARRIERS + 8u * (uint32_t)i; };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+    if (!p.described) pdl_wait();
     // late tiles, which see the most keys, come first - across all kv heads
     const int kvh = blockIdx.x % p.nkv, slice = blockIdx.z;
     Q8Tile t;

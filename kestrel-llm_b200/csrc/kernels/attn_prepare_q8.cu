@@ -26,6 +26,7 @@ struct PrepParams {
     float *ks, *vs;
     void *q_out;
     int S, nseq, table_width, table_stride, page_size, cache_pages, T, nq, nkv, hd, rot, rot_mode, units;
+    int described;                  // positions, cu and table were on the device before the kernel in front of this one began
     float eps, rot_scale;
 };
 
@@ -308,11 +309,12 @@ __global__ void __launch_bounds__(THREADS) attn_prepare_q8_fast_kernel(const Pre
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane & 7, mine = tid >> 3;
     const int half = TURN == TURN_NONE ? 0 : TURN == TURN_HALF ? HD / 2 : p.rot >> 1;
     const int kv_ctas = p.units * p.nkv;
+    if (!p.described) pdl_wait();
 
     if ((int)blockIdx.x >= kv_ctas) {
         // ---- one token's queries, 32 heads at a time
         const int t = blockIdx.x - kv_ctas;
-        if (t >= p.cu[p.nseq]) { pdl_wait(); return; }      // the step's description was there before the kernel in front of this one began
+        if (t >= p.cu[p.nseq]) { pdl_wait(); return; }
         if (TURN != TURN_NONE) {
             const int pos = p.positions[t];
             for (int j = tid; j < half; j += THREADS) cs[0][j] = sizeof(T) == 4 ? turn(pos, p.inv_freq[j], p.rot_scale) : turn_fast(pos, p.inv_freq[j], p.rot_scale);
@@ -385,7 +387,8 @@ __global__ void __launch_bounds__(THREADS) attn_prepare_q8_kernel(const PrepPara
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane % LPR, mine = warp * RPW + lane / LPR;
     const int half = p.rot >> 1;
     const int kv_ctas = p.units * p.nkv;
-    const int n_tokens = p.cu[p.nseq];              // the step's description was there before the kernel in front of this one began
+    if (!p.described) pdl_wait();
+    const int n_tokens = p.cu[p.nseq];
 
     if ((int)blockIdx.x >= kv_ctas) {
         // ---- one token's queries
@@ -501,7 +504,7 @@ KESTREL_API int kestrel_attn_prepare_q8(const float *partial, int S, long long s
                                         float norm_eps, const float *inv_freq, int rot, int rot_mode, float rot_scale, const int *positions,
                                         const int *cu_seqlens, int nseq, const int *block_table, int table_width, int table_stride, int page_size,
                                         int cache_pages, void *k_cache, void *v_cache, float *k_scale, float *v_scale, void *q_out, int dtype, int T, int nq,
-                                        int nkv, int hd, int write_kv, kestrel_stream_t stream) {
+                                        int nkv, int hd, int write_kv, int described, kestrel_stream_t stream) {
     if (T == 0 || nseq == 0) return 0;
     KESTREL_REQUIRE(T > 0 && nseq > 0 && S > 0 && nq > 0 && nkv > 0, "attn_prepare_q8: bad sizes");
     KESTREL_REQUIRE(dtype == KESTREL_F32 || dtype == KESTREL_BF16, "attn_prepare_q8: unknown dtype %d", dtype);
@@ -517,7 +520,7 @@ KESTREL_API int kestrel_attn_prepare_q8(const float *partial, int S, long long s
     p.partial = partial; p.bias = bias; p.q_w = q_norm_w; p.k_w = k_norm_w; p.inv_freq = inv_freq; p.slice_stride = (size_t)slice_stride;
     p.positions = positions; p.cu = cu_seqlens; p.table = block_table; p.k = (int8_t *)k_cache; p.v = (int8_t *)v_cache; p.ks = k_scale; p.vs = v_scale;
     p.q_out = q_out; p.S = S; p.nseq = nseq; p.table_width = table_width; p.table_stride = table_stride; p.page_size = page_size;
-    p.cache_pages = cache_pages; p.T = T; p.nq = nq; p.nkv = nkv; p.hd = hd; p.rot = rot; p.rot_mode = rot_mode; p.eps = norm_eps; p.rot_scale = rot_scale;
+    p.cache_pages = cache_pages; p.T = T; p.nq = nq; p.nkv = nkv; p.hd = hd; p.rot = rot; p.rot_mode = rot_mode; p.eps = norm_eps; p.rot_scale = rot_scale; p.described = described;
     // n tokens touch at most (n + 14) / 16 + 1 blocks, and no more than n
     const long long units = write_kv ? (T < ((long long)T + 30ll * nseq) / 16 ? (long long)T : ((long long)T + 30ll * nseq) / 16) : 0;
     KESTREL_REQUIRE(units * nkv + T < (1ll << 31), "attn_prepare_q8: %d tokens of %d requests exceed the grid", T, nseq);

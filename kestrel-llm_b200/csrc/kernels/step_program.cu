@@ -281,7 +281,7 @@ struct Walk {
                                                          (const float *)op.w, op.rot, op.rot_mode, op.rot_scale, dev + layout[KB_O_POSITIONS],
                                                          dev + layout[KB_O_CU_SEQLENS], n, dev + layout[KB_O_TABLES] + (size_t)op.group * n * W, W, W,
                                                          op.page_size, op.cache_pages, (void *)op.k_cache, (void *)op.v_cache, op.k_scale, op.v_scale, o.ptr,
-                                                         pg.dtype, T, op.nq, op.nkv, op.hd, op.flag, stream);
+                                                         pg.dtype, T, op.nq, op.nkv, op.hd, op.flag, 1, stream);
                         else
                             rc = kestrel_attn_prepare((const float *)qkv.ptr, qkv.slices, (long long)T * qkv.cols, qkv.bias, op.w2, op.w3, op.eps,
                                                       (const float *)op.w, op.rot, op.rot_mode, op.rot_scale, dev + layout[KB_O_POSITIONS],
@@ -308,7 +308,7 @@ struct Walk {
                             rc = kestrel_attention_q8(q.ptr, op.k_cache, op.v_cache, op.k_scale, op.v_scale, o.ptr, scratch, floats, cu_h, kv_h,
                                                       dev + layout[KB_O_CU_SEQLENS], dev + layout[KB_O_KV_LENS],
                                                       dev + layout[KB_O_TABLES] + (size_t)op.group * n * W, n, layout[KB_MAX_COUNT], layout[KB_MAX_KV_LEN], W, W,
-                                                      op.page_size, op.cache_pages, T, op.nq, op.nkv, op.hd, op.window, op.scale, pg.dtype, stream);
+                                                      op.page_size, op.cache_pages, T, op.nq, op.nkv, op.hd, op.window, op.scale, pg.dtype, 1, stream);
                             if (rc > 0) launches += rc, rc = 0;
                         }
                         break;

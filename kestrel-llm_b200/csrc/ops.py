@@ -385,14 +385,16 @@ def attn_prepare_q8(qkv: Partials, q_norm_w: Optional[torch.Tensor], k_norm_w: O
                     inv_freq: Optional[torch.Tensor], rotary_dim: int, positions: torch.Tensor, cu_seqlens: torch.Tensor,
                     block_table: torch.Tensor, page_size: int, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                     v_scale: torch.Tensor, q_out: torch.Tensor, nq: int, nkv: int, hd: int, write_kv: bool = True, rot_mode: int = 0,
-                    rot_scale: float = 1.0) -> None:
+                    rot_scale: float = 1.0, described: bool = False) -> None:
     """`attn_prepare` into pages of 8-bit codes: bias, per-head RMSNorm, rotation (angles of any int32 position to float32 accuracy);
     q to q_out (float32 or bfloat16), K and V as int8 codes in [-127, 127] and one float32 scale for every ``Q8_BLOCK`` tokens and head:
     value = code * scale, scale = max(2^-64, largest magnitude / 127) over what the block has met, codes rounded to nearest even.
     Where a step's tokens raise the scale of a block that earlier steps began, its codes are rounded again, so a block's codes depend on
     how a sequence was cut into steps (by at most half a step of the scale for each rise).  A block that met a number that is not finite
     has a scale that is not a number, until its page begins anew.  The tokens of request i are cu_seqlens[i] to cu_seqlens[i + 1] - 1, at
-    consecutive positions; rows of q_out behind the last request are left as they are, and so is a token whose page is absent."""
+    consecutive positions; rows of q_out behind the last request are left as they are, and so is a token whose page is absent.
+    ``described``: positions, cu_seqlens and block_table were on the device before the kernel in front of this one on the stream began,
+    as a copy leaves them; the launch reads them while that kernel still runs."""
     dev = q_out.device
     _need(q_out, "attn_prepare_q8.q_out", dims=2)
     T = q_out.shape[0]
@@ -416,7 +418,7 @@ def attn_prepare_q8(qkv: Partials, q_norm_w: Optional[torch.Tensor], k_norm_w: O
             qkv.data.data_ptr(), qkv.slices, qkv.slice_stride, _p(qkv.bias), _p(q_norm_w), _p(k_norm_w), norm_eps, _p(inv_freq),
             rotary_dim, rot_mode, rot_scale, positions.data_ptr(), cu_seqlens.data_ptr(), n, block_table.data_ptr(), block_table.shape[1],
             block_table.stride(0), page_size, k_cache.shape[0], k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-            v_scale.data_ptr(), q_out.data_ptr(), _code(q_out, "attn_prepare_q8.q_out"), T, nq, nkv, hd, 1 if write_kv else 0, _stream()))
+            v_scale.data_ptr(), q_out.data_ptr(), _code(q_out, "attn_prepare_q8.q_out"), T, nq, nkv, hd, 1 if write_kv else 0, described, _stream()))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -426,13 +428,14 @@ def _q8_scratch(device: int, n: int, max_count: int, max_kv: int, T: int, nq: in
 
 
 def attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, out: torch.Tensor,
-                 batch, block_table: torch.Tensor, page_size: int, nq: int, nkv: int, hd: int, window: int, scale: float) -> None:
+                 batch, block_table: torch.Tensor, page_size: int, nq: int, nkv: int, hd: int, window: int, scale: float,
+                 described: bool = False) -> None:
     """Causal attention of this step's queries (float32 or bfloat16 [T, nq * hd]) over their requests' pages of 8-bit codes
     (`attn_prepare_q8`), or over the last ``window`` keys.  ``batch`` is the step's description: ``num_tokens``, ``num_seqs``,
     ``cu_seqlens`` and ``kv_lens`` (int32 on the device), their host copies ``cu_seqlens_host`` and ``kv_lens_host``, ``max_count``,
     ``max_kv_len`` and ``captured`` (the launch is being recorded for replay with other lengths: every request then brings at most
-    ``max_count`` tokens).  Rows of ``out`` behind the last request are left as they are.  Kernels find their tiles on the device;
-    sums and softmax statistics are float32."""
+    ``max_count`` tokens).  ``described``: as `attn_prepare_q8` has it, of the batch and block_table.  Rows of ``out`` behind the last
+    request are left as they are.  Kernels find their tiles on the device; sums and softmax statistics are float32."""
     dev = q.device
     _need(q, "attention_q8.q", dims=2)
     _need(out, "attention_q8.out", q.dtype, 2)
@@ -460,7 +463,7 @@ def attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
         rc = lib.kestrel_attention_q8(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), out.data_ptr(), _p(scratch), floats,
             cu, kv, batch.cu_seqlens.data_ptr(), batch.kv_lens.data_ptr(), block_table.data_ptr(), n, max_count, max_kv,
-            block_table.shape[1], block_table.stride(0), page_size, k_cache.shape[0], T, nq, nkv, hd, window, scale, code, _stream())
+            block_table.shape[1], block_table.stride(0), page_size, k_cache.shape[0], T, nq, nkv, hd, window, scale, code, described, _stream())
     if rc < 0:
         raise KernelError(lib.kestrel_last_error().decode("utf-8", "replace"))
     global launches

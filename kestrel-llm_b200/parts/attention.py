@@ -80,10 +80,10 @@ class GroupedQueryAttention(Mixer):
             ops.attn_prepare_q8(self.qkv.forward(x), self.q_norm, self.k_norm, self.qk_norm_eps or 0.0, rot.inv_freq if rot else None,
                                 rot.dim if rot else 0, batch.positions, batch.cu_seqlens, table, cache.page_size, cache.k, cache.v, cache.k_scale,
                                 cache.v_scale, q, self.heads, self.kv_heads, self.head_dim, cache.writable, rot.mode if rot else 0,
-                                rot.scale if rot else 1.0)
+                                rot.scale if rot else 1.0, described=True)
             a = torch.empty_like(q)
             ops.attention_q8(q, cache.k, cache.v, cache.k_scale, cache.v_scale, a, batch, table, cache.page_size, self.heads, self.kv_heads,
-                             self.head_dim, self.window, self.scale)
+                             self.head_dim, self.window, self.scale, described=True)
             return self.out.forward(a, residual=residual)
         prepare = dict(q_norm_w=self.q_norm, k_norm_w=self.k_norm, norm_eps=self.qk_norm_eps or 0.0,
                        inv_freq=rot.inv_freq if rot else None, rotary_dim=rot.dim if rot else 0, positions=batch.positions,

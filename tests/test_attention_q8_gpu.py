@@ -1,4 +1,6 @@
 """Attention over pages of 8-bit codes, against float64."""
+from types import SimpleNamespace
+
 import pytest
 
 from q8_util import BLOCK, attend64, planes, rows_of, step
@@ -204,9 +206,35 @@ def test_two_streams_at_once():
         _near(s, out.view(-1, nq, hd).double(), want, size, "bfloat16")
 
 
+def test_a_description_that_kernels_write():
+    """Lengths and tables that kernels in front of the call wrote count as they stand then, and copied ones give the same bits early."""
+    import torch
+    from kestrel_llm_b200.csrc import ops
+    for portions in ([(1, 3000)] * 9, [(1, 40)], [(200, 300)], [(300, 0), (1, 9)]):
+        for dtype in (torch.bfloat16, torch.float32):
+            s = step(portions, 16)
+            k, ks, v, vs = planes(s, 2, 128)
+            q = torch.randn((s.num_tokens, 8 * 128), device="cuda").to(dtype)
+            got = []
+            for described in (True, False, False):
+                out = torch.full_like(q, float("nan"))
+                lens, table = s.kv_lens.clone(), s.table.clone()
+                if not described:               # the smallest lengths and no pages, until a moment before the call
+                    lens -= torch.tensor(s.starts, dtype=torch.int32, device="cuda")
+                    table.fill_(-1)
+                torch.cuda.synchronize()
+                if not described:
+                    torch.add(lens, torch.tensor(s.starts, dtype=torch.int32, device="cuda"), out=lens)
+                    torch.maximum(table, s.table, out=table)
+                here = SimpleNamespace(**{**vars(s), "kv_lens": lens})
+                ops.attention_q8(q, k, v, ks, vs, out, here, table, 16, 8, 2, 128, 0, 0.1, described=described)
+                got.append(out)
+            assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+            assert torch.isfinite(got[0]).all()
+
+
 def test_refusals():
     import torch
-    from types import SimpleNamespace
     from kestrel_llm_b200.csrc import ops
     nq, nkv, hd, page = 4, 2, 64, 16
     s = step([(3, 20)], page)
