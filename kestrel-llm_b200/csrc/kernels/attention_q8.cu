@@ -252,7 +252,8 @@ constexpr int MAX_SLICES = 32;
 enum Kernel { CORES, DECODE, TC };
 struct Part {
     Kernel kernel = CORES;
-    int rows_above = 0, rows_upto = 0, rows_per_tile = 0, tiles = 0, slices = 1, longest = 0;
+    int rows_above = 0, rows_upto = 0, rows_per_tile = 0, slices = 1, longest = 0;
+    long long tiles = 0;
     int ctas = 0, most_rows = 0, row_tiles = 0;
     long long scratch = 0;              // floats
     long long key_tiles = 0;             // of 64, over all requests and kv heads
@@ -270,7 +271,7 @@ int slices_for(long long ctas, int slots, int keys, int least) {
 // Rows follow from the host's copy of cu_seqlens; without it every request brings max_count tokens at most.
 void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, int max_kv, int T, int nq, int nkv, int hd, int window, int dtype) {
     const int G = nq / nkv;
-    auto seen_of = [&](int keys, long long rows) { return window > 0 ? std::min(keys, window + (int)((rows - 1) / G)) : keys; };
+    auto seen_of = [&](int keys, long long rows) { return window > 0 ? (int)std::min<long long>(keys, window + (rows - 1) / G) : keys; };
     constexpr int FEW = 512;                // rows of a portion that may go to the decode kernel
     const bool cores = dtype != KESTREL_BF16 || (hd != 64 && hd != 128);
     Part small, large;
@@ -318,10 +319,12 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
         if (rows <= 0) return;
         Part &p = rows <= small.rows_upto ? small : large;
         const int seen = seen_of(keys, rows);
-        p.tiles += times * (int)((rows + p.rows_per_tile - 1) / p.rows_per_tile);
+        const long long each = (rows + p.rows_per_tile - 1) / p.rows_per_tile;
+        // requests that may all bring so many rows still share the step's tokens
+        p.tiles += times == 1 ? each : std::min(times * each, times + (long long)T * G / p.rows_per_tile);
         p.longest = std::max(p.longest, seen);
         p.most_rows = std::max(p.most_rows, (int)std::min<long long>(rows, p.rows_upto));
-        p.key_tiles += (long long)times * nkv * ((seen + 63) / 64) * ((rows + p.rows_per_tile - 1) / p.rows_per_tile);
+        p.key_tiles += times * each * nkv * ((seen + 63) / 64);
     };
     if (cu) {
         for (int i = 0; i < nseq; ++i) count((long long)(cu[i + 1] - cu[i]) * G, kv[i], 1);
@@ -341,8 +344,8 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
             p->scratch = p->slices ? 0 : q8_decode_scratch(p->ctas, hd);
         } else {
             // the tensor cores: one CTA an SM, slices of two key tiles at least
-            p->slices = p->kernel == TC ? slices_for((long long)p->tiles * nkv, kestrel_sms(), p->longest, 256)
-                                        : slices_for((long long)p->tiles * nkv, kestrel_sms() * 2, p->longest, 256);
+            p->slices = p->kernel == TC ? slices_for(p->tiles * nkv, kestrel_sms(), p->longest, 256)
+                                        : slices_for(p->tiles * nkv, kestrel_sms() * 2, p->longest, 256);
             p->scratch = p->slices > 1 ? (long long)T * nq * p->slices * (hd + 2) : 0;
         }
         pl.part[pl.parts++] = *p;
@@ -379,6 +382,12 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
     KESTREL_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)scratch) & 15) == 0, "attention_q8: tensors must start on 16 bytes");
     Plan pl;
     make_plan(pl, cu_host, kv_host, nseq, max_count, max_kv, T, nq, nkv, hd, window, dtype);
+    for (int i = 0; i < pl.parts; ++i) {
+        const Part &part = pl.part[i];
+        KESTREL_REQUIRE(part.tiles * nkv < (1ll << 31) && (part.kernel != DECODE || part.key_tiles / nkv < (1ll << 31)),
+                        "attention_q8: %lld row tiles and %lld key tiles of %d kv heads exceed the grid", part.tiles, part.key_tiles, nkv);
+        KESTREL_REQUIRE(part.scratch == 0 || (scratch && part.scratch <= scratch_floats), "attention_q8: scratch of %lld floats is needed, %lld given", part.scratch, scratch_floats);
+    }
     int launches = 0;
     for (int i = 0; i < pl.parts; ++i) {
         const Part &part = pl.part[i];
@@ -389,7 +398,6 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
         p.nq = nq; p.nkv = nkv; p.hd = hd; p.window = window; p.slices = part.slices; p.scale = scale; p.described = described;
         p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1;
         p.rows_above = part.rows_above; p.rows_upto = part.rows_upto; p.rows_per_tile = part.rows_per_tile; p.row_tiles = part.row_tiles;
-        KESTREL_REQUIRE(part.scratch == 0 || (scratch && part.scratch <= scratch_floats), "attention_q8: scratch of %lld floats is needed, %lld given", part.scratch, scratch_floats);
         p.part_o = scratch;
         int rc;
         if (part.kernel == DECODE) {
@@ -398,8 +406,8 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
             launches += part.slices ? 1 : 2;
         } else {
             p.part_ml = scratch ? scratch + (long long)T * nq * part.slices * hd : nullptr;
-            rc = part.kernel == TC ? q8_launch_tc(p, part.tiles, stream) : q8_launch_plain(p, dtype, part.tiles, stream);
-            if (rc == 0 && part.slices > 1) rc = q8_launch_merge(p, dtype, part.tiles, stream);
+            rc = part.kernel == TC ? q8_launch_tc(p, (int)part.tiles, stream) : q8_launch_plain(p, dtype, (int)part.tiles, stream);
+            if (rc == 0 && part.slices > 1) rc = q8_launch_merge(p, dtype, (int)part.tiles, stream);
             launches += part.slices > 1 ? 2 : 1;
         }
         if (rc) return rc;

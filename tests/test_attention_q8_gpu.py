@@ -233,6 +233,51 @@ def test_a_description_that_kernels_write():
             assert torch.isfinite(got[0]).all()
 
 
+@pytest.mark.parametrize("portions", [[(1, 900)] * 3, [(200, 300), (1, 70)], [(20, 40)]])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_window_of_every_size(portions, dtype):
+    """Windows beyond the longest request hide nothing, up to the largest int32."""
+    got = []
+    for window in (0, 10000, 2 ** 31 - 1):
+        out, want, size = _run(step(portions, 16), 8, 2, 128, window, dtype)
+        _near(step(portions, 16), out, want, size, dtype)
+        got.append(out)
+    assert got[0].equal(got[1]) and got[0].equal(got[2])
+
+
+def test_recorded_portions_share_the_tokens():
+    """A step recorded for eight requests of up to 300 tokens, 320 in all, and replayed with other cuts of them."""
+    import torch
+    from kestrel_llm_b200.csrc import ops
+    nq, nkv, hd = 8, 2, 128
+    most = [(300, 0)] + [(0, 0)] * 7
+    first = step([(300, 200)] + [(2, 498)] * 7, 16)
+    for dtype in (torch.bfloat16, torch.float32):
+        s = step(most, 16)
+        s.table, s.pages, s.num_tokens, s.max_kv_len, s.captured = first.table, first.pages, 320, 500, True
+        k, ks, v, vs = planes(first, nkv, hd)
+        q = torch.randn((320, nq * hd), device="cuda").to(dtype)
+        out = torch.empty_like(q)
+        run = lambda: ops.attention_q8(q, k, v, ks, vs, out, s, s.table, 16, nq, nkv, hd, 0, hd ** -0.5)  # noqa: E731
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        for cuts in ([(300, 200)] + [(2, 498)] * 7, [(40, 100)] * 8, [(1, 499)] * 8, [(0, 0), (17, 3), (128, 0), (129, 371), (0, 0), (3, 400), (1, 0), (42, 42)]):
+            now = step(cuts, 16)
+            now.table, now.num_tokens = first.table, 320
+            s.cu_seqlens.copy_(now.cu_seqlens)
+            s.kv_lens.copy_(now.kv_lens)
+            out.fill_(float("nan"))
+            graph.replay()
+            want, size = attend64(q, k, ks, v, vs, now, nq, nkv, hd, 0, hd ** -0.5)
+            _near(now, out.view(-1, nq, hd).double(), want, size, "float32" if dtype is torch.float32 else "bfloat16")
+
+
 def test_refusals():
     import torch
     from kestrel_llm_b200.csrc import ops
