@@ -14,6 +14,11 @@
 
 #define Q8_BLOCK KESTREL_Q8_BLOCK
 
+// The tensor-core kernels mask a key by a score of minus infinity, which a product with zero would turn into no number.  So a block's scale
+// counts as 2^-64 at least, which is what an append writes at least, and a row's factor as 2^-84: their product is a float32 number.  What
+// that changes is a value of 2^-57 at most, and a score of 2^-63 times its block's scale at most.
+constexpr float Q8_LEAST_SCALE = 5.421010862427522e-20f, Q8_LEAST_FACTOR = 5.169878828456423e-26f;
+
 struct Q8Params {
     const void *q;                  // [T, nq * hd] float32 or bfloat16
     void *out;                      // [T, nq * hd], as q

@@ -441,7 +441,7 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                 }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            const float scale_g = __uint_as_float((uint32_t)(127 - up) << 23) * p.scale * (1.4426950408889634f * 16777216.0f);
+            const float scale_g = fmaxf(__uint_as_float((uint32_t)(127 - up) << 23) * p.scale * (1.4426950408889634f * 16777216.0f), Q8_LEAST_FACTOR);
             const float bias_g = sum * (-128.0f / 16777216.0f);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -496,8 +496,8 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                     }
                 }
                 const float *sc = reinterpret_cast<const float *>(ring + R::SCALES + stage * 32);
-                // zero counts as 2^-100; what is no number stays that
-                const float sk = sc[warp] < 7.9e-31f ? 7.9e-31f : sc[warp], sv = sc[4 + warp] < 7.9e-31f ? 7.9e-31f : sc[4 + warp];
+                // (what is no number stays that)
+                const float sk = sc[warp] < Q8_LEAST_SCALE ? Q8_LEAST_SCALE : sc[warp], sv = sc[4 + warp] < Q8_LEAST_SCALE ? Q8_LEAST_SCALE : sc[4 + warp];
                 const float lv = log2_fast(sv), rv = rcp_fast(sv);
                 if (kbase >= w.k_first && kbase + 16 <= w.k_end && kbase + 15 <= min_pos && kbase >= max_low) {
                     weigh<NT, false>(s, o, m, l, row_scale, sk, lv, rv, kbase, my_key, pos, low);

@@ -182,7 +182,7 @@ __device__ __forceinline__ void convert(const Q8Params &p, const int *table, int
             // A scale that is no positive number becomes one that makes the sum of a row that sees the block no number, and no other's:
             // the weights of such a row come out as 2^0 against a reference that nothing else reaches, and 1 / s_v is NaN.
             const bool bad = !(sk >= 0.f && sk <= 3.4e38f && sv >= 0.f && sv <= 3.4e38f);
-            const float k = bad ? 1e-30f : fmaxf(sk, 7.9e-31f), v = fmaxf(sv, 7.9e-31f);      // zero counts as 2^-100
+            const float k = bad ? Q8_LEAST_SCALE : fmaxf(sk, Q8_LEAST_SCALE), v = fmaxf(sv, Q8_LEAST_SCALE);
             if (lane < BLOCKS)
                 sts128(base + L::SCALES + ((i & 3) * BLOCKS + lane) * 16, make_uint4(__float_as_uint(k), __float_as_uint(bad ? 3e4f : log2_fast(v)),
                                                                                      bad ? 0x7fc00000u : __float_as_uint(1.0f / v), 0));
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
         const int my_pos = row_ok ? t.pos_begin + (tile_row + r) / t.G : -1;
         // the keys that this row sees in this slice: [see_lo, see_hi)
         const int see_lo = max(k_first, p.window > 0 ? my_pos - p.window + 1 : 0), see_hi = min(my_pos + 1, k_hi_x);
-        const float row_scale = row_up[HALVES ? r : x * BM + r] * p.scale * 1.4426950408889634f;
+        const float row_scale = fmaxf(row_up[HALVES ? r : x * BM + r] * p.scale * 1.4426950408889634f, Q8_LEAST_FACTOR);
         // warps none of whose 32 rows exist skip the arithmetic
         const bool warp_has_rows = 32 * (warp & 3) < rows_x;
         const uint32_t lane_base = ((uint32_t)(32 * (warp & 3))) << 16;

@@ -89,6 +89,23 @@ def test_scales_and_queries_of_every_size(portions, hd):
     _near(s, *_run(s, nq, nkv, hd, 0, "bfloat16", q=q, planes_=(k, ks, v, vs)), "bfloat16")
 
 
+@pytest.mark.parametrize("portions", [[(1, 40)] * 2, [(1, 1)], [(100, 5)], [(300, 20)]])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("scale", [0.1, 2.0 ** -100])
+def test_keys_and_queries_of_nothing_leave_the_mask_alone(portions, hd, scale):
+    """Scores that vanish - keys whose scale is zero or the least, queries of 2^-70, a factor of 2^-100 - weigh alike; a hidden key, whatever its scale, nothing."""
+    import torch
+    s = step(portions, 16)
+    nq, nkv = 8, 2
+    for keys in (0.0, 2.0 ** -64):
+        k, ks, v, vs = planes(s, nkv, hd)
+        ks = torch.where(torch.isnan(ks), ks, keys)
+        q = (torch.randn((s.num_tokens, nq * hd), device="cuda") * 2.0 ** -70).bfloat16()
+        _near(s, *_run(s, nq, nkv, hd, 0, "bfloat16", scale=scale, q=q, planes_=(k, ks, v, vs)), "bfloat16")
+        got, _, _ = _run(s, nq, nkv, hd, 0, "bfloat16", scale=scale, q=q, planes_=(k, ks, v, torch.where(torch.isnan(vs), vs, 0.0)))
+        assert (got.abs() <= 2.0 ** -57).all()
+
+
 @pytest.mark.parametrize("portions,bad", [([(1, 40), (1, 40)], 0), ([(100, 0)], 60), ([(300, 20)], 130)])
 @pytest.mark.parametrize("nq,nkv,hd", [(4, 4, 128), (8, 1, 64), (2, 2, 80)])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
