@@ -155,6 +155,14 @@ __device__ __forceinline__ Block find_block(const PrepParams &p, int unit) {
             tokens = p.cu[i + 1] - first;
             if (tokens > 0) {
                 pos = p.positions[first];
+                if (pos < 0) {                      // tokens in front of position 0 have no page
+                    const int gone = pos > -tokens ? -pos : tokens;
+                    first += gone;
+                    tokens -= gone;
+                    pos += gone;
+                }
+            }
+            if (tokens > 0) {
                 n = (pos + tokens - 1) / Q8_BLOCK - pos / Q8_BLOCK + 1;
             }
         }

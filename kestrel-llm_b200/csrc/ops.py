@@ -392,7 +392,7 @@ def attn_prepare_q8(qkv: Partials, q_norm_w: Optional[torch.Tensor], k_norm_w: O
     Where a step's tokens raise the scale of a block that earlier steps began, its codes are rounded again, so a block's codes depend on
     how a sequence was cut into steps (by at most half a step of the scale for each rise).  A block that met a number that is not finite
     has a scale that is not a number, until its page begins anew.  The tokens of request i are cu_seqlens[i] to cu_seqlens[i + 1] - 1, at
-    consecutive positions; rows of q_out behind the last request are left as they are, and so is a token whose page is absent.
+    consecutive positions; rows of q_out behind the last request are left as they are, and so is a token whose page is absent or whose position is below 0.
     ``described``: positions, cu_seqlens and block_table were on the device before the kernel in front of this one on the stream began,
     as a copy leaves them; the launch reads them while that kernel still runs."""
     dev = q_out.device

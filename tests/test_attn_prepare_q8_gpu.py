@@ -193,6 +193,37 @@ def test_a_layer_that_reads_only_writes_nothing():
     assert ((q.view(20, nq, hd).double() - q64).abs() <= E * 1.5 * q64.abs().amax(-1, keepdim=True)).all()
 
 
+@pytest.mark.parametrize("hd", [64, 80])
+def test_tokens_in_front_of_position_zero_are_left_out(hd):
+    """A request from position -20 on: its queries are turned back, its keys and values begin at position 0."""
+    import torch
+    nq, nkv = 4, 2
+    s = step([(10, 0), (3, 7)], 16)
+    k, ks, v, vs = planes(s, nkv, hd)
+    inputs = _inputs(s, nq, nkv, hd, 2, hd, True, True)
+    early = step([(30, 0), (3, 7)], 16)
+    early.positions[:30] = torch.arange(-20, 10, dtype=torch.int32)
+    early.table = s.table
+    longer = (torch.cat([torch.full((2, 20, inputs[0].shape[2]), 1e4, device="cuda"), inputs[0]], 1),) + inputs[1:]
+    got = []
+    for st, x in ((s, inputs), (early, longer)):
+        p = [t.clone() for t in (k, ks, v, vs)]
+        q = torch.full((st.num_tokens, nq * hd), float("nan"), device="cuda")
+        _append(st, x, *p, q, nq, nkv, hd, hd)
+        got.append(p + [q[-13:]])
+        assert torch.isfinite(q).all()
+    for a, b in zip(*got):
+        assert torch.equal(a.view(torch.uint8), b.contiguous().view(torch.uint8))
+    none = step([(5, 0)], 16)
+    none.positions.copy_(torch.arange(-2 ** 31, -2 ** 31 + 5))
+    q = torch.full((5, nq * hd), float("nan"), device="cuda")
+    p = [t.clone() for t in (k, ks, v, vs)]
+    _append(none, (inputs[0][:, :5].contiguous(),) + inputs[1:], *p, q, nq, nkv, hd, hd)
+    assert torch.isfinite(q).all()
+    for a, b in zip(p, (k, ks, v, vs)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_refusals():
     import torch
     from kestrel_llm_b200.csrc import ops
