@@ -392,7 +392,8 @@ def attn_prepare_q8(qkv: Partials, q_norm_w: Optional[torch.Tensor], k_norm_w: O
     Where a step's tokens raise the scale of a block that earlier steps began, its codes are rounded again, so a block's codes depend on
     how a sequence was cut into steps (by at most half a step of the scale for each rise).  A block that met a number that is not finite
     has a scale that is not a number, until its page begins anew.  The tokens of request i are cu_seqlens[i] to cu_seqlens[i + 1] - 1, at
-    consecutive positions; rows of q_out behind the last request are left as they are, and so is a token whose page is absent or whose position is below 0.
+    consecutive positions; rows of q_out behind the last request are left as they are, and so is a token whose page is absent or whose position is
+    below 0.
     ``described``: positions, cu_seqlens and block_table were on the device before the kernel in front of this one on the stream began,
     as a copy leaves them; the launch reads them while that kernel still runs."""
     dev = q_out.device
@@ -451,9 +452,13 @@ def attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     _need_q8("attention_q8", k_cache, v_cache, k_scale, v_scale, nkv, page_size, hd, dev)
     lib, code = library(), _code(q, "attention_q8.q")
     max_count, max_kv = batch.max_count, batch.max_kv_len
+    if max_kv > block_table.shape[1] * page_size and not batch.captured:
+        raise KernelError(f"attention_q8: {max_kv} keys in block tables of {block_table.shape[1]} pages of {page_size}")
     cu = kv = None
     if not batch.captured and max_count > 1:        # steps of single tokens need no look at the lengths
-        cu, kv = (ctypes.c_int * (n + 1))(*batch.cu_seqlens_host), (ctypes.c_int * n)(*batch.kv_lens_host)
+        if len(batch.cu_seqlens_host) <= n or len(batch.kv_lens_host) < n:
+            raise KernelError(f"attention_q8: a host's description of fewer than {n} requests")
+        cu, kv = (ctypes.c_int * (n + 1))(*batch.cu_seqlens_host[:n + 1]), (ctypes.c_int * n)(*batch.kv_lens_host[:n])
     with _on(dev):
         if cu is None:
             floats = _q8_scratch(dev.index, n, max_count, max_kv, T, nq, nkv, hd, window, code)
