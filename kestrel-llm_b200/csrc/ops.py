@@ -508,7 +508,7 @@ def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, top
     got = TokenLogprobs(None if ids is None else buf.as_strided((R,), (1,), 0), buf.as_strided((R,), (1,), R),
                         buf.view(torch.int32).as_strided((R, top), (top or 1, 1), 2 * R), buf.as_strided((R, top), (top or 1, 1), (2 + top) * R))
     with _on(dev):
-        _check(library().kestrel_token_logprobs(logits.data_ptr(), logits.stride(0), R, V, _p(ids), top, _p(got.logprobs), got.entropy.data_ptr(),
+        _check(library().kestrel_token_logprobs(logits.data_ptr(), logits.stride(0) if R > 1 else V, R, V, _p(ids), top, _p(got.logprobs), got.entropy.data_ptr(),
                                                 got.top_ids.data_ptr(), got.top_logprobs.data_ptr(), _stream()))
     return got
 

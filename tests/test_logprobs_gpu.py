@@ -111,6 +111,8 @@ def test_tokens_outside_the_vocabulary_and_no_tokens():
     assert torch.isnan(got.logprobs).tolist() == [True, True, False, False] and got.top_ids.shape == (4, 0)
     none = ops.token_logprobs(x, None, 3)
     assert none.logprobs is None and torch.equal(none.entropy, got.entropy)
+    one = ops.token_logprobs(x[2].clone()[:, None].t(), ids[2:3], 3)         # a row alone may have any stride
+    assert torch.equal(one.logprobs, got.logprobs[2:3]) and torch.equal(one.top_ids, none.top_ids[2:3])
     empty = ops.token_logprobs(x[:0], ids[:0], 3)
     assert empty.logprobs.shape == (0,) and empty.top_ids.shape == (0, 3)
 
