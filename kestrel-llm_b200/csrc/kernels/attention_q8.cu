@@ -15,6 +15,20 @@ namespace {
 // the true 32-bit path, and the one of head sizes that the tensor-core kernels do not take.
 constexpr int BM = 32, BN = 64, THREADS = 128;
 
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+    float2 d;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+    return d;
+}
+__device__ __forceinline__ void fma_pair(uint64_t &c, uint64_t a, uint64_t b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b)); }
+// code i of four: as the low byte of the number 2^23 + (c + 128), which a byte permutation makes (a conversion takes four times as long)
+__device__ __forceinline__ float code(uint32_t biased, int i) { return __uint_as_float(__byte_perm(biased, 0x4b000000u, 0x7440 + i)) - 8388736.0f; }
+
 template <int HDP> constexpr int lds_k() { return HDP + 4; }          // padded rows: sixteen lanes read sixteen keys without bank conflicts
 template <int HDP> constexpr size_t plain_smem() { return sizeof(float) * ((size_t)BM * lds_k<HDP>() + 2 * (size_t)BN * lds_k<HDP>() + BM * (BN + 4) + BN); }
 
@@ -31,20 +45,39 @@ __global__ void __launch_bounds__(THREADS) attention_q8_plain_kernel(const Q8Par
     if (!q8_find_tile(p, blockIdx.x, t)) return;
     int lo, hi;
     q8_slice(t, p.slices, slice, BN, lo, hi);
-    for (int i = tid; i < BM * HDP; i += THREADS) {
-        const int r = i / HDP, d = i % HDP;
-        float x = 0.f;
-        if (r < t.rows && d < p.hd) x = to_f32<T>(((const T *)p.q)[q8_out_row(p, t, kvh, r) * p.hd + d]);
-        Q[r * LD + d] = x;
+    // The four runs of a chunk of 16 dimensions lie a quarter of a row apart, so that the neighbours that hold a row's chunks write 16 bytes
+    // side by side.
+    auto place = [](int d, int run) { return run * (HDP / 4) + d / 4; };
+    // the queries, sixteen numbers a thread and turn, all of them in flight
+#pragma unroll
+    for (int i = 0; i < (BM * (HDP / 16) + THREADS - 1) / THREADS; ++i) {
+        const int r = (tid + i * THREADS) / (HDP / 16), d = (tid + i * THREADS) % (HDP / 16) * 16;
+        if (r >= BM) break;
+        const bool there = r < t.rows && d < p.hd;
+        const T *src = (const T *)p.q + (there ? q8_out_row(p, t, kvh, r) * p.hd + d : 0);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (there) {
+                if (sizeof(T) == 4) {
+                    x = *reinterpret_cast<const float4 *>(src + j);
+                } else {
+                    const uint2 u = *reinterpret_cast<const uint2 *>(src + j);
+                    x = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+                }
+            }
+            *reinterpret_cast<float4 *>(Q + r * LD + place(d, j / 4)) = x;
+        }
     }
-    float m[4], l[4], o[4][DV];
+    float m[4], l[4];
+    uint64_t o[4][DV / 2];
     int pos[4], low[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
-        for (int d = 0; d < DV; ++d) o[i][d] = 0.f;
+        for (int d = 0; d < DV / 2; ++d) o[i][d] = 0;
         const int r = 4 * rg + i;
         pos[i] = r < t.rows ? t.pos_begin + (t.row0 + r) / t.G : -1;
         low[i] = p.window > 0 ? max(0, pos[i] - p.window + 1) : 0;
@@ -78,32 +111,35 @@ __global__ void __launch_bounds__(THREADS) attention_q8_plain_kernel(const Q8Par
             const uint32_t kw[4] = {kq[i].x, kq[i].y, kq[i].z, kq[i].w}, vw[4] = {vq[i].x, vq[i].y, vq[i].z, vq[i].w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const char4 k = *reinterpret_cast<const char4 *>(&kw[j]), v = *reinterpret_cast<const char4 *>(&vw[j]);
-                *reinterpret_cast<float4 *>(K + r * LD + d + 4 * j) = make_float4(k.x * ks[i], k.y * ks[i], k.z * ks[i], k.w * ks[i]);
-                *reinterpret_cast<float4 *>(V + r * LD + d + 4 * j) = make_float4(v.x, v.y, v.z, v.w);
+                const uint32_t k = kw[j] ^ 0x80808080u, v = vw[j] ^ 0x80808080u;
+                *reinterpret_cast<float4 *>(K + r * LD + place(d, j)) = make_float4(code(k, 0) * ks[i], code(k, 1) * ks[i], code(k, 2) * ks[i], code(k, 3) * ks[i]);
+                *reinterpret_cast<float4 *>(V + r * LD + place(d, j)) = make_float4(code(v, 0), code(v, 1), code(v, 2), code(v, 3));
             }
             if (d == 0) sv_s[r] = vs[i];
         }
         __syncthreads();
         if (kb + BN < hi) fetch(kb + BN);
-        float s[4][4] = {};
+        uint64_t s2[4][4] = {};             // even and odd dimensions' sums
 #pragma unroll 4
         for (int d = 0; d < HDP; d += 4) {
-            float4 a[4], b[4];
+            ulonglong2 a[4], b[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4 *>(Q + (4 * rg + i) * LD + d);
+            for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const ulonglong2 *>(Q + (4 * rg + i) * LD + d);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4 *>(K + (kg + 16 * j) * LD + d);
+            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const ulonglong2 *>(K + (kg + 16 * j) * LD + d);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    s[i][j] = fmaf(a[i].x, b[j].x, s[i][j]);
-                    s[i][j] = fmaf(a[i].y, b[j].y, s[i][j]);
-                    s[i][j] = fmaf(a[i].z, b[j].z, s[i][j]);
-                    s[i][j] = fmaf(a[i].w, b[j].w, s[i][j]);
+                    fma_pair(s2[i][j], a[i].x, b[j].x);
+                    fma_pair(s2[i][j], a[i].y, b[j].y);
                 }
         }
+        float s[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[i][j] = halves(s2[i][j]).x + halves(s2[i][j]).y;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float mx = -INFINITY;
@@ -131,7 +167,10 @@ __global__ void __launch_bounds__(THREADS) attention_q8_plain_kernel(const Q8Par
             for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
             l[i] = l[i] * alpha + sum;
 #pragma unroll
-            for (int d = 0; d < DV; ++d) o[i][d] *= alpha;
+            for (int d = 0; d < DV / 2; ++d) {
+                const float2 x = halves(o[i][d]);
+                o[i][d] = pair(x.x * alpha, x.y * alpha);
+            }
         }
         __syncwarp();               // a row's probabilities are its own sixteen lanes'
 #pragma unroll 2
@@ -146,13 +185,11 @@ __global__ void __launch_bounds__(THREADS) attention_q8_plain_kernel(const Q8Par
             for (int k = 0; k < 4; ++k)
 #pragma unroll
                 for (int d = 0; d < DV; d += 4) {
-                    const float4 x = *reinterpret_cast<const float4 *>(V + (j + k) * LD + 4 * kg + 16 * d);
+                    const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(V + (j + k) * LD + 4 * kg + 16 * d);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        o[i][d] = fmaf(pr[i][k], x.x, o[i][d]);
-                        o[i][d + 1] = fmaf(pr[i][k], x.y, o[i][d + 1]);
-                        o[i][d + 2] = fmaf(pr[i][k], x.z, o[i][d + 2]);
-                        o[i][d + 3] = fmaf(pr[i][k], x.w, o[i][d + 3]);
+                        fma_pair(o[i][d / 2], pair(pr[i][k], pr[i][k]), x.x);
+                        fma_pair(o[i][d / 2 + 1], pair(pr[i][k], pr[i][k]), x.y);
                     }
                 }
         }
@@ -162,24 +199,22 @@ __global__ void __launch_bounds__(THREADS) attention_q8_plain_kernel(const Q8Par
         const int r = 4 * rg + i;
         if (r >= t.rows) continue;
         const size_t row = q8_out_row(p, t, kvh, r);
-        if (p.slices > 1) {
+        const float inv = p.slices > 1 ? 1.0f : 1.0f / l[i];
 #pragma unroll
-            for (int d = 0; d < DV; ++d) {
-                const int at = 4 * kg + 16 * (d & ~3) + (d & 3);
-                if (at < p.hd) p.part_o[(row * p.slices + slice) * p.hd + at] = o[i][d];
-            }
-            if (kg == 0) {
-                p.part_ml[(row * p.slices + slice) * 2] = m[i];
-                p.part_ml[(row * p.slices + slice) * 2 + 1] = l[i];
-            }
-        } else {
-            const float inv = 1.0f / l[i];
-#pragma unroll
-            for (int d = 0; d < DV; ++d) {
-                const int at = 4 * kg + 16 * (d & ~3) + (d & 3);
-                if (at < p.hd) ((T *)p.out)[row * p.hd + at] = from_f32<T>(o[i][d] * inv);
+        for (int d = 0; d < DV; d += 4) {
+            const int at = 4 * kg + 16 * d, dim = at % (HDP / 4) * 4 + at / (HDP / 4) * 4;      // four neighbours, and where they belong
+            if (dim >= p.hd) continue;
+            const float2 x = halves(o[i][d / 2]), y = halves(o[i][d / 2 + 1]);
+            if (p.slices > 1) {
+                *reinterpret_cast<float4 *>(p.part_o + (row * p.slices + slice) * p.hd + dim) = make_float4(x.x, x.y, y.x, y.y);
+            } else if (sizeof(T) == 4) {
+                *reinterpret_cast<float4 *>((T *)p.out + row * p.hd + dim) = make_float4(x.x * inv, x.y * inv, y.x * inv, y.y * inv);
+            } else {
+                const __nv_bfloat162 a = __floats2bfloat162_rn(x.x * inv, x.y * inv), b = __floats2bfloat162_rn(y.x * inv, y.y * inv);
+                *reinterpret_cast<uint2 *>((T *)p.out + row * p.hd + dim) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
             }
         }
+        if (p.slices > 1 && kg == 0) *reinterpret_cast<float2 *>(p.part_ml + (row * p.slices + slice) * 2) = make_float2(m[i], l[i]);
     }
 }
 
@@ -343,9 +378,11 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
             p->slices = q8_decode_cluster((long long)nseq * p->row_tiles * nkv, (p->longest + 63) / 64, p->key_tiles, hd, p->most_rows);
             p->scratch = p->slices ? 0 : q8_decode_scratch(p->ctas, hd);
         } else {
-            // the tensor cores: one CTA an SM, slices of two key tiles at least
+            // The tensor cores: one CTA an SM, slices of two key tiles at least.  The CUDA cores: two CTAs an SM, which a key tile takes 6 us, the
+            // merge 3: slices of one tile, and CTAs for two rounds (float32, 16 / 4 heads of 128: 8 tokens behind 400 keys 19 us, 49 with slices of
+            // 256 keys; 411 tokens 52 us, 63 with CTAs for one round; eight single tokens behind 3,000 keys 63 us, 61 with one round).
             p->slices = p->kernel == TC ? slices_for(p->tiles * nkv, kestrel_sms(), p->longest, 256)
-                                        : slices_for(p->tiles * nkv, kestrel_sms() * 2, p->longest, 256);
+                                        : slices_for(p->tiles * nkv, kestrel_sms() * 4, p->longest, BN);
             p->scratch = p->slices > 1 ? (long long)T * nq * p->slices * (hd + 2) : 0;
         }
         pl.part[pl.parts++] = *p;
