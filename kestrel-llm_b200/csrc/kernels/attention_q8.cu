@@ -287,6 +287,7 @@ constexpr int MAX_SLICES = 32;
 enum Kernel { CORES, DECODE, TC };
 struct Part {
     Kernel kernel = CORES;
+    Q8Form form = Q8_EIGHT;
     int rows_above = 0, rows_upto = 0, rows_per_tile = 0, slices = 1, longest = 0;
     long long tiles = 0;
     int ctas = 0, most_rows = 0, row_tiles = 0;
@@ -308,11 +309,11 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
     const int G = nq / nkv;
     auto seen_of = [&](int keys, long long rows) { return window > 0 ? (int)std::min<long long>(keys, window + (rows - 1) / G) : keys; };
     constexpr int FEW = 512;                // rows of a portion that may go to the decode kernel
-    const bool cores = dtype != KESTREL_BF16 || (hd != 64 && hd != 128);
+    const bool cores = hd != 64 && hd != 128, wide = dtype != KESTREL_BF16;
     Part small, large;
     small.kernel = cores ? CORES : DECODE;
-    small.rows_upto = cores ? 0x7fffffff : 16;
-    if (!cores && cu) {
+    small.rows_upto = cores || wide ? 0x7fffffff : 16;
+    if (!cores && !wide && cu) {
         // Short portions go to the decode kernel, which reads a request's keys again for every 16 rows, if that leaves no portion to the other
         // kernel: where every pair has its CTAs at once and their work is little (32 / 8 heads of 128, one request, behind 500 keys: 16 tokens
         // 10.9 us against 14.9, 64 tokens 13.8 against 16.7, 128 tokens 16.9 against 17.8; 64 tokens behind 2,000 keys 27 against 19; four
@@ -333,14 +334,14 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
         }
         const long long pairs = (long long)nseq * ((most + 15) / 16) * nkv;
         if (all && most > 16 && tiles <= (single ? 24 : 8) * 2ll * kestrel_sms() &&
-            (q8_decode_cluster(pairs, (longest + 63) / 64, tiles, hd, most) > 0 || (single && pairs <= q8_decode_ctas(tiles, hd, most))))
+            (q8_decode_cluster(pairs, (longest + 63) / 64, tiles, hd, Q8_SIXTEEN) > 0 || (single && pairs <= q8_decode_ctas(tiles, hd, Q8_SIXTEEN))))
             small.rows_upto = FEW;
     }
     large.kernel = TC;
     large.rows_above = small.rows_upto;
     large.rows_upto = 0x7fffffff;
     large.rows_per_tile = 256;
-    if (!cores && cu) {
+    if (!cores && !wide && cu) {
         // while tiles of 128 rows fit the SMs at once, a CTA takes one and its key tiles go to the two streams in turn
         long long tiles = 0;
         for (int i = 0; i < nseq; ++i) {
@@ -349,7 +350,7 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
         }
         if (tiles * nkv <= kestrel_sms()) large.rows_per_tile = 128;
     }
-    small.rows_per_tile = cores ? BM : 16;
+    small.rows_per_tile = cores ? BM : wide ? 8 : 16;
     auto count = [&](long long rows, int keys, int times) {
         if (rows <= 0) return;
         Part &p = rows <= small.rows_upto ? small : large;
@@ -372,10 +373,11 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
     for (Part *p : {&small, &large}) {
         if (!p->tiles) continue;
         if (p->kernel == DECODE) {
-            if (p->most_rows <= 8) p->rows_per_tile = 8;
-            p->ctas = q8_decode_ctas(p->key_tiles, hd, p->most_rows);
+            p->form = wide ? Q8_WIDE : p->most_rows <= 8 ? Q8_EIGHT : Q8_SIXTEEN;
+            p->rows_per_tile = p->form == Q8_SIXTEEN ? 16 : 8;
+            p->ctas = q8_decode_ctas(p->key_tiles, hd, p->form);
             p->row_tiles = (p->most_rows + p->rows_per_tile - 1) / p->rows_per_tile;
-            p->slices = q8_decode_cluster((long long)nseq * p->row_tiles * nkv, (p->longest + 63) / 64, p->key_tiles, hd, p->most_rows);
+            p->slices = q8_decode_cluster((long long)nseq * p->row_tiles * nkv, (p->longest + 63) / 64, p->key_tiles, hd, p->form);
             p->scratch = p->slices ? 0 : q8_decode_scratch(p->ctas, hd);
         } else {
             // The tensor cores: one CTA an SM, slices of two key tiles at least.  The CUDA cores: two CTAs an SM, which a key tile takes 6 us, the
@@ -421,7 +423,7 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
     make_plan(pl, cu_host, kv_host, nseq, max_count, max_kv, T, nq, nkv, hd, window, dtype);
     for (int i = 0; i < pl.parts; ++i) {
         const Part &part = pl.part[i];
-        KESTREL_REQUIRE(part.tiles * nkv < (1ll << 31) && (part.kernel != DECODE || part.key_tiles / nkv < (1ll << 31)),
+        KESTREL_REQUIRE(part.tiles * nkv < (1ll << 31) && (part.kernel != DECODE || (part.key_tiles / nkv < (1ll << 31) && (long long)nseq * part.row_tiles < (1ll << 31))),
                         "attention_q8: %lld row tiles and %lld key tiles of %d kv heads exceed the grid", part.tiles, part.key_tiles, nkv);
         KESTREL_REQUIRE(part.scratch == 0 || (scratch && part.scratch <= scratch_floats), "attention_q8: scratch of %lld floats is needed, %lld given", part.scratch, scratch_floats);
     }
@@ -439,7 +441,7 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
         int rc;
         if (part.kernel == DECODE) {
             p.part_ml = scratch ? scratch + 2ll * part.ctas * 16 * hd : nullptr;
-            rc = q8_launch_decode(p, part.ctas, stream);
+            rc = q8_launch_decode(p, part.form, part.ctas, stream);
             launches += part.slices ? 1 : 2;
         } else {
             p.part_ml = scratch ? scratch + (long long)T * nq * part.slices * hd : nullptr;

@@ -25,6 +25,7 @@
 
 #include <cuda_fp16.h>
 #include <math.h>
+#include <type_traits>
 
 __device__ int g_q8d_error = 0;
 
@@ -33,13 +34,16 @@ namespace {
 constexpr int THREADS = 160, BN = 64, MAX_CLUSTER = 8;      // four consumer warps and the loader; keys of a tile
 constexpr uint32_t MAGIC = 0x64646464u;     // high byte of the float16 numbers 1024 .. 1279
 
-// NT: column tiles of eight rows.  One: three CTAs an SM; two: two.
-template <int HD, int NT> struct Ring {
-    static constexpr int STAGES = (NT == 1 ? 3 : 4) * (128 / HD), CTAS = NT == 1 ? 3 : 2;
+// NT: column tiles of eight rows.  One: three CTAs an SM; two, or one of float32: two.
+template <int HD, int NT, typename T> struct Ring {
+    static constexpr bool THREE = NT == 1 && sizeof(T) == 2;
+    static constexpr int STAGES = (THREE ? 3 : 4) * (128 / HD), CTAS = THREE ? 3 : 2;
     static constexpr int LDO = HD + 4;      // row of a warp's outputs, in floats, when the four warps meet
     static constexpr uint32_t PLANE = BN * HD, STAGE = 2 * PLANE;
     static constexpr uint32_t SCALES = STAGES * STAGE, BARS = SCALES + STAGES * 32, MEET = BARS + 16 * STAGES, BYTES = MEET + 4 * 8 * NT * (LDO + 2) * 4;
 };
+
+template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : 1; }
 
 __device__ __forceinline__ uint32_t hsub2(uint32_t a) {             // - 1152 from both halves
     uint32_t d;
@@ -65,6 +69,18 @@ __device__ __forceinline__ float rcp_fast(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// two numbers as pairs of float16 parts, the largest first: three of them leave 2^-33 of a number, or 2^-25
+template <int PARTS>
+__device__ __forceinline__ void split(float lo, float hi, uint32_t (&part)[PARTS]) {
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+        part[i] = pack_f16(lo, hi);
+        if (i + 1 == PARTS) break;
+        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&part[i]));
+        lo -= x.x;
+        hi -= x.y;
+    }
 }
 __device__ __forceinline__ void mma_f16(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -169,7 +185,10 @@ struct Line {
     }
 };
 
-// CTA u's stretch begins here; the CTA whose stretch holds tile `at`
+// Stretches that the line is cut into: one for every CTA, but of two tiles at least - a recorded launch may meet a shorter line than it was
+// made for, and a CTA without tiles would leave its part of a pair unwritten
+__device__ __forceinline__ int stretches(long long length, int ctas) { return (int)max(1ll, min((long long)ctas, length / 2)); }
+// stretch u begins here; the stretch that holds tile `at`
 __device__ __forceinline__ long long stretch(long long u, long long length, int ctas) { return u * length / ctas; }
 __device__ __forceinline__ int holder(long long at, long long length, int ctas) { return (int)(((at + 1) * ctas - 1) / length); }
 
@@ -179,7 +198,7 @@ struct Walk {
     long long at, end, begin;           // next tile, end of the stretch, place of the pair's first tile
     int seq, n, kvh, row0;              // the pair; n: its tiles, row0: its first row among the request's
     // the part
-    int G, row_tiles, all_rows, rows, tok_begin, pos_begin, k_first, k_end, from, to;
+    int G, row_tiles, all_rows, rows, tok_begin, pos_begin, k_first, k_end, from, to, seen_from, seen_to;
     const int *table;
     bool whole;
 
@@ -193,14 +212,15 @@ struct Walk {
         if (n == 0) return;
         row0 = rt * p.rows_per_tile;
         describe();
-        rows = min(p.rows_per_tile, all_rows - row0);
-        from = (int)((long long)n * rank / ranks);
-        to = (int)((long long)n * (rank + 1) / ranks);
+        see();
+        from = seen_from + (int)((long long)(seen_to - seen_from) * rank / ranks);
+        to = seen_from + (int)((long long)(seen_to - seen_from) * (rank + 1) / ranks);
         whole = ranks == 1;
     }
     __device__ __forceinline__ Walk(const Q8Params &p_, long long length) : p(p_), n(0) {
-        at = stretch(blockIdx.x, length, gridDim.x);
-        end = stretch(blockIdx.x + 1, length, gridDim.x);
+        const int cuts = stretches(length, gridDim.x);
+        at = stretch(min((int)blockIdx.x, cuts), length, cuts);
+        end = stretch(min((int)blockIdx.x + 1, cuts), length, cuts);
         G = p.nq / p.nkv;
         if (at >= end) return;
         const Line line{p};
@@ -221,6 +241,13 @@ struct Walk {
         k_first = p.window > 0 ? max(0, pos_begin - p.window + 1) : 0;
         table = p.block_table + (size_t)seq * p.table_stride;
     }
+    // the pair's rows, and the tiles that some of them see
+    __device__ __forceinline__ void see() {
+        rows = min(p.rows_per_tile, all_rows - row0);
+        const int first = k_first / BN, last_pos = pos_begin + (row0 + rows - 1) / G;
+        seen_from = p.window > 0 ? max(0, pos_begin + row0 / G - p.window + 1) / BN - first : 0;
+        seen_to = last_pos / BN - first + 1;
+    }
     // the next part: tiles [from, to) of the pair; false at the end of the stretch
     __device__ __forceinline__ bool next() {
         if (at >= end) return false;
@@ -238,11 +265,13 @@ struct Walk {
                 }
             }
         }
-        rows = min(p.rows_per_tile, all_rows - row0);
+        see();
         from = (int)(at - begin);
         to = (int)min((long long)n, end - begin);
         whole = from == 0 && to == n;
         at = begin + to;
+        from = max(from, seen_from);
+        to = min(to, seen_to);
         return true;
     }
     __device__ __forceinline__ size_t out_row(int r) const { return (size_t)(tok_begin + (row0 + r) / G) * p.nq + kvh * G + (row0 + r) % G; }
@@ -253,8 +282,8 @@ template <int HD> __device__ __forceinline__ float *part_out(const Q8Params &p, 
 __device__ __forceinline__ float2 *part_ml(const Q8Params &p, long long part, int row) { return reinterpret_cast<float2 *>(p.part_ml) + part * 16 + row; }
 
 // A block's scores s - (key g, rows 2 c and 2 c + 1), (key g + 8, the same) - become weights; the rows' references, sums and outputs follow.
-// sk: the keys' scale, lv and rv: log2 and reciprocal of the values'.  MASKED: some row does not see the block whole.
-template <int NT, bool MASKED, int NO>
+// sk: the keys' scale, lv and rv: log2 and reciprocal of the values', or of its power of two (WIDE).  MASKED: some row does not see the block whole.
+template <int NT, bool MASKED, bool WIDE, int NO>
 __device__ __forceinline__ void weigh(float (&s)[NT][4], float (&o)[NT][NO][4], float (&m)[NT][2], float (&l)[NT][2], const float (&row_scale)[NT][2], float sk,
                                       float lv, float rv, int kbase, int my_key, const int (&pos)[NT][2], const int (&low)[NT][2]) {
     float mx[NT][2], ck[NT][2];
@@ -275,9 +304,9 @@ __device__ __forceinline__ void weigh(float (&s)[NT][4], float (&o)[NT][NO][4], 
             // in base-2 units, with the value's scale: x = s * ck + lv
             mx[nt][i] = fmaf(fmaxf(s[nt][i], s[nt][2 + i]), ck[nt][i], lv);
             if (MASKED && none[nt][i]) mx[nt][i] = -INFINITY;
-            grow |= mx[nt][i] > m[nt][i] + 8.f || (m[nt][i] == -INFINITY && mx[nt][i] > -INFINITY);
+            grow |= mx[nt][i] > m[nt][i] + (WIDE ? 0.f : 8.f) || (m[nt][i] == -INFINITY && mx[nt][i] > -INFINITY);
         }
-    // the reference moves once the maximum has outgrown it by 8: weights stay below 2^8
+    // The reference moves once the maximum has outgrown it by 8: weights stay below 2^8.  (Float32: with the maximum.)
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -286,7 +315,7 @@ __device__ __forceinline__ void weigh(float (&s)[NT][4], float (&o)[NT][NO][4], 
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) mx[nt][i] = fmaxf(mx[nt][i], __shfl_xor_sync(0xffffffffu, mx[nt][i], x));
                 if (mx[nt][i] > m[nt][i]) {
-                    const float alpha = m[nt][i] == -INFINITY ? 0.f : exp2_fast(m[nt][i] - mx[nt][i]);
+                    const float alpha = m[nt][i] == -INFINITY ? 0.f : WIDE ? exp2f(m[nt][i] - mx[nt][i]) : exp2_fast(m[nt][i] - mx[nt][i]);
                     m[nt][i] = mx[nt][i];
                     l[nt][i] *= alpha;
 #pragma unroll
@@ -298,21 +327,23 @@ __device__ __forceinline__ void weigh(float (&s)[NT][4], float (&o)[NT][NO][4], 
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const float shift = lv - (m[nt][i] == -INFINITY ? 0.f : m[nt][i]);
+            // (float32: times 2^14, so that a weight with its scale's other factor stays below 2^15, and its parts leave 2^-39 of the largest)
+            const float shift = lv - (m[nt][i] == -INFINITY ? 0.f : m[nt][i]) + (WIDE ? 14.f : 0.f);
             float &a = s[nt][i], &b = s[nt][2 + i];
-            a = exp2_fast(fmaf(a, ck[nt][i], shift));
-            b = exp2_fast(fmaf(b, ck[nt][i], shift));
+            a = WIDE ? exp2f(fmaf(a, ck[nt][i], shift)) : exp2_fast(fmaf(a, ck[nt][i], shift));
+            b = WIDE ? exp2f(fmaf(b, ck[nt][i], shift)) : exp2_fast(fmaf(b, ck[nt][i], shift));
             if (MASKED && none[nt][i]) a = b = 0.f;
             else l[nt][i] = fmaf(a + b, rv, l[nt][i]);
         }
 }
 
-template <int HD, int NT, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS, Ring<HD, NT>::CTAS)
+template <typename T, int HD, int NT, bool CLUSTER>
+__global__ void __launch_bounds__(THREADS, Ring<HD, NT, T>::CTAS)
 attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Q8Params p) {
     pdl_launch_dependents();
-    using R = Ring<HD, NT>;
-    constexpr int KS = HD / 16, HALVES = HD / 64, ROWS = 8 * NT;
+    using R = Ring<HD, NT, T>;
+    constexpr int KS = HD / 16, HALVES = HD / 64, ROWS = 8 * NT, PARTS = parts_of<T>();
+    constexpr bool WIDE = PARTS > 1;
     constexpr uint32_t FIN_ML = ROWS * HD * 4;
     extern __shared__ uint8_t q8d_smem[];
     const uint32_t base = (smem_u32(q8d_smem) + 1023u) & ~1023u;
@@ -343,10 +374,15 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     // eight neighbouring numbers of an output row
     auto store = [&](size_t at, const float *acc, float L) {
         const float inv = 1.0f / L;
-        __nv_bfloat162 b[4];
+        if constexpr (WIDE) {
+            *reinterpret_cast<float4 *>((float *)p.out + at) = make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+            *reinterpret_cast<float4 *>((float *)p.out + at + 4) = make_float4(acc[4] * inv, acc[5] * inv, acc[6] * inv, acc[7] * inv);
+        } else {
+            __nv_bfloat162 b[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) b[j] = __floats2bfloat162_rn(acc[2 * j] * inv, acc[2 * j + 1] * inv);
-        *reinterpret_cast<uint4 *>((__nv_bfloat16 *)p.out + at) = *reinterpret_cast<uint4 *>(b);
+            for (int j = 0; j < 4; ++j) b[j] = __floats2bfloat162_rn(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+            *reinterpret_cast<uint4 *>((__nv_bfloat16 *)p.out + at) = *reinterpret_cast<uint4 *>(b);
+        }
     };
 
     if (warp == 4) {
@@ -398,32 +434,35 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     while (next()) {
         // Queries as fragments, in float16: a row is multiplied by the power of two that brings its largest number to [64, 128), so that
         // a bfloat16 number keeps its bits down to 2^-21 of that, and the rest is off by 2^-31 of it.
-        uint32_t qb[NT][KS][2];
+        // float32: three parts of a number, which leave 2^-31 of the row's largest.
+        uint32_t qb[PARTS][NT][KS][2];
         float row_scale[NT][2], bias[NT][2];            // of rows 2 c and 2 c + 1
         int pos[NT][2], low[NT][2], min_pos = 0x7fffffff, max_low = 0;      // (the last two of the rows that are there)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int r = 8 * nt + g;
-            uint4 q[HALVES][2];
+            constexpr int VECS = WIDE ? 4 : 2;
+            uint4 q[HALVES][VECS];
             uint32_t big = 0;
 #pragma unroll
             for (int j = 0; j < HALVES; ++j) {
-                q[j][0] = q[j][1] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int k = 0; k < VECS; ++k) q[j][k] = make_uint4(0, 0, 0, 0);
                 if (r < w.rows) {
-                    const uint4 *src = reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)p.q + w.out_row(r) * HD + 64 * j + 16 * c);
-                    q[j][0] = src[0];
-                    q[j][1] = src[1];
+                    const uint4 *src = reinterpret_cast<const uint4 *>((const T *)p.q + w.out_row(r) * HD + 64 * j + 16 * c);
+#pragma unroll
+                    for (int k = 0; k < VECS; ++k) q[j][k] = src[k];
                 }
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
+                for (int k = 0; k < VECS; ++k) {
                     const uint32_t *u = reinterpret_cast<const uint32_t *>(&q[j][k]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) big = max(big, max(u[e] & 0x7fffu, (u[e] >> 16) & 0x7fffu));
+                    for (int e = 0; e < 4; ++e) big = max(big, WIDE ? u[e] & 0x7fffffffu : max(u[e] & 0x7fffu, (u[e] >> 16) & 0x7fffu));
                 }
             }
             big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
             big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-            const int e = (int)(big >> 7);              // biased exponent of the largest; 255: not finite, as it is
+            const int e = (int)(big >> (WIDE ? 23 : 7));         // biased exponent of the largest; 255: not finite, as it is
             const int up = big == 0 || e == 255 ? 0 : 127 + 6 - max(e, 63);      // (below 2^-64 nothing weighs)
             const float f = __uint_as_float((uint32_t)(127 + up) << 23);
             float sum = 0.f;
@@ -431,18 +470,27 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
             for (int j = 0; j < HALVES; ++j)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {           // k-step 4 j + k: dimensions 64 j + 16 c + 4 k ..
-                    const uint32_t a = reinterpret_cast<const uint32_t *>(&q[j][k >> 1])[2 * (k & 1)], b = reinterpret_cast<const uint32_t *>(&q[j][k >> 1])[2 * (k & 1) + 1];
-                    const uint32_t x = pack_f16(__uint_as_float(a << 16) * f, __uint_as_float(a & 0xffff0000u) * f);
-                    const uint32_t y = pack_f16(__uint_as_float(b << 16) * f, __uint_as_float(b & 0xffff0000u) * f);
-                    qb[nt][4 * j + k][0] = x;
-                    qb[nt][4 * j + k][1] = y;
-                    const float2 fx = __half22float2(*reinterpret_cast<const __half2 *>(&x)), fy = __half22float2(*reinterpret_cast<const __half2 *>(&y));
-                    sum += (fx.x + fx.y) + (fy.x + fy.y);
+                    uint32_t x[PARTS], y[PARTS];
+                    if constexpr (WIDE) {
+                        split<PARTS>(__uint_as_float(q[j][k].x) * f, __uint_as_float(q[j][k].y) * f, x);
+                        split<PARTS>(__uint_as_float(q[j][k].z) * f, __uint_as_float(q[j][k].w) * f, y);
+                    } else {
+                        const uint32_t a = reinterpret_cast<const uint32_t *>(&q[j][k >> 1])[2 * (k & 1)], b = reinterpret_cast<const uint32_t *>(&q[j][k >> 1])[2 * (k & 1) + 1];
+                        x[0] = pack_f16(__uint_as_float(a << 16) * f, __uint_as_float(a & 0xffff0000u) * f);
+                        y[0] = pack_f16(__uint_as_float(b << 16) * f, __uint_as_float(b & 0xffff0000u) * f);
+                        const float2 fx = __half22float2(*reinterpret_cast<const __half2 *>(x)), fy = __half22float2(*reinterpret_cast<const __half2 *>(y));
+                        sum += (fx.x + fx.y) + (fy.x + fy.y);
+                    }
+#pragma unroll
+                    for (int i = 0; i < PARTS; ++i) {
+                        qb[i][nt][4 * j + k][0] = x[i];
+                        qb[i][nt][4 * j + k][1] = y[i];
+                    }
                 }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            const float scale_g = fmaxf(__uint_as_float((uint32_t)(127 - up) << 23) * p.scale * (1.4426950408889634f * 16777216.0f), Q8_LEAST_FACTOR);
-            const float bias_g = sum * (-128.0f / 16777216.0f);
+            const float scale_g = fmaxf(__uint_as_float((uint32_t)(127 - up) << 23) * p.scale * (1.4426950408889634f * (WIDE ? 1.0f : 16777216.0f)), Q8_LEAST_FACTOR);
+            const float bias_g = WIDE ? 0.f : sum * (-128.0f / 16777216.0f);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 row_scale[nt][i] = __shfl_sync(0xffffffffu, scale_g, 8 * c + 4 * i);
@@ -490,26 +538,50 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const uint32_t x0 = u0[k] ^ 0x80808080u, x1 = u1[k] ^ 0x80808080u;
-                        const uint32_t a[4] = {__byte_perm(x0, 0, 0x4140), __byte_perm(x1, 0, 0x4140), __byte_perm(x0, 0, 0x4342), __byte_perm(x1, 0, 0x4342)};
+                        if constexpr (WIDE) {
+                            // small parts first, and every k-step from zero: the unit's sums are cut off rather than rounded
+                            const uint32_t a[4] = {hsub2(__byte_perm(x0, MAGIC, 0x4140)), hsub2(__byte_perm(x1, MAGIC, 0x4140)),
+                                                   hsub2(__byte_perm(x0, MAGIC, 0x4342)), hsub2(__byte_perm(x1, MAGIC, 0x4342))};
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a, qb[nt][4 * j + k][0], qb[nt][4 * j + k][1]);
+                            for (int nt = 0; nt < NT; ++nt) {
+                                float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                                for (int i = PARTS - 1; i >= 0; --i) mma_f16(t, a, qb[i][nt][4 * j + k][0], qb[i][nt][4 * j + k][1]);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) s[nt][i] += t[i];
+                            }
+                        } else {
+                            const uint32_t a[4] = {__byte_perm(x0, 0, 0x4140), __byte_perm(x1, 0, 0x4140), __byte_perm(x0, 0, 0x4342), __byte_perm(x1, 0, 0x4342)};
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a, qb[0][nt][4 * j + k][0], qb[0][nt][4 * j + k][1]);
+                        }
                     }
                 }
                 const float *sc = reinterpret_cast<const float *>(ring + R::SCALES + stage * 32);
                 // (what is no number stays that)
                 const float sk = sc[warp] < Q8_LEAST_SCALE ? Q8_LEAST_SCALE : sc[warp], sv = sc[4 + warp] < Q8_LEAST_SCALE ? Q8_LEAST_SCALE : sc[4 + warp];
-                const float lv = log2_fast(sv), rv = rcp_fast(sv);
+                // float32: the values' scale is a power of two, which is exact as a logarithm, and a factor in [1, 2) on the weights
+                const bool number = sv <= 3.4e38f;
+                const float rv = WIDE ? 1.0f / __uint_as_float(__float_as_uint(sv) & 0x7f800000u) : rcp_fast(sv);
+                const float lv = !WIDE ? log2_fast(sv) : number ? (float)((int)(__float_as_uint(sv) >> 23) - 127) : __uint_as_float(0x7fc00000u);
                 if (kbase >= w.k_first && kbase + 16 <= w.k_end && kbase + 15 <= min_pos && kbase >= max_low) {
-                    weigh<NT, false>(s, o, m, l, row_scale, sk, lv, rv, kbase, my_key, pos, low);
+                    weigh<NT, false, WIDE>(s, o, m, l, row_scale, sk, lv, rv, kbase, my_key, pos, low);
                 } else {
-                    weigh<NT, true>(s, o, m, l, row_scale, sk, lv, rv, kbase, my_key, pos, low);
+                    weigh<NT, true, WIDE>(s, o, m, l, row_scale, sk, lv, rv, kbase, my_key, pos, low);
                 }
                 // out += w V: the transposed weights' pairs are keys 2 c, 2 c + 1 of both halves
-                uint32_t b[NT][2];
+                uint32_t b[PARTS][NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    b[nt][0] = transpose(pack_f16(s[nt][0], s[nt][1]));
-                    b[nt][1] = transpose(pack_f16(s[nt][2], s[nt][3]));
+                    const float factor = WIDE && number ? sv * rv : 1.f;
+                    uint32_t x[PARTS], y[PARTS];
+                    split<PARTS>(s[nt][0] * factor, s[nt][1] * factor, x);
+                    split<PARTS>(s[nt][2] * factor, s[nt][3] * factor, y);
+#pragma unroll
+                    for (int i = 0; i < PARTS; ++i) {
+                        b[i][nt][0] = transpose(x[i]);
+                        b[i][nt][1] = transpose(y[i]);
+                    }
                 }
                 uint32_t v[4][HD / 32];
                 if (HD == 128) {                            // this thread's 16 dimensions
@@ -533,8 +605,19 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                                             hsub2(__byte_perm(p3, MAGIC, 0x4140)), hsub2(__byte_perm(p3, MAGIC, 0x4342))};
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma_f16(o[nt][2 * k], a0, b[nt][0], b[nt][1]);
-                        mma_f16(o[nt][2 * k + 1], a1, b[nt][0], b[nt][1]);
+                        if constexpr (WIDE) {
+                            float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int i = PARTS - 1; i >= 0; --i) {
+                                mma_f16(t0, a0, b[i][nt][0], b[i][nt][1]);
+                                mma_f16(t1, a1, b[i][nt][0], b[i][nt][1]);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[nt][2 * k][i] += t0[i], o[nt][2 * k + 1][i] += t1[i];
+                        } else {
+                            mma_f16(o[nt][2 * k], a0, b[0][nt][0], b[0][nt][1]);
+                            mma_f16(o[nt][2 * k + 1], a1, b[0][nt][0], b[0][nt][1]);
+                        }
                     }
                 }
             }
@@ -634,7 +717,7 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                 }
 #pragma unroll
                 for (int s = 0; s < MAX_CLUSTER; ++s) {
-                    const float f = ml[s].x == -INFINITY ? 0.f : exp2_fast(ml[s].x - M);
+                    const float f = ml[s].x == -INFINITY ? 0.f : exp2f(ml[s].x - M);
                     if (s >= p.slices || (f == 0.f && ml[s].y == ml[s].y)) continue;       // (a sum that is no number stays that)
                     L = fmaf(ml[s].y, f, L);
                     acc[0] = fmaf(x[s][0].x, f, acc[0]); acc[1] = fmaf(x[s][0].y, f, acc[1]); acc[2] = fmaf(x[s][0].z, f, acc[2]); acc[3] = fmaf(x[s][0].w, f, acc[3]);
@@ -649,11 +732,11 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 
 // Joins the parts of the pairs that lie in several CTAs' stretches: a warp a row, HD / 32 neighbouring dimensions a lane, eight parts'
 // outputs in flight.
-template <int HD>
+template <typename T, int HD>
 __global__ void __launch_bounds__(256) attention_q8_join_kernel(const Q8Params p, int ctas) {
     pdl_launch_dependents();
     constexpr int DL = HD / 32;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.x, kvh = blockIdx.y, G = p.nq / p.nkv;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.x / p.row_tiles, rt = blockIdx.x - seq * p.row_tiles, kvh = blockIdx.y, G = p.nq / p.nkv;
     if (!p.described) pdl_wait();
     const Line line{p};
     int before = 0, all = 0, row_tiles;
@@ -664,12 +747,13 @@ __global__ void __launch_bounds__(256) attention_q8_join_kernel(const Q8Params p
     }
     const long long length = (long long)__reduce_add_sync(0xffffffffu, all) * p.nkv;
     const int n = line.tiles_of(seq, row_tiles);
-    const long long begin = (long long)__reduce_add_sync(0xffffffffu, before) * p.nkv + ((long long)blockIdx.z * p.nkv + kvh) * n;
+    const long long begin = (long long)__reduce_add_sync(0xffffffffu, before) * p.nkv + ((long long)rt * p.nkv + kvh) * n;
     pdl_wait();
-    if (n == 0 || (int)blockIdx.z >= row_tiles) return;
+    if (n == 0 || rt >= row_tiles) return;
+    ctas = stretches(length, ctas);
     const int u0 = holder(begin, length, ctas), u1 = holder(begin + n - 1, length, ctas);
     if (u0 == u1) return;
-    const int tok_begin = p.cu_seqlens[seq], row0 = blockIdx.z * p.rows_per_tile, rows = min(p.rows_per_tile, (p.cu_seqlens[seq + 1] - tok_begin) * G - row0);
+    const int tok_begin = p.cu_seqlens[seq], row0 = rt * p.rows_per_tile, rows = min(p.rows_per_tile, (p.cu_seqlens[seq + 1] - tok_begin) * G - row0);
     const long long first = 2ll * u0 + (begin > stretch(u0, length, ctas) ? 1 : 0);      // in its own CTA the pair's part is the last one
     auto part_of = [&](int k) { return k == 0 ? first : 2ll * (u0 + k); };
     const int parts = u1 - u0 + 1;
@@ -702,21 +786,24 @@ __global__ void __launch_bounds__(256) attention_q8_join_kernel(const Q8Params p
             }
         }
         const float inv = 1.0f / L;
-        __nv_bfloat16 *out = (__nv_bfloat16 *)p.out + ((size_t)(tok_begin + (row0 + r) / G) * p.nq + kvh * G + (row0 + r) % G) * HD + lane * DL;
+        T *out = (T *)p.out + ((size_t)(tok_begin + (row0 + r) / G) * p.nq + kvh * G + (row0 + r) % G) * HD + lane * DL;
 #pragma unroll
-        for (int d = 0; d < DL; d += 2) *reinterpret_cast<__nv_bfloat162 *>(out + d) = __floats2bfloat162_rn(acc[d] * inv, acc[d + 1] * inv);
+        for (int d = 0; d < DL; d += 2) {
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(out + d) = make_float2(acc[d] * inv, acc[d + 1] * inv);
+            else *reinterpret_cast<__nv_bfloat162 *>(out + d) = __floats2bfloat162_rn(acc[d] * inv, acc[d + 1] * inv);
+        }
     }
 }
 
-template <int HD, int NT> constexpr size_t decode_smem() { return Ring<HD, NT>::BYTES + 1024; }
+template <typename T, int HD, int NT> constexpr size_t decode_smem() { return Ring<HD, NT, T>::BYTES + 1024; }
 
 // all but the grid and the stream of a launch in clusters
-template <int HD, int NT>
+template <typename T, int HD, int NT>
 int cluster_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int size) {
-    if (cudaFuncSetAttribute(attention_q8_decode_kernel<HD, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)decode_smem<HD, NT>()) != cudaSuccess)
+    if (cudaFuncSetAttribute(attention_q8_decode_kernel<T, HD, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)decode_smem<T, HD, NT>()) != cudaSuccess)
         return kestrel_fail(-3, "attention_q8: cannot raise the shared-memory limit: %s", cudaGetErrorString(cudaGetLastError()));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = decode_smem<HD, NT>();
+    cfg.dynamicSmemBytes = decode_smem<T, HD, NT>();
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = size;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -725,7 +812,7 @@ int cluster_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int size)
     return 0;
 }
 
-template <int HD, int NT>
+template <typename T, int HD, int NT>
 int launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
     CUtensorMap mk, mv;
     const long long lines = (long long)p.cache_pages * p.nkv * p.page_size * HD / 128;
@@ -738,70 +825,75 @@ int launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
         // a CTA, or a cluster of them, a pair
         cudaLaunchConfig_t cfg = {};
         cudaLaunchAttribute attr[2];
-        rc = cluster_config<HD, NT>(cfg, attr, p.slices);
+        rc = cluster_config<T, HD, NT>(cfg, attr, p.slices);
         if (rc) return rc;
         cfg.gridDim = dim3((unsigned)p.nseq * p.row_tiles * p.nkv * p.slices);
         cfg.stream = stream;
         attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs = g_kestrel_pdl ? 2 : 1;
-        cudaLaunchKernelEx(&cfg, attention_q8_decode_kernel<HD, NT, true>, mk, mv, p);
+        cudaLaunchKernelEx(&cfg, attention_q8_decode_kernel<T, HD, NT, true>, mk, mv, p);
         return kestrel_check_launch("attention_q8 decode");
     }
-    if (cudaFuncSetAttribute(attention_q8_decode_kernel<HD, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)decode_smem<HD, NT>()) != cudaSuccess)
+    if (cudaFuncSetAttribute(attention_q8_decode_kernel<T, HD, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)decode_smem<T, HD, NT>()) != cudaSuccess)
         return kestrel_fail(-3, "attention_q8: cannot raise the shared-memory limit: %s", cudaGetErrorString(cudaGetLastError()));
-    kestrel_launch(attention_q8_decode_kernel<HD, NT, false>, dim3(ctas), dim3(THREADS), decode_smem<HD, NT>(), stream, mk, mv, p);
+    kestrel_launch(attention_q8_decode_kernel<T, HD, NT, false>, dim3(ctas), dim3(THREADS), decode_smem<T, HD, NT>(), stream, mk, mv, p);
     rc = kestrel_check_launch("attention_q8 decode");
     if (rc) return rc;
-    kestrel_launch(attention_q8_join_kernel<HD>, dim3(p.nseq, p.nkv, p.row_tiles), dim3(256), 0, stream, p, ctas);
+    kestrel_launch(attention_q8_join_kernel<T, HD>, dim3((unsigned)p.nseq * p.row_tiles, p.nkv), dim3(256), 0, stream, p, ctas);
     return kestrel_check_launch("attention_q8 join");
 }
 
 // Clusters of `size` CTAs that the current device holds at once.  A cluster lies within one GPC, so they are fewer than the CTAs' places
 // divided by their size.  Asked of the runtime once a device, head size, rows and size.
-template <int HD, int NT>
+template <typename T, int HD, int NT>
 int resident_clusters(int size) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
-    if (cluster_config<HD, NT>(cfg, attr, size)) return 0;
+    if (cluster_config<T, HD, NT>(cfg, attr, size)) return 0;
     cfg.gridDim = dim3(size);
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, attention_q8_decode_kernel<HD, NT, true>, &cfg) != cudaSuccess) {
+    if (cudaOccupancyMaxActiveClusters(&n, attention_q8_decode_kernel<T, HD, NT, true>, &cfg) != cudaSuccess) {
         cudaGetLastError();
         return 0;
     }
     return n;
 }
 
+// calls f with the kernel's types and sizes: (T, head size, column tiles)
+template <typename F>
+auto with_form(Q8Form form, int hd, F f) {
+    auto sized = [&](auto t, auto nt) { return hd == 64 ? f(t, std::integral_constant<int, 64>(), nt) : f(t, std::integral_constant<int, 128>(), nt); };
+    using One = std::integral_constant<int, 1>;
+    return form == Q8_WIDE ? sized(0.f, One()) : form == Q8_EIGHT ? sized(__nv_bfloat16(), One()) : sized(__nv_bfloat16(), std::integral_constant<int, 2>());
+}
+
 }  // namespace
 
-int q8_launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
-    if (p.rows_per_tile == 8) return p.hd == 64 ? launch_decode<64, 1>(p, ctas, stream) : launch_decode<128, 1>(p, ctas, stream);
-    return p.hd == 64 ? launch_decode<64, 2>(p, ctas, stream) : launch_decode<128, 2>(p, ctas, stream);
+int q8_launch_decode(const Q8Params &p, Q8Form form, int ctas, cudaStream_t stream) {
+    return with_form(form, p.hd, [&](auto t, auto hd, auto nt) { return launch_decode<decltype(t), hd(), nt()>(p, ctas, stream); });
 }
 
 // As many as are resident at once.  A stretch of fewer than two tiles costs more to begin and to join than it takes.
-int q8_decode_ctas(long long tiles, int hd, int most_rows) {
-    const long long most = (most_rows <= 8 ? (hd == 64 ? Ring<64, 1>::CTAS : Ring<128, 1>::CTAS) : (hd == 64 ? Ring<64, 2>::CTAS : Ring<128, 2>::CTAS)) * (long long)kestrel_sms();
+int q8_decode_ctas(long long tiles, int hd, Q8Form form) {
+    const long long most = with_form(form, hd, [](auto t, auto h, auto nt) { return Ring<h(), nt(), decltype(t)>::CTAS; }) * (long long)kestrel_sms();
     return (int)(tiles / 2 < 1 ? 1 : tiles / 2 < most ? tiles / 2 : most);
 }
 
 // CTAs a pair, or 0 for stretches.  As many as let every cluster be resident, up to 8, and two tiles each; taken where the longest pair's
 // share is no more than six tiles above a stretch, which is about what the join kernel takes.
-int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int hd, int most_rows) {
-    static DeviceTable<4 * (MAX_CLUSTER + 1)> known;
+int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int hd, Q8Form form) {
+    static DeviceTable<6 * (MAX_CLUSTER + 1)> known;
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess) {
         cudaGetLastError();
         dev = -1;
     }
-    const long long stretch = (tiles + q8_decode_ctas(tiles, hd, most_rows) - 1) / q8_decode_ctas(tiles, hd, most_rows);
+    const long long ctas = q8_decode_ctas(tiles, hd, form), stretch = (tiles + ctas - 1) / ctas;
     for (int size = longest_tiles / 2 < MAX_CLUSTER ? (longest_tiles < 2 ? 1 : longest_tiles / 2) : MAX_CLUSTER; size >= 1; --size) {
         if ((longest_tiles + size - 1) / size > stretch + 6) return 0;
-        const int at = ((hd == 64 ? 2 : 0) + (most_rows <= 8 ? 1 : 0)) * (MAX_CLUSTER + 1) + size;
-        const int n = known.get(dev, at, [&] {
-            return hd == 64 ? (most_rows <= 8 ? resident_clusters<64, 1>(size) : resident_clusters<64, 2>(size))
-                            : (most_rows <= 8 ? resident_clusters<128, 1>(size) : resident_clusters<128, 2>(size));
+        const int n = known.get(dev, (2 * (int)form + (hd == 64)) * (MAX_CLUSTER + 1) + size, [&] {
+            return with_form(form, hd, [&](auto t, auto h, auto nt) { return resident_clusters<decltype(t), h(), nt()>(size); });
         });
         if (pairs <= n) return size;
     }

@@ -10,12 +10,14 @@ pytestmark = pytest.mark.gpu
 
 def _tolerance(out, size, dtype, keys):
     """float32: scores of up to 256 products and sums over up to 2^17 keys in a few partial sums, 2^-24 each, of numbers that are at most
-    their keys' weighted magnitudes; exponentials within 2^-21: 2^-14 of these magnitudes.  bfloat16: the output is rounded by half a step,
+    their keys' weighted magnitudes; exponentials within 2^-21: 2^-14 of these magnitudes.  A weight - a probability times its value's scale's
+    power of two - is held in three float16 parts that leave 2^-39 of the row's largest, times a code of at most 127, where the key that
+    holds the largest has codes of 64 and more: 2^-38 of the row's largest magnitude for every key.  bfloat16: the output is rounded by half a step,
     2^-8 of it; weights - a key's probability times its value's scale - are rounded to float16, 2^-11 of them each and at least 2^-25 of the
     row's largest, whose own magnitudes are the row's largest too; scores sum in float32: 2^-10 of the magnitudes, and 2^-24 of the row's
     largest for every key."""
     if dtype == "float32":
-        return 2.0 ** -14 * size
+        return 2.0 ** -14 * size + keys * 2.0 ** -38 * size.amax(-1, keepdim=True)
     return 2.0 ** -8 * out.abs() + 2.0 ** -10 * size + keys * 2.0 ** -24 * size.amax(-1, keepdim=True)
 
 
@@ -260,6 +262,35 @@ def test_a_window_of_every_size(portions, dtype):
         _near(step(portions, 16), out, want, size, dtype)
         got.append(out)
     assert got[0].equal(got[1]) and got[0].equal(got[2])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_recorded_single_tokens_of_short_requests(dtype):
+    """Recorded for contexts of up to 65,536, replayed with far shorter ones: less work than the launch was cut for."""
+    import torch
+    from kestrel_llm_b200.csrc import ops
+    nq, nkv, hd, n = 8, 2, 128, 40
+    held = step([(1, 300)] * n, 16)
+    k, ks, v, vs = planes(held, nkv, hd)
+    k.div_(4, rounding_mode="trunc")                # scores of a few units
+    q = torch.randn((n, nq * hd), device="cuda").to(getattr(torch, dtype))
+    out = torch.empty_like(q)
+    s = step([(1, 300)] * n, 16)
+    s.table, s.captured, s.max_kv_len = held.table, True, 65536
+    run = lambda: ops.attention_q8(q, k, v, ks, vs, out, s, s.table, 16, nq, nkv, hd, 0, 0.01)  # noqa: E731
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for contexts in ([300] * n, [0] * n, [100] * n, list(range(3, 3 + 7 * n, 7)), [0] * (n - 1) + [300]):
+        now = step([(1, c) for c in contexts], 16)
+        now.table = held.table
+        s.kv_lens.copy_(now.kv_lens)
+        out.fill_(float("nan"))
+        graph.replay()
+        want, size = attend64(q, k, ks, v, vs, now, nq, nkv, hd, 0, 0.01)
+        _near(now, out.view(-1, nq, hd).double(), want, size, dtype)
 
 
 def test_recorded_portions_share_the_tokens():
