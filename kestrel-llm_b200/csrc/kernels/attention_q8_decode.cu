@@ -131,7 +131,8 @@ template <int HD> __device__ __forceinline__ uint32_t chunk_at(int k, int c) {
     return line * 128 + ((at ^ (line & 7)) << 4);
 }
 
-// The line of key tiles: request i's pairs lie behind those of the requests before it, row tile by row tile and in these kv head by kv head.
+// The line of key tiles: request i's pairs lie behind those of the requests before it, kv head by kv head and in these row tile by row tile: the
+// first, the last, the second, the last but one, ..., so that neighbours, which see few keys of a prompt and many, weigh together like others.
 // All pairs of a request have the tiles that its first or its last row sees.
 struct Line {
     const Q8Params &p;
@@ -192,11 +193,15 @@ __device__ __forceinline__ int stretches(long long length, int ctas) { return (i
 __device__ __forceinline__ long long stretch(long long u, long long length, int ctas) { return u * length / ctas; }
 __device__ __forceinline__ int holder(long long at, long long length, int ctas) { return (int)(((at + 1) * ctas - 1) / length); }
 
+// The k-th row tile of a request's kv head on the line, and a row tile's place there
+__device__ __forceinline__ int nth_row_tile(int k, int row_tiles) { return k & 1 ? row_tiles - 1 - k / 2 : k / 2; }
+__device__ __forceinline__ int place_of_row_tile(int rt, int row_tiles) { return 2 * rt < row_tiles ? 2 * rt : 2 * (row_tiles - 1 - rt) + 1; }
+
 // One CTA's parts of pairs, one after the other
 struct Walk {
     const Q8Params &p;
     long long at, end, begin;           // next tile, end of the stretch, place of the pair's first tile
-    int seq, n, kvh, row0;              // the pair; n: its tiles, row0: its first row among the request's
+    int seq, n, kvh, nth, row0;         // the pair; n: its tiles, nth: its row tile's place, row0: its first row among the request's
     // the part
     int G, row_tiles, all_rows, rows, tok_begin, pos_begin, k_first, k_end, from, to, seen_from, seen_to;
     const int *table;
@@ -228,8 +233,8 @@ struct Walk {
         n = line.tiles_of(seq, row_tiles);
         const int pair = (int)((at - begin) / n);
         begin += (long long)pair * n;
-        kvh = pair % p.nkv;
-        row0 = pair / p.nkv * p.rows_per_tile;
+        kvh = pair / row_tiles;
+        nth = pair - kvh * row_tiles;
         describe();
     }
     __device__ __forceinline__ void describe() {
@@ -253,11 +258,10 @@ struct Walk {
         if (at >= end) return false;
         if (at >= begin + n) {
             begin += n;
-            if (++kvh == p.nkv) {
-                kvh = 0;
-                row0 += p.rows_per_tile;
-                if (row0 >= all_rows) {
-                    row0 = 0;
+            if (++nth == row_tiles) {
+                nth = 0;
+                if (++kvh == p.nkv) {
+                    kvh = 0;
                     const Line line{p};
                     do n = line.tiles_of(++seq, row_tiles);
                     while (n == 0 && seq < p.nseq);
@@ -265,6 +269,7 @@ struct Walk {
                 }
             }
         }
+        row0 = nth_row_tile(nth, row_tiles) * p.rows_per_tile;
         see();
         from = (int)(at - begin);
         to = (int)min((long long)n, end - begin);
@@ -747,7 +752,7 @@ __global__ void __launch_bounds__(256) attention_q8_join_kernel(const Q8Params p
     }
     const long long length = (long long)__reduce_add_sync(0xffffffffu, all) * p.nkv;
     const int n = line.tiles_of(seq, row_tiles);
-    const long long begin = (long long)__reduce_add_sync(0xffffffffu, before) * p.nkv + ((long long)rt * p.nkv + kvh) * n;
+    const long long begin = (long long)__reduce_add_sync(0xffffffffu, before) * p.nkv + ((long long)kvh * row_tiles + place_of_row_tile(rt, row_tiles)) * n;
     pdl_wait();
     if (n == 0 || rt >= row_tiles) return;
     ctas = stretches(length, ctas);
