@@ -333,7 +333,7 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
             tiles += (rows + 15) / 16 * nkv * ((seen_of(kv[i], rows) + 63) / 64);
         }
         const long long pairs = (long long)nseq * ((most + 15) / 16) * nkv;
-        if (all && most > 16 && tiles <= (single ? 24 : 8) * 2ll * kestrel_sms() &&
+        if (all && most > 16 && pairs <= 2ll * kestrel_sms() && tiles <= (single ? 24 : 8) * 2ll * kestrel_sms() &&
             (q8_decode_cluster(pairs, (longest + 63) / 64, tiles, hd, Q8_SIXTEEN) > 0 || (single && pairs <= q8_decode_ctas(tiles, hd, Q8_SIXTEEN))))
             small.rows_upto = FEW;
     }
@@ -377,7 +377,8 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
             p->rows_per_tile = p->form == Q8_SIXTEEN ? 16 : 8;
             p->ctas = q8_decode_ctas(p->key_tiles, hd, p->form);
             p->row_tiles = (p->most_rows + p->rows_per_tile - 1) / p->rows_per_tile;
-            p->slices = q8_decode_cluster((long long)nseq * p->row_tiles * nkv, (p->longest + 63) / 64, p->key_tiles, hd, p->form);
+            if (p->row_tiles == 1) p->tiles = nseq;
+            p->slices = q8_decode_cluster(p->tiles * nkv, (p->longest + 63) / 64, p->key_tiles, hd, p->form);
             p->scratch = p->slices ? 0 : q8_decode_scratch(p->ctas, hd);
         } else {
             // The tensor cores: one CTA an SM, slices of two key tiles at least.  The CUDA cores: two CTAs an SM, which a key tile takes 6 us, the
@@ -423,7 +424,7 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
     make_plan(pl, cu_host, kv_host, nseq, max_count, max_kv, T, nq, nkv, hd, window, dtype);
     for (int i = 0; i < pl.parts; ++i) {
         const Part &part = pl.part[i];
-        KESTREL_REQUIRE(part.tiles * nkv < (1ll << 31) && (part.kernel != DECODE || (part.key_tiles / nkv < (1ll << 31) && (long long)nseq * part.row_tiles < (1ll << 31))),
+        KESTREL_REQUIRE(part.tiles * nkv * std::max(part.slices, 1) < (1ll << 31) && (part.kernel != DECODE || (part.key_tiles / nkv < (1ll << 31) && (long long)nseq * part.row_tiles < (1ll << 31))),
                         "attention_q8: %lld row tiles and %lld key tiles of %d kv heads exceed the grid", part.tiles, part.key_tiles, nkv);
         KESTREL_REQUIRE(part.scratch == 0 || (scratch && part.scratch <= scratch_floats), "attention_q8: scratch of %lld floats is needed, %lld given", part.scratch, scratch_floats);
     }
@@ -437,6 +438,7 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
         p.nq = nq; p.nkv = nkv; p.hd = hd; p.window = window; p.slices = part.slices; p.scale = scale; p.described = described;
         p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1;
         p.rows_above = part.rows_above; p.rows_upto = part.rows_upto; p.rows_per_tile = part.rows_per_tile; p.row_tiles = part.row_tiles;
+        p.tiles = (int)part.tiles;
         p.part_o = scratch;
         int rc;
         if (part.kernel == DECODE) {

@@ -32,6 +32,7 @@ struct Q8Params {
     int nseq, table_width, table_stride, page_size, cache_pages, nq, nkv, hd, window, slices;
     int rows_above, rows_upto;      // this launch takes the requests with rows_above < (token, head) rows per kv head <= rows_upto
     int rows_per_tile, row_tiles;   // row_tiles: most of a request
+    int tiles;                      // row tiles of all requests, or the requests where row_tiles is 1
     int page_shift;                 // log2 of the page size, or -1
     int described;                  // the step's description was on the device before the kernel in front of this one began
     float scale;

@@ -210,12 +210,17 @@ struct Walk {
     // the rank-th of `ranks` equal parts of a pair
     __device__ __forceinline__ Walk(const Q8Params &p_, int pair, int rank, int ranks) : p(p_), at(0), end(0), begin(0), kvh(pair % p_.nkv) {
         G = p.nq / p.nkv;
-        seq = pair / p.nkv / p.row_tiles;
-        const int rt = pair / p.nkv - seq * p.row_tiles;
+        n = 0;
+        seq = pair / p.nkv;
+        row0 = 0;
+        if (p.row_tiles > 1) {          // late row tiles, which see the most keys, come first
+            Q8Tile t;
+            if (!q8_find_tile(p, p.tiles - 1 - seq, t)) return;
+            seq = t.seq;
+            row0 = t.row0;
+        }
         n = Line{p}.tiles_of(seq, row_tiles);
-        if (rt >= row_tiles) n = 0;
         if (n == 0) return;
-        row0 = rt * p.rows_per_tile;
         describe();
         see();
         from = seen_from + (int)((long long)(seen_to - seen_from) * rank / ranks);
@@ -832,7 +837,7 @@ int launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
         cudaLaunchAttribute attr[2];
         rc = cluster_config<T, HD, NT>(cfg, attr, p.slices);
         if (rc) return rc;
-        cfg.gridDim = dim3((unsigned)p.nseq * p.row_tiles * p.nkv * p.slices);
+        cfg.gridDim = dim3((unsigned)p.tiles * p.nkv * p.slices);
         cfg.stream = stream;
         attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[1].val.programmaticStreamSerializationAllowed = 1;
@@ -885,8 +890,11 @@ int q8_decode_ctas(long long tiles, int hd, Q8Form form) {
     return (int)(tiles / 2 < 1 ? 1 : tiles / 2 < most ? tiles / 2 : most);
 }
 
-// CTAs a pair, or 0 for stretches.  As many as let every cluster be resident, up to 8, and two tiles each; taken where the longest pair's
-// share is no more than six tiles above a stretch, which is about what the join kernel takes.
+// CTAs a pair, or 0 for stretches.  Where every pair can have its CTAs at once, as many as let every cluster be resident, up to 8, and two
+// tiles each; taken where the longest pair's share is no more than six tiles above a stretch, which is about what the join kernel takes.  Where
+// there are more pairs, one, if the wait for the last one is worth what pairs cost a stretch: some five tiles' time each, and the join
+// (32 / 8 heads of 128, bfloat16: 256 requests behind 300, 1,000, 2,000 keys 48, 109, 198 us, in stretches 77, 133, 220; behind 20 to 1,805
+// 107 and 211; 64 behind 300, 1,000, 4,095 16, 39, 138, in stretches 22, 39, 102; 411 float32 tokens of one request, 16 / 4 heads, 27 and 39).
 int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int hd, Q8Form form) {
     static DeviceTable<6 * (MAX_CLUSTER + 1)> known;
     int dev = -1;
@@ -894,15 +902,18 @@ int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int h
         cudaGetLastError();
         dev = -1;
     }
-    const long long ctas = q8_decode_ctas(tiles, hd, form), stretch = (tiles + ctas - 1) / ctas;
-    for (int size = longest_tiles / 2 < MAX_CLUSTER ? (longest_tiles < 2 ? 1 : longest_tiles / 2) : MAX_CLUSTER; size >= 1; --size) {
-        if ((longest_tiles + size - 1) / size > stretch + 6) return 0;
-        const int n = known.get(dev, (2 * (int)form + (hd == 64)) * (MAX_CLUSTER + 1) + size, [&] {
+    auto resident = [&](int size) {
+        return known.get(dev, (2 * (int)form + (hd == 64)) * (MAX_CLUSTER + 1) + size, [&] {
             return with_form(form, hd, [&](auto t, auto h, auto nt) { return resident_clusters<decltype(t), h(), nt()>(size); });
         });
-        if (pairs <= n) return size;
+    };
+    const long long ctas = q8_decode_ctas(tiles, hd, form), stretch = (tiles + ctas - 1) / ctas;
+    for (int size = longest_tiles / 2 < MAX_CLUSTER ? (longest_tiles < 2 ? 1 : longest_tiles / 2) : MAX_CLUSTER; size >= 1; --size) {
+        if ((longest_tiles + size - 1) / size > stretch + 6) break;
+        if (pairs <= resident(size)) return size;
     }
-    return 0;
+    const int at_once = resident(1);
+    return at_once > 0 && pairs > at_once && longest_tiles <= 25 * pairs / (2 * at_once) + 15 ? 1 : 0;
 }
 
 long long q8_decode_scratch(int ctas, int hd) { return 2ll * ctas * 16 * (hd + 2); }
