@@ -1,8 +1,9 @@
-// Attention over pages of int8 codes: the kernel on the CUDA cores, which takes every head size, float32 and bfloat16, the merge of key
-// slices, and the entry point that decides which kernel takes which requests.  Formulas in attention_q8.cuh.
+// Attention over pages of int8 codes: the kernel on the CUDA cores, for head sizes other than 64 and 128, the merge of key slices, and the
+// entry point that decides which kernel takes which requests.  Formulas in attention_q8.cuh.
 #include "attention_q8.cuh"
 
 #include <algorithm>
+#include <climits>
 #include <math.h>
 
 namespace {
@@ -11,8 +12,10 @@ namespace {
 // A CTA takes 32 rows and walks its keys in tiles of 64: codes are widened to float32 in shared memory, the keys' times their scale,
 // scores and outputs are register tiles of 4 rows by 4 keys (by HDP / 16 dimensions), the softmax runs online with float32 statistics.
 // The values' scales enter with the weights: the weight of a key that a row may not see is zero whatever its scale is, and a code is
-// always a number, so that what is not finite stays with the rows that see it.  Bound by the float32 units and shared memory; this is
-// the true 32-bit path, and the one of head sizes that the tensor-core kernels do not take.
+// always a number, so that what is not finite stays with the rows that see it.  Products are pairs of float32 multiply-adds.  Bound by
+// shared memory: of a 16-byte load by four rows or keys come eight such instructions, and a tile of 64 keys takes a CTA 6 us.
+// 411 tokens of one request, 16 / 4 heads of 80: 51 us in float32 and bfloat16, 8.5 TFLOP/s; of 256 95 us, 14.6; eight single tokens behind 3,000
+// keys, heads of 80, 64 us, of 256 144 us.
 constexpr int BM = 32, BN = 64, THREADS = 128;
 
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
@@ -220,7 +223,7 @@ __global__ void __launch_bounds__(THREADS) attention_q8_plain_kernel(const Q8Par
 
 // ---- merge -------------------------------------------------------------------------------------------
 // A warp takes a row: lane s holds slice s's maximum and sum, the outputs are added in ascending order of the slices; a lane takes four
-// neighbouring dimensions, four slices' in flight.
+// neighbouring dimensions, four slices' in flight.  Bound by latency: 3 us behind a portion of 500 tokens, 16 heads of 64 in two slices.
 template <typename T>
 __global__ void __launch_bounds__(256) attention_q8_merge_kernel(const Q8Params p) {
     pdl_launch_dependents();
@@ -316,9 +319,9 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
     if (!cores && !wide && cu) {
         // Short portions go to the decode kernel, which reads a request's keys again for every 16 rows, if that leaves no portion to the other
         // kernel: where every pair has its CTAs at once and their work is little (32 / 8 heads of 128, one request, behind 500 keys: 16 tokens
-        // 10.9 us against 14.9, 64 tokens 13.8 against 16.7, 128 tokens 16.9 against 17.8; 64 tokens behind 2,000 keys 27 against 19; four
-        // requests of about 64 tokens, more pairs than CTAs, 30 against 10), and beside single tokens, which are a launch of the kernel anyway,
-        // for three times that (four requests of 2 to 8 tokens behind 2,000 keys 15 against 32, behind 8,000 34 against 51).
+        // 12.0 us against 15.7, 64 tokens 14.7 against 17.4, 128 tokens 18.0 against 18.6; 64 tokens behind 2,000 keys 27 against 20; four
+        // requests of about 64 tokens behind 100, more pairs than CTAs, 19 against 12), and beside single tokens, which are a launch of the kernel
+        // anyway, for three times that (four requests of 2 to 8 tokens behind 2,000 keys 17 against 35, behind 8,000 37 against 59).
         long long tiles = 0;
         int most = 0, longest = 0;
         bool single = false, all = true;
@@ -342,13 +345,24 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
     large.rows_upto = 0x7fffffff;
     large.rows_per_tile = 256;
     if (!cores && !wide && cu) {
-        // while tiles of 128 rows fit the SMs at once, a CTA takes one and its key tiles go to the two streams in turn
-        long long tiles = 0;
-        for (int i = 0; i < nseq; ++i) {
-            const long long rows = (long long)(cu[i + 1] - cu[i]) * G;
-            if (rows > small.rows_upto) tiles += (rows + 127) / 128;
-        }
-        if (tiles * nkv <= kestrel_sms()) large.rows_per_tile = 128;
+        // While tiles of 128 rows fit the SMs at once, a CTA may take one, and its key tiles go to the two streams in turn.  What a CTA has to do
+        // is rows times keys of its slice, and slices cost their merge, as much as 128 rows' 380 keys (32 / 8 heads of 128: 256 tokens 12 us in
+        // tiles of 128, 15 of 256; 500 behind 1,500 39 and 47, where only the latter need slices; 300 behind 2,000 43 and 39;
+        // 16 / 4 heads of 64, 500 tokens of a window of 1,024, in two slices and four, 21 and 23).
+        auto work = [&](int rows_per_tile) {
+            long long tiles = 0;
+            int longest = 0;
+            for (int i = 0; i < nseq; ++i) {
+                const long long rows = (long long)(cu[i + 1] - cu[i]) * G;
+                if (rows <= small.rows_upto) continue;
+                tiles += (rows + rows_per_tile - 1) / rows_per_tile;
+                longest = std::max(longest, seen_of(kv[i], rows));
+            }
+            const int slices = slices_for(tiles * nkv, kestrel_sms(), longest, 256);
+            return tiles * nkv > kestrel_sms() ? LLONG_MAX : (long long)rows_per_tile * (longest / slices) + (slices > 1 ? 128 * 380 : 0);
+        };
+        const long long halves = work(128);
+        if (halves < LLONG_MAX && halves / 8 * 7 <= work(256)) large.rows_per_tile = 128;
     }
     small.rows_per_tile = cores ? BM : wide ? 8 : 16;
     auto count = [&](long long rows, int keys, int times) {

@@ -1,23 +1,35 @@
-// Attention over pages of int8 codes with few rows: single tokens and short portions.  Head sizes 64 and 128, bfloat16
-// queries.  Formulas in attention_q8.cuh.
+// Attention over pages of int8 codes with few rows: single tokens and short portions in bfloat16, and all of float32.  Head sizes 64 and 128.
+// Formulas in attention_q8.cuh.
 //
-// The work is cut evenly, whatever the requests' lengths: all key tiles of 64 of all pairs - of a kv head and up to 16 (token, query head)
-// rows of a request - stand in one line, and every CTA takes as many of them as the next.  A CTA walks its stretch pair by pair.  A pair that lies
-// within one CTA's stretch is finished there; the others leave (maximum, sum, outputs) of their parts in scratch, two parts a CTA at most,
-// and the merge kernel below joins them in the order of the keys.  Where the pairs are few and short (CLUSTER) the CTAs of a cluster share one
-// pair instead, evenly, and join their parts in each other's shared memory: a kernel less.
+// The work is pairs - a kv head and up to 8 or 16 (token, query head) rows of a request - of key tiles of 64.  How CTAs take them
+// (q8_decode_cluster has both sides' times):
+//   - the CTAs of a cluster of up to 8 share one pair, evenly, and join their parts in each other's shared memory: few, short pairs;
+//   - a CTA a pair, late rows first, more CTAs than there is room for: many pairs, none long;
+//   - stretches: all key tiles of all pairs stand in one line, and every CTA takes as many of them as the next, whatever the requests' lengths.
+//     A CTA walks its stretch pair by pair.  A pair that lies within one CTA's stretch is finished there; the others leave (maximum, sum,
+//     outputs) of their parts in scratch, two parts a CTA at most, and the join kernel below adds them in the order of the keys.
 //
 // A loader warp brings tiles by TMA into a ring of stages, codes of K and V side by side, and the scales of their four blocks beside
 // them, running ahead over the pairs' borders; four consumer warps take one block of 16 keys each.  Codes go from shared memory straight
 // into the fragments of mma.sync.m16n8k16 (float16, float32 sums), as the operand of sixteen rows: 16 keys by 8 query rows of scores,
 // 16 dimensions by 8 query rows of outputs, so that four heads a group leave half of a product unused and not three quarters, and a
-// thread's softmax holds four scores.  The weights change places between the two products by transposing 8 by 8 tiles.  A code of V is the low byte of the float16 number 1024 + (c + 128), made
-// by a byte permutation and freed of 1152 by one subtraction of pairs.  A code of K is the float16 number (c + 128) 2^-24, a subnormal
-// one, which the permutation alone makes; the scores' sums begin with -128 2^-24 times the row's sum of queries instead of zero.  (The same
-// for V would leave 128 times the weights' sum in the outputs, of which they are a hundredth where many keys weigh alike.)
-// The order of a product's inner index is free as long as both operands share it, which is used twice: a thread's 16 neighbouring
-// dimensions of a key are one 16-byte load and four k-steps of the scores, and the columns of the scores stand for keys in an order that
-// lets every load of a warp touch each bank once.  Bound by HBM: 2 hd bytes a key and kv head; some 0.6 instructions a code to widen it.
+// thread's softmax holds four scores.  The weights change places between the two products by transposing 8 by 8 tiles.  A code of V is the
+// low byte of the float16 number 1024 + (c + 128), made by a byte permutation and freed of 1152 by one subtraction of pairs.  A code of K
+// is the float16 number (c + 128) 2^-24, a subnormal one, which the permutation alone makes; the scores' sums begin with -128 2^-24 times
+// the row's sum of queries instead of zero.  (The same for V would leave 128 times the weights' sum in the outputs, of which they are a
+// hundredth where many keys weigh alike.)  The order of a product's inner index is free as long as both operands share it, which is used
+// twice: a thread's 16 neighbouring dimensions of a key are one 16-byte load and four k-steps of the scores, and the columns of the scores
+// stand for keys in an order that lets every load of a warp touch each bank once.
+//
+// float32: a query and a weight are three float16 parts each, whose products with codes are exact, so that a score or an output is a sum
+// of exact products as in float32, at three times the matrix instructions; these cut their sums off instead of rounding them, so every
+// k-step begins at zero, smallest part first, and is added in float32.  Errors against 64 bits are those of float32 multiply-adds
+// (2e-7 of the outputs' size on random data, as the CUDA cores').  Codes of K are freed of their 1152 like those of V here.
+//
+// Bound by HBM with bfloat16: 2 hd bytes a key and kv head; some 0.6 instructions a code to widen it.  32 / 8 heads of 128: 64 requests
+// behind up to 4,095 keys (407 MB) 83 us, 4.9 TB/s; two behind 65,535 (235 MB) 50 us, 4.7 TB/s; one behind 1,003 6.4 us, of which latency
+// is nearly all; with a head size of 64, where a tile has half the bytes and the same softmax, 64 behind up to 4,095 69 us, 2.9 TB/s.
+// float32: 64 behind 3,000 131 us, 3.0 TB/s, and 411 tokens of two requests, 16 / 4 heads, 23 us (CUDA cores: 39).
 #include "attention_q8.cuh"
 #include "tcgen05.cuh"
 
@@ -741,7 +753,7 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 }
 
 // Joins the parts of the pairs that lie in several CTAs' stretches: a warp a row, HD / 32 neighbouring dimensions a lane, eight parts'
-// outputs in flight.
+// outputs in flight.  Bound by the latency of a few dependent loads: 3 to 4 us behind the stretches of 64 or two requests.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) attention_q8_join_kernel(const Q8Params p, int ctas) {
     pdl_launch_dependents();
@@ -891,7 +903,9 @@ int q8_decode_ctas(long long tiles, int hd, Q8Form form) {
 }
 
 // CTAs a pair, or 0 for stretches.  Where every pair can have its CTAs at once, as many as let every cluster be resident, up to 8, and two
-// tiles each; taken where the longest pair's share is no more than six tiles above a stretch, which is about what the join kernel takes.  Where
+// tiles each; taken where the longest pair's share is no more than six tiles above a stretch, which is about what the join kernel takes (32 / 8 heads of 128: a request behind 1,003 keys
+// 6.5 us with 8 CTAs a pair, 16 with one, 10 in stretches; two behind 65,535 126 us with 8, 55 in stretches; 32 behind 500 13 with one, 17 in
+// stretches; 8 behind 4,095 18 with 6, 23 in stretches).  Where
 // there are more pairs, one, if the wait for the last one is worth what pairs cost a stretch: some five tiles' time each, and the join
 // (32 / 8 heads of 128, bfloat16: 256 requests behind 300, 1,000, 2,000 keys 48, 109, 198 us, in stretches 77, 133, 220; behind 20 to 1,805
 // 107 and 211; 64 behind 300, 1,000, 4,095 16, 39, 138, in stretches 22, 39, 102; 411 float32 tokens of one request, 16 / 4 heads, 27 and 39).

@@ -5,7 +5,8 @@
 // from the product to the codes, so that the block's largest magnitude is known before anything is rounded.  The others take one token's
 // queries.  A block that earlier steps began and whose scale rises is read back and rounded again by the CTA that owns it: one owner a
 // block, no atomics.  A row (one head of one token) belongs to LPR lanes that hold four neighbouring numbers each (NV times); the members
-// of a rotation pair meet in shared memory.  Bound by the product's float32 bytes.
+// of a rotation pair meet in shared memory.  Bound by the product's float32 bytes; at 2,048 tokens, 32 / 8 heads of 128, rotated and normed
+// (71 MB), 20 us, 3.5 TB/s, which instructions hold back: cosines, sums over a row, codes.  64 requests' tokens 7 us and one 4 us: latency.
 //
 // Angles are products of an int32 position and a float32 frequency, reduced in float64: a float32 product is off by 2^-24 of an angle that
 // reaches 10^5 radians, 0.006 of one, by which every far key would be turned.
