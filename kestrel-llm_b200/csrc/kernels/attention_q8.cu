@@ -341,7 +341,6 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
             small.rows_upto = FEW;
     }
     large.kernel = TC;
-    large.rows_above = small.rows_upto;
     large.rows_upto = 0x7fffffff;
     large.rows_per_tile = 256;
     if (!cores && !wide && cu) {
@@ -349,21 +348,40 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
         // is rows times keys of its slice, and slices cost their merge, as much as 128 rows' 380 keys (32 / 8 heads of 128: 256 tokens 12 us in
         // tiles of 128, 15 of 256; 500 behind 1,500 39 and 47, where only the latter need slices; 300 behind 2,000 43 and 39;
         // 16 / 4 heads of 64, 500 tokens of a window of 1,024, in two slices and four, 21 and 23).
-        auto work = [&](int rows_per_tile) {
+        // Single tokens beside portions come along where the SMs hold all of it at once and that takes no longer than a launch of the decode
+        // kernel for them: what 128 rows' 400 keys take, and 55 more for every key tile of a CTA's (16 / 4 heads of 64, a window of 1,024: 500
+        // tokens beside twelve single ones 22 us, in two launches 29; 32 / 8 heads of 128: 300 behind 2,000 beside six 43 and 52, 256 beside
+        // eight behind 300 14 and 22, but beside one behind 3,000 37 and 24, and twelve portions of 30 beside 50 behind 2,000 165 and 71).
+        auto work = [&](int rows_above, int rows_per_tile) {
             long long tiles = 0;
             int longest = 0;
             for (int i = 0; i < nseq; ++i) {
                 const long long rows = (long long)(cu[i + 1] - cu[i]) * G;
-                if (rows <= small.rows_upto) continue;
+                if (rows <= rows_above) continue;
                 tiles += (rows + rows_per_tile - 1) / rows_per_tile;
                 longest = std::max(longest, seen_of(kv[i], rows));
             }
             const int slices = slices_for(tiles * nkv, kestrel_sms(), longest, 256);
             return tiles * nkv > kestrel_sms() ? LLONG_MAX : (long long)rows_per_tile * (longest / slices) + (slices > 1 ? 128 * 380 : 0);
         };
-        const long long halves = work(128);
-        if (halves < LLONG_MAX && halves / 8 * 7 <= work(256)) large.rows_per_tile = 128;
+        long long halves = work(small.rows_upto, 128), whole = work(small.rows_upto, 256), singles = 0;
+        bool portions = false;
+        for (int i = 0; i < nseq; ++i) {
+            const long long rows = (long long)(cu[i + 1] - cu[i]) * G;
+            if (rows > small.rows_upto) portions = true;
+            else if (rows > 0) singles += (seen_of(kv[i], rows) + 63) / 64 * (long long)nkv;
+        }
+        if (portions && singles && std::min(halves, whole) < LLONG_MAX) {
+            const long long all_halves = work(0, 128), all_whole = work(0, 256);
+            if (std::min(all_halves, all_whole) <= std::min(halves, whole) + 128 * (400 + 55 * singles / (3 * kestrel_sms()))) {
+                small.rows_upto = 0;
+                halves = all_halves;
+                whole = all_whole;
+            }
+        }
+        if (halves < LLONG_MAX && halves / 8 * 7 <= whole) large.rows_per_tile = 128;
     }
+    large.rows_above = small.rows_upto;
     small.rows_per_tile = cores ? BM : wide ? 8 : 16;
     auto count = [&](long long rows, int keys, int times) {
         if (rows <= 0) return;
@@ -396,8 +414,8 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
             p->scratch = p->slices ? 0 : q8_decode_scratch(p->ctas, hd);
         } else {
             // The tensor cores: one CTA an SM, slices of two key tiles at least.  The CUDA cores: two CTAs an SM, which a key tile takes 6 us, the
-            // merge 3: slices of one tile, and CTAs for two rounds (float32, 16 / 4 heads of 128: 8 tokens behind 400 keys 19 us, 49 with slices of
-            // 256 keys; 411 tokens 52 us, 63 with CTAs for one round; eight single tokens behind 3,000 keys 63 us, 61 with one round).
+            // merge 3: slices of one tile, and CTAs for two rounds (16 / 4 heads of 80: 8 tokens behind 400 keys 19 us, 45 with slices of 256
+            // keys; 411 tokens 51 us, 63 with CTAs for one round).
             p->slices = p->kernel == TC ? slices_for(p->tiles * nkv, kestrel_sms(), p->longest, 256)
                                         : slices_for(p->tiles * nkv, kestrel_sms() * 4, p->longest, BN);
             p->scratch = p->slices > 1 ? (long long)T * nq * p->slices * (hd + 2) : 0;

@@ -143,6 +143,9 @@ template <int HD> __device__ __forceinline__ uint32_t chunk_at(int k, int c) {
     return line * 128 + ((at ^ (line & 7)) << 4);
 }
 
+// a / b for a >= 0, b > 0: a division of 64 bits takes ten times one of 32
+__device__ __forceinline__ long long over(long long a, long long b) { return (a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b); }
+
 // The line of key tiles: request i's pairs lie behind those of the requests before it, kv head by kv head and in these row tile by row tile: the
 // first, the last, the second, the last but one, ..., so that neighbours, which see few keys of a prompt and many, weigh together like others.
 // All pairs of a request have the tiles that its first or its last row sees.
@@ -175,7 +178,7 @@ struct Line {
     // the request in which tile `at` lies, and its first tile's place
     __device__ __forceinline__ int request_at(long long at, long long &begin) const {
         const int lane = threadIdx.x & 31;
-        const int want = (int)(at / p.nkv);         // on one kv head's line a request holds its place
+        const int want = (int)over(at, p.nkv);      // on one kv head's line a request holds its place
         int before = 0;
         for (int base = 0; base < p.nseq; base += 32) {
             const int n = place_of(base + lane);
@@ -202,8 +205,8 @@ struct Line {
 // made for, and a CTA without tiles would leave its part of a pair unwritten
 __device__ __forceinline__ int stretches(long long length, int ctas) { return (int)max(1ll, min((long long)ctas, length / 2)); }
 // stretch u begins here; the stretch that holds tile `at`
-__device__ __forceinline__ long long stretch(long long u, long long length, int ctas) { return u * length / ctas; }
-__device__ __forceinline__ int holder(long long at, long long length, int ctas) { return (int)(((at + 1) * ctas - 1) / length); }
+__device__ __forceinline__ long long stretch(long long u, long long length, int ctas) { return over(u * length, ctas); }
+__device__ __forceinline__ int holder(long long at, long long length, int ctas) { return (int)over((at + 1) * ctas - 1, length); }
 
 // The k-th row tile of a request's kv head on the line, and a row tile's place there
 __device__ __forceinline__ int nth_row_tile(int k, int row_tiles) { return k & 1 ? row_tiles - 1 - k / 2 : k / 2; }
@@ -248,7 +251,7 @@ struct Walk {
         const Line line{p};
         seq = line.request_at(at, begin);
         n = line.tiles_of(seq, row_tiles);
-        const int pair = (int)((at - begin) / n);
+        const int pair = (int)over(at - begin, n);
         begin += (long long)pair * n;
         kvh = pair / row_tiles;
         nth = pair - kvh * row_tiles;

@@ -505,12 +505,12 @@ def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, top
         if ids.shape[0] != R:
             raise KernelError(f"token_logprobs: {ids.shape[0]} tokens for {R} rows")
     buf = logits.new_empty(2 * R * (1 + top))       # one piece of memory: an allocation costs the host as much as a launch
-    got = TokenLogprobs(None if ids is None else buf.as_strided((R,), (1,), 0), buf.as_strided((R,), (1,), R),
-                        buf.view(torch.int32).as_strided((R, top), (top or 1, 1), 2 * R), buf.as_strided((R, top), (top or 1, 1), (2 + top) * R))
-    with _on(dev):
-        _check(library().kestrel_token_logprobs(logits.data_ptr(), logits.stride(0) if R > 1 else V, R, V, _p(ids), top, _p(got.logprobs), got.entropy.data_ptr(),
-                                                got.top_ids.data_ptr(), got.top_logprobs.data_ptr(), _stream()))
-    return got
+    at = buf.data_ptr()
+    with _on(dev):                                  # the kernel first: the host makes its views while it runs
+        _check(library().kestrel_token_logprobs(logits.data_ptr(), logits.stride(0) if R > 1 else V, R, V, _p(ids), top, at, at + 4 * R, at + 8 * R,
+                                                at + 4 * (2 + top) * R, _stream()))
+    return TokenLogprobs(None if ids is None else buf.as_strided((R,), (1,), 0), buf.as_strided((R,), (1,), R),
+                         buf.view(torch.int32).as_strided((R, top), (top or 1, 1), 2 * R), buf.as_strided((R, top), (top or 1, 1), (2 + top) * R))
 
 
 def argmax(logits: torch.Tensor, out: torch.Tensor) -> None:
