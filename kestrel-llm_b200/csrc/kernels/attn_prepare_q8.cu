@@ -324,13 +324,17 @@ __global__ void __launch_bounds__(THREADS) attn_prepare_q8_fast_kernel(const Pre
         // ---- one token's queries, 32 heads at a time
         const int t = blockIdx.x - kv_ctas;
         if (t >= p.cu[p.nseq]) { pdl_wait(); return; }
-        if (TURN != TURN_NONE) {
+        // in front of the wait, or while the product is on its way
+        auto angles = [&] {
+            if (TURN == TURN_NONE) return;
             const int pos = p.positions[t];
             for (int j = tid; j < half; j += THREADS) cs[0][j] = sizeof(T) == 4 ? turn(pos, p.inv_freq[j], p.rot_scale) : turn_fast(pos, p.inv_freq[j], p.rot_scale);
-        }
+        };
+        if (p.described) angles();
         pdl_wait();
         Eighth<T, HD, TURN> r;
         r.load(p, t, mine, sub, mine < p.nq);
+        if (!p.described) angles();
         __syncthreads();
         for (int h0 = 0;;) {
             const int h = h0 + mine;
@@ -351,12 +355,14 @@ __global__ void __launch_bounds__(THREADS) attn_prepare_q8_fast_kernel(const Pre
     const int there = bl.pos0 % Q8_BLOCK;           // codes that earlier steps left in the block
     const int idx = bl.pos0 / p.page_size;
     const int page = idx < p.table_width ? p.table[(size_t)bl.seq * p.table_stride + idx] : -1;
-    if (TURN != TURN_NONE) {
+    auto angles = [&] {
+        if (TURN == TURN_NONE) return;
         for (int i = tid; i < bl.count * half; i += THREADS) {
             const int n = TURN == TURN_HALF ? i / (HD / 2) : i / half, j = i - n * half;
             cs[n][j] = sizeof(T) == 4 ? turn(bl.pos0 + n, p.inv_freq[j], p.rot_scale) : turn_fast(bl.pos0 + n, p.inv_freq[j], p.rot_scale);
         }
-    }
+    };
+    if (p.described) angles();
     pdl_wait();
     if (page < 0 || page >= p.cache_pages) return;  // no page to write to
     const size_t row0 = ((size_t)page * p.nkv + kvh) * p.page_size + (bl.pos0 - idx * p.page_size) - there;
@@ -367,6 +373,7 @@ __global__ void __launch_bounds__(THREADS) attn_prepare_q8_fast_kernel(const Pre
     const float k_before = there ? p.ks[row0 / Q8_BLOCK] : 0.f, v_before = there ? p.vs[row0 / Q8_BLOCK] : 0.f;
     Eighth<T, HD, TURN> r;
     r.load(p, bl.t0 + n, p.nq + (is_k ? 0 : p.nkv) + kvh, sub, n < bl.count);
+    if (!p.described) angles();
     __syncthreads();                                // the cosines and sines
     if (is_k) {
         if (p.k_w) r.norm(p, p.k_w, sub);
