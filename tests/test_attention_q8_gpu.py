@@ -147,6 +147,39 @@ def test_a_query_that_is_not_finite_stays_in_its_row(tokens):
     assert ((got - want).abs() <= _tolerance(want, size, "bfloat16", s.max_kv_len))[~bad].all()
 
 
+@pytest.mark.parametrize("portions", [[(1, 100)] * 3, [(150, 30)]])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_float32_scales_and_queries_of_every_size(portions, hd):
+    """Values from 2^-60 to 2^60 beside one another, and float32 queries whose rows differ as much and use all of their bits."""
+    import torch
+    s = step(portions, 16)
+    nq, nkv = 8, 2
+    k, ks, v, vs = planes(s, nkv, hd)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    powers = torch.randint(-60, 61, vs.shape, generator=gen, device="cuda")
+    vs = torch.where(torch.isnan(vs), vs, 2.0 ** powers * (1 + torch.rand(vs.shape, generator=gen, device="cuda")))
+    q = torch.randn((s.num_tokens, nq * hd), generator=gen, device="cuda")
+    q = (q.view(-1, nq, hd) * 2.0 ** torch.randint(-40, 41, (s.num_tokens, nq, 1), generator=gen, device="cuda")).view(q.shape)
+    ks = ks * 2.0 ** -44
+    _near(s, *_run(s, nq, nkv, hd, 0, "float32", q=q, planes_=(k, ks, v, vs)), "float32")
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+@pytest.mark.parametrize("hd", [64, 128, 80])
+def test_a_float32_query_that_is_not_finite_stays_in_its_row(tokens, hd):
+    import torch
+    s = step([(tokens, 70), (tokens, 3)], 16)
+    nq, nkv = 8, 2
+    q = torch.randn((s.num_tokens, nq * hd), device="cuda")
+    bad = torch.zeros((s.num_tokens, nq), dtype=torch.bool, device="cuda")
+    for i, (t, h, x) in enumerate(((0, 1, "nan"), (s.num_tokens - 1, 4, "inf"), (s.num_tokens - 1, 7, "-inf"))):
+        q.view(-1, nq, hd)[t, h, 3 + i] = float(x)
+        bad[t, h] = True
+    got, want, size = _run(s, nq, nkv, hd, 0, "float32", q=q)
+    assert torch.isnan(got[bad]).all() and torch.isfinite(got[~bad]).all()
+    assert ((got - want).abs() <= _tolerance(want, size, "float32", s.max_kv_len))[~bad].all()
+
+
 def test_append_then_attend_then_replay():
     """A prompt appended in portions and decoded on: attention over what the append wrote, eager and replayed from a graph with other contents."""
     import torch
