@@ -180,6 +180,27 @@ def test_a_float32_query_that_is_not_finite_stays_in_its_row(tokens, hd):
     assert ((got - want).abs() <= _tolerance(want, size, "float32", s.max_kv_len))[~bad].all()
 
 
+@pytest.mark.parametrize("portions", [[(1, 100), (1, 500)], [(200, 300)]])
+def test_pages_beyond_four_gigabytes(portions):
+    """A plane of 2^32 codes and more: offsets of codes need more than 32 bits."""
+    import torch
+    nq, nkv, hd = 8, 8, 128
+    s = step(portions, 16, extra_pages=280000)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    p = []
+    for _ in range(2):
+        p += [torch.zeros((s.pages, nkv, 16, hd), dtype=torch.int8, device="cuda"), torch.full((s.pages, nkv, 1), float("nan"), device="cuda")]
+    assert p[0].numel() > 2 ** 32
+    s.table[s.table >= 0] = (s.pages - 1 - torch.arange(int((s.table >= 0).sum()), device="cuda") * 2).int()
+    used = s.table[s.table >= 0].long()
+    for codes, scales in ((p[0], p[1]), (p[2], p[3])):
+        codes[used] = torch.randint(-127, 128, (len(used), nkv, 16, hd), generator=gen, device="cuda", dtype=torch.int8)
+        scales[used] = torch.exp(torch.randn((len(used), nkv, 1), generator=gen, device="cuda")) / 64
+    for dtype in ("bfloat16", "float32"):
+        got, want, size = _run(s, nq, nkv, hd, 0, dtype, scale=0.01, planes_=p)
+        _near(s, got, want, size, dtype)
+
+
 def test_append_then_attend_then_replay():
     """A prompt appended in portions and decoded on: attention over what the append wrote, eager and replayed from a graph with other contents."""
     import torch

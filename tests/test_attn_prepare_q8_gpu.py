@@ -193,6 +193,30 @@ def test_a_layer_that_reads_only_writes_nothing():
     assert ((q.view(20, nq, hd).double() - q64).abs() <= E * 1.5 * q64.abs().amax(-1, keepdim=True)).all()
 
 
+def test_pages_beyond_four_gigabytes():
+    """A plane of 2^32 codes and more: what is written to its last pages is what is written to others."""
+    import torch
+    nq, nkv, hd = 4, 8, 128
+    s = step([(40, 5), (3, 30)], 16)
+    inputs = _inputs(s, nq, nkv, hd, 1, hd, True, False)
+    small = [t.clone() for t in planes(s, nkv, hd)]
+    pages = 280000
+    large = [torch.zeros((pages,) + t.shape[1:], dtype=t.dtype, device="cuda") for t in small]
+    assert large[0].numel() > 2 ** 32
+    for a, b in zip(large, small):
+        a[-s.pages:] = b
+    far = step([(40, 5), (3, 30)], 16)
+    far.table[far.table >= 0] += pages - s.pages
+    got = []
+    for st, p in ((s, small), (far, large)):
+        q = torch.empty((st.num_tokens, nq * hd), device="cuda")
+        _append(st, inputs, *p, q, nq, nkv, hd, hd)
+        got.append([t[-s.pages:] for t in p] + [q])
+    for a, b in zip(*got):
+        assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+    assert all(not t[:-s.pages].any() for t in large)
+
+
 @pytest.mark.parametrize("hd", [64, 80])
 def test_tokens_in_front_of_position_zero_are_left_out(hd):
     """A request from position -20 on: its queries are turned back, its keys and values begin at position 0."""
