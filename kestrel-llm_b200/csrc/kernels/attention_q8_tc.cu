@@ -44,9 +44,12 @@ constexpr float STEP = 8.0f;                            // log2 units by which a
 
 enum { Q_FULL = 0, K_FULL = 1, K_EMPTY = 3, V_FULL = 5, V_EMPTY = 7, S_FULL = 9, P_FULL = 11, PV_DONE = 13, SCALES_FULL = 15, BARS = 19 };
 
-template <int HD> struct Lay {
+template <int HD, bool HALVES> struct Lay {
     static constexpr uint32_t PANEL = 128 * 128, PANELS = HD / 64, TILE = PANELS * PANEL;       // 128 rows of HD float16 numbers
-    static constexpr uint32_t Q = 0, K = 2 * TILE, V = 4 * TILE, SCALES = 6 * TILE;             // Q_A Q_B | two stages of K | of V
+    static constexpr uint32_t Q = 0, K = (HALVES ? 1 : 2) * TILE, V = K + 2 * TILE;             // Q_A (Q_B) | two stages of K | of V
+    // codes on their way: two tiles of K and of V where there is room for them
+    static constexpr int AHEAD = HD == 128 && !HALVES ? 0 : 2;
+    static constexpr uint32_t CODES = V + 2 * TILE, RAW = 128 * HD, SCALES = CODES + 2 * AHEAD * RAW;
     static constexpr uint32_t ROWS = SCALES + 4 * BLOCKS * 16, BARRIERS = ROWS + 256 * 4, TMEM = BARRIERS + 8 * BARS, BYTES = TMEM + 16;
     static constexpr uint32_t TMEM_COLS = 512, O = 256;                                         // S_A S_B at 0 and 128, O_A O_B behind
 };
@@ -129,6 +132,11 @@ __device__ __forceinline__ uint4 ldg128(const int8_t *p) {
     asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
 // eight codes as eight float16 numbers
 __device__ __forceinline__ uint4 widen(uint32_t a, uint32_t b) {
     a ^= 0x80808080u;
@@ -138,14 +146,17 @@ __device__ __forceinline__ uint4 widen(uint32_t a, uint32_t b) {
 }
 
 // One plane's widening, by four warps of which this is the w-th: key tiles of 128 into a ring of two stages at `ring`.  A warp's load is one
-// unit: 512 bytes, 4 keys at head size 128 and 8 at 64.  A warp always has four units in flight: once one is widened the load of the fourth
-// after it starts, over the tiles' borders.  A quarter-warp's stores of 16 bytes go to two keys and every other chunk, which the swizzle
+// unit: 512 bytes, 4 keys at head size 128 and 8 at 64.  Codes come by cp.async, two tiles ahead, every lane's into places that it alone
+// reads.  Where shared memory has no room for them a warp has four units in flight in registers: once one is widened the load of the fourth
+// after it starts, over the tiles' borders.  (32 / 8 heads of 128, 500 tokens behind 1,500 32 us, 38 through registers; 16 / 4 of 64, 2,048
+// tokens 43 and 45; with one tile ahead, for which the larger layout has room, a prompt of 2,048 tokens of 32 / 8 heads of 128 59, 57
+// through registers.)  A quarter-warp's stores of 16 bytes go to two keys and every other chunk, which the swizzle
 // spreads over all banks.  Both planes' warps run the same instructions: with a copy for each, and all of a tile unrolled, the kernel
 // waited for its code, and for what did not fit its registers.
-template <int HD>
+template <int HD, bool HALVES>
 __device__ __forceinline__ void convert(const Q8Params &p, const int *table, int kvh, const int8_t *plane, int w, bool scaled, int lane, int k_lo, int n_tiles,
-                                        uint32_t base, uint32_t ring, int full0, int empty0, int error) {
-    using L = Lay<HD>;
+                                        uint32_t base, uint32_t ring, uint32_t codes, int full0, int empty0, int error) {
+    using L = Lay<HD, HALVES>;
     constexpr int KEYS = 512 / HD, MINE = BN / KEYS / 4, DEEP = 4;         // units of a tile that are this warp's: 8, or 4
     auto bar = [&](int i) { return base + L::BARRIERS + 8u * (uint32_t)i; };
     const int key = w * KEYS + (HD == 128 ? (lane >> 2) & 3 : lane >> 2);                   // among the keys of the four warps' units: 16, or 32
@@ -157,30 +168,48 @@ __device__ __forceinline__ void convert(const Q8Params &p, const int *table, int
     auto rows_of = [&](int i) { return i < n_tiles ? q8_row_of(p, table, kvh, k_lo + i * BN + (lane & 7) * Q8_BLOCK) : 0; };
     auto load = [&](int rows, int u) {
         const int row = __shfl_sync(0xffffffffu, rows, HD == 128 ? u : 2 * u + (w >> 1));
-        return ldg128(plane + (size_t)row * HD);
+        return plane + (size_t)row * HD;
     };
-    int rows = rows_of(0), rows_next = rows_of(1);
-    uint4 q[DEEP];
+    // tile i's codes, asked for into this lane's own places of slot i % 2
+    const uint32_t mine = base + codes + w * (MINE * 512) + lane * 16;
+    auto fetch = [&](int i, int rows) {
+        const uint32_t to = mine + (i & 1) * L::RAW;
+        if (i < n_tiles) {
 #pragma unroll
-    for (int u = 0; u < DEEP; ++u) q[u] = load(rows, u);
+            for (int u = 0; u < MINE; ++u) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u * 512), "l"(load(rows, u)) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int rows = rows_of(0), rows_next = rows_of(1), rows_after = L::AHEAD > 0 ? rows_of(2) : 0;
+    uint4 q[DEEP];
+    if constexpr (L::AHEAD > 0) {
+        fetch(0, rows);
+        fetch(1, rows_next);
+    } else {
+#pragma unroll
+        for (int u = 0; u < DEEP; ++u) q[u] = ldg128(load(rows, u));
+    }
 #pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {
         const int b = i & 1;
         float sk = 0.f, sv = 0.f;
         if (scaled && lane < BLOCKS) sk = p.ks[rows / Q8_BLOCK], sv = p.vs[rows / Q8_BLOCK];
-        const int rows_after = rows_of(i + 2);
+        const int rows_last = rows_of(i + (L::AHEAD > 0 ? 3 : 2));
+        if constexpr (L::AHEAD > 0) asm volatile("cp.async.wait_group 1;" ::: "memory");
         if (!mbar_wait(bar(empty0 + b), (uint32_t)((i >> 1) + 1) & 1u)) { atomicExch(&g_q8t_error, error); break; }
 #pragma unroll 1
         for (int h = 0; h < MINE; h += DEEP) {
 #pragma unroll
             for (int u = 0; u < DEEP; ++u) {
                 const uint32_t off = b * L::TILE + (uint32_t)(h + u) * (4 * KEYS * 128);
+                if constexpr (L::AHEAD > 0) q[u] = lds128(mine + b * L::RAW + (h + u) * 512);
                 sts128(at0 + off, widen(q[u].x, q[u].y));
                 sts128(at1 + off, widen(q[u].z, q[u].w));
                 // behind the last tile the rows are 0: a load that nothing waits for
-                q[u] = h + DEEP < MINE ? load(rows, h + DEEP + u) : load(rows_next, u);
+                if constexpr (L::AHEAD == 0) q[u] = ldg128(h + DEEP < MINE ? load(rows, h + DEEP + u) : load(rows_next, u));
             }
         }
+        if constexpr (L::AHEAD > 0) fetch(i + 2, rows_after);      // into the slot that was just read
         if (scaled) {
             // Slot i % 4 is free: tile i's stage was, so S(i - 2) is done, before which every thread was through with tile i - 4.
             // A scale that is no positive number becomes one that makes the sum of a row that sees the block no number, and no other's:
@@ -197,14 +226,19 @@ __device__ __forceinline__ void convert(const Q8Params &p, const int *table, int
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(full0 + b));
         rows = rows_next;
-        rows_next = rows_after;
+        if (L::AHEAD > 0) {
+            rows_next = rows_after;
+            rows_after = rows_last;
+        } else {
+            rows_next = rows_last;
+        }
     }
 }
 
 template <int HD, bool HALVES>
 __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Params p) {
     pdl_launch_dependents();
-    using L = Lay<HD>;
+    using L = Lay<HD, HALVES>;
     // float16 x float16 -> float32, M = 128; S: both operands K-major, N = 128; PV: B is MN-major, N = head size
     constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
     constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
@@ -256,7 +290,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
         if (warp >= 12) {
             const bool is_v = warp >= 16;
             if (n_tiles > 0)
-                convert<HD>(p, t.table, kvh, is_v ? p.v : p.k, warp & 3, warp == 12, lane, k_lo, n_tiles, base, is_v ? L::V : L::K, is_v ? V_FULL : K_FULL,
+                convert<HD, HALVES>(p, t.table, kvh, is_v ? p.v : p.k, warp & 3, warp == 12, lane, k_lo, n_tiles, base, is_v ? L::V : L::K,
+                            L::CODES + (is_v ? L::AHEAD * L::RAW : 0), is_v ? V_FULL : K_FULL,
                             is_v ? V_EMPTY : K_EMPTY, is_v ? 4 : 3);
         } else if (warp == 8 && lane == 0 && n_tiles > 0) {
             // ---- issuer
@@ -389,8 +424,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
         const int k_hi_x = x == 0 ? k_hi_a : k_hi;
         const bool row_ok = r < rows_x;
         const int my_pos = row_ok ? t.pos_begin + (tile_row + r) / t.G : -1;
-        // the keys that this row sees in this slice: [see_lo, see_hi)
-        const int see_lo = max(k_first, p.window > 0 ? my_pos - p.window + 1 : 0), see_hi = min(my_pos + 1, k_hi_x);
+        // the keys that this row sees in this slice: [see_lo, see_hi); a row that is not there sees all, which asks for no mask
+        const int see_lo = row_ok ? max(k_first, p.window > 0 ? my_pos - p.window + 1 : 0) : 0, see_hi = row_ok ? min(my_pos + 1, k_hi_x) : 0x7fffffff;
         const float row_scale = fmaxf(row_up[HALVES ? r : x * BM + r] * p.scale * 1.4426950408889634f, Q8_LEAST_FACTOR);
         // warps none of whose 32 rows exist skip the arithmetic
         const bool warp_has_rows = 32 * (warp & 3) < rows_x;
@@ -417,8 +452,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
                     // keys this row may not see count as minus infinity
                     const int lo = see_lo - kbase, hi = see_hi - kbase;
 #pragma unroll
-                    for (int j = 0; j < BN; ++j)
-                        if (j < lo || j >= hi) a[j] = 0xff800000u;
+                    for (int c = 0; c < BN; c += 32) {
+                        const uint32_t from = lo <= c ? ~0u : lo >= c + 32 ? 0u : ~0u << (lo - c), upto = hi >= c + 32 ? ~0u : hi <= c ? 0u : ~(~0u << (hi - c));
+                        const uint32_t seen = from & upto;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!(seen & 1u << j)) a[c + j] = 0xff800000u;
+                    }
                 }
                 float mx = -INFINITY;
 #pragma unroll
@@ -566,7 +606,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const Q8Par
 
 template <int HD, bool HALVES>
 int launch_tc(const Q8Params &p, int tiles, cudaStream_t stream) {
-    constexpr int smem = Lay<HD>::BYTES + 1024;
+    constexpr int smem = Lay<HD, HALVES>::BYTES + 1024;
+    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
     // the registers dealt out inside are those of the launch: with fewer the softmax groups would wait for the difference
     static const int regs = [] {
         cudaFuncAttributes a;
