@@ -319,9 +319,9 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
     if (!cores && !wide && cu) {
         // Short portions go to the decode kernel, which reads a request's keys again for every 16 rows, if that leaves no portion to the other
         // kernel: where every pair has its CTAs at once and their work is little (32 / 8 heads of 128, one request, behind 500 keys: 16 tokens
-        // 12.0 us against 15.7, 64 tokens 14.7 against 17.4, 128 tokens 18.0 against 18.6; 64 tokens behind 2,000 keys 27 against 20; four
-        // requests of about 64 tokens behind 100, more pairs than CTAs, 19 against 12), and beside single tokens, which are a launch of the kernel
-        // anyway, for three times that (four requests of 2 to 8 tokens behind 2,000 keys 17 against 35, behind 8,000 37 against 59).
+        // 11.9 us against 14.8, 64 tokens 14.7 against 16.7, 128 tokens 17.7 against 17.8; 64 tokens behind 2,000 keys 27 against 19; four
+        // requests of about 64 tokens behind 100, more pairs than CTAs, 19 against 11), and beside single tokens, which are a launch of the kernel
+        // anyway, for three times that (requests of 2, 4, 6 and 8 tokens behind 2,000 keys 17 against 18, behind 8,000 36 against 54).
         long long tiles = 0;
         int most = 0, longest = 0;
         bool single = false, all = true;
@@ -345,13 +345,13 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
     large.rows_per_tile = 256;
     if (!cores && !wide && cu) {
         // While tiles of 128 rows fit the SMs at once, a CTA may take one, and its key tiles go to the two streams in turn.  What a CTA has to do
-        // is rows times keys of its slice, and slices cost their merge, as much as 128 rows' 380 keys (32 / 8 heads of 128: 256 tokens 12 us in
-        // tiles of 128, 15 of 256; 500 behind 1,500 39 and 47, where only the latter need slices; 300 behind 2,000 43 and 39;
-        // 16 / 4 heads of 64, 500 tokens of a window of 1,024, in two slices and four, 21 and 23).
+        // is rows times keys of its slice, and slices cost their merge, as much as 128 rows' 380 keys; for as much to do, tiles of 128 take four
+        // fifths of the time (32 / 8 heads of 128: 256 tokens 11 us in tiles of 128, 14 of 256; 500 behind 1,500 32 and 43, where only the latter
+        // need slices; 300 behind 2,000 35 and 38; 500 behind 8,000 102 and 111).
         // Single tokens beside portions come along where the SMs hold all of it at once and that takes no longer than a launch of the decode
         // kernel for them: what 128 rows' 400 keys take, and 55 more for every key tile of a CTA's (16 / 4 heads of 64, a window of 1,024: 500
-        // tokens beside twelve single ones 22 us, in two launches 29; 32 / 8 heads of 128: 300 behind 2,000 beside six 43 and 52, 256 beside
-        // eight behind 300 14 and 22, but beside one behind 3,000 37 and 24, and twelve portions of 30 beside 50 behind 2,000 165 and 71).
+        // tokens beside twelve single ones 20 us, in two launches 28; 32 / 8 heads of 128: 300 behind 2,000 beside six 35 and 51, 256 beside
+        // eight behind 300 12 and 21, but beside one behind 3,000 31 and 22, 200 beside four behind 8,000 93 and 35).
         auto work = [&](int rows_above, int rows_per_tile) {
             long long tiles = 0;
             int longest = 0;
@@ -379,7 +379,7 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
                 whole = all_whole;
             }
         }
-        if (halves < LLONG_MAX && halves / 8 * 7 <= whole) large.rows_per_tile = 128;
+        if (halves < LLONG_MAX && halves / 5 * 4 <= whole) large.rows_per_tile = 128;
     }
     large.rows_above = small.rows_upto;
     small.rows_per_tile = cores ? BM : wide ? 8 : 16;

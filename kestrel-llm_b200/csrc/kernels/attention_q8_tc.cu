@@ -6,9 +6,9 @@
 //   warps 0-3, 4-7   softmax of A and of B: a thread owns a row, its 128 scores in registers; P goes back over S in TMEM as float16;
 //   warp 8           one thread issues S_X = Q_X K^T and O_X += P_X V, tcgen05.mma M = 128, N = 128 (N = head size), in the order
 //                    S_A S_B | PV_A S_A' PV_B S_B' | ..., so that one row tile is multiplied while the other is softmaxed;
-//   warps 12-15      read the codes of K from the cache, 16 bytes a lane, widen them to float16 in registers and write them to shared
-//                    memory in the swizzled layout of an operand, two stages ahead of the products at most; eight lanes of warp 12 bring
-//                    the blocks' scales along;
+//   warps 12-15      bring the codes of K from the cache, 16 bytes a lane, widen them to float16 and write them to shared memory in the
+//                    swizzled layout of an operand, two stages ahead of the products at most; eight lanes of warp 12 bring the blocks'
+//                    scales along;
 //   warps 16-19      the same for V.
 // A code is widened as the low byte of the float16 number 1024 + (c + 128), less 1152: a permutation for two codes and a subtraction of
 // pairs.  Reading codes and not 16-bit numbers halves what a CTA fetches; the widening, 32,768 codes a key tile, takes some 1,800 of the
@@ -25,9 +25,11 @@
 // HALVES: a CTA with one row tile (up to 128 rows), whose even key tiles go to stream A and odd ones to B, over the same queries; the rows'
 // two states are merged at the end.  Every wait is bounded.
 //
-// Bound by the softmax's issue slots: 2,600 cycles a pair of row tiles and key tile, of which the products take 2,048 at head size 128; a
-// CTA's beginning - queries, first codes - takes some 8,000.  32 / 8 heads of 128: a prompt of 2,048 tokens 57 us, 600 TFLOP/s, of 8,192
-// 646 us, 850 TFLOP/s; 500 tokens behind 1,500 39 us.
+// Bound by a row tile's chain: from its scores to its weights 2,900 cycles (4,000 where both streams' warps are at it), from there to the next
+// scores 1,850, of which its products are 1,024; a pair of row tiles and a key tile take 4,850 cycles, where the products alone would take
+// 2,048 at head size 128.  (At head size 64 TMEM has room for weights beside the scores, so that the next scores are there at once: 2 % faster
+// at 8,192 tokens, 3 % slower or the same at 500, not kept.)  A CTA's beginning - queries, table, first codes - takes some 6,000.
+// 32 / 8 heads of 128: a prompt of 2,048 tokens 57 us, 600 TFLOP/s, of 8,192 650 us, 850 TFLOP/s; 500 tokens behind 1,500 31 us, 470 TFLOP/s.
 #include "attention_q8.cuh"
 #include "tcgen05.cuh"
 
