@@ -9,8 +9,10 @@
 //     A CTA walks its stretch pair by pair.  A pair that lies within one CTA's stretch is finished there; the others leave (maximum, sum,
 //     outputs) of their parts in scratch, two parts a CTA at most, and the join kernel below adds them in the order of the keys.
 //
-// A loader warp brings tiles by TMA into a ring of stages, codes of K and V side by side, and the scales of their four blocks beside
-// them, running ahead over the pairs' borders; four consumer warps take one block of 16 keys each.  Codes go from shared memory straight
+// A loader warp brings tiles by cp.async into a ring of stages, codes of K and V side by side in lines of 128 bytes, swizzled so that lines
+// meet in all banks, and the scales of their four blocks beside them, running ahead over the pairs' borders; four consumer warps take one
+// block of 16 keys each.  (Tiles by TMA, a copy a page and plane, are no faster with pages of 64 and slower with pages of 16, whose copies
+// are of 2,048 bytes: 256 requests behind 1,000 keys 102 us, 109 by TMA.)  Codes go from shared memory straight
 // into the fragments of mma.sync.m16n8k16 (float16, float32 sums), as the operand of sixteen rows: 16 keys by 8 query rows of scores,
 // 16 dimensions by 8 query rows of outputs, so that four heads a group leave half of a product unused and not three quarters, and a
 // thread's softmax holds four scores.  The weights change places between the two products by transposing 8 by 8 tiles.  A code of V is the
@@ -27,8 +29,8 @@
 // (2e-7 of the outputs' size on random data, as the CUDA cores').  Codes of K are freed of their 1152 like those of V here.
 //
 // Bound by HBM with bfloat16: 2 hd bytes a key and kv head; some 0.6 instructions a code to widen it.  32 / 8 heads of 128: 64 requests
-// behind up to 4,095 keys (407 MB) 83 us, 4.9 TB/s; two behind 65,535 (235 MB) 50 us, 4.7 TB/s; one behind 1,003 6.4 us, of which latency
-// is nearly all; with a head size of 64, where a tile has half the bytes and the same softmax, 64 behind up to 4,095 69 us, 2.9 TB/s.
+// behind up to 4,095 keys (407 MB) 81 us, 5.0 TB/s; two behind 65,535 (235 MB) 50 us, 4.7 TB/s; one behind 1,003 6.3 us, of which latency
+// is nearly all; with a head size of 64, where a tile has half the bytes and the same softmax, 64 behind up to 4,095 57 us, 3.6 TB/s.
 // float32: 64 behind 3,000 131 us, 3.0 TB/s, and 411 tokens of two requests, 16 / 4 heads, 23 us (CUDA cores: 39).
 #include "attention_q8.cuh"
 #include "tcgen05.cuh"
@@ -131,8 +133,8 @@ __device__ __forceinline__ uint2 lds64(uint32_t at) {
     return v;
 }
 
-// Key, among the eight of a half tile, that row n of the scores stands for.  A tile's lines of 128 bytes are swizzled as TMA writes
-// them: 16-byte chunk c of line i lies at c ^ (i % 8).  Head size 128: a key is a line; eight lanes of a 16-byte load hold rows
+// Key, among the eight of a half tile, that row n of the scores stands for.  A tile's lines of 128 bytes are swizzled:
+// 16-byte chunk c of line i lies at c ^ (i % 8).  Head size 128: a key is a line; eight lanes of a 16-byte load hold rows
 // 2 i and 2 i + 1, whose keys are four lines apart, so that their chunks fall into different halves of the banks; the values' loads of
 // sixteen lanes hold the even (or odd) rows, which are neighbouring keys.  Head size 64: a line is two keys.
 template <int HD> __device__ __forceinline__ int key_of_row(int n) { return HD == 128 ? (n >> 1) + 4 * (n & 1) : n ^ ((n >> 1) & 1); }
@@ -364,8 +366,8 @@ __device__ __forceinline__ void weigh(float (&s)[NT][4], float (&o)[NT][NO][4], 
 
 template <typename T, int HD, int NT, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, Ring<HD, NT, T>::CTAS)
-attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Q8Params p) {
-    pdl_launch_dependents();
+attention_q8_decode_kernel(const Q8Params p) {
+    if (CLUSTER) pdl_launch_dependents();               // (stretches let the join kernel in at their end)
     using R = Ring<HD, NT, T>;
     constexpr int KS = HD / 16, HALVES = HD / 64, ROWS = 8 * NT, PARTS = parts_of<T>();
     constexpr bool WIDE = PARTS > 1;
@@ -377,8 +379,8 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     auto empty_bar = [&](int s) { return base + R::BARS + 8u * (R::STAGES + s); };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        // a stage is full when its codes are there (the loader's bytes) and eight lanes' scales
-        for (int s = 0; s < R::STAGES; ++s) { mbar_init(full_bar(s), 1 + 8); mbar_init(empty_bar(s), 4); }
+        // a stage is full when what the loader's lanes have asked for is there
+        for (int s = 0; s < R::STAGES; ++s) { mbar_init(full_bar(s), 32); mbar_init(empty_bar(s), 4); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -411,29 +413,31 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     };
 
     if (warp == 4) {
-        // ---- loader: lane l brings the l-th box of a tile, K and V; lanes 0-3 (4-7) bring its blocks' scales of K (V)
-        const int box = p.page_size % 64 == 0 ? 64 : p.page_size % 32 == 0 ? 32 : 16, boxes = BN / box;
+        // ---- loader: 512 bytes at a time, sixteen a lane, to where the swizzle wants them; lanes 0-3 (4-7) bring the blocks' scales of K (V)
+        constexpr int UNITS = 16 * HD / 512;            // of a block
         const float *scales = lane < 4 ? p.ks : p.vs;
+        const int8_t *src_k = p.k + lane * 16, *src_v = p.v + lane * 16;
+        const uint32_t to = base + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);
         bool ok = true;
         while (ok && next()) {
             const int kb0 = w.k_first / BN * BN;
             for (int i = w.from; i < w.to; ++i) {
                 const int kb = kb0 + i * BN;
-                const int box_row = lane < boxes ? q8_row_of(p, w.table, w.kvh, kb + lane * box) : 0;
                 const int block_row = lane < 8 ? q8_row_of(p, w.table, w.kvh, kb + (lane & 3) * Q8_BLOCK) : 0;
                 if (!mbar_wait(empty_bar(stage), phase ^ 1u)) { atomicExch(&g_q8d_error, 1); ok = false; break; }
-                if (lane == 0) mbar_expect_tx(full_bar(stage), R::STAGE);
-                __syncwarp();
-                if (lane < boxes) {
-                    const uint32_t dst = base + stage * R::STAGE + lane * box * HD;
-                    const int line = HD == 128 ? box_row : box_row >> 1;
-                    tma_load_2d(dst, &map_k, full_bar(stage), 0, line);
-                    tma_load_2d(dst + R::PLANE, &map_v, full_bar(stage), 0, line);
+#pragma unroll
+                for (int b = 0; b < BN / Q8_BLOCK; ++b) {
+                    const size_t row = (size_t)__shfl_sync(0xffffffffu, block_row, b) * HD;
+#pragma unroll
+                    for (int u = 0; u < UNITS; ++u) {
+                        // (four lines further on the swizzle turns its third bit)
+                        const uint32_t dst = (u & 1 ? to ^ 64u : to) + stage * R::STAGE + b * 16 * HD + u * 512;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src_k + row + u * 512) : "memory");
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + R::PLANE), "l"(src_v + row + u * 512) : "memory");
+                    }
                 }
-                if (lane < 8) {
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(base + R::SCALES + stage * 32 + lane * 4), "l"(scales + block_row / Q8_BLOCK) : "memory");
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full_bar(stage)) : "memory");
-                }
+                if (lane < 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(base + R::SCALES + stage * 32 + lane * 4), "l"(scales + block_row / Q8_BLOCK) : "memory");
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full_bar(stage)) : "memory");
                 if (++stage == R::STAGES) stage = 0, phase ^= 1u;
             }
         }
@@ -711,6 +715,9 @@ attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         first_part = false;
     }
     }   // consumers
+    // At the beginning this let the join kernel's CTAs, and those of the launch behind it, in a few at a time: 64 requests behind 4,095 keys,
+    // heads of 64, took 83 us instead of 69.
+    if (!CLUSTER) pdl_launch_dependents();
 
     if (CLUSTER && !w.whole) {
         // the parts of one pair, in ascending order of the keys; the rows are shared out among the CTAs.  Every thread takes part in the
@@ -839,13 +846,7 @@ int cluster_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int size)
 
 template <typename T, int HD, int NT>
 int launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
-    CUtensorMap mk, mv;
-    const long long lines = (long long)p.cache_pages * p.nkv * p.page_size * HD / 128;
-    const int box = (p.page_size % 64 == 0 ? 64 : p.page_size % 32 == 0 ? 32 : 16) * HD / 128;
-    // two codes as one 16-bit element: the copy moves lines of 128 bytes, whatever they hold
-    int rc = kestrel_tensor_map_bf16(&mk, p.k, lines, 64, 64, box);
-    if (rc == 0) rc = kestrel_tensor_map_bf16(&mv, p.v, lines, 64, 64, box);
-    if (rc) return rc;
+    int rc;
     if (p.slices > 0) {
         // a CTA, or a cluster of them, a pair
         cudaLaunchConfig_t cfg = {};
@@ -857,12 +858,12 @@ int launch_decode(const Q8Params &p, int ctas, cudaStream_t stream) {
         attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs = g_kestrel_pdl ? 2 : 1;
-        cudaLaunchKernelEx(&cfg, attention_q8_decode_kernel<T, HD, NT, true>, mk, mv, p);
+        cudaLaunchKernelEx(&cfg, attention_q8_decode_kernel<T, HD, NT, true>, p);
         return kestrel_check_launch("attention_q8 decode");
     }
     if (cudaFuncSetAttribute(attention_q8_decode_kernel<T, HD, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)decode_smem<T, HD, NT>()) != cudaSuccess)
         return kestrel_fail(-3, "attention_q8: cannot raise the shared-memory limit: %s", cudaGetErrorString(cudaGetLastError()));
-    kestrel_launch(attention_q8_decode_kernel<T, HD, NT, false>, dim3(ctas), dim3(THREADS), decode_smem<T, HD, NT>(), stream, mk, mv, p);
+    kestrel_launch(attention_q8_decode_kernel<T, HD, NT, false>, dim3(ctas), dim3(THREADS), decode_smem<T, HD, NT>(), stream, p);
     rc = kestrel_check_launch("attention_q8 decode");
     if (rc) return rc;
     kestrel_launch(attention_q8_join_kernel<T, HD>, dim3((unsigned)p.nseq * p.row_tiles, p.nkv), dim3(256), 0, stream, p, ctas);
@@ -910,8 +911,8 @@ int q8_decode_ctas(long long tiles, int hd, Q8Form form) {
 // 6.5 us with 8 CTAs a pair, 16 with one, 10 in stretches; two behind 65,535 126 us with 8, 55 in stretches; 32 behind 500 13 with one, 17 in
 // stretches; 8 behind 4,095 18 with 6, 23 in stretches).  Where
 // there are more pairs, one, if the wait for the last one is worth what pairs cost a stretch: some five tiles' time each, and the join
-// (32 / 8 heads of 128, bfloat16: 256 requests behind 300, 1,000, 2,000 keys 48, 109, 198 us, in stretches 77, 133, 220; behind 20 to 1,805
-// 107 and 211; 64 behind 300, 1,000, 4,095 16, 39, 138, in stretches 22, 39, 102; 411 float32 tokens of one request, 16 / 4 heads, 27 and 39).
+// (32 / 8 heads of 128, bfloat16: 256 requests behind 300, 1,000, 2,000 keys 46, 102, 184 us, in stretches 77, 133, 220; behind 20 to 1,805
+// 98 and 211; 64 behind 300, 1,000 15, 37, in stretches 22, 39, behind 4,095 138 and 99; 411 float32 tokens of one request, 16 / 4 heads, 27 and 39).
 int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int hd, Q8Form form) {
     static DeviceTable<6 * (MAX_CLUSTER + 1)> known;
     int dev = -1;
