@@ -8,7 +8,7 @@
 // With x_j the score in base-2 units the tensor-core kernels hold
 //     w_j = 2^(x_j + log2 s_v(j) - m),   out = sum_j w_j c_v(j),   l = sum_j w_j / s_v(j),
 // so that w_j, rounded to float16 for the second product, lies in [0, 2^8] whatever the size of the values, one exponential serves both
-// sums, and (m, l, out) of two key ranges merge as those of any online softmax.  o = out / l.
+// sums, and (m, l, out) of two key ranges merge as those of any online softmax.  o = out / l.  (float32: attention_q8_decode.cu.)
 #pragma once
 #include "common.cuh"
 

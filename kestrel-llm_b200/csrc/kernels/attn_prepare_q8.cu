@@ -324,11 +324,12 @@ __global__ void __launch_bounds__(THREADS) attn_prepare_q8_fast_kernel(const Pre
         // ---- one token's queries, 32 heads at a time
         const int t = blockIdx.x - kv_ctas;
         if (t >= p.cu[p.nseq]) { pdl_wait(); return; }
-        // in front of the wait, or while the product is on its way
+        // in front of the wait, or while the product is on its way; half is no more than 64
+        int pos = 0;
+        float freq = 0.f;
+        if (TURN != TURN_NONE && tid < half) pos = p.positions[t], freq = p.inv_freq[tid];
         auto angles = [&] {
-            if (TURN == TURN_NONE) return;
-            const int pos = p.positions[t];
-            for (int j = tid; j < half; j += THREADS) cs[0][j] = sizeof(T) == 4 ? turn(pos, p.inv_freq[j], p.rot_scale) : turn_fast(pos, p.inv_freq[j], p.rot_scale);
+            if (TURN != TURN_NONE && tid < half) cs[0][tid] = sizeof(T) == 4 ? turn(pos, freq, p.rot_scale) : turn_fast(pos, freq, p.rot_scale);
         };
         if (p.described) angles();
         pdl_wait();

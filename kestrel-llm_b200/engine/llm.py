@@ -414,7 +414,8 @@ class LLM:
                 raise ValueError(f"a prompt of {len(p)} tokens exceeds max_model_len {self.engine.max_model_len}")
         out: List[List[TokenScore]] = [[] for _ in texts]
         engine, cache = self.engine, self.engine.cache
-        budget = min(self.options.max_step_tokens, self.options.prefill_batch)
+        # a step's logits, all of its rows', stay within a gigabyte
+        budget = max(1, min(self.options.max_step_tokens, self.options.prefill_batch, (1 << 28) // engine.vocab_size))
         waiting = [i for i, p in enumerate(texts) if len(p) > 1]
         running: List[Tuple[int, int]] = []              # (text, request id)
         try:
