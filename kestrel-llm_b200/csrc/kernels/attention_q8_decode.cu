@@ -3,7 +3,7 @@
 //
 // The work is pairs - a kv head and up to 8 or 16 (token, query head) rows of a request - of key tiles of 64.  How CTAs take them
 // (q8_decode_cluster has both sides' times):
-//   - the CTAs of a cluster of up to 8 share one pair, evenly, and join their parts in each other's shared memory: few, short pairs;
+//   - the CTAs of a cluster of up to 16 share one pair, evenly, and join their parts in each other's shared memory: few, short pairs;
 //   - a CTA a pair, late rows first, more CTAs than there is room for: many pairs, none long;
 //   - stretches: all key tiles of all pairs stand in one line, and every CTA takes as many of them as the next, whatever the requests' lengths.
 //     A CTA walks its stretch pair by pair.  A pair that lies within one CTA's stretch is finished there; the others leave (maximum, sum,
@@ -45,7 +45,7 @@ __device__ int g_q8d_error = 0;
 
 namespace {
 
-constexpr int THREADS = 160, BN = 64, MAX_CLUSTER = 8;      // four consumer warps and the loader; keys of a tile
+constexpr int THREADS = 160, BN = 64, MAX_CLUSTER = 16;     // four consumer warps and the loader; keys of a tile
 constexpr uint32_t MAGIC = 0x64646464u;     // high byte of the float16 numbers 1024 .. 1279
 
 // NT: column tiles of eight rows.  One: three CTAs an SM; two, or one of float32: two.
@@ -724,39 +724,51 @@ attention_q8_decode_kernel(const Q8Params p) {
         // barriers; no CTA leaves while its shared memory may still be read.
         const int rank = blockIdx.x % p.slices;
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-        if (warp < 4) {
+        // MOST: parts at most, 8 or 16
+        auto join = [&](auto most) {
+            constexpr int MOST = most();
             for (int idx = tid; idx < ROWS * (HD / 8); idx += 128) {
                 const int r = idx / (HD / 8), d = (idx % (HD / 8)) * 8;
                 if (r >= w.rows) break;
                 if (r % p.slices != rank) continue;
-                // all parts' numbers in flight at once
-                float2 ml[MAX_CLUSTER];
-                float4 x[MAX_CLUSTER][2];
+                // all parts' maxima and sums and eight parts' outputs in flight at once
+                float2 ml[MOST];
 #pragma unroll
-                for (int s = 0; s < MAX_CLUSTER; ++s) {
-                    ml[s] = make_float2(-INFINITY, 0.f);
-                    if (s >= p.slices) continue;
-                    ml[s] = ld_cluster2(in_cluster(base + FIN_ML + 8 * r, s));
-                    x[s][0] = ld_cluster4(in_cluster(base + (r * HD + d) * 4, s));
-                    x[s][1] = ld_cluster4(in_cluster(base + (r * HD + d + 4) * 4, s));
-                }
+                for (int s = 0; s < MOST; ++s) ml[s] = s < p.slices ? ld_cluster2(in_cluster(base + FIN_ML + 8 * r, s)) : make_float2(-INFINITY, 0.f);
                 float M = -INFINITY, L = 0.f, acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
                 bool fine = true;
 #pragma unroll
-                for (int s = 0; s < MAX_CLUSTER; ++s) {
-                    fine = fine && ml[s].x == ml[s].x;      // a wait gave up: nothing is written
-                    M = fmaxf(M, ml[s].x);
-                }
+                for (int s0 = 0; s0 < MOST; s0 += 8) {
+                    float4 x[8][2];
 #pragma unroll
-                for (int s = 0; s < MAX_CLUSTER; ++s) {
-                    const float f = ml[s].x == -INFINITY ? 0.f : exp2f(ml[s].x - M);
-                    if (s >= p.slices || (f == 0.f && ml[s].y == ml[s].y)) continue;       // (a sum that is no number stays that)
-                    L = fmaf(ml[s].y, f, L);
-                    acc[0] = fmaf(x[s][0].x, f, acc[0]); acc[1] = fmaf(x[s][0].y, f, acc[1]); acc[2] = fmaf(x[s][0].z, f, acc[2]); acc[3] = fmaf(x[s][0].w, f, acc[3]);
-                    acc[4] = fmaf(x[s][1].x, f, acc[4]); acc[5] = fmaf(x[s][1].y, f, acc[5]); acc[6] = fmaf(x[s][1].z, f, acc[6]); acc[7] = fmaf(x[s][1].w, f, acc[7]);
+                    for (int s = 0; s < 8; ++s) {
+                        if (s0 + s >= p.slices) continue;
+                        x[s][0] = ld_cluster4(in_cluster(base + (r * HD + d) * 4, s0 + s));
+                        x[s][1] = ld_cluster4(in_cluster(base + (r * HD + d + 4) * 4, s0 + s));
+                    }
+                    if (s0 == 0) {
+#pragma unroll
+                        for (int s = 0; s < MOST; ++s) {
+                            fine = fine && ml[s].x == ml[s].x;      // a wait gave up: nothing is written
+                            M = fmaxf(M, ml[s].x);
+                        }
+                    }
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) {
+                        const float2 part = ml[s0 + s];
+                        const float f = part.x == -INFINITY ? 0.f : exp2f(part.x - M);
+                        if (s0 + s >= p.slices || (f == 0.f && part.y == part.y)) continue;     // (a sum that is no number stays that)
+                        L = fmaf(part.y, f, L);
+                        acc[0] = fmaf(x[s][0].x, f, acc[0]); acc[1] = fmaf(x[s][0].y, f, acc[1]); acc[2] = fmaf(x[s][0].z, f, acc[2]); acc[3] = fmaf(x[s][0].w, f, acc[3]);
+                        acc[4] = fmaf(x[s][1].x, f, acc[4]); acc[5] = fmaf(x[s][1].y, f, acc[5]); acc[6] = fmaf(x[s][1].z, f, acc[6]); acc[7] = fmaf(x[s][1].w, f, acc[7]);
+                    }
                 }
                 if (fine) store(w.out_row(r) * HD + d, acc, L);
             }
+        };
+        if (warp < 4) {
+            if (p.slices <= 8) join(std::integral_constant<int, 8>());
+            else join(std::integral_constant<int, MAX_CLUSTER>());
         }
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
@@ -834,6 +846,9 @@ template <typename T, int HD, int NT>
 int cluster_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int size) {
     if (cudaFuncSetAttribute(attention_q8_decode_kernel<T, HD, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)decode_smem<T, HD, NT>()) != cudaSuccess)
         return kestrel_fail(-3, "attention_q8: cannot raise the shared-memory limit: %s", cudaGetErrorString(cudaGetLastError()));
+    // more than eight CTAs a cluster are not on every device; how many such clusters this one holds is asked below
+    if (size > 8 && cudaFuncSetAttribute(attention_q8_decode_kernel<T, HD, NT, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return kestrel_fail(-3, "attention_q8: clusters of %d: %s", size, cudaGetErrorString(cudaGetLastError()));
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = decode_smem<T, HD, NT>();
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -907,7 +922,8 @@ int q8_decode_ctas(long long tiles, int hd, Q8Form form) {
 }
 
 // CTAs a pair, or 0 for stretches.  Where every pair can have its CTAs at once, as many as let every cluster be resident, up to 8, and two
-// tiles each; taken where the longest pair's share is no more than six tiles above a stretch, which is about what the join kernel takes (32 / 8 heads of 128: a request behind 1,003 keys
+// tiles each, or up to 16 where these have four (two requests behind 8,000 keys 15 us, 18 with 8; one behind 4,095 in float32 12 and 15; one
+// behind 2,000 9 and 8); taken where the longest pair's share is no more than six tiles above a stretch, which is about what the join kernel takes (32 / 8 heads of 128: a request behind 1,003 keys
 // 6.5 us with 8 CTAs a pair, 16 with one, 10 in stretches; two behind 65,535 126 us with 8, 55 in stretches; 32 behind 500 13 with one, 17 in
 // stretches; 8 behind 4,095 18 with 6, 23 in stretches).  Where
 // there are more pairs, one, if the wait for the last one is worth what pairs cost a stretch: some five tiles' time each, and the join
@@ -926,7 +942,8 @@ int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int h
         });
     };
     const long long ctas = q8_decode_ctas(tiles, hd, form), stretch = (tiles + ctas - 1) / ctas;
-    for (int size = longest_tiles / 2 < MAX_CLUSTER ? (longest_tiles < 2 ? 1 : longest_tiles / 2) : MAX_CLUSTER; size >= 1; --size) {
+    const int most = longest_tiles >= 4 * MAX_CLUSTER ? MAX_CLUSTER : 8;
+    for (int size = longest_tiles / 2 < most ? (longest_tiles < 2 ? 1 : longest_tiles / 2) : most; size >= 1; --size) {
         if ((longest_tiles + size - 1) / size > stretch + 6) break;
         if (pairs <= resident(size)) return size;
     }

@@ -67,7 +67,7 @@ def test_head_sizes_and_float32_against_float64(portions, nq, nkv, hd, page, win
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("portions", [[(1, 70000)], [(3, 20000), (1, 9)], [(40, 9000)]])
+@pytest.mark.parametrize("portions", [[(1, 70000)], [(3, 20000), (1, 9)], [(40, 9000)], [(1, 5000)], [(2, 4500), (1, 300)], [(1, 6200)] * 3])
 def test_long_contexts(portions, dtype):
     s = step(portions, 64)
     _near(s, *_run(s, 8, 2, 128, 0, dtype), dtype)
