@@ -781,8 +781,7 @@ __global__ void __launch_bounds__(256) attention_q8_join_kernel(const Q8Params p
     pdl_launch_dependents();
     constexpr int DL = HD / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.x / p.row_tiles, rt = blockIdx.x - seq * p.row_tiles, kvh = blockIdx.y, G = p.nq / p.nkv;
-    if (!p.described) pdl_wait();
-    const Line line{p};
+    const Line line{p};                 // (the description is there: every CTA of the stretches has waited for it before it let this kernel in)
     int before = 0, all = 0, row_tiles;
     for (int i = lane; i < p.nseq; i += 32) {
         const int n = line.place_of(i);
