@@ -382,7 +382,14 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
         if (halves < LLONG_MAX && halves / 5 * 4 <= whole) large.rows_per_tile = 128;
     }
     large.rows_above = small.rows_upto;
-    small.rows_per_tile = cores ? BM : wide ? 8 : 16;
+    // float32: sixteen rows at head size 64, where they fit the registers (32 / 8 heads, 300 tokens behind 600 53 us, 64 in tiles of eight;
+    // at 128, with spilled registers, 30 and 25 for 411 tokens)
+    bool sixteen = !wide;
+    if (wide && hd == 64) {
+        if (!cu) sixteen = (long long)max_count * G > 8;
+        else for (int i = 0; i < nseq; ++i) sixteen |= (long long)(cu[i + 1] - cu[i]) * G > 8;
+    }
+    small.rows_per_tile = cores ? BM : sixteen ? 16 : 8;
     auto count = [&](long long rows, int keys, int times) {
         if (rows <= 0) return;
         Part &p = rows <= small.rows_upto ? small : large;
@@ -405,8 +412,8 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
     for (Part *p : {&small, &large}) {
         if (!p->tiles) continue;
         if (p->kernel == DECODE) {
-            p->form = wide ? Q8_WIDE : p->most_rows <= 8 ? Q8_EIGHT : Q8_SIXTEEN;
-            p->rows_per_tile = p->form == Q8_SIXTEEN ? 16 : 8;
+            if (p->most_rows <= 8) p->rows_per_tile = 8;
+            p->form = p->rows_per_tile == 8 ? (wide ? Q8_WIDE_EIGHT : Q8_EIGHT) : wide ? Q8_WIDE_SIXTEEN : Q8_SIXTEEN;
             p->ctas = q8_decode_ctas(p->key_tiles, hd, p->form);
             p->row_tiles = (p->most_rows + p->rows_per_tile - 1) / p->rows_per_tile;
             if (p->row_tiles == 1) p->tiles = nseq;

@@ -107,7 +107,7 @@ __device__ __forceinline__ size_t q8_out_row(const Q8Params &p, const Q8Tile &t,
 }
 
 // attention_q8_decode.cu: requests of few rows and float32, head sizes 64 and 128; one or two kernels
-enum Q8Form { Q8_EIGHT, Q8_SIXTEEN, Q8_WIDE };          // tiles of 8 or 16 rows (Q8Params.rows_per_tile) of bfloat16, of 8 of float32
+enum Q8Form { Q8_EIGHT, Q8_SIXTEEN, Q8_WIDE_EIGHT, Q8_WIDE_SIXTEEN };      // tiles of 8 or 16 rows (Q8Params.rows_per_tile) of bfloat16, of float32
 int q8_launch_decode(const Q8Params &p, Q8Form form, int ctas, cudaStream_t stream);
 int q8_decode_ctas(long long tiles, int hd, Q8Form form);       // for so many (row tile, kv head, 64 keys)
 int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int hd, Q8Form form);        // CTAs a pair (Q8Params.slices), or 0: ctas in stretches

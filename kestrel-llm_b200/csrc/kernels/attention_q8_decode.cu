@@ -23,15 +23,16 @@
 // twice: a thread's 16 neighbouring dimensions of a key are one 16-byte load and four k-steps of the scores, and the columns of the scores
 // stand for keys in an order that lets every load of a warp touch each bank once.
 //
-// float32: a query and a weight are three float16 parts each, whose products with codes are exact, so that a score or an output is a sum
-// of exact products as in float32, at three times the matrix instructions; these cut their sums off instead of rounding them, so every
-// k-step begins at zero, smallest part first, and is added in float32.  Errors against 64 bits are those of float32 multiply-adds
-// (2e-7 of the outputs' size on random data, as the CUDA cores').  Codes of K are freed of their 1152 like those of V here.
+// float32: a query and a weight are two float16 parts each, which leave 2^-22 of it or, of a row's small ones, 2^-31 of the largest query and
+// 2^-39 of the largest weight.  (A third part would leave less than float32 itself; outputs on random data are off by 2.3e-7 of their norm
+// with two parts, 2.2e-7 with three, 4e-7 in PyTorch's float32, and the third takes a fifth of the time.)  Products with codes are exact.  The
+// matrix instructions cut their sums off instead of rounding them, so every k-step begins at zero, smaller part first, and is added in
+// float32.  Codes of K are freed of their 1152 like those of V here.
 //
 // Bound by HBM with bfloat16: 2 hd bytes a key and kv head; some 0.6 instructions a code to widen it.  32 / 8 heads of 128: 64 requests
-// behind up to 4,095 keys (407 MB) 81 us, 5.0 TB/s; two behind 65,535 (235 MB) 50 us, 4.7 TB/s; one behind 1,003 6.3 us, of which latency
-// is nearly all; with a head size of 64, where a tile has half the bytes and the same softmax, 64 behind up to 4,095 57 us, 3.6 TB/s.
-// float32: 64 behind 3,000 131 us, 3.0 TB/s, and 411 tokens of two requests, 16 / 4 heads, 23 us (CUDA cores: 39).
+// behind up to 4,095 keys (407 MB) 80 us, 5.1 TB/s; two behind 65,535 (235 MB) 49 us, 4.8 TB/s; one behind 1,003 6.3 us, of which latency
+// is nearly all; with a head size of 64, where a tile has half the bytes and the same softmax, 64 behind up to 4,095 55 us, 3.7 TB/s.
+// float32: 64 behind 3,000 115 us, 3.5 TB/s, and 411 tokens of two requests, 16 / 4 heads, 20 us (CUDA cores: 39).
 #include "attention_q8.cuh"
 #include "tcgen05.cuh"
 
@@ -57,7 +58,7 @@ template <int HD, int NT, typename T> struct Ring {
     static constexpr uint32_t SCALES = STAGES * STAGE, BARS = SCALES + STAGES * 32, MEET = BARS + 16 * STAGES, BYTES = MEET + 4 * 8 * NT * (LDO + 2) * 4;
 };
 
-template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : 1; }
+template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 2 : 1; }
 
 __device__ __forceinline__ uint32_t hsub2(uint32_t a) {             // - 1152 from both halves
     uint32_t d;
@@ -84,7 +85,7 @@ __device__ __forceinline__ float rcp_fast(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// two numbers as pairs of float16 parts, the largest first: three of them leave 2^-33 of a number, or 2^-25
+// two numbers as pairs of float16 parts, the larger first: two of them leave 2^-22 of a number, or 2^-25
 template <int PARTS>
 __device__ __forceinline__ void split(float lo, float hi, uint32_t (&part)[PARTS]) {
 #pragma unroll
@@ -354,7 +355,7 @@ __device__ __forceinline__ void weigh(float (&s)[NT][4], float (&o)[NT][NO][4], 
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            // (float32: times 2^14, so that a weight with its scale's other factor stays below 2^15, and its parts leave 2^-39 of the largest)
+            // (float32: times 2^14, so that a weight with its scale's other factor stays below 2^15, and its parts leave no more than 2^-39 of the largest)
             const float shift = lv - (m[nt][i] == -INFINITY ? 0.f : m[nt][i]) + (WIDE ? 14.f : 0.f);
             float &a = s[nt][i], &b = s[nt][2 + i];
             a = WIDE ? exp2f(fmaf(a, ck[nt][i], shift)) : exp2_fast(fmaf(a, ck[nt][i], shift));
@@ -463,7 +464,7 @@ attention_q8_decode_kernel(const Q8Params p) {
     while (next()) {
         // Queries as fragments, in float16: a row is multiplied by the power of two that brings its largest number to [64, 128), so that
         // a bfloat16 number keeps its bits down to 2^-21 of that, and the rest is off by 2^-31 of it.
-        // float32: three parts of a number, which leave 2^-31 of the row's largest.
+        // float32: two parts of a number.
         uint32_t qb[PARTS][NT][KS][2];
         float row_scale[NT][2], bias[NT][2];            // of rows 2 c and 2 c + 1
         int pos[NT][2], low[NT][2], min_pos = 0x7fffffff, max_low = 0;      // (the last two of the rows that are there)
@@ -900,12 +901,13 @@ int resident_clusters(int size) {
     return n;
 }
 
-// calls f with the kernel's types and sizes: (T, head size, column tiles)
+// calls f with the kernel's types and sizes: (T, head size, column tiles); float32 in tiles of 16 rows is for head size 64 alone
 template <typename F>
 auto with_form(Q8Form form, int hd, F f) {
     auto sized = [&](auto t, auto nt) { return hd == 64 ? f(t, std::integral_constant<int, 64>(), nt) : f(t, std::integral_constant<int, 128>(), nt); };
     using One = std::integral_constant<int, 1>;
-    return form == Q8_WIDE ? sized(0.f, One()) : form == Q8_EIGHT ? sized(__nv_bfloat16(), One()) : sized(__nv_bfloat16(), std::integral_constant<int, 2>());
+    if (form == Q8_WIDE_SIXTEEN) return f(0.f, std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+    return form == Q8_WIDE_EIGHT ? sized(0.f, One()) : form == Q8_EIGHT ? sized(__nv_bfloat16(), One()) : sized(__nv_bfloat16(), std::integral_constant<int, 2>());
 }
 
 }  // namespace
@@ -927,9 +929,9 @@ int q8_decode_ctas(long long tiles, int hd, Q8Form form) {
 // stretches; 8 behind 4,095 18 with 6, 23 in stretches).  Where
 // there are more pairs, one, if the wait for the last one is worth what pairs cost a stretch: some five tiles' time each, and the join
 // (32 / 8 heads of 128, bfloat16: 256 requests behind 300, 1,000, 2,000 keys 46, 102, 184 us, in stretches 77, 133, 220; behind 20 to 1,805
-// 98 and 211; 64 behind 300, 1,000 15, 37, in stretches 22, 39, behind 4,095 138 and 99; 411 float32 tokens of one request, 16 / 4 heads, 27 and 39).
+// 98 and 211; 64 behind 300, 1,000 15, 37, in stretches 22, 39, behind 4,095 138 and 99; 411 float32 tokens of one request, 16 / 4 heads, 25 and 39).
 int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int hd, Q8Form form) {
-    static DeviceTable<6 * (MAX_CLUSTER + 1)> known;
+    static DeviceTable<8 * (MAX_CLUSTER + 1)> known;
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess) {
         cudaGetLastError();

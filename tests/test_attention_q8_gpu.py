@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 def _tolerance(out, size, dtype, keys):
     """float32: scores of up to 256 products and sums over up to 2^17 keys in a few partial sums, 2^-24 each, of numbers that are at most
     their keys' weighted magnitudes; exponentials within 2^-21: 2^-14 of these magnitudes.  A weight - a probability times its value's scale's
-    power of two - is held in three float16 parts that leave 2^-39 of the row's largest, times a code of at most 127, where the key that
+    power of two - is held in float16 parts that leave 2^-22 of it or 2^-39 of the row's largest, times a code of at most 127, where the key that
     holds the largest has codes of 64 and more: 2^-38 of the row's largest magnitude for every key.  bfloat16: the output is rounded by half a step,
     2^-8 of it; weights - a key's probability times its value's scale - are rounded to float16, 2^-11 of them each and at least 2^-25 of the
     row's largest, whose own magnitudes are the row's largest too; scores sum in float32: 2^-10 of the magnitudes, and 2^-24 of the row's
