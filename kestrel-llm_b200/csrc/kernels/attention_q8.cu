@@ -465,7 +465,8 @@ KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const v
         const Part &part = pl.part[i];
         KESTREL_REQUIRE(part.tiles * nkv * std::max(part.slices, 1) < (1ll << 31) && (part.kernel != DECODE || (part.key_tiles / nkv < (1ll << 31) && (long long)nseq * part.row_tiles < (1ll << 31))),
                         "attention_q8: %lld row tiles and %lld key tiles of %d kv heads exceed the grid", part.tiles, part.key_tiles, nkv);
-        KESTREL_REQUIRE(part.scratch == 0 || (scratch && part.scratch <= scratch_floats), "attention_q8: scratch of %lld floats is needed, %lld given", part.scratch, scratch_floats);
+        if (part.scratch > 0 && (!scratch || part.scratch > scratch_floats))
+            return kestrel_fail(-KESTREL_Q8_NEEDS_SCRATCH, "attention_q8: scratch of %lld floats is needed, %lld given", part.scratch, scratch_floats);
     }
     int launches = 0;
     for (int i = 0; i < pl.parts; ++i) {

@@ -344,6 +344,7 @@ def attention_plain(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 # ---- pages of 8-bit codes -------------------------------------------------------------------------
 
 Q8_BLOCK = _cdecl.constants()["KESTREL_Q8_BLOCK"]       # tokens that share a scale
+_Q8_NEEDS_SCRATCH = -_cdecl.constants()["KESTREL_Q8_NEEDS_SCRATCH"]
 
 
 def _need_q8(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, nkv: int, page_size: int, hd: int,
@@ -398,10 +399,12 @@ def attn_prepare_q8(qkv: Partials, q_norm_w: Optional[torch.Tensor], k_norm_w: O
     as a copy leaves them; the launch reads them while that kernel still runs."""
     dev = q_out.device
     _need(q_out, "attn_prepare_q8.q_out", dims=2)
-    T = q_out.shape[0]
+    T, i32 = q_out.shape[0], torch.int32
     if qkv.tokens != T or qkv.width != (nq + 2 * nkv) * hd or q_out.shape[1] != nq * hd:
         raise KernelError("attn_prepare_q8: shapes differ")
-    _need_ints("attn_prepare_q8", dev, positions=positions, cu_seqlens=cu_seqlens)
+    if not (positions.dtype is cu_seqlens.dtype is i32 and positions.dim() == cu_seqlens.dim() == 1 and positions.is_contiguous()
+            and cu_seqlens.is_contiguous() and positions.get_device() == cu_seqlens.get_device() == dev.index):
+        _need_ints("attn_prepare_q8", dev, positions=positions, cu_seqlens=cu_seqlens)
     _need_table("attn_prepare_q8", block_table, dev)
     n = cu_seqlens.shape[0] - 1
     if positions.shape[0] != T or n < 1 or block_table.shape[0] < n:
@@ -438,37 +441,46 @@ def attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     ``max_count`` tokens).  ``described``: as `attn_prepare_q8` has it, of the batch and block_table.  Rows of ``out`` behind the last
     request are left as they are.  Kernels find their tiles on the device; sums and softmax statistics are float32."""
     dev = q.device
-    _need(q, "attention_q8.q", dims=2)
-    _need(out, "attention_q8.out", q.dtype, 2)
-    T, n = q.shape[0], batch.num_seqs
-    if q.shape[1] != nq * hd or out.shape != q.shape or out.device != dev:
-        raise KernelError(f"attention_q8: queries {tuple(q.shape)} and outputs {tuple(out.shape)} of {nq} heads of {hd}")
-    if T != batch.num_tokens:
-        raise KernelError(f"attention_q8: {T} query rows for a step of {batch.num_tokens} tokens")
-    _need_ints("attention_q8", dev, cu_seqlens=batch.cu_seqlens, kv_lens=batch.kv_lens)
+    T, n = batch.num_tokens, batch.num_seqs
+    cu_dev, kv_dev = batch.cu_seqlens, batch.kv_lens
+    if not (q.is_cuda and q.is_contiguous() and out.is_contiguous() and out.dtype is q.dtype and q.shape == out.shape == (T, nq * hd)
+            and out.get_device() == dev.index):
+        _need(q, "attention_q8.q", dims=2)
+        _need(out, "attention_q8.out", q.dtype, 2)
+        if q.shape[1] != nq * hd or out.shape != q.shape or out.device != dev:
+            raise KernelError(f"attention_q8: queries {tuple(q.shape)} and outputs {tuple(out.shape)} of {nq} heads of {hd}")
+        raise KernelError(f"attention_q8: {q.shape[0]} query rows for a step of {T} tokens")
+    if not (cu_dev.dtype is kv_dev.dtype is torch.int32 and cu_dev.dim() == kv_dev.dim() == 1 and cu_dev.get_device() == kv_dev.get_device() == dev.index
+            and cu_dev.is_contiguous() and kv_dev.is_contiguous()):
+        _need_ints("attention_q8", dev, cu_seqlens=cu_dev, kv_lens=kv_dev)
     _need_table("attention_q8", block_table, dev)
-    if batch.cu_seqlens.shape[0] < n + 1 or batch.kv_lens.shape[0] < n or block_table.shape[0] < n:
+    rows, width = block_table.shape
+    if cu_dev.shape[0] <= n or kv_dev.shape[0] < n or rows < n:
         raise KernelError(f"attention_q8: a description of fewer than {n} requests")
     _need_q8("attention_q8", k_cache, v_cache, k_scale, v_scale, nkv, page_size, hd, dev)
     lib, code = library(), _code(q, "attention_q8.q")
     max_count, max_kv = batch.max_count, batch.max_kv_len
-    if max_kv > block_table.shape[1] * page_size and not batch.captured:
-        raise KernelError(f"attention_q8: {max_kv} keys in block tables of {block_table.shape[1]} pages of {page_size}")
+    if max_kv > width * page_size and not batch.captured:
+        raise KernelError(f"attention_q8: {max_kv} keys in block tables of {width} pages of {page_size}")
     cu = kv = None
     if not batch.captured and max_count > 1:        # steps of single tokens need no look at the lengths
         if len(batch.cu_seqlens_host) <= n or len(batch.kv_lens_host) < n:
             raise KernelError(f"attention_q8: a host's description of fewer than {n} requests")
         cu, kv = (ctypes.c_int * (n + 1))(*batch.cu_seqlens_host[:n + 1]), (ctypes.c_int * n)(*batch.kv_lens_host[:n])
+    floats, scratch = 0, None
     with _on(dev):
         if cu is None:
             floats = _q8_scratch(dev.index, n, max_count, max_kv, T, nq, nkv, hd, window, code)
-        else:
+        while True:                                     # (most steps with portions need no scratch: asked for once the call says so)
+            if floats:
+                scratch = torch.empty(floats, dtype=torch.float32, device=dev)
+            rc = lib.kestrel_attention_q8(
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), out.data_ptr(), _p(scratch), floats,
+                cu, kv, cu_dev.data_ptr(), kv_dev.data_ptr(), block_table.data_ptr(), n, max_count, max_kv,
+                width, block_table.stride(0), page_size, k_cache.shape[0], T, nq, nkv, hd, window, scale, code, described, _stream())
+            if rc != _Q8_NEEDS_SCRATCH or floats:
+                break
             floats = lib.kestrel_attention_q8_scratch(cu, kv, n, max_count, max_kv, T, nq, nkv, hd, window, code)
-        scratch = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
-        rc = lib.kestrel_attention_q8(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), out.data_ptr(), _p(scratch), floats,
-            cu, kv, batch.cu_seqlens.data_ptr(), batch.kv_lens.data_ptr(), block_table.data_ptr(), n, max_count, max_kv,
-            block_table.shape[1], block_table.stride(0), page_size, k_cache.shape[0], T, nq, nkv, hd, window, scale, code, described, _stream())
     if rc < 0:
         raise KernelError(lib.kestrel_last_error().decode("utf-8", "replace"))
     global launches

@@ -475,6 +475,7 @@ KESTREL_API int kestrel_attn_planner_last_launches(void *planner);
  * A plane of the cache is int8 codes [pages, nkv, page_size, hd] in [-127, 127] and float32 scales [pages, nkv, page_size / KESTREL_Q8_BLOCK];
  * a value is code * scale, and KESTREL_Q8_BLOCK consecutive tokens share the scale of their head. */
 #define KESTREL_Q8_BLOCK 16
+#define KESTREL_Q8_NEEDS_SCRATCH 8     /* minus that, of kestrel_attention_q8: nothing was launched */
 /* Bias, per-head norm and rotation of a step's product (float32 [S, T, (nq + 2 nkv) hd]; rot_mode 0 rotate-half, 1 interleaved); queries to q_out
  * (float32 or bfloat16), keys and values to their blocks.  A block's scale is max(2^-64, largest magnitude / 127) over what it has met since its
  * first token; codes that earlier steps left in it are rounded again where it rises.  A block that met a value that is not finite has a scale that is
@@ -484,7 +485,7 @@ KESTREL_API int kestrel_attn_planner_last_launches(void *planner);
 KESTREL_API int kestrel_attn_prepare_q8(const float *partial, int S, long long slice_stride, const float *bias, const float *q_norm_w, const float *k_norm_w, float norm_eps, const float *inv_freq, int rot, int rot_mode, float rot_scale, const int *positions, const int *cu_seqlens, int nseq, const int *block_table, int table_width, int table_stride, int page_size, int cache_pages, void *k_cache, void *v_cache, float *k_scale, float *v_scale, void *q_out, int dtype, int T, int nq, int nkv, int hd, int write_kv, int described, kestrel_stream_t stream);
 /* Causal attention of a step's queries over such pages; q and out float32 or bfloat16 [T, nq hd].  cu_host and kv_host are the host's copies of
  * cu_seqlens and kv_lens, or NULL where only the bounds are known (a step recorded for replay).  scratch holds kestrel_attention_q8_scratch floats.
- * Returns the number of kernels launched. */
+ * Returns the number of kernels launched, or -KESTREL_Q8_NEEDS_SCRATCH where scratch is too small. */
 KESTREL_API long long kestrel_attention_q8_scratch(const int *cu_host, const int *kv_host, int nseq, int max_count, int max_kv, int T, int nq, int nkv, int hd, int window, int dtype);
 KESTREL_API int kestrel_attention_q8(const void *q, const void *k_cache, const void *v_cache, const float *k_scale, const float *v_scale, void *out, float *scratch, long long scratch_floats, const int *cu_host, const int *kv_host, const int *cu_seqlens, const int *kv_lens, const int *block_table, int nseq, int max_count, int max_kv, int table_width, int table_stride, int page_size, int cache_pages, int T, int nq, int nkv, int hd, int window, float scale, int dtype, int described, kestrel_stream_t stream);
 
