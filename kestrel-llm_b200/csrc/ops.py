@@ -425,9 +425,16 @@ def attn_prepare_q8(qkv: Partials, q_norm_w: Optional[torch.Tensor], k_norm_w: O
             v_scale.data_ptr(), q_out.data_ptr(), _code(q_out, "attn_prepare_q8.q_out"), T, nq, nkv, hd, 1 if write_kv else 0, described, _stream()))
 
 
+@functools.lru_cache(maxsize=256)
+def _q8_ones(n: int):
+    """The host's cu_seqlens of n requests of one token."""
+    return (ctypes.c_int * (n + 1))(*range(n + 1))
+
+
 @functools.lru_cache(maxsize=1024)
 def _q8_scratch(device: int, n: int, max_count: int, max_kv: int, T: int, nq: int, nkv: int, hd: int, window: int, code: int) -> int:
-    """Floats of scratch that a step of single tokens, or a recorded one, needs on the current device: a matter of its sizes."""
+    """Floats of scratch that a step of which only the sizes are known needs on the current device: what a recorded step takes, and what one of
+    single tokens begins with."""
     return library().kestrel_attention_q8_scratch(None, None, n, max_count, max_kv, T, nq, nkv, hd, window, code)
 
 
@@ -463,13 +470,16 @@ def attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     if max_kv > width * page_size and not batch.captured:
         raise KernelError(f"attention_q8: {max_kv} keys in block tables of {width} pages of {page_size}")
     cu = kv = None
-    if not batch.captured and max_count > 1:        # steps of single tokens need no look at the lengths
-        if len(batch.cu_seqlens_host) <= n or len(batch.kv_lens_host) < n:
+    if not batch.captured:
+        cu_host, kv_host = batch.cu_seqlens_host, batch.kv_lens_host
+        if len(cu_host) > n and len(kv_host) >= n:      # which kernel, and how it is cut, is a matter of all lengths
+            cu = _q8_ones(n) if max_count == 1 and T == n else (ctypes.c_int * (n + 1))(*cu_host[:n + 1])
+            kv = (ctypes.c_int * n)(*kv_host[:n])
+        elif max_count > 1:
             raise KernelError(f"attention_q8: a host's description of fewer than {n} requests")
-        cu, kv = (ctypes.c_int * (n + 1))(*batch.cu_seqlens_host[:n + 1]), (ctypes.c_int * n)(*batch.kv_lens_host[:n])
     floats, scratch = 0, None
     with _on(dev):
-        if cu is None:
+        if max_count == 1 or cu is None:
             floats = _q8_scratch(dev.index, n, max_count, max_kv, T, nq, nkv, hd, window, code)
         while True:                                     # (most steps with portions need no scratch: asked for once the call says so)
             if floats:
@@ -478,9 +488,12 @@ def attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
                 q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), out.data_ptr(), _p(scratch), floats,
                 cu, kv, cu_dev.data_ptr(), kv_dev.data_ptr(), block_table.data_ptr(), n, max_count, max_kv,
                 width, block_table.stride(0), page_size, k_cache.shape[0], T, nq, nkv, hd, window, scale, code, described, _stream())
-            if rc != _Q8_NEEDS_SCRATCH or floats:
+            if rc != _Q8_NEEDS_SCRATCH:
                 break
-            floats = lib.kestrel_attention_q8_scratch(cu, kv, n, max_count, max_kv, T, nq, nkv, hd, window, code)
+            needed = lib.kestrel_attention_q8_scratch(cu, kv, n, max_count, max_kv, T, nq, nkv, hd, window, code)
+            if needed <= floats:
+                break
+            floats = needed
     if rc < 0:
         raise KernelError(lib.kestrel_last_error().decode("utf-8", "replace"))
     global launches

@@ -1,0 +1,69 @@
+"""How a step of attention over pages of 8-bit codes is cut: by its requests' own lengths, and safely where these are not known."""
+from types import SimpleNamespace
+
+import pytest
+
+from q8_util import attend64, planes, step
+from test_attention_q8_gpu import _near
+
+pytestmark = pytest.mark.gpu
+
+
+def _inputs(s, nq, nkv, hd, dtype):
+    import torch
+    k, ks, v, vs = planes(s, nkv, hd)
+    q = torch.randn((s.num_tokens, nq * hd), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").to(getattr(torch, dtype))
+    return q, k, ks, v, vs
+
+
+def _attend(s, nq, nkv, hd, q, k, ks, v, vs, out):
+    """Kernels that the call launched."""
+    from kestrel_llm_b200.csrc import ops
+    before = ops.launches
+    ops.attention_q8(q, k, v, ks, vs, out, s, s.table, s.page, nq, nkv, hd, 0, hd ** -0.5)
+    return ops.launches - before
+
+
+def _check(s, nq, nkv, hd, dtype, q, k, ks, v, vs, out):
+    from kestrel_llm_b200.csrc import ops
+    ops.raise_on_kernel_error()
+    want, size = attend64(q, k, ks, v, vs, s, nq, nkv, hd, 0, hd ** -0.5)
+    _near(s, out.view(s.num_tokens, nq, hd).double(), want, size, dtype)
+
+
+@pytest.mark.parametrize("contexts,launches", [([16000] + [300] * 26, 2), ([300] * 26 + [16000], 2), ([4000] * 27, 1), ([16000] + [300] * 7, 2), ([1003], 1)])
+def test_one_long_request_among_short_ones_is_shared_out(contexts, launches):
+    """A cluster a pair (one kernel) would leave a long request to two CTAs while the others wait; stretches are two kernels."""
+    import torch
+    nq, nkv, hd = 32, 8, 128
+    s = step([(1, c) for c in contexts], 64)
+    x = _inputs(s, nq, nkv, hd, "bfloat16")
+    out = torch.full_like(x[0], float("nan"))
+    assert _attend(s, nq, nkv, hd, *x, out) == launches
+    _check(s, nq, nkv, hd, "bfloat16", *x, out)
+
+
+@pytest.mark.parametrize("nq,nkv", [(40, 1), (34, 2)])
+@pytest.mark.parametrize("contexts", [[1000] * 10, [700, 3, 2000], [0]])
+def test_more_than_sixteen_query_heads_a_kv_head(nq, nkv, contexts):
+    """Single tokens of more rows than the kernel for few rows takes at once: no launch for requests of fewer rows, which there are none of."""
+    import torch
+    s = step([(1, c) for c in contexts], 16)
+    x = _inputs(s, nq, nkv, 128, "bfloat16")
+    out = torch.full_like(x[0], float("nan"))
+    assert _attend(s, nq, nkv, 128, *x, out) == 1
+    _check(s, nq, nkv, 128, "bfloat16", *x, out)
+
+
+def test_host_lists_of_single_tokens_that_are_missing_or_longer():
+    import torch
+    nq, nkv, hd = 8, 2, 64
+    s = step([(1, 90), (1, 4000), (1, 3)], 16)
+    x = _inputs(s, nq, nkv, hd, "float32")
+    outs = []
+    for kw in (dict(), dict(cu_seqlens_host=[], kv_lens_host=[]), dict(cu_seqlens_host=s.cu_seqlens_host + [3], kv_lens_host=s.kv_lens_host + [9])):
+        out = torch.full_like(x[0], float("nan"))
+        _attend(SimpleNamespace(**{**vars(s), **kw}), nq, nkv, hd, *x, out)
+        _check(s, nq, nkv, hd, "float32", *x, out)
+        outs.append(out)
+    assert torch.equal(outs[0], outs[2])
