@@ -337,7 +337,7 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
         }
         const long long pairs = (long long)nseq * ((most + 15) / 16) * nkv;
         if (all && most > 16 && pairs <= 2ll * kestrel_sms() && tiles <= (single ? 24 : 8) * 2ll * kestrel_sms() &&
-            (q8_decode_cluster(pairs, (longest + 63) / 64, tiles, hd, Q8_SIXTEEN) > 0 || (single && pairs <= q8_decode_ctas(tiles, hd, Q8_SIXTEEN))))
+            (q8_decode_cluster(pairs, (longest + 63) / 64, tiles, hd, Q8_SIXTEEN, true) > 0 || (single && pairs <= q8_decode_ctas(tiles, hd, Q8_SIXTEEN))))
             small.rows_upto = FEW;
     }
     large.kernel = TC;
@@ -417,7 +417,7 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
             p->ctas = q8_decode_ctas(p->key_tiles, hd, p->form);
             p->row_tiles = (p->most_rows + p->rows_per_tile - 1) / p->rows_per_tile;
             if (p->row_tiles == 1) p->tiles = nseq;
-            p->slices = q8_decode_cluster(p->tiles * nkv, (p->longest + 63) / 64, p->key_tiles, hd, p->form);
+            p->slices = q8_decode_cluster(p->tiles * nkv, (p->longest + 63) / 64, p->key_tiles, hd, p->form, cu != nullptr);
             p->scratch = p->slices ? 0 : q8_decode_scratch(p->ctas, hd);
         } else {
             // The tensor cores: one CTA an SM, slices of two key tiles at least.  The CUDA cores: two CTAs an SM, which a key tile takes 6 us, the

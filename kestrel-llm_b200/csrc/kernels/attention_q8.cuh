@@ -110,7 +110,8 @@ __device__ __forceinline__ size_t q8_out_row(const Q8Params &p, const Q8Tile &t,
 enum Q8Form { Q8_EIGHT, Q8_SIXTEEN, Q8_WIDE_EIGHT, Q8_WIDE_SIXTEEN };      // tiles of 8 or 16 rows (Q8Params.rows_per_tile) of bfloat16, of float32
 int q8_launch_decode(const Q8Params &p, Q8Form form, int ctas, cudaStream_t stream);
 int q8_decode_ctas(long long tiles, int hd, Q8Form form);       // for so many (row tile, kv head, 64 keys)
-int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int hd, Q8Form form);        // CTAs a pair (Q8Params.slices), or 0: ctas in stretches
+// CTAs a pair (Q8Params.slices), or 0: ctas in stretches; exact: by the requests' own lengths, else by bounds of them
+int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int hd, Q8Form form, bool exact);
 long long q8_decode_scratch(int ctas, int hd);          // floats: part_o, then part_ml
 int q8_decode_error();                                  // its bounded waits' error word; synchronises
 // attention_q8_tc.cu: tiles of up to 256 rows, head sizes 64 and 128, bfloat16

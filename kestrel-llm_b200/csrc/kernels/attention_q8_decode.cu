@@ -922,15 +922,22 @@ int q8_decode_ctas(long long tiles, int hd, Q8Form form) {
     return (int)(tiles / 2 < 1 ? 1 : tiles / 2 < most ? tiles / 2 : most);
 }
 
-// CTAs a pair, or 0 for stretches.  Where every pair can have its CTAs at once, as many as let every cluster be resident, up to 8, and two
-// tiles each, or up to 16 where these have four (two requests behind 8,000 keys 15 us, 18 with 8; one behind 4,095 in float32 12 and 15; one
-// behind 2,000 9 and 8); taken where the longest pair's share is no more than six tiles above a stretch, which is about what the join kernel takes (32 / 8 heads of 128: a request behind 1,003 keys
-// 6.5 us with 8 CTAs a pair, 16 with one, 10 in stretches; two behind 65,535 126 us with 8, 55 in stretches; 32 behind 500 13 with one, 17 in
-// stretches; 8 behind 4,095 18 with 6, 23 in stretches).  Where
-// there are more pairs, one, if the wait for the last one is worth what pairs cost a stretch: some five tiles' time each, and the join
-// (32 / 8 heads of 128, bfloat16: 256 requests behind 300, 1,000, 2,000 keys 46, 102, 184 us, in stretches 77, 133, 220; behind 20 to 1,805
-// 98 and 211; 64 behind 300, 1,000 15, 37, in stretches 22, 39, behind 4,095 138 and 99; 411 float32 tokens of one request, 16 / 4 heads, 25 and 39).
-int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int hd, Q8Form form) {
+// CTAs a pair, or 0 for stretches.  (Times in us; bfloat16, 32 / 8 heads of 128 | of 64 | float32 of 128 | of 64.)
+// Where every pair can have its CTAs at once, as many as let every cluster be resident, up to 8, and two tiles each, or up to 16 where these have
+// four; taken where the longest pair's share is no more than six tiles above a stretch, which is about what the join kernel takes:
+//     1 request behind 1,003: 8 CTAs 6.2 | 5.5 | 6.6 | 5.9, stretches 7.8 | 7.1 | 8.6 | 7.9;   1 behind 4,095: 16 CTAs 10 | 8.3 | 11 | 9.2, 8 10 | 8.7 | 12.5 | 11
+//     2 behind 8,000: 16 CTAs 15 | 12 | 28 | 24, 8 18 | 14 | 23 | 18, stretches 17 | 15 | 19 | 15 (float32 holds fewer such clusters: stretches)
+//     8 behind 4,095: rule 18 | 14 | 24 | 20, stretches 20 | 17 | 28 | 22;   32 behind 500: one CTA 13 | 10 | 14 | 11, stretches 17 | 15 | 20 | 16
+//     27 behind 4,000: two CTAs 40 | 30 | 78 | 62, stretches 45 | 39 | 67 | 49 (float32: taken);   55 behind 4,000: one 71 | 50 | 125 | 107, stretches 82 | 58 | 128 | 90
+// Where only bounds are known (a recorded step, whose requests may be far shorter than the longest) a share is sixteen tiles at most: 8 requests
+// behind 6,000, shares of 16, 23 | 17 | 46 | - against 25 | 21 | 36 in stretches, one behind 6,000 and seven behind 300 21 | 16 | 21 against 17 | 15 | 17, but
+// one behind 16,000 and seven behind 300, shares of 42, 45 | 34 | 48 against 22 | 19 | 25.  Stretches follow the real lengths.
+// Where there are more pairs, one CTA, if the wait for the last one is worth what pairs cost a stretch: some five tiles' time each, and the join:
+//     256 behind 300: one 45 | 35 | 69 | 55, stretches 71 | 51 | 93 | 66;   behind 2,000: 172 | 123 | 264 | 208 and 203 | 143 | 312 | 221
+//     256 behind 20 to 1,805: 94 | 73 | 149 | 120 and 205 | 156 | 301 | 222;   one behind 4,000 and 255 behind 300: 52 | 40 | 73 and 73 | 52 | 96
+//     64 behind 1,000: 35 | 26 | 44 | 34 and 38 | 29 | 52 | 37;   behind 4,095: 111 | 82 | 143 | 111 and 97 | 67 | 148 | 104;   one behind 1,500 and 63 behind 20: 19 | 16 | 24 and 14 | 11 | 19
+//     411 float32 tokens of one request, 16 / 4 heads of 128: 25 and 35
+int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int hd, Q8Form form, bool exact) {
     static DeviceTable<8 * (MAX_CLUSTER + 1)> known;
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess) {
@@ -945,7 +952,8 @@ int q8_decode_cluster(long long pairs, int longest_tiles, long long tiles, int h
     const long long ctas = q8_decode_ctas(tiles, hd, form), stretch = (tiles + ctas - 1) / ctas;
     const int most = longest_tiles >= 4 * MAX_CLUSTER ? MAX_CLUSTER : 8;
     for (int size = longest_tiles / 2 < most ? (longest_tiles < 2 ? 1 : longest_tiles / 2) : most; size >= 1; --size) {
-        if ((longest_tiles + size - 1) / size > stretch + 6) break;
+        const int share = (longest_tiles + size - 1) / size;
+        if (share > stretch + 6 || (!exact && share > 16)) break;
         if (pairs <= resident(size)) return size;
     }
     const int at_once = resident(1);

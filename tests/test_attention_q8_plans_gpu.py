@@ -67,3 +67,29 @@ def test_host_lists_of_single_tokens_that_are_missing_or_longer():
         _check(s, nq, nkv, hd, "float32", *x, out)
         outs.append(out)
     assert torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("nq,nkv,bound,launches,replays", [
+    (32, 8, 16384, 2, [[16000] + [300] * 7, [300] * 8, [0] * 7 + [16000], [16000] * 8]),       # shares of 42 tiles in clusters of 6: stretches
+    (32, 8, 1024, 1, [[1000] + [20] * 7, [1000] * 8])])                                        # shares of three: clusters
+def test_recorded_steps_are_cut_for_requests_of_any_length(nq, nkv, bound, launches, replays):
+    import torch
+    hd = 128
+    held = step([(1, bound - 1)] * 8, 64)
+    q, k, ks, v, vs = _inputs(held, nq, nkv, hd, "bfloat16")
+    k.div_(4, rounding_mode="trunc")                # scores of a few units
+    out = torch.empty_like(q)
+    s = step([(1, bound - 1)] * 8, 64)
+    s.table, s.captured, s.max_kv_len = held.table, True, bound
+    assert _attend(s, nq, nkv, hd, q, k, ks, v, vs, out) == launches
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _attend(s, nq, nkv, hd, q, k, ks, v, vs, out)
+    for contexts in replays:
+        now = step([(1, c) for c in contexts], 64)
+        now.table = held.table
+        s.kv_lens.copy_(now.kv_lens)
+        out.fill_(float("nan"))
+        graph.replay()
+        _check(now, nq, nkv, hd, "bfloat16", q, k, ks, v, vs, out)
