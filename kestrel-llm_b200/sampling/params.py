@@ -3,6 +3,7 @@
 """
 from __future__ import annotations
 
+import operator
 from dataclasses import dataclass, field
 from typing import Optional, Tuple
 
@@ -23,8 +24,13 @@ class SamplingParams:
     logprobs: Optional[int] = None    # report every token's log probability and this many of the likeliest alternatives (0..32); None: no report
 
     def __post_init__(self):
-        if self.logprobs is not None and not 0 <= int(self.logprobs) <= 32:
-            raise ValueError(f"logprobs {self.logprobs} outside 0..32")
+        if self.logprobs is not None:
+            try:
+                self.logprobs = operator.index(self.logprobs)
+            except TypeError:
+                raise ValueError(f"logprobs {self.logprobs!r} is no whole number") from None
+            if not 0 <= self.logprobs <= 32:
+                raise ValueError(f"logprobs {self.logprobs} outside 0..32")
         if not 1 <= int(self.repetition_window) <= 64:
             raise ValueError(f"repetition_window {self.repetition_window} outside 1..64")
         if self.repetition_penalty >= 1e3:
