@@ -54,7 +54,7 @@ class GroupedQueryAttention(Mixer):
         self.graph_safe = heads // kv_heads <= 16
 
     def cache_spec(self) -> PagedKVSpec:
-        return PagedKVSpec(self.kv_heads, self.head_dim, self.window, codes=self.head_dim % 16 == 0 and self.head_dim <= 256)
+        return PagedKVSpec(self.kv_heads, self.head_dim, self.window, codes=self.head_dim % 16 == 0)
 
     def weight_slots(self) -> List[WeightSlot]:
         p = self.prefix
