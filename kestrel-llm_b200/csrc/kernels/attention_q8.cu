@@ -381,6 +381,9 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
         }
         if (halves < LLONG_MAX && halves / 5 * 4 <= whole) large.rows_per_tile = 128;
     }
+    // Recorded for no more than 128 rows a request (more than 16 query heads a kv head, single tokens): likewise (40 / 1 heads, ten requests behind
+    // 1,000 keys 12.1 us in tiles of 128, 13.7 of 256; 64 of them 18.6 and 23.0; 72 / 2 heads, 32 behind 2,000 24 and 32).
+    if (!cores && !wide && !cu && (long long)max_count * G <= 128) large.rows_per_tile = 128;
     large.rows_above = small.rows_upto;
     // float32: sixteen rows at head size 64, where they fit the registers (32 / 8 heads, 300 tokens behind 600 53 us, 64 in tiles of eight;
     // at 128, with spilled registers, 30 and 25 for 411 tokens)
@@ -403,7 +406,7 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
     };
     if (cu) {
         for (int i = 0; i < nseq; ++i) count((long long)(cu[i + 1] - cu[i]) * G, kv[i], 1);
-    } else if ((long long)max_count * G <= small.rows_upto) {
+    } else if ((long long)max_count * G <= small.rows_upto || G > small.rows_upto) {
         count((long long)max_count * G, max_kv, nseq);
     } else {                            // any request may be of either kind: both launches are made for all of them
         count(std::min<long long>(small.rows_upto, (long long)max_count * G), max_kv, nseq);

@@ -71,7 +71,8 @@ def test_host_lists_of_single_tokens_that_are_missing_or_longer():
 
 @pytest.mark.parametrize("nq,nkv,bound,launches,replays", [
     (32, 8, 16384, 2, [[16000] + [300] * 7, [300] * 8, [0] * 7 + [16000], [16000] * 8]),       # shares of 42 tiles in clusters of 6: stretches
-    (32, 8, 1024, 1, [[1000] + [20] * 7, [1000] * 8])])                                        # shares of three: clusters
+    (32, 8, 1024, 1, [[1000] + [20] * 7, [1000] * 8]),                                         # shares of three: clusters
+    (40, 1, 1024, 2, [[1000] + [20] * 7, [1000] * 8, [0] * 8])])                               # the portions' kernel and its merge, nothing for fewer rows
 def test_recorded_steps_are_cut_for_requests_of_any_length(nq, nkv, bound, launches, replays):
     import torch
     hd = 128
