@@ -54,9 +54,9 @@ struct State {
     }
 };
 
-// order of the numbers as that of unsigned integers, never 0
+// order of the numbers as that of unsigned integers, never 0; what is no number counts as minus infinity, as the threads' maxima have it
 __device__ __forceinline__ uint32_t key_of(float x) {
-    const uint32_t u = __float_as_uint(x + 0.f);                    // -0 counts as 0
+    const uint32_t u = __float_as_uint(x == x ? x + 0.f : -INFINITY);       // -0 counts as 0
     const uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
     return k ? k : 1u;
 }

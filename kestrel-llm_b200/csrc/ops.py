@@ -518,7 +518,8 @@ def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, top
     """Natural log probabilities under softmax(logits[r]), logits float32 [R, V] with neighbouring columns (rows may be further apart):
     of the given tokens ``ids`` (int32 [R]; an id outside the vocabulary gets NaN), and of the ``top`` likeliest tokens, at most
     ``MAX_TOP_LOGPROBS`` of them, most likely first, equal ones by id; and every distribution's entropy.  A logit of minus infinity has
-    probability zero; a row of nothing else, or with a logit of plus infinity or NaN, has NaN for log probabilities and entropy."""
+    probability zero; a row of nothing else, or with a logit of plus infinity or NaN, has NaN for log probabilities and entropy, and its
+    likeliest tokens are those of its logits with NaN as minus infinity."""
     if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1 or not logits.is_cuda:
         _need(logits, "token_logprobs.logits", torch.float32, 2)
     R, V = logits.shape

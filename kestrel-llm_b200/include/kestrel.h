@@ -494,7 +494,8 @@ KESTREL_API int kestrel_attention_q8_error(void);
 
 /* ---- log probabilities ---- */
 /* Of every row of logits float32 [R, ld], V of them: the log probability of ids[r] (ids may be NULL; an id outside [0, V) gives NaN), the entropy
- * in nats (entropy may be NULL), and the `top` likeliest tokens, most likely first, ties to the lowest id. */
+ * in nats (entropy may be NULL), and the `top` likeliest tokens, most likely first, ties to the lowest id, NaN
+ * as minus infinity. */
 #define KESTREL_LOGPROBS_MAX_TOP 32
 KESTREL_API int kestrel_token_logprobs(const float *logits, long long ld, int R, int V, const int *ids, int top, float *logprobs, float *entropy, int *top_ids, float *top_logprobs, kestrel_stream_t stream);
 
