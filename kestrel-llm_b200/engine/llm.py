@@ -400,7 +400,7 @@ class LLM:
     def score(self, prompts: Sequence[Sequence[int]], top: int = 0) -> List[List[TokenScore]]:
         """The log probability of every token of every prompt after its first, given the tokens before it, with the ``top`` likeliest tokens
         at its place: how well the model foresees a text, and what a cache of another type changes.  Runs steps of its own, while no request
-        is live; nothing of the prompts stays in the cache."""
+        is live; nothing of the prompts stays in the cache, and later requests sample what they would have sampled."""
         if self.has_unfinished():
             raise RuntimeError("score() runs steps of its own: requests are live")
         if not 0 <= top <= min(ops.MAX_TOP_LOGPROBS, self.engine.vocab_size):
@@ -418,6 +418,7 @@ class LLM:
         budget = max(1, min(self.options.max_step_tokens, self.options.prefill_batch, (1 << 28) // engine.vocab_size))
         waiting = [i for i, p in enumerate(texts) if len(p) > 1]
         running: List[Tuple[int, int]] = []              # (text, request id)
+        started = 0
         try:
             while waiting or running:
                 # as many texts at once as the step has tokens, and the cache slots and pages for all of their tokens
@@ -428,8 +429,8 @@ class LLM:
                     held = [sum(cache.num_blocks(r, g) for _, r in running) for g in range(cache.num_groups)]
                     if running and any(pages > cache.free_pages(g) + held[g] for g in range(cache.num_groups)):
                         break
-                    rid = self._next_id
-                    self._next_id += 1
+                    rid = -1 - started               # not a number of the requests', whose seeds come from theirs
+                    started += 1
                     engine.admit(rid)
                     running.append((i, rid))
                     waiting.pop(0)
