@@ -382,6 +382,11 @@ def _need_table(what: str, block_table: torch.Tensor, device: torch.device) -> N
                           f"got {block_table.dtype} {tuple(block_table.shape)} on {block_table.device}")
 
 
+def _row_stride(block_table: torch.Tensor) -> int:
+    """Of a table of one row the stride says nothing."""
+    return block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1]
+
+
 def attn_prepare_q8(qkv: Partials, q_norm_w: Optional[torch.Tensor], k_norm_w: Optional[torch.Tensor], norm_eps: float,
                     inv_freq: Optional[torch.Tensor], rotary_dim: int, positions: torch.Tensor, cu_seqlens: torch.Tensor,
                     block_table: torch.Tensor, page_size: int, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -421,7 +426,7 @@ def attn_prepare_q8(qkv: Partials, q_norm_w: Optional[torch.Tensor], k_norm_w: O
         _check(library().kestrel_attn_prepare_q8(
             qkv.data.data_ptr(), qkv.slices, qkv.slice_stride, _p(qkv.bias), _p(q_norm_w), _p(k_norm_w), norm_eps, _p(inv_freq),
             rotary_dim, rot_mode, rot_scale, positions.data_ptr(), cu_seqlens.data_ptr(), n, block_table.data_ptr(), block_table.shape[1],
-            block_table.stride(0), page_size, k_cache.shape[0], k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+            _row_stride(block_table), page_size, k_cache.shape[0], k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
             v_scale.data_ptr(), q_out.data_ptr(), _code(q_out, "attn_prepare_q8.q_out"), T, nq, nkv, hd, 1 if write_kv else 0, described, _stream()))
 
 
@@ -487,7 +492,7 @@ def attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
             rc = lib.kestrel_attention_q8(
                 q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), out.data_ptr(), _p(scratch), floats,
                 cu, kv, cu_dev.data_ptr(), kv_dev.data_ptr(), block_table.data_ptr(), n, max_count, max_kv,
-                width, block_table.stride(0), page_size, k_cache.shape[0], T, nq, nkv, hd, window, scale, code, described, _stream())
+                width, _row_stride(block_table), page_size, k_cache.shape[0], T, nq, nkv, hd, window, scale, code, described, _stream())
             if rc != _Q8_NEEDS_SCRATCH:
                 break
             needed = lib.kestrel_attention_q8_scratch(cu, kv, n, max_count, max_kv, T, nq, nkv, hd, window, code)

@@ -94,3 +94,22 @@ def test_recorded_steps_are_cut_for_requests_of_any_length(nq, nkv, bound, launc
         out.fill_(float("nan"))
         graph.replay()
         _check(now, nq, nkv, hd, "bfloat16", q, k, ks, v, vs, out)
+
+
+def test_a_block_table_of_one_row_whatever_its_stride_says():
+    import torch
+    from kestrel_llm_b200.csrc import ops
+    nq, nkv, hd, page = 8, 2, 64, 16
+    s = step([(1, 90)], page)
+    inv_freq = torch.ones(hd // 2, device="cuda")
+    qkv = torch.randn((1, 1, (nq + 2 * nkv) * hd), device="cuda")
+    x = _inputs(s, nq, nkv, hd, "bfloat16")
+    got = []
+    for table in (s.table, s.table.reshape(-1, 1).clone().t()):
+        assert table.shape == s.table.shape
+        q, k, ks, v, vs = (t.clone() for t in x)
+        out = torch.empty_like(q)
+        ops.attn_prepare_q8(ops.Partials(qkv), None, None, 0.0, inv_freq, hd, s.positions, s.cu_seqlens, table, page, k, v, ks, vs, q, nq, nkv, hd)
+        ops.attention_q8(q, k, v, ks, vs, out, s, table, page, nq, nkv, hd, 0, hd ** -0.5)
+        got.append((k, v, q, out))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
