@@ -12,7 +12,8 @@ vocabulary 151936), bfloat16, random weights; prompts are uniform random token i
 one decode step of the whole batch at a context that ends at 4,096 tokens; the ids a step picks
 are the next step's input (on the device), and the cache pages are handed out in a scattered
 order, as after long serving.  `--layers` runs fewer layers of the same sizes (the record names
-both numbers); layer sizes never shrink.
+both numbers); layer sizes never shrink.  `--cache-dtype int8` keeps keys and values as 8-bit
+codes; the record's metric says so.
 
 `--workload mix14b`: 32 requests with prompts of 128 to 2,048 tokens (seed-fixed) and 256 greedy
 tokens each at the sizes of Qwen3-14B, through `LLM.add_request` / `LLM.step`, prompt portions
@@ -726,6 +727,7 @@ def main() -> int:
     ap.add_argument("--impl", default="ours", choices=["ours", "reference"])
     ap.add_argument("--skip-points", action="store_true", help="leave out batch 1 and 64")
     ap.add_argument("--page-size", type=int, default=16, help="tokens per cache page (default 16)")
+    ap.add_argument("--cache-dtype", default="", choices=["", "int8"], help="the default workload with a cache of 8-bit codes (default: the model's type)")
     ap.add_argument("--context", type=int, default=CONTEXT, help="context length at which the decode steps end (default 4096)")
     ap.add_argument("--prefill-tokens", type=int, default=PREFILL_TOKENS, help="tokens of the prefill step (default 2048)")
     ap.add_argument("--workload", default="decode8b", choices=["decode8b", "mix14b", "32b", "zidivik", "tidavik", "toredra", "korirax", "tuganex", "fasanex"],
@@ -773,12 +775,18 @@ def main() -> int:
     longest = max(CONTEXT, PREFILL_TOKENS) + 64
     opts = EngineOptions(dtype="bfloat16", page_size=args.page_size, batch_max=max_batch, max_model_len=longest,
                          max_tokens=max(max_batch * (CONTEXT + 64), longest), max_step_tokens=max(PREFILL_TOKENS, max_batch),
-                         prefill_batch=PREFILL_TOKENS)
+                         prefill_batch=PREFILL_TOKENS, cache_dtype=args.cache_dtype)
     llm = LLM(model, dtype="bfloat16", options=opts)
     engine = llm.engine
     engine.cache.shuffle_free(0)                     # pages in a scattered order, as after long serving
-    for t in engine.cache.k + engine.cache.v:        # cache contents for the synthetic contexts
-        if t is not None:
+    for t in engine.cache.k + engine.cache.v + engine.cache.k_scale + engine.cache.v_scale:       # cache contents for the synthetic contexts
+        if t is None:
+            continue
+        if t.dtype == torch.int8:
+            t.random_(-127, 128)
+        elif engine.cache.codes:
+            t.fill_(0.5 / 73)                        # codes of equal probability have a standard deviation of 73
+        else:
             t.normal_(0.0, 0.5)
     rng = np.random.default_rng(0)
     pk = peaks()
@@ -789,7 +797,7 @@ def main() -> int:
     per_layer = (cfg.q_size + 2 * cfg.kv_size) * cfg.hidden_size + cfg.hidden_size * cfg.q_size \
         + 3 * cfg.intermediate_size * cfg.hidden_size
     weight_bytes = esz * (L * per_layer + cfg.vocab_size * cfg.hidden_size)
-    kv_bytes_per_token = L * 2 * cfg.kv_size * esz
+    kv_bytes_per_token = engine.cache.bytes_per_token()
 
     def timed(fn, n):
         torch.cuda.synchronize()
@@ -908,6 +916,9 @@ def main() -> int:
                      "frac": round(achieved / pk["hbm_gbs"], 4)},
         "points": out_points, "clocks": clocks.summary(),
     }
+    if engine.cache.codes:
+        rec["metric"] += ", cache of 8-bit codes"
+        rec["config"]["cache_dtype"] = args.cache_dtype
     print(json.dumps(rec))
     return 0
 
