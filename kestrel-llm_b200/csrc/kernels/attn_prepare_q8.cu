@@ -6,10 +6,17 @@
 // queries.  A block that earlier steps began and whose scale rises is read back and rounded again by the CTA that owns it: one owner a
 // block, no atomics.  A row (one head of one token) belongs to LPR lanes that hold four neighbouring numbers each (NV times); the members
 // of a rotation pair meet in shared memory.  Bound by the product's float32 bytes; at 2,048 tokens, 32 / 8 heads of 128, rotated and normed
-// (71 MB), 20 us, 3.5 TB/s, which instructions hold back: cosines, sums over a row, codes.  64 requests' tokens 7 us and one 4 us: latency.
+// (71 MB), 18 us in a row of calls and 23 from cold caches, 3.9 and 3.1 TB/s, which instructions hold back: cosines, sums over a row, codes.
+// 64 requests' tokens 4.0 us and one 3.7, from cold caches 6.2 and 8.0 (a product in 8 slices): latency.  The general form (heads other than 64 and
+// 128, rotate-half pairs over part of a head) has pairs meet in shared memory: the same prompt with half of each head rotated 32 us, with heads of 80
+// 32, 16 / 4 heads of 256 35.
 //
 // Angles are products of an int32 position and a float32 frequency, reduced in float64: a float32 product is off by 2^-24 of an angle that
 // reaches 10^5 radians, 0.006 of one, by which every far key would be turned.
+//
+// A code is the whole number next to a float32 product with the scale's reciprocal, and the float32 product of a code with a ratio of scales where a
+// scale has risen: within 1/2 + 2^-17 and 1/2 + 2^-16 of the quotient.  (Divisions instead: 2,048 tokens 18.8 us.  The number itself is off by
+// some 2^-15 of a step.)
 #include "attention_q8.cuh"
 
 #include <math.h>
@@ -33,8 +40,8 @@ struct PrepParams {
 
 __device__ __forceinline__ float4 add4(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 
-// cosine and sine of position * frequency, times the encoding's scale: the product is exact in float64, and what whole turns leave of it
-// is off by 2^-23 at most
+// Cosine and sine of position * frequency, times the encoding's scale.  What whole turns leave of the angle is off by its rounding to float32,
+// 2^-23, and by what float64 loses: 2^-25 below position 2^28, 2^-22 at the largest; sincosf is within two units.
 __device__ __forceinline__ float2 turn(int pos, float freq, float scale) {
     const double angle = (double)pos * (double)freq, turns = rint(angle * 0.15915494309189535);
     float s, c;
@@ -125,7 +132,7 @@ struct Row {
     }
 };
 
-// Four codes as one word.  x / scale as a product with the reciprocal: off by 2^-23 of at most 127 steps.  Added to 1.5 * 2^23 a number is
+// Four codes as one word.  x / scale as a product with the reciprocal, which is off by 2^-24 of itself: 2^-17 of a step at most.  Added to 1.5 * 2^23 a number is
 // rounded to a whole one, ties to even, whose two's complement is the low byte; no number is above the one that the scale came from.
 __device__ __forceinline__ uint32_t codes_word(float a, float b, float c, float d, float inv) {
     constexpr float M = 12582912.0f;
@@ -205,7 +212,9 @@ __device__ __forceinline__ void round_again(int8_t *codes, int n, float ratio) {
 // and a warp works on four rows: a third of the instructions of the general form, which is bound by them.
 enum { TURN_NONE, TURN_HALF, TURN_NEXT };
 
-// (cosine, sine) as the codes and bfloat16 queries need them: within 2^-21
+// The same for steps with bfloat16 queries, their keys' codes included: __cosf and __sinf are off by 2^-21.2 and 2^-21.4 on [-pi, pi], so with the
+// angle's 2^-22.7 a cosine is within 2^-20 of one, an absolute error, times the scale: 2^-12 of a code's step, and 2^-11 of a bfloat16 query's
+// rounding.  Below position 2^28; 2^-19.8 at the largest.  (sincosf instead: 2,048 tokens 18.5 us, 17.9 so.)
 __device__ __forceinline__ float2 turn_fast(int pos, float freq, float scale) {
     const double angle = (double)pos * (double)freq, turns = rint(angle * 0.15915494309189535);
     const float r = (float)fma(turns, -6.283185307179586, angle);

@@ -392,9 +392,10 @@ def attn_prepare_q8(qkv: Partials, q_norm_w: Optional[torch.Tensor], k_norm_w: O
                     block_table: torch.Tensor, page_size: int, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                     v_scale: torch.Tensor, q_out: torch.Tensor, nq: int, nkv: int, hd: int, write_kv: bool = True, rot_mode: int = 0,
                     rot_scale: float = 1.0, described: bool = False) -> None:
-    """`attn_prepare` into pages of 8-bit codes: bias, per-head RMSNorm, rotation (angles of any int32 position to float32 accuracy);
-    q to q_out (float32 or bfloat16), K and V as int8 codes in [-127, 127] and one float32 scale for every ``Q8_BLOCK`` tokens and head:
-    value = code * scale, scale = max(2^-64, largest magnitude / 127) over what the block has met, codes rounded to nearest even.
+    """`attn_prepare` into pages of 8-bit codes: bias, per-head RMSNorm, rotation (angles of any int32 position in float64, cosines and sines to
+    float32 accuracy, or off by up to 2^-20 ``rot_scale`` where q_out is bfloat16 and the head size 64 or 128); q to q_out (float32 or bfloat16),
+    K and V as int8 codes in [-127, 127] and one float32 scale for every ``Q8_BLOCK`` tokens and head: value = code * scale,
+    scale = max(2^-64, largest magnitude / 127) over what the block has met, a code within 1/2 + 2^-17 of the number / scale.
     Where a step's tokens raise the scale of a block that earlier steps began, its codes are rounded again, so a block's codes depend on
     how a sequence was cut into steps (by at most half a step of the scale for each rise).  A block that met a number that is not finite
     has a scale that is not a number, until its page begins anew.  The tokens of request i are cu_seqlens[i] to cu_seqlens[i + 1] - 1, at
