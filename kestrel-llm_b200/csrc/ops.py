@@ -7,6 +7,7 @@ first call raises.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 import os
@@ -431,10 +432,11 @@ def attn_prepare_q8(qkv: Partials, q_norm_w: Optional[torch.Tensor], k_norm_w: O
             v_scale.data_ptr(), q_out.data_ptr(), _code(q_out, "attn_prepare_q8.q_out"), T, nq, nkv, hd, 1 if write_kv else 0, described, _stream()))
 
 
-@functools.lru_cache(maxsize=256)
-def _q8_ones(n: int):
-    """The host's cu_seqlens of n requests of one token."""
-    return (ctypes.c_int * (n + 1))(*range(n + 1))
+@functools.lru_cache(maxsize=64)
+def _q8_ints(values):
+    """(address, memory) of a tuple or range as the library takes whole numbers: a step's layers ask for the same ones."""
+    memory = array.array("i", values)
+    return memory.buffer_info()[0], memory
 
 
 @functools.lru_cache(maxsize=1024)
@@ -479,8 +481,9 @@ def attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     if not batch.captured:
         cu_host, kv_host = batch.cu_seqlens_host, batch.kv_lens_host
         if len(cu_host) > n and len(kv_host) >= n:      # which kernel, and how it is cut, is a matter of all lengths
-            cu = _q8_ones(n) if max_count == 1 and T == n else (ctypes.c_int * (n + 1))(*cu_host[:n + 1])
-            kv = (ctypes.c_int * n)(*kv_host[:n])
+            # (the memory is held until the call returns)
+            cu, cu_memory = _q8_ints(range(n + 1) if max_count == 1 and T == n else tuple(cu_host[:n + 1]))
+            kv, kv_memory = _q8_ints(tuple(kv_host[:n]))
         elif max_count > 1:
             raise KernelError(f"attention_q8: a host's description of fewer than {n} requests")
     floats, scratch = 0, None
