@@ -322,6 +322,8 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
         // 11.9 us against 14.8, 64 tokens 14.7 against 16.7, 128 tokens 17.7 against 17.8; 64 tokens behind 2,000 keys 27 against 19; four
         // requests of about 64 tokens behind 100, more pairs than CTAs, 19 against 11), and beside single tokens, which are a launch of the kernel
         // anyway, for three times that (requests of 2, 4, 6 and 8 tokens behind 2,000 keys 17 against 18, behind 8,000 36 against 54).
+        // (32 / 8 heads of 64: 16 tokens behind 500 8.4 against 11.9, 64 11.6 and 13.1, 64 behind 2,000 21 and 15, four of 64 behind 100 14 and 8.3,
+        // 2 to 8 behind 8,000 27 and 40; 24 / 8 of 128: 10.7 and 13.8, 14.4 and 16.4, 26 and 18, 18 and 10.6, 36 and 50.)
         long long tiles = 0;
         int most = 0, longest = 0;
         bool single = false, all = true;
@@ -348,10 +350,14 @@ void make_plan(Plan &pl, const int *cu, const int *kv, int nseq, int max_count, 
         // is rows times keys of its slice, and slices cost their merge, as much as 128 rows' 380 keys; for as much to do, tiles of 128 take four
         // fifths of the time (32 / 8 heads of 128: 256 tokens 11 us in tiles of 128, 14 of 256; 500 behind 1,500 32 and 43, where only the latter
         // need slices; 300 behind 2,000 35 and 38; 500 behind 8,000 102 and 111).
+        // (32 / 8 heads of 64: 256 tokens 8.1 and 10.8, 500 behind 1,500 27 and 36, 300 behind 2,000 28 and 30, 500 behind 8,000 86 and 94, 2,048 63 and 48;
+        // 24 / 8 of 128: 10.5 and 14.4, 31 and 38, 30 and 34, 105 and 83, 60 and 52.  Where tiles of 128 just miss the SMs they would still be faster at times:
+        // 16 / 4 of 64, 2,048 tokens 32 and 43; 24 / 8 of 128, 1,000 tokens 25 and 30.)
         // Single tokens beside portions come along where the SMs hold all of it at once and that takes no longer than a launch of the decode
         // kernel for them: what 128 rows' 400 keys take, and 55 more for every key tile of a CTA's (16 / 4 heads of 64, a window of 1,024: 500
         // tokens beside twelve single ones 20 us, in two launches 28; 32 / 8 heads of 128: 300 behind 2,000 beside six 35 and 51, 256 beside
         // eight behind 300 12 and 21, but beside one behind 3,000 31 and 22, 200 beside four behind 8,000 93 and 35).
+        // (32 / 8 heads of 64: 29 and 37, 9.9 and 14.7, 27 and 16, 79 and 25; 24 / 8 of 128: 35 and 39 - not taken -, 12 and 18, 30 and 20, 57 and 32.)
         auto work = [&](int rows_above, int rows_per_tile) {
             long long tiles = 0;
             int longest = 0;

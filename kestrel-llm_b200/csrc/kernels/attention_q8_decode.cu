@@ -933,6 +933,7 @@ int q8_decode_ctas(long long tiles, int hd, Q8Form form) {
 // Where only bounds are known (a recorded step, whose requests may be far shorter than the longest) a share is sixteen tiles at most: 8 requests
 // behind 6,000, shares of 16, 23 | 17 | 46 | - against 25 | 21 | 36 in stretches, one behind 6,000 and seven behind 300 21 | 16 | 21 against 17 | 15 | 17, but
 // one behind 16,000 and seven behind 300, shares of 42, 45 | 34 | 48 against 22 | 19 | 25.  Stretches follow the real lengths.
+// (Recorded steps of like requests pay for that: 27 behind 4,000 45 instead of 40, 55 of them 82 instead of 70.)
 // Where there are more pairs, one CTA, if the wait for the last one is worth what pairs cost a stretch: some five tiles' time each, and the join:
 //     256 behind 300: one 45 | 35 | 69 | 55, stretches 71 | 51 | 93 | 66;   behind 2,000: 172 | 123 | 264 | 208 and 203 | 143 | 312 | 221
 //     256 behind 20 to 1,805: 94 | 73 | 149 | 120 and 205 | 156 | 301 | 222;   one behind 4,000 and 255 behind 300: 52 | 40 | 73 and 73 | 52 | 96
