@@ -94,3 +94,18 @@ def test_scores_from_codes_are_those_of_the_definition(model_dirs, monkeypatch, 
         if mistake == "heads exchanged" and cfg["num_key_value_heads"] == 1:
             continue
         assert rms(got - scores(mistake)) > 2 * allowed, mistake
+
+
+@pytest.mark.parametrize("name", ["D", "E", "F"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_the_runner_and_the_walk_cut_steps_alike(model_dirs, name, dtype):
+    """Heads of 64 and 128, windows, more than sixteen query heads a kv head: both plan by the requests' own lengths, so their bits agree."""
+    from kestrel_llm_b200 import SamplingParams
+    prompts = _prompts(name, (1, 33, 70, 129))
+    outs = []
+    for native in (True, False):
+        llm = _llm(model_dirs, name, dtype, cuda_graphs=False, native_step=native)
+        assert llm.engine.cache.codes and (llm.engine.runner is not None) == native
+        got = llm.generate(prompts, SamplingParams(max_tokens=20, ignore_eos=True, logprobs=2))
+        outs.append([(o.token_ids, [(s.logprob, s.entropy, s.top) for s in o.logprobs]) for o in got])
+    assert outs[0] == outs[1]
